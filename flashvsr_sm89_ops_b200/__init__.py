@@ -16,6 +16,9 @@ from .fused_adaln import fused_ln_modulate, fused_gate_add  # noqa: E402
 from .fp8_quant import quantize_fp8, FP8_MAX  # noqa: E402
 from .fp8_linear import FP8Linear, convert_linears_fp8  # noqa: E402
 from .fp8_ffn import FP8FFN, convert_ffn_fp8  # noqa: E402
+from .fp4_quant import FP4_MAX, FP4Tensor, dequantize_fp4, quantize_fp4  # noqa: E402
+from .fp4_linear import FP4FFN, FP4Linear, convert_linears_fp4, ffn_fp4, fp4_mm  # noqa: E402
+from .fused_residual_norm import fused_residual_norm  # noqa: E402
 from .integrate import enable  # noqa: E402
 from .tiling import auto_tile_limits, plan_tiles, render_tiled, tile_weight  # noqa: E402
 
@@ -30,6 +33,16 @@ __all__ = [
     "convert_linears_fp8",
     "FP8FFN",
     "convert_ffn_fp8",
+    "FP4_MAX",
+    "FP4Tensor",
+    "quantize_fp4",
+    "dequantize_fp4",
+    "fp4_mm",
+    "ffn_fp4",
+    "FP4Linear",
+    "FP4FFN",
+    "convert_linears_fp4",
+    "fused_residual_norm",
     "plan_tiles",
     "render_tiled",
     "auto_tile_limits",

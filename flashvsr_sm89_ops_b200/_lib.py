@@ -25,6 +25,14 @@ FVB_SCALE_TENSOR = 0
 FVB_SCALE_ROW = 1
 FVB_EPI_NONE = 0
 FVB_EPI_GELU_AMAX = 1
+FVB_FP4_NV = 1
+FVB_FP4_MX = 2
+FVB_BF16 = 0
+FVB_F16 = 1
+FVB_F32 = 2
+FVB_NORM_NONE = 0
+FVB_NORM_RMS = 1
+FVB_NORM_LAYER = 2
 
 _lib = None
 _lock = threading.Lock()
@@ -74,6 +82,18 @@ _SIGS = {
     "fvb_causal_topk_pooled_csr": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp,
                                           _vp, _vp]),
     "fvb_causal_topk_pooled": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _vp]),
+    "fvb_fp4_codes_bytes": (_sz, [_i64, _i64]),
+    "fvb_fp4_scales_bytes": (_sz, [_i64, _i64, _int]),
+    "fvb_quant_fp4": (_int, [_vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
+    "fvb_dequant_fp4": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _vp, _vp]),
+    "fvb_fp4_gemm": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int, _int, _vp, _vp, _i64, _vp,
+                            _i64, _i64, _i64, _vp, _vp]),
+    "fvb_fp4_ffn_workspace_bytes": (_sz, [_i64, _i64]),
+    "fvb_fp4_ffn": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _int, _int, _vp, _vp, _vp, _vp, _vp,
+                           _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "fvb_residual_norm": (_int, [_vp, _vp, _vp, _int, _f32, _int, _vp, _vp, _f32, _int, _vp, _vp,
+                                 _vp, _vp, _f32, _i64, _i64, _i64, _vp, _vp, _int, _vp, _vp, _vp,
+                                 _vp]),
 }
 
 
@@ -133,6 +153,8 @@ def _kernels_per_call(name: str, args) -> int:
         return 4
     if name == "fvb_causal_topk_mask":
         return 3
+    if name == "fvb_fp4_ffn":
+        return 2
     if name in ("fvb_device_error", "fvb_abi_version", "fvb_last_error", "fvb_copy_window_h2d"):
         return 0  # no kernel (fvb_copy_window_h2d is a copy-engine transfer)
     return 1

@@ -1,0 +1,386 @@
+// Quantisation to microscaled 4-bit and back (fp4.cuh has the formats and the layout).
+//
+// Both directions move each element once and compute a few operations on it, so HBM bounds
+// them.  A thread's unit is 16 elements of one row: one nv block, or half an mx block whose
+// other half is the neighbouring lane's.  nv needs the row's amax before its first code, so
+// the row waits in registers (one warp up to 2048 elements, four warps up to 16384); longer
+// rows are read twice.  mx blocks are independent and are dealt to threads flat.
+#include "fp4.cuh"
+
+namespace fvb {
+namespace fp4 {
+
+template <typename T>
+struct Raw {
+  static constexpr int kVec = (int)sizeof(T);  // 16-byte vectors of 16 elements
+  uint4 v[kVec];
+};
+
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(float x) { return x; }
+
+// elements [k0, k0 + 16) of a row of K; zeros past its end.  vec: the row is 16-byte aligned
+template <typename T>
+__device__ __forceinline__ void load16(Raw<T>& r, const T* __restrict__ row, int64_t k0, int64_t K,
+                                       bool vec) {
+  if (vec && k0 + 16 <= K) {
+    const uint4* p = reinterpret_cast<const uint4*>(row + k0);
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kVec; ++i) r.v[i] = ld_stream(p + i);
+  } else {
+    T* e = reinterpret_cast<T*>(r.v);
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kVec; ++i) r.v[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (k0 + i < K) e[i] = row[k0 + i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const Raw<T>& r, float* f) {
+  const T* e = reinterpret_cast<const T*>(r.v);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = to_f32(e[i]);
+}
+
+// largest finite magnitude of the 16; bad: whether one is not finite
+template <typename T>
+__device__ __forceinline__ float amax16(const Raw<T>& r, bool& bad) {
+  float m;
+  if constexpr (sizeof(T) == 2) {
+    // packed 16-bit maxima that keep a NaN
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(r.v);
+    T2 a = __habs2(p[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a = __hmax2_nan(a, __habs2(p[i]));
+    const T* e = reinterpret_cast<const T*>(&a);
+    m = to_f32(__hmax_nan(e[0], e[1]));
+  } else {
+    uint32_t b = 0u;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(r.v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b = max(b, p[i] & 0x7FFFFFFFu);
+    m = __uint_as_float(b);
+  }
+  bad = !(m < INFINITY);
+  if (bad) {
+    float f[16];
+    unpack16(r, f);
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float a = fabsf(f[i]);
+      if (a < INFINITY) m = fmaxf(m, a);
+    }
+  }
+  return m;
+}
+
+template <typename T>
+struct QuantArgs {
+  const T* x;
+  int64_t ld, M, K;
+  uint8_t* codes;
+  uint8_t* scales;
+  float* row_scale;
+  int64_t pitch;  // bytes of one row of codes
+  int64_t tiles;  // scale tiles along a row
+  bool vec;
+};
+
+// codes and scale of one nv unit
+template <typename T>
+__device__ __forceinline__ void nv_store(const QuantArgs<T>& a, int64_t m, int64_t u,
+                                         const Raw<T>& r, float amax, bool bad, float rs, float ik) {
+  const uint32_t c = nv_scale(amax, ik);
+  if (u * 8 < a.pitch) {
+    float f[16];
+    unpack16(r, f);
+    *reinterpret_cast<uint2*>(a.codes + m * a.pitch + u * 8) =
+        bad ? make_uint2(0u, 0u) : nv_codes16(f, c, rs);
+  }
+  a.scales[scale_at(m, u, a.tiles)] = (uint8_t)(bad ? 0x7Fu : c);
+}
+
+// nv, the row held in registers: WPR warps a row, NB units a thread
+template <typename T, int NB, int WPR>
+__global__ void __launch_bounds__(WPR == 1 ? 256 : 32 * WPR) quant_nv_kernel(const QuantArgs<T> a) {
+  constexpr int T_ROW = 32 * WPR;
+  const int64_t m = WPR == 1 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  if (m >= a.M) return;  // whole warps, and with WPR > 1 no block has such a row
+  const int t = WPR == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const T* row = a.x + m * a.ld;
+  const int units = (int)(a.tiles * 4);
+  Raw<T> r[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) load16(r[i], row, (int64_t)(t + i * T_ROW) * 16, a.K, a.vec);
+  float am[NB], top = 0.f;
+  uint32_t bad = 0u;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    bool b;
+    am[i] = amax16(r[i], b);
+    bad |= (uint32_t)b << i;
+    top = fmaxf(top, am[i]);
+  }
+  top = warp_max(top);
+  if (WPR > 1) {
+    __shared__ float red[WPR];
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) top = fmaxf(top, red[i]);
+  }
+  const int k = row_exponent(top);
+  const float rs = pow2i(k), ik = pow2i(-k);
+  if (t == 0) a.row_scale[m] = rs;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const int u = t + i * T_ROW;
+    if (u < units) nv_store(a, m, u, r[i], am[i], (bad >> i) & 1u, rs, ik);
+  }
+}
+
+// nv, rows too long for the registers of four warps: the row is read twice (the second time
+// from L2, which holds the rows in flight)
+template <typename T>
+__global__ void __launch_bounds__(256) quant_nv_long_kernel(const QuantArgs<T> a) {
+  const int64_t m = blockIdx.x;
+  const T* row = a.x + m * a.ld;
+  const int64_t units = a.tiles * 4;
+  float top = 0.f;
+  for (int64_t u = threadIdx.x; u < units; u += 256) {
+    Raw<T> r;
+    bool b;
+    load16(r, row, u * 16, a.K, a.vec);
+    top = fmaxf(top, amax16(r, b));
+  }
+  __shared__ float red[8];
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+  const int k = row_exponent(top);
+  const float rs = pow2i(k), ik = pow2i(-k);
+  if (threadIdx.x == 0) a.row_scale[m] = rs;
+  for (int64_t u = threadIdx.x; u < units; u += 256) {
+    Raw<T> r;
+    bool b;
+    load16(r, row, u * 16, a.K, a.vec);
+    const float am = amax16(r, b);
+    nv_store(a, m, u, r, am, b, rs, ik);
+  }
+}
+
+// mx: units dealt flat, lanes 2i and 2i + 1 share a block
+template <typename T>
+__global__ void __launch_bounds__(256) quant_mx_kernel(const QuantArgs<T> a) {
+  const int64_t units = a.tiles * 8;  // per row; a multiple of 8, so a block's lanes are neighbours
+  const int64_t total = a.M * units;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  // whole warps run every turn of the loop (the shuffle needs both lanes)
+  for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += stride) {
+    const int64_t i = i0 + threadIdx.x;
+    const int64_t m = i < total ? i / units : a.M - 1;
+    const int64_t u = i < total ? i - m * units : 0;
+    Raw<T> r;
+    load16(r, a.x + m * a.ld, u * 16, a.K, a.vec);
+    bool bad;
+    float am = amax16(r, bad);
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+    const bool other = __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;  // by every lane
+    bad = bad || other;
+    if (i >= total) continue;
+    const int e = mx_exponent(am);
+    if (u * 8 < a.pitch) {
+      float f[16];
+      unpack16(r, f);
+      *reinterpret_cast<uint2*>(a.codes + m * a.pitch + u * 8) =
+          bad ? make_uint2(0u, 0u) : mx_codes16(f, e);
+    }
+    // scales past the last block are 0, not the exponent of an empty block (also byte 0)
+    if ((u & 1) == 0) a.scales[scale_at(m, u >> 1, a.tiles)] = (uint8_t)(bad ? 0xFF : e + 127);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+
+// the values that codes stand for; one thread per 16 elements
+template <typename T, int FMT>
+__global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict__ codes,
+                                                      const uint8_t* __restrict__ scales,
+                                                      const float* __restrict__ row_scale,
+                                                      int rs_row, int64_t M, int64_t K,
+                                                      int64_t pitch, int64_t tiles,
+                                                      T* __restrict__ out) {
+  const int64_t units = (K + 15) / 16, total = M * units;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t m = i / units, u = i - m * units;
+    const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + m * pitch + u * 8));
+    const uint32_t b = __ldg(scales + scale_at(m, FMT == FVB_FP4_NV ? u : u >> 1, tiles));
+    float s;
+    if (FMT == FVB_FP4_NV)
+      s = e4m3_value(b) * (row_scale ? __ldg(row_scale + (rs_row ? m : 0)) : 1.0f);
+    else
+      s = b == 0xFFu ? __uint_as_float(0x7FC00000u) : pow2i((int)b - 127);
+    uint32_t h[8];
+    e2m1x8_to_f16(c.x, h);
+    e2m1x8_to_f16(c.y, h + 4);
+    Raw<T> o;
+    T* e = reinterpret_cast<T*>(o.v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      e[2 * j] = from_f32<T>(f.x * s);
+      e[2 * j + 1] = from_f32<T>(f.y * s);
+    }
+    T* p = out + m * K + u * 16;
+    if (K % (16 / (int)sizeof(T)) == 0 && u * 16 + 16 <= K) {
+#pragma unroll
+      for (int j = 0; j < Raw<T>::kVec; ++j) reinterpret_cast<uint4*>(p)[j] = o.v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (u * 16 + j < K) p[j] = e[j];
+    }
+  }
+}
+
+static unsigned flat_grid(int64_t total) {
+  const int64_t blocks = (total + 255) / 256, most = (int64_t)sm_count() * 64;
+  return (unsigned)(blocks < most ? blocks : most);
+}
+
+template <typename T>
+static int quant(const void* x, int64_t ld, int64_t M, int64_t K, int fmt, void* codes,
+                 void* scales, float* row_scale, cudaStream_t st) {
+  QuantArgs<T> a;
+  a.x = (const T*)x;
+  a.ld = ld;
+  a.M = M;
+  a.K = K;
+  a.codes = (uint8_t*)codes;
+  a.scales = (uint8_t*)scales;
+  a.row_scale = row_scale;
+  a.pitch = code_pitch(K);
+  a.tiles = scale_tiles(K, fmt);
+  a.vec = aligned16(x) && (ld * (int64_t)sizeof(T)) % 16 == 0;
+  if (fmt == FVB_FP4_MX) {
+    quant_mx_kernel<T><<<flat_grid(M * a.tiles * 8), 256, 0, st>>>(a);
+    return check_launch("fvb_quant_fp4");
+  }
+  const int64_t units = a.tiles * 4;
+  const unsigned g8 = (unsigned)((M + 7) / 8), g1 = (unsigned)M;
+  if (units <= 32)
+    quant_nv_kernel<T, 1, 1><<<g8, 256, 0, st>>>(a);
+  else if (units <= 64)
+    quant_nv_kernel<T, 2, 1><<<g8, 256, 0, st>>>(a);
+  else if (units <= 96)
+    quant_nv_kernel<T, 3, 1><<<g8, 256, 0, st>>>(a);
+  else if (units <= 128)
+    quant_nv_kernel<T, 4, 1><<<g8, 256, 0, st>>>(a);
+  else if (units <= 256)
+    quant_nv_kernel<T, 2, 4><<<g1, 128, 0, st>>>(a);
+  else if (units <= 640)
+    quant_nv_kernel<T, 5, 4><<<g1, 128, 0, st>>>(a);
+  else if (units <= 1024)
+    quant_nv_kernel<T, 8, 4><<<g1, 128, 0, st>>>(a);
+  else
+    quant_nv_long_kernel<T><<<g1, 256, 0, st>>>(a);
+  return check_launch("fvb_quant_fp4");
+}
+
+template <typename T>
+static int dequant(const void* codes, const void* scales, const float* row_scale, int rs_row,
+                   int64_t M, int64_t K, int fmt, void* out, cudaStream_t st) {
+  const unsigned grid = flat_grid(M * ((K + 15) / 16));
+  const int64_t pitch = code_pitch(K), tiles = scale_tiles(K, fmt);
+  if (fmt == FVB_FP4_NV)
+    dequant_kernel<T, FVB_FP4_NV><<<grid, 256, 0, st>>>((const uint8_t*)codes,
+                                                        (const uint8_t*)scales, row_scale, rs_row,
+                                                        M, K, pitch, tiles, (T*)out);
+  else
+    dequant_kernel<T, FVB_FP4_MX><<<grid, 256, 0, st>>>((const uint8_t*)codes,
+                                                        (const uint8_t*)scales, nullptr, 0, M, K,
+                                                        pitch, tiles, (T*)out);
+  return check_launch("fvb_dequant_fp4");
+}
+
+}  // namespace fp4
+}  // namespace fvb
+
+extern "C" {
+
+size_t fvb_fp4_codes_bytes(int64_t M, int64_t K) {
+  return M > 0 && K > 0 ? (size_t)(M * fvb::fp4::code_pitch(K)) : 0;
+}
+
+size_t fvb_fp4_scales_bytes(int64_t M, int64_t K, int fmt) {
+  if (M <= 0 || K <= 0 || (fmt != FVB_FP4_NV && fmt != FVB_FP4_MX)) return 0;
+  return (size_t)((M + 127) / 128 * fvb::fp4::scale_tiles(K, fmt)) * 512;
+}
+
+int fvb_quant_fp4(const void* x, int dtype, int64_t ld, int64_t M, int64_t K, int fmt, void* codes,
+                  void* scales, float* row_scale, fvb_stream_t stream) {
+  using namespace fvb;
+  FVB_REQUIRE(M >= 0 && K >= 0, "fvb_quant_fp4: negative size");
+  FVB_REQUIRE(M < (1ll << 31) && K < (1ll << 31), "fvb_quant_fp4: size");
+  FVB_REQUIRE(fmt == FVB_FP4_NV || fmt == FVB_FP4_MX, "fvb_quant_fp4: format %d", fmt);
+  FVB_REQUIRE(dtype == FVB_BF16 || dtype == FVB_F16 || dtype == FVB_F32, "fvb_quant_fp4: dtype %d",
+              dtype);
+  if (M == 0 || K == 0) return FVB_OK;
+  if (ld == 0) ld = K;
+  FVB_REQUIRE(ld >= K || M == 1, "fvb_quant_fp4: row pitch %lld < K %lld", (long long)ld,
+              (long long)K);
+  FVB_REQUIRE(x && codes && scales, "fvb_quant_fp4: NULL pointer");
+  FVB_REQUIRE(fmt == FVB_FP4_MX || row_scale, "fvb_quant_fp4: nv needs row_scale");
+  FVB_REQUIRE(aligned16(codes) && aligned16(scales),
+              "fvb_quant_fp4: codes and scales must be 16-byte aligned");
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FVB_BF16)
+    return fp4::quant<__nv_bfloat16>(x, ld, M, K, fmt, codes, scales, row_scale, st);
+  if (dtype == FVB_F16) return fp4::quant<__half>(x, ld, M, K, fmt, codes, scales, row_scale, st);
+  return fp4::quant<float>(x, ld, M, K, fmt, codes, scales, row_scale, st);
+}
+
+int fvb_dequant_fp4(const void* codes, const void* scales, const float* row_scale, int rs_mode,
+                    int64_t M, int64_t K, int fmt, int dtype, void* out, fvb_stream_t stream) {
+  using namespace fvb;
+  FVB_REQUIRE(M >= 0 && K >= 0, "fvb_dequant_fp4: negative size");
+  FVB_REQUIRE(M < (1ll << 31) && K < (1ll << 31), "fvb_dequant_fp4: size");
+  FVB_REQUIRE(fmt == FVB_FP4_NV || fmt == FVB_FP4_MX, "fvb_dequant_fp4: format %d", fmt);
+  FVB_REQUIRE(dtype == FVB_BF16 || dtype == FVB_F16 || dtype == FVB_F32,
+              "fvb_dequant_fp4: dtype %d", dtype);
+  FVB_REQUIRE(rs_mode == FVB_SCALE_TENSOR || rs_mode == FVB_SCALE_ROW, "fvb_dequant_fp4: rs_mode");
+  if (M == 0 || K == 0) return FVB_OK;
+  FVB_REQUIRE(codes && scales && out, "fvb_dequant_fp4: NULL pointer");
+  FVB_REQUIRE(aligned16(codes) && aligned16(scales) && aligned16(out),
+              "fvb_dequant_fp4: pointers must be 16-byte aligned");
+  cudaStream_t st = (cudaStream_t)stream;
+  const int rr = rs_mode == FVB_SCALE_ROW;
+  if (dtype == FVB_BF16)
+    return fp4::dequant<__nv_bfloat16>(codes, scales, row_scale, rr, M, K, fmt, out, st);
+  if (dtype == FVB_F16)
+    return fp4::dequant<__half>(codes, scales, row_scale, rr, M, K, fmt, out, st);
+  return fp4::dequant<float>(codes, scales, row_scale, rr, M, K, fmt, out, st);
+}
+
+}  // extern "C"

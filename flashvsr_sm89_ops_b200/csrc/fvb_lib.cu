@@ -8,3 +8,6 @@
 #include "bsa.cu"
 #include "noalloc.cu"
 #include "crop_copy.cu"
+#include "fp4_quant.cu"
+#include "gemm_fp4.cu"
+#include "residual_norm.cu"

@@ -1,0 +1,212 @@
+"""4-bit Linear and FFN on hand-written block-scaled tcgen05 products (sm_100a).
+
+The 4-bit counterparts of fp8_linear.py and fp8_ffn.py (whose reference is
+fp8_linear.py:16-67 and fp8_ffn.py:75-115): the weight is quantised once, every forward
+quantises its input and multiplies.  ``FP4FFN`` keeps its hidden state in 4 bits: the first
+product's epilogue applies bias and GELU(tanh) and writes mx codes, so no 16-bit hidden state
+exists.  Inference only, like the rest of the pack.
+"""
+from __future__ import annotations
+
+import re
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from .fp4_quant import _FMTS, FP4Tensor, fp4_format, quantize_fp4
+
+
+def _vector(t, n, what, device):
+    """A bf16 vector of n entries for the kernel (None stays None)."""
+    if t is None:
+        return None
+    if t.numel() != n:
+        raise ValueError(f"{what} must have {n} entries, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the operands on {device}")
+    if t.dtype != torch.bfloat16:
+        t = t.to(torch.bfloat16)
+    return t.reshape(-1).contiguous() if t.dim() != 1 or not t.is_contiguous() else t
+
+
+def _residual(r, M, N, what, device):
+    """(residual as [M, N] with unit column stride, its row pitch)."""
+    if r is None:
+        return None, 0
+    if r.dtype != torch.bfloat16 or r.numel() != M * N or r.shape[-1] != N:
+        raise ValueError(f"{what}: residual must be bf16 [{M}, {N}], got {r.dtype} {tuple(r.shape)}")
+    if r.device != device:
+        raise ValueError(f"{what}: residual is on {r.device}, the operands on {device}")
+    if r.dim() != 2:
+        r = r.reshape(M, N)
+    if (N > 1 and r.stride(1) != 1) or (M > 1 and r.stride(0) < N):
+        r = r.contiguous()
+    return r, (r.stride(0) if M > 1 else N)
+
+
+def _out(out, M, N, what, device):
+    if out is None:
+        return torch.empty((M, N), dtype=torch.bfloat16, device=device)
+    if out.dtype != torch.bfloat16 or out.numel() != M * N or not out.is_contiguous() \
+            or out.device != device:
+        raise ValueError(f"{what}: out must be a contiguous bf16 [{M}, {N}] tensor on {device}")
+    return out
+
+
+def fp4_mm(a: FP4Tensor, w: FP4Tensor, bias: torch.Tensor | None = None,
+           out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+           gate: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16(a w^T + bias), or bf16(residual + gate * (a w^T + bias)) with a residual.
+
+    a [M, K] and w [N, K] of the same format; bias and gate [N], residual [M, N].  fp32 sums
+    and epilogue, one rounding.  out (contiguous [M, N]) may be the residual.
+    """
+    _lib.require_cuda(a.codes, w.codes)
+    M, K = a.shape
+    N = w.shape[0]
+    dev = a.codes.device
+    if a.fmt != w.fmt:
+        raise ValueError(f"fp4_mm: formats differ ({a.fmt} x {w.fmt})")
+    if w.shape[1] != K:
+        raise ValueError(f"fp4_mm: K mismatch {a.shape} x {w.shape}")
+    if w.codes.device != dev:
+        raise ValueError("fp4_mm: operands are on different devices")
+    if gate is not None and residual is None:
+        raise ValueError("fp4_mm: gate needs a residual")
+    bias = _vector(bias, N, "fp4_mm: bias", dev)
+    gate = _vector(gate, N, "fp4_mm: gate", dev)
+    residual, ldr = _residual(residual, M, N, "fp4_mm", dev)
+    out = _out(out, M, N, "fp4_mm", dev)
+    _lib.call("fvb_fp4_gemm", a.codes.data_ptr(), a.scales.data_ptr(), _lib.ptr(a.row_scale),
+              a.row_mode(), w.codes.data_ptr(), w.scales.data_ptr(), _lib.ptr(w.row_scale),
+              w.row_mode(), _FMTS[a.fmt], _lib.ptr(bias), _lib.ptr(residual), ldr, _lib.ptr(gate),
+              M, N, K, out.data_ptr(), _lib.stream_of(out))
+    return out
+
+
+def ffn_fp4(a: FP4Tensor, w0: FP4Tensor, b0: torch.Tensor | None, w2: FP4Tensor,
+            b2: torch.Tensor | None, residual: torch.Tensor | None = None,
+            gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+            workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """y = mx(gelu_tanh(a w0^T + b0)) w2^T + b2 in one call; bf16(y), or
+    bf16(residual + gate * y) with a residual.
+
+    a [M, D] and w0 [F, D] share a format, w2 [N, F] is mx (the hidden state's format: its
+    blocks need nothing of the rest of their row, so the first product writes them itself).
+    workspace: uint8, at least fvb_fp4_ffn_workspace_bytes(M, F), 256-byte aligned.
+    """
+    _lib.require_cuda(a.codes, w0.codes, w2.codes)
+    M, D = a.shape
+    F, N = w0.shape[0], w2.shape[0]
+    dev = a.codes.device
+    if a.fmt != w0.fmt:
+        raise ValueError(f"ffn_fp4: formats differ ({a.fmt} x {w0.fmt})")
+    if w2.fmt != "mx":
+        raise ValueError("ffn_fp4: w2 must be mx, the hidden state's format")
+    if w0.shape[1] != D or w2.shape[1] != F:
+        raise ValueError(f"ffn_fp4: shapes {a.shape}, {w0.shape}, {w2.shape} do not chain")
+    if w0.codes.device != dev or w2.codes.device != dev:
+        raise ValueError("ffn_fp4: operands are on different devices")
+    if gate is not None and residual is None:
+        raise ValueError("ffn_fp4: gate needs a residual")
+    b0 = _vector(b0, F, "ffn_fp4: b0", dev)
+    b2 = _vector(b2, N, "ffn_fp4: b2", dev)
+    gate = _vector(gate, N, "ffn_fp4: gate", dev)
+    residual, ldr = _residual(residual, M, N, "ffn_fp4", dev)
+    out = _out(out, M, N, "ffn_fp4", dev)
+    need = _lib.load().fvb_fp4_ffn_workspace_bytes(M, F)
+    if workspace is None:
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+    elif workspace.numel() * workspace.element_size() < need or workspace.device != dev:
+        raise ValueError(f"ffn_fp4: workspace needs {need} bytes on {dev}")
+    _lib.call("fvb_fp4_ffn", a.codes.data_ptr(), a.scales.data_ptr(), _lib.ptr(a.row_scale),
+              a.row_mode(), w0.codes.data_ptr(), w0.scales.data_ptr(), _lib.ptr(w0.row_scale),
+              w0.row_mode(), _FMTS[a.fmt], _lib.ptr(b0), w2.codes.data_ptr(), w2.scales.data_ptr(),
+              _lib.ptr(b2), _lib.ptr(residual), ldr, _lib.ptr(gate), M, D, F, N, out.data_ptr(),
+              workspace.data_ptr(), _lib.stream_of(out))
+    return out
+
+
+class FP4Linear(nn.Module):
+    """nn.Linear replacement with 4-bit weights and activations (cf. FP8Linear)."""
+
+    def __init__(self, linear: nn.Linear, fmt: str = "nv"):
+        super().__init__()
+        fp4_format(fmt)
+        self.fmt = fmt
+        self.in_features = linear.in_features
+        self.out_features = linear.out_features
+        q = quantize_fp4(linear.weight.detach(), fmt)
+        self.weight = nn.Parameter(q.codes, requires_grad=False)
+        self.register_buffer("w_scales", q.scales, persistent=False)
+        self.register_buffer("w_row_scale", q.row_scale, persistent=False)
+        if linear.bias is not None:
+            self.bias = nn.Parameter(linear.bias.detach().to(torch.bfloat16).clone(),
+                                     requires_grad=False)
+        else:
+            self.bias = None
+
+    def weight_fp4(self) -> FP4Tensor:
+        rs = self.w_row_scale  # a model cast to bf16 casts it too: a power of two, so exactly
+        return FP4Tensor(self.weight.data, self.w_scales, None if rs is None else rs.float(),
+                         (self.out_features, self.in_features), self.fmt)
+
+    def forward(self, x):
+        shape = x.shape
+        y = fp4_mm(quantize_fp4(x.reshape(-1, shape[-1]), self.fmt), self.weight_fp4(), self.bias)
+        return y.reshape(*shape[:-1], self.out_features)
+
+    def extra_repr(self):
+        return f"in={self.in_features}, out={self.out_features}, fmt={self.fmt}"
+
+
+class FP4FFN(nn.Module):
+    """Replacement for a DiT FFN ``Sequential(Linear, GELU(tanh), Linear)`` whose two Linears
+    are FP4Linear, the second mx (cf. FP8FFN)."""
+
+    def __init__(self, lin0: FP4Linear, lin2: FP4Linear):
+        super().__init__()
+        if lin2.fmt != "mx":
+            raise ValueError("FP4FFN: the second linear must be mx")
+        self.lin0 = lin0
+        self.lin2 = lin2
+
+    def ffn(self, a: FP4Tensor, residual=None, gate=None):
+        """The FFN of an already quantised input, with the block's gated residual."""
+        return ffn_fp4(a, self.lin0.weight_fp4(), self.lin0.bias, self.lin2.weight_fp4(),
+                       self.lin2.bias, residual=residual, gate=gate)
+
+    def forward(self, x):
+        shape = x.shape
+        y = self.ffn(quantize_fp4(x.reshape(-1, shape[-1]), self.lin0.fmt))
+        return y.reshape(*shape[:-1], self.lin2.out_features)
+
+
+_PATTERNS = {"self": r"^blocks\.\d+\.self_attn\.[qkvo]$", "cross": r"^blocks\.\d+\.cross_attn\.[qkvo]$"}
+
+
+def convert_linears_fp4(model: nn.Module, parts=("ffn",), fmt: str = "nv") -> int:
+    """Swap the DiT blocks' Linears of `parts` (ffn, self, cross) for 4-bit ones; returns the
+    count.  ``blocks.i.ffn`` becomes an FP4FFN whose first linear has `fmt`.  Same module names
+    as convert_linears_fp8 (fp8_linear.py:45-67)."""
+    fp4_format(fmt)
+    unknown = set(parts) - {"ffn", "self", "cross"}
+    if unknown:
+        raise ValueError(f"convert_linears_fp4: unknown parts {sorted(unknown)} (ffn|self|cross)")
+    n = 0
+    pats = [re.compile(_PATTERNS[p]) for p in parts if p in _PATTERNS]
+    ffn = re.compile(r"^blocks\.\d+\.ffn$") if "ffn" in parts else None
+    for name, mod in list(model.named_modules()):
+        parent_name, _, leaf = name.rpartition(".")
+        if ffn is not None and ffn.match(name) and isinstance(mod, nn.Sequential) \
+                and type(mod[0]) is nn.Linear and type(mod[2]) is nn.Linear:
+            new = FP4FFN(FP4Linear(mod[0], fmt), FP4Linear(mod[2], "mx"))
+            n += 2
+        elif type(mod) is nn.Linear and any(p.match(name) for p in pats):
+            new = FP4Linear(mod, fmt)
+            n += 1
+        else:
+            continue
+        setattr(model.get_submodule(parent_name) if parent_name else model, leaf, new)
+    return n

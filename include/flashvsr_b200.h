@@ -309,6 +309,76 @@ FVB_API int fvb_causal_topk_pooled(const float* aq, const float* ak, int64_t H, 
                                    int64_t NK, int64_t d, int64_t per_row, float ratio,
                                    uint8_t* keep, fvb_stream_t stream);
 
+/* ------------------------------------------------- microscaled 4-bit operators
+ * No counterpart in the reference, whose narrowest type is FP8.  E2M1 codes (0, .5, 1, 1.5, 2,
+ * 3, 4, 6 and a sign) with one scale per block of a row:
+ *   FVB_FP4_NV  blocks of 16, E4M3 scales, and one fp32 power of two per row (row_scale)
+ *   FVB_FP4_MX  blocks of 32, E8M0 scales 2^(floor(log2 amax) - 2), no row_scale
+ * codes: [M, ceil(K / 32) * 16] bytes, two codes to a byte, even element in the low nibble, a
+ *   row padded with zero codes to a multiple of 32 elements.
+ * scales: 512-byte tiles of 128 rows x 4 blocks, row-major ([ceil(M/128), ceil(blocks/4)]);
+ *   block j of row m is byte (m % 32) * 16 + (m % 128) / 32 * 4 + j % 4 of its tile.  Blocks
+ *   past a row's last are 0; rows past M are never read back.
+ * All these buffers are 16-byte aligned. */
+#define FVB_FP4_NV 1
+#define FVB_FP4_MX 2
+#define FVB_BF16 0
+#define FVB_F16 1
+#define FVB_F32 2
+FVB_API size_t fvb_fp4_codes_bytes(int64_t M, int64_t K);
+FVB_API size_t fvb_fp4_scales_bytes(int64_t M, int64_t K, int fmt);
+
+/* x [M, K] (dtype FVB_BF16 / F16 / F32, row pitch ld elements, 0 = K, any alignment) -> codes,
+ * scales and, for nv, row_scale [M].  Rounding is to nearest even, decided exactly; a block
+ * that holds a NaN or an infinity has a NaN scale and counts as its finite values in the row's
+ * maximum. */
+FVB_API int fvb_quant_fp4(const void* x, int dtype, int64_t ld, int64_t M, int64_t K, int fmt,
+                          void* codes, void* scales, float* row_scale, fvb_stream_t stream);
+/* The values the codes stand for, [M, K] contiguous of `dtype` (rounded once).  row_scale:
+ * [M] (FVB_SCALE_ROW), [1] (FVB_SCALE_TENSOR) or NULL (1). */
+FVB_API int fvb_dequant_fp4(const void* codes, const void* scales, const float* row_scale,
+                            int rs_mode, int64_t M, int64_t K, int fmt, int dtype, void* out,
+                            fvb_stream_t stream);
+
+/* out = bf16(y), or bf16(residual + gate * y) with a residual, where
+ *   y[m, n] = rsA[m] * rsW[n] * sum_k A[m, k] W[n, k] + bias[n]
+ * A [M, K] and W [N, K] in 4 bits of the same format; rsA / rsW as in fvb_dequant_fp4 (a_mode,
+ * w_mode; ignored for mx).  bias, gate [N] bf16 or NULL, residual [M, N] bf16 with row pitch
+ * ldr (0 = N) or NULL, out [M, N] bf16 (may be the residual).  Any M, N, K: the sums are fp32
+ * on the tcgen05 block-scaled tensor cores and out is rounded once. */
+FVB_API int fvb_fp4_gemm(const void* A, const void* sfA, const float* rsA, int a_mode, const void* W,
+                         const void* sfW, const float* rsW, int w_mode, int fmt, const void* bias,
+                         const void* residual, int64_t ldr, const void* gate, int64_t M, int64_t N,
+                         int64_t K, void* out, fvb_stream_t stream);
+
+/* A DiT FFN in 4 bits: h = mx(gelu_tanh(A W0^T + b0)), out as fvb_fp4_gemm of h and W2.
+ * A [M, D] and W0 [F, D] of format fmt, W2 [N, F] mx.  h is quantised from fp32 in the first
+ * product's epilogue.  workspace: fvb_fp4_ffn_workspace_bytes(M, F), 256-byte aligned. */
+FVB_API size_t fvb_fp4_ffn_workspace_bytes(int64_t M, int64_t F);
+FVB_API int fvb_fp4_ffn(const void* A, const void* sfA, const float* rsA, int a_mode, const void* W0,
+                        const void* sfW0, const float* rsW0, int w_mode, int fmt, const void* b0,
+                        const void* W2, const void* sfW2, const void* b2, const void* residual,
+                        int64_t ldr, const void* gate, int64_t M, int64_t D, int64_t F, int64_t N,
+                        void* out, void* workspace, fvb_stream_t stream);
+
+/* The seam between two branches, with norms on both sides of it:
+ *   x_out = residual_scale * x + gate * (post(y) * post_w + post_b)
+ *   h     = (norm(x_out) * w + b) * (1 + scale) + shift
+ * x, y, x_out [B, L, D] bf16; gate [B, D] (gate_rows 0) or [B, L, D] (gate_rows 1); scale, shift
+ * [B, D]; post_w, post_b, w, b [D]; all bf16, any of them NULL.  post: FVB_NORM_NONE / RMS /
+ * LAYER, norm: RMS / LAYER.  fp32 between loads and stores: h is normed from the unrounded sum.
+ * out [B, L, D] bf16 (NULL with fmt != 0), and with fmt the 4-bit codes of the unrounded h
+ * ([B * L, D]; codes, scales, row_scale).  D % 8 == 0, D <= 16384. */
+#define FVB_NORM_NONE 0
+#define FVB_NORM_RMS 1
+#define FVB_NORM_LAYER 2
+FVB_API int fvb_residual_norm(const void* x, const void* y, const void* gate, int gate_rows,
+                              float residual_scale, int post, const void* post_w,
+                              const void* post_b, float post_eps, int norm, const void* w,
+                              const void* b, const void* scale, const void* shift, float eps,
+                              int64_t B, int64_t L, int64_t D, void* x_out, void* out, int fmt,
+                              void* codes, void* scales, float* row_scale, fvb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
