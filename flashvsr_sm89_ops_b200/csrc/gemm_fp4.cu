@@ -10,10 +10,11 @@
 //               into a ring of shared-memory stages
 //   warp 1      MMA issuer: copies a group of scale tiles into TMEM (tcgen05.cp), then issues
 //               the group's block-scaled MMAs (K = 64 each) into the fp32 accumulator
-//   warps 2..9  epilogue: two warps per TMEM lane quarter take the tile's 32-column chunks in
-//               turn, each thread one row; bf16 through a swizzled staging buffer and a TMA
-//               store.  A chunk is one mx block of a row, so the 4-bit output needs no exchange
-//               between threads and the hidden state of an FFN never exists in 16 bits.
+//   warps 2..   epilogue (8 warps, 16 with GELU): the warps of a TMEM lane quarter take the
+//               tile's 64-column chunks in turn, each thread one row; bf16 through a swizzled
+//               staging buffer and a TMA store.  A chunk is two mx blocks of a row, so the
+//               4-bit output needs no exchange between threads and the hidden state of an FFN
+//               never exists in 16 bits.
 //
 // TMEM (512 columns): two accumulators of BN columns and two buffers of scale columns.  With
 // BN = 256 that is more than 512, so the second accumulator starts at column 192: the tiles'
@@ -30,11 +31,12 @@ namespace gemm4 {
 
 constexpr int BM = 128;
 constexpr int kRowBytes = 128;  // one K block of a row: 256 elements
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kStageOut = 32 * 64;  // an epilogue warp's staging: 32 rows x 32 bf16
+constexpr int kStageOut = 32 * 128;  // an epilogue warp's staging: 32 rows x 64 bf16
 
 enum { kPlain = 0, kResidual = 1, kGeluMx = 2 };
+
+// epilogue warps, a multiple of 4
+__host__ __device__ constexpr int epi_warps(int epi) { return epi == kGeluMx ? 16 : 8; }
 
 struct Args {
   int M, N, K;
@@ -47,14 +49,18 @@ struct Args {
   __nv_bfloat16* out;         // row pitch ldo
   int64_t ldr, ldo;
   int tma_out;      // whether `out` suits a TMA store
-  int vec_n;        // whether the per-column vectors and res may be read 16 bytes at a time
+  int vec_res;      // whether res may be read 16 bytes at a time
   uint8_t* hcodes;  // kGeluMx
   uint8_t* hscales;
   int64_t hpitch, htiles;
 };
 
-template <int FMT, int BN, bool PAIR>
+template <int FMT, int BN, int EPI, bool PAIR>
 struct Shape {
+  static constexpr int kEpiWarps = epi_warps(EPI);
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kOutBytes = EPI == kGeluMx ? 0 : kEpiWarps * kStageOut;
+  static constexpr int kColBytes = 3 * BN * 4;  // the tile's column scales, biases and gates
   static constexpr int kTilesK = FMT == FVB_FP4_NV ? 4 : 2;  // scale tiles per K block
   static constexpr int kGroups = kTilesK / 2;                // TMEM groups of two scale tiles
   static constexpr int kMmas = 4 / kGroups;                  // MMAs (K = 64) per group
@@ -65,7 +71,7 @@ struct Shape {
   static constexpr int kBytesSfA = kGroups * 1024;
   static constexpr int kBytesSfB = kGroups * kSfTilesB * 1024;
   static constexpr int kBytes = kBytesA + kBytesB + kBytesSfA + kBytesSfB;
-  static constexpr int kFixed = kEpiWarps * kStageOut + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int kFixed = kOutBytes + kColBytes + 1024 /*align*/ + 256 /*barriers*/;
   static constexpr int kFit = (227 * 1024 - kFixed) / kBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr size_t kSmem = (size_t)kStages * kBytes + kFixed;
@@ -99,12 +105,13 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t da, uint64_t db, ui
 #undef FVB_MMA4
 }
 
-// one 512-byte scale tile -> 4 TMEM columns of 32 lanes, repeated in the four lane quarters
+// descriptor of one 512-byte scale tile: unswizzled 8-row x 16-byte core matrices, 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// the tile -> 4 TMEM columns of 32 lanes, repeated in the four lane quarters
 template <bool PAIR>
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint32_t saddr) {
-  // unswizzled 8-row x 16-byte core matrices, 128 bytes apart
-  const uint64_t desc = (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) |
-                        ((uint64_t)1 << 46);
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
   if (PAIR)
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
                  : "memory");
@@ -121,14 +128,25 @@ __host__ __device__ constexpr uint32_t idesc4(int M, int N) {
          ((FMT == FVB_FP4_MX ? 1u : 0u) << 23) | ((uint32_t)(M >> 4) << 24);
 }
 
-// GELU(tanh) in fp32: x * sigmoid(2 u) = x / (1 + 2^(-2 u log2 e)), u = sqrt(2/pi) (x + c x^3)
-__device__ __forceinline__ float gelu_f32(float x) {
-  const float t = x * x;
-  const float u = x * __fmaf_rn(t, -2.0f * 0.7978845608028654f * 0.044715f * 1.4426950408889634f,
-                                -2.0f * 0.7978845608028654f * 1.4426950408889634f);
+// GELU(tanh) of two values in fp32: x * sigmoid(2 u) = x / (1 + 2^v), u = sqrt(2/pi) (x + c x^3),
+// v = -2 u log2(e).  One reciprocal of the product serves both: 1 / a = b / (a b).  v is held
+// at 60 so the product stays finite; x / 2^60 is then already far below any step of the codes
+// next to it, and 0.5 x (1 + tanh u) in fp32 has long been 0.
+__device__ __forceinline__ void gelu2(float& x0, float& x1) {
+  const float k1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, k3 = k1 * 0.044715f;
+  const uint64_t x = f2_pack(x0, x1);
+  const uint64_t v = f2_mul(x, f2_fma(f2_mul(x, x), f2_pack(k3, k3), f2_pack(k1, k1)));
+  float v0, v1;
+  f2_unpack(v, v0, v1);
+  const float a = 1.0f + ex2_approx(fminf(v0, 60.0f)), b = 1.0f + ex2_approx(fminf(v1, 60.0f));
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(u)));
-  return x * r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  f2_unpack(f2_mul(f2_mul(x, f2_pack(r, r)), f2_pack(b, a)), x0, x1);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // keeps a NaN
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 __device__ __forceinline__ void load_cols8(const __nv_bfloat16* p, int c, int N, bool vec, float* v) {
@@ -139,25 +157,13 @@ __device__ __forceinline__ void load_cols8(const __nv_bfloat16* p, int c, int N,
     for (int i = 0; i < 8; ++i) v[i] = c + i < N ? __bfloat162float(p[c + i]) : 0.f;
   }
 }
-__device__ __forceinline__ void load_cols8(const float* p, int c, int N, bool vec, float* v) {
-  if (vec && c + 8 <= N) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p + c));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p + c + 4));
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < N ? p[c + i] : 0.f;
-  }
-}
-
 template <int FMT, int BN, int EPI, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSfA,
                     const __grid_constant__ CUtensorMap tmSfB,
                     const __grid_constant__ CUtensorMap tmOut, const Args args) {
-  using S = Shape<FMT, BN, PAIR>;
+  using S = Shape<FMT, BN, EPI, PAIR>;
   constexpr int STAGES = S::kStages;
   constexpr int TM = PAIR ? 2 * BM : BM;
   extern __shared__ uint8_t smem_raw[];
@@ -168,7 +174,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sSfA = sB + STAGES * S::kBytesB;
   uint8_t* sSfB = sSfA + STAGES * S::kBytesSfA;
   uint8_t* sOut = sSfB + STAGES * S::kBytesSfB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + kEpiWarps * kStageOut);
+  float* sCol = reinterpret_cast<float*>(sOut + S::kOutBytes);  // [3][BN]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::kOutBytes + S::kColBytes);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;   // [2] accumulator finished
   uint64_t* tempty = tfull + 2;       // [2] accumulator (its shared columns) read
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
+      mbar_init(&tempty[b], PAIR ? 2 * S::kEpiWarps : S::kEpiWarps);
       mbar_init(&sfree[b], 1);
     }
     mbar_init(drain, 1);
@@ -290,9 +297,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the loop, so addresses and descriptors stay warp-uniform (the form
+    // the tensor instructions take them in); one elected lane issues.
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc4<FMT>(TM, BN);
+      const bool leader = elect_one();
       const int ksteps = (args.K + 63) / 64;
+      const uint64_t descA = smem_desc_sw128(smem_u32(sA), 16, 1024);
+      const uint64_t descB = smem_desc_sw128(smem_u32(sB), 16, 1024);
+      const uint64_t descFA = scale_desc(smem_u32(sSfA));
+      const uint64_t descFB = scale_desc(smem_u32(sSfB));
       int stage = 0;
       uint32_t phase = 0;
       int t = 0;
@@ -306,187 +320,234 @@ __global__ void __launch_bounds__(kThreads, 1)
             S::kOverlap
                 ? (t == 0 || mbar_wait(&tempty[buf ^ 1], (uint32_t)((t - 1) >> 1) & 1u, 0x402u))
                 : mbar_wait(&tempty[buf], ((uint32_t)(t >> 1) & 1u) ^ 1u, 0x402u);
-        if (!clear) break;
+        if (!__all_sync(0xffffffffu, clear)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf ? S::kAcc1 : 0);
         const int nt = (tile % n_tiles) * BN;
         const uint32_t shift = BN < 128 ? (uint32_t)((nt & 127) >> 5) : 0u;
         for (int kb = 0; kb < kblocks && ok; ++kb) {
-          if (!mbar_wait(&full[stage], phase, 0x403u)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, 0x403u))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + stage * S::kBytesA);
-          const uint32_t b0 = smem_u32(sB + stage * S::kBytesB);
-          const uint32_t fa0 = smem_u32(sSfA + stage * S::kBytesSfA);
-          const uint32_t fb0 = smem_u32(sSfB + stage * S::kBytesSfB);
+          const uint64_t da = descA + (uint32_t)(stage * (S::kBytesA >> 4));
+          const uint64_t db = descB + (uint32_t)(stage * (S::kBytesB >> 4));
+          const uint64_t fa = descFA + (uint32_t)(stage * (S::kBytesSfA >> 4));
+          const uint64_t fb = descFB + (uint32_t)(stage * (S::kBytesSfB >> 4));
+          const int left = ksteps - kb * 4;  // K steps from this block on
 #pragma unroll
-          for (int g = 0; g < S::kGroups; ++g, ++grp) {
-            if (kb * 4 + g * S::kMmas >= ksteps) break;
-            const uint32_t sb = grp & 1u;
-            if (!mbar_wait(&sfree[sb], ((grp >> 1) & 1u) ^ 1u, 0x405u)) {
-              ok = false;
-              break;
-            }
-            const uint32_t sfa = tmem + (uint32_t)S::kSf + sb * (uint32_t)S::kSfCols;
-            const uint32_t sfb = sfa + 8u;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              cp_scales<PAIR>(sfa + 4u * i, fa0 + g * 1024 + i * 512);
-#pragma unroll
-              for (int r = 0; r < S::kSfTilesB; ++r)
-                cp_scales<PAIR>(sfb + (uint32_t)(4 * S::kSfTilesB * i + 4 * r),
-                                fb0 + (g * S::kSfTilesB + r) * 1024 + i * 512);
-            }
-#pragma unroll
-            for (int i = 0; i < S::kMmas; ++i) {
-              const int ks = g * S::kMmas + i;  // K step inside the block
-              if (kb * 4 + ks < ksteps) {
-                const int ti = FMT == FVB_FP4_NV ? i : i >> 1;            // scale tile
-                const uint32_t id = FMT == FVB_FP4_NV ? 0u : (i & 1) * 2u;  // byte in its column
-                mma_fp4<FMT, PAIR>(d, smem_desc_sw128(a0 + ks * 32, 16, 1024),
-                                   smem_desc_sw128(b0 + ks * 32, 16, 1024),
-                                   idesc | (id << 4) | (id << 29), sfa + 4u * ti,
-                                   sfb + (uint32_t)(4 * S::kSfTilesB * ti) + shift,
-                                   (kb | ks) != 0 ? 1u : 0u);
+          for (int g = 0; g < S::kGroups; ++g) {
+            if (g * S::kMmas < left) {
+              const uint32_t sb = grp & 1u;
+              if (!__all_sync(0xffffffffu, mbar_wait(&sfree[sb], ((grp >> 1) & 1u) ^ 1u, 0x405u))) {
+                ok = false;
+                break;
               }
+              const uint32_t sfa = tmem + (uint32_t)S::kSf + sb * (uint32_t)S::kSfCols;
+              const uint32_t sfb = sfa + 8u;
+              if (leader) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  cp_scales<PAIR>(sfa + 4u * i, fa + (g * 1024 + i * 512) / 16);
+#pragma unroll
+                  for (int r = 0; r < S::kSfTilesB; ++r)
+                    cp_scales<PAIR>(sfb + (uint32_t)(4 * S::kSfTilesB * i + 4 * r),
+                                    fb + ((g * S::kSfTilesB + r) * 1024 + i * 512) / 16);
+                }
+#pragma unroll
+                for (int i = 0; i < S::kMmas; ++i) {
+                  const int ks = g * S::kMmas + i;  // K step inside the block
+                  if (ks < left) {
+                    const int ti = FMT == FVB_FP4_NV ? i : i >> 1;            // scale tile
+                    const uint32_t id = FMT == FVB_FP4_NV ? 0u : (i & 1) * 2u;  // byte in its column
+                    mma_fp4<FMT, PAIR>(d, da + 2 * ks, db + 2 * ks, idesc | (id << 4) | (id << 29),
+                                       sfa + 4u * ti, sfb + (uint32_t)(4 * S::kSfTilesB * ti) + shift,
+                                       (kb | ks) != 0 ? 1u : 0u);
+                  }
+                }
+                if (PAIR) tc_commit_pair(&sfree[sb]);
+                else tc_commit(&sfree[sb]);
+              }
+              ++grp;
+              any = true;
             }
-            any = true;
-            if (PAIR) tc_commit_pair(&sfree[sb]);
-            else tc_commit(&sfree[sb]);
           }
           if (!ok) break;
-          if (PAIR) tc_commit_pair_both(&empty[stage], 0x3);
-          else tc_commit(&empty[stage]);
+          if (leader) {
+            if (PAIR) tc_commit_pair_both(&empty[stage], 0x3);
+            else tc_commit(&empty[stage]);
+          }
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) {
+        if (ok && leader) {
           if (PAIR) tc_commit_pair_both(&tfull[buf], 0x3);
           else tc_commit(&tfull[buf]);
         }
+        __syncwarp();
       }
       // every MMA issued above completes before TMEM is freed
       if (any) {
-        if (PAIR) tc_commit_pair(drain);
-        else tc_commit(drain);
+        if (leader) {
+          if (PAIR) tc_commit_pair(drain);
+          else tc_commit(drain);
+        }
+        __syncwarp();
         mbar_wait(drain, 0, 0x40Bu);
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue
+    // G warps per TMEM lane quarter (warp % 4) take the tile's 64-column chunks in turn, each
+    // thread one row of a chunk
+    constexpr int G = S::kEpiWarps / 4;
+    constexpr int kChunks = BN / 64;
     const int q = warp & 3;
-    const int half = (warp - 2) >> 2;
+    const int sub = (warp - 2) >> 2;
+    const int et = (int)threadIdx.x - 64;
     uint8_t* stg = sOut + (size_t)(warp - 2) * kStageOut;
-    constexpr int kChunks = BN / 32;
+    auto release = [&](int b) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_remote(tempty0_c + 8u * b);
+        else mbar_arrive(&tempty[b]);
+      }
+    };
+    // the tile's column vectors go through shared memory: read from global one tile ahead,
+    // so that no thread waits for them between the accumulator and the store
+    float cs = 1.f, cb = 0.f, cg = 1.f;
+    auto columns = [&](int tile) {
+      const int c = (tile % n_tiles) * BN + et;
+      if (tile < num_tiles && et < BN && c < args.N) {
+        if (args.sw) cs = __ldg(args.sw + (args.sw_row ? c : 0));
+        if (args.bias) cb = __bfloat162float(args.bias[c]);
+        if (EPI == kResidual && args.gate) cg = __bfloat162float(args.gate[c]);
+      }
+    };
+    columns(unit);
+    bool ok = true;
     int t = 0;
     for (int tile = unit; tile < num_tiles; tile += units, ++t) {
       const int buf = t & 1;
       const int m0 = (tile / n_tiles) * TM + (int)rank * BM;
       const int n0 = (tile % n_tiles) * BN;
-      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[buf], (uint32_t)(t >> 1) & 1u, 0x404u))) break;
-      tc_fence_after();
       const int row = m0 + q * 32 + lane;
       const bool row_ok = row < args.M;
       float sa = 1.0f;
       if (args.sa) sa = args.sa_row ? (row_ok ? __ldg(args.sa + row) : 0.f) : __ldg(args.sa);
-      const float sw0 = args.sw && !args.sw_row ? __ldg(args.sw) : 1.0f;
+      asm volatile("bar.sync 1, %0;" ::"r"(S::kEpiWarps * 32) : "memory");  // last tile's readers
+      if (et < BN) {
+        sCol[et] = cs;
+        sCol[BN + et] = cb;
+        if (EPI == kResidual) sCol[2 * BN + et] = cg;
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(S::kEpiWarps * 32) : "memory");
+      columns(tile + units);
+      // a warp whose wait ran out goes on to the barriers above, which its neighbours may be at,
+      // and does nothing else
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&tfull[buf], (uint32_t)(t >> 1) & 1u, 0x404u));
+      if (!ok) continue;
+      tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf ? S::kAcc1 : 0);
+      const uint64_t sa2 = f2_pack(sa, sa);
+      // chunk order: the columns shared with the other accumulator first (the first
+      // accumulator's last chunk, the second's first)
+      const int first = S::kOverlap && buf == 0 ? kChunks - 1 : 0;
+      if (sub >= kChunks || (S::kOverlap && sub != 0)) release(buf);  // reads no shared column
 #pragma unroll 1
-      for (int i = 0; i < kChunks / 2; ++i) {
-        // the first accumulator's shared columns are its last 64: start with those
-        int c = 2 * i + half;
-        if (S::kOverlap && buf == 0) c = (c + kChunks - 2) & (kChunks - 1);
-        const int col0 = n0 + c * 32;
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(acc + (uint32_t)(c * 32), r);
+      for (int i = sub; i < kChunks; i += G) {
+        const int c = (i + first) & (kChunks - 1);
+        const int col0 = n0 + c * 64;
+        uint32_t r[64];
+        tmem_ld_32x32b_x32(acc + (uint32_t)(c * 64), r);
+        tmem_ld_32x32b_x32(acc + (uint32_t)(c * 64 + 32), r + 32);
         tmem_ld_wait();
-        if (i == (S::kOverlap ? 0 : kChunks / 2 - 1)) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (PAIR) mbar_arrive_remote(tempty0_c + 8u * buf);
-            else mbar_arrive(&tempty[buf]);
+        if (S::kOverlap ? i == 0 : i + G >= kChunks) release(buf);
+        float* v = reinterpret_cast<float*>(r);
+        if (col0 < args.N) {  // warp-uniform
+          const float4* s4 = reinterpret_cast<const float4*>(sCol + c * 64);
+          const float4* b4 = reinterpret_cast<const float4*>(sCol + BN + c * 64);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float4 s = s4[j], b = b4[j];
+            f2_unpack(f2_fma(f2_pack(v[4 * j], v[4 * j + 1]), f2_mul(sa2, f2_pack(s.x, s.y)),
+                             f2_pack(b.x, b.y)),
+                      v[4 * j], v[4 * j + 1]);
+            f2_unpack(f2_fma(f2_pack(v[4 * j + 2], v[4 * j + 3]), f2_mul(sa2, f2_pack(s.z, s.w)),
+                             f2_pack(b.z, b.w)),
+                      v[4 * j + 2], v[4 * j + 3]);
           }
-        }
-        if (col0 >= args.N) {  // warp-uniform
-          // the hidden state's scales past its last block: the next product reads whole tiles
-          if (EPI == kGeluMx && row_ok && (col0 >> 5) < args.htiles * 4)
-            args.hscales[fp4::scale_at(row, col0 >> 5, args.htiles)] = 0;
-          continue;
-        }
-        float v[32];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int cg = col0 + g * 8;
-          float s[8], b[8];
-          if (args.sw && args.sw_row) {
-            load_cols8(args.sw, cg, args.N, args.vec_n, s);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = sw0;
-          }
-          if (args.bias) {
-            load_cols8(args.bias, cg, args.N, args.vec_n, b);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = 0.f;
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            v[g * 8 + j] = __fmaf_rn(__uint_as_float(r[g * 8 + j]), sa * s[j], b[j]);
         }
         if (EPI == kGeluMx) {
-          float am = 0.f;
-          bool bad = false;
+          // two mx blocks of this row
+          uint32_t byte[2] = {0u, 0u};
+          uint4 code[2];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            v[j] = col0 + j < args.N ? gelu_f32(v[j]) : 0.f;
-            bad |= !(fabsf(v[j]) < INFINITY);
-            am = fmaxf(am, fabsf(v[j]));
-          }
-          if (bad) {
-            am = 0.f;
-          }
-          const int e = fp4::mx_exponent(am);
-          if (row_ok) {
-            uint4 o = make_uint4(0u, 0u, 0u, 0u);
-            if (!bad) {
-              const uint2 lo = fp4::mx_codes16(v, e), hi = fp4::mx_codes16(v + 16, e);
-              o = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          for (int h = 0; h < 2; ++h) {
+            code[h] = make_uint4(0u, 0u, 0u, 0u);
+            const int cb0 = col0 + h * 32;
+            if (cb0 >= args.N) continue;  // past the last block: a zero scale
+            float* x = v + h * 32;
+            float am = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              gelu2(x[j], x[j + 1]);
+              if (cb0 + 32 > args.N) {  // columns past N carry whatever scales lie past W's rows
+                if (cb0 + j >= args.N) x[j] = 0.f;
+                if (cb0 + j + 1 >= args.N) x[j + 1] = 0.f;
+              }
+              am = max_nan(max_nan(am, fabsf(x[j])), fabsf(x[j + 1]));
             }
-            *reinterpret_cast<uint4*>(args.hcodes + (int64_t)row * args.hpitch + (col0 >> 1)) = o;
-            args.hscales[fp4::scale_at(row, col0 >> 5, args.htiles)] = (uint8_t)(bad ? 0xFF : e + 127);
+            if (am < INFINITY) {
+              const int e = fp4::mx_exponent(am);
+              byte[h] = (uint32_t)(e + 127);
+              const uint2 lo = fp4::mx_codes16(x, e), hi = fp4::mx_codes16(x + 16, e);
+              code[h] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+              byte[h] = 0xFFu;
+            }
+          }
+          if (row_ok && (col0 >> 5) < args.htiles * 4) {
+            uint8_t* hp = args.hcodes + (int64_t)row * args.hpitch + (col0 >> 1);
+            if (col0 < args.N) *reinterpret_cast<uint4*>(hp) = code[0];
+            if (col0 + 32 < args.N) *reinterpret_cast<uint4*>(hp + 16) = code[1];
+            *reinterpret_cast<uint16_t*>(args.hscales + fp4::scale_at(row, col0 >> 5, args.htiles)) =
+                (uint16_t)(byte[0] | (byte[1] << 8));
           }
           continue;
         }
+        if (col0 >= args.N) continue;
         if (EPI == kResidual) {
           const __nv_bfloat16* rp = args.res + (int64_t)row * args.ldr;
+          const float4* g4 = reinterpret_cast<const float4*>(sCol + 2 * BN + c * 64);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int cg = col0 + g * 8;
-            float x[8], gt[8];
-            load_cols8(rp, row_ok ? cg : args.N, args.N, args.vec_n, x);
-            if (args.gate) {
-              load_cols8(args.gate, cg, args.N, args.vec_n, gt);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) gt[j] = 1.f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[g * 8 + j] = __fmaf_rn(gt[j], v[g * 8 + j], x[j]);
+          for (int g = 0; g < 8; ++g) {
+            float x[8];
+            load_cols8(rp, row_ok ? col0 + g * 8 : args.N, args.N, args.vec_res, x);
+            const float4 ga = g4[2 * g], gb = g4[2 * g + 1];
+            float* y = v + g * 8;
+            y[0] = __fmaf_rn(ga.x, y[0], x[0]);
+            y[1] = __fmaf_rn(ga.y, y[1], x[1]);
+            y[2] = __fmaf_rn(ga.z, y[2], x[2]);
+            y[3] = __fmaf_rn(ga.w, y[3], x[3]);
+            y[4] = __fmaf_rn(gb.x, y[4], x[4]);
+            y[5] = __fmaf_rn(gb.y, y[5], x[5]);
+            y[6] = __fmaf_rn(gb.z, y[6], x[6]);
+            y[7] = __fmaf_rn(gb.w, y[7], x[7]);
           }
         }
         if (args.tma_out) {
           if (lane == 0) tma_store_wait_read<0>();
           __syncwarp();
-          // 64-byte swizzle: 16-byte chunk g of row l lands at chunk g ^ (l / 2 % 4)
+          // 128-byte swizzle: 16-byte chunk g of row l lands at chunk g ^ (l % 8)
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<uint4*>(stg + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)) =
+          for (int g = 0; g < 8; ++g)
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((g ^ (lane & 7)) << 4)) =
                 f32_to_bf16x8(v + g * 8);
           fence_proxy_async_smem();
           __syncwarp();
@@ -497,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (row_ok) {
           __nv_bfloat16* op = args.out + (int64_t)row * args.ldo;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
+          for (int j = 0; j < 64; ++j)
             if (col0 + j < args.N) op[col0 + j] = __float2bfloat16_rn(v[j]);
         }
       }
@@ -527,7 +588,7 @@ struct Operand {
 
 template <int FMT, int BN, int EPI, bool PAIR>
 static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_t st) {
-  using S = Shape<FMT, BN, PAIR>;
+  using S = Shape<FMT, BN, EPI, PAIR>;
   const int64_t pitch = fp4::code_pitch(a.K);
   const int64_t tiles = fp4::scale_tiles(a.K, FMT);
   CUtensorMap tmA, tmB, tmSfA, tmSfB, tmO;
@@ -549,7 +610,7 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   tmO = tmA;  // unused unless tma_out
   if (a.tma_out) {
     rc = make_tmap_2d(&tmO, a.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.N,
-                      (uint64_t)a.M, (uint64_t)a.ldo * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+                      (uint64_t)a.M, (uint64_t)a.ldo * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
   auto kern = fp4_gemm_kernel<FMT, BN, EPI, PAIR>;
@@ -566,7 +627,7 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   const int num = (int)n_tiles64;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   if (PAIR) {
@@ -635,11 +696,6 @@ static int operands(const char* who, const void* A, const void* sfA, const float
   return FVB_OK;
 }
 
-static bool vec_cols(const Args& g) {
-  return (!g.sw || !g.sw_row || aligned16(g.sw)) && (!g.bias || aligned16(g.bias)) &&
-         (!g.gate || aligned16(g.gate)) && (!g.res || (aligned16(g.res) && g.ldr % 8 == 0));
-}
-
 }  // namespace gemm4
 }  // namespace fvb
 
@@ -673,7 +729,7 @@ int fvb_fp4_gemm(const void* A, const void* sfA, const float* rsA, int a_mode, c
   a.out = (__nv_bfloat16*)out;
   a.ldo = N;
   a.tma_out = aligned16(out) && N % 8 == 0;
-  a.vec_n = gemm4::vec_cols(a);
+  a.vec_res = residual && aligned16(residual) && ldr % 8 == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (residual) return gemm4::dispatch_fmt<gemm4::kResidual>(fmt, a, oa, ow, st);
   return gemm4::dispatch_fmt<gemm4::kPlain>(fmt, a, oa, ow, st);
@@ -712,7 +768,6 @@ int fvb_fp4_ffn(const void* A, const void* sfA, const float* rsA, int a_mode, co
   a.hscales = hs;
   a.hpitch = fp4::code_pitch(F);
   a.htiles = fp4::scale_tiles(F, FVB_FP4_MX);
-  a.vec_n = gemm4::vec_cols(a);
   rc = gemm4::dispatch_fmt<gemm4::kGeluMx>(fmt, a, oa, ow, (cudaStream_t)stream);
   if (rc) return rc;
   return fvb_fp4_gemm(hc, hs, nullptr, FVB_SCALE_TENSOR, W2, sfW2, nullptr, FVB_SCALE_TENSOR,
