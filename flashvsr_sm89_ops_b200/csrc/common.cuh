@@ -51,6 +51,10 @@ int sm_count();  // cached multiprocessor count of the current device
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes,
                  uint64_t inner, uint64_t outer, uint64_t row_bytes, uint32_t box_inner,
                  uint32_t box_outer, CUtensorMapSwizzle swizzle);
+// 3-D tensor, dim0 contiguous, strides of dim1 and dim2 in bytes; unswizzled boxes.
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t dim0,
+                 uint64_t dim1, uint64_t dim2, uint64_t stride1, uint64_t stride2, uint32_t box0,
+                 uint32_t box1, uint32_t box2);
 
 // Device-side error word: kernels that give up on a bounded wait record a code
 // here; the host reads it back with fvb_device_error().  (The library is one

@@ -8,22 +8,29 @@
 // One persistent CTA per SM, or one CTA pair per two SMs, warp-specialised:
 //   warp 0      TMA producer: 256-element (128-byte) K blocks of A and W and their scale tiles
 //               into a ring of shared-memory stages
-//   warp 1      MMA issuer: copies a group of scale tiles into TMEM (tcgen05.cp), then issues
-//               the group's block-scaled MMAs (K = 64 each) into the fp32 accumulator
-//   warps 2..   epilogue (8 warps, 16 with GELU): the warps of a TMEM lane quarter take the
-//               tile's 64-column chunks in turn, each thread one row; bf16 through a swizzled
-//               staging buffer and a TMA store.  A chunk is two mx blocks of a row, so the
-//               4-bit output needs no exchange between threads and the hidden state of an FFN
-//               never exists in 16 bits.
+//   warp 1      MMA issuer: copies a K block's scale tiles into TMEM (tcgen05.cp), then issues
+//               its four block-scaled MMAs (K = 64 each) into the fp32 accumulator
+//   warps 2..   epilogue: the warps of a TMEM lane quarter take the tile's 64-column chunks in
+//               turn; bf16 through a swizzled staging buffer and a TMA store, a residual into
+//               the same buffer by TMA while the tile is still being multiplied
 //
-// TMEM (512 columns): two accumulators of BN columns and two buffers of scale columns.  With
-// BN = 256 that is more than 512, so the second accumulator starts at column 192: the tiles'
-// accumulators share 64 columns, the epilogue reads those first, and the next tile's MMAs start
-// when they have been read instead of when the whole tile has.
+// TMEM (512 columns): two accumulators of BN columns, so that a tile's epilogue runs under the
+// next tile's MMAs, and at least two buffers of a K block's scales.  With BN = 256 that is
+// more than 512, so the second accumulator starts at column 128: the two share half their
+// columns, the epilogue's warps read those first, and the next tile's MMAs start when they have
+// been read.
 //
-// The scale columns of a group are overwritten two groups later, after a wait for the MMAs that
-// read them: the issue order orders a copy before the MMAs after it, but nothing orders an MMA
-// before a copy after it.
+// A scale buffer is overwritten after a wait for the MMAs that read it: the issue order puts a
+// copy before the MMAs after it, but nothing puts an MMA before a copy after it.  The wait is on
+// the ring stage's own barrier; a commit and a wait for every scale tile measured 84.6 us on
+// 8448 x 1536 x 8960, where one for every K block takes 49.
+//
+// Shared-memory bandwidth (128 bytes a clock per SM) is what the operands, their TMA writes and
+// the epilogue share, and it is nearly used up: a 256-element K block of a 256 x 256 pair tile
+// reads 32 KB and writes 38 KB per CTA in the 512 clocks of its MMAs.  So the epilogue reads
+// TMEM in the 16x256b shape, where a thread holds 2 columns of every 8 for 4 rows: a 64-column
+// chunk's scales and biases then cost a warp 24 wavefronts of shared memory, where a thread
+// that holds a whole row reads all 64 columns' and costs it 128.
 #include "fp4.cuh"
 
 namespace fvb {
@@ -33,10 +40,14 @@ constexpr int BM = 128;
 constexpr int kRowBytes = 128;  // one K block of a row: 256 elements
 constexpr int kStageOut = 32 * 128;  // an epilogue warp's staging: 32 rows x 64 bf16
 
+constexpr int kStageCodes = 32 * 32;  // with GELU: 32 rows x 64 codes
+
 enum { kPlain = 0, kResidual = 1, kGeluMx = 2 };
 
-// epilogue warps, a multiple of 4
-__host__ __device__ constexpr int epi_warps(int epi) { return epi == kGeluMx ? 16 : 8; }
+// epilogue warps: one per TMEM lane quarter and 64-column chunk, at most 8.  16 for BN = 256 left
+// the GELU epilogue 96 registers a thread and measured 119 us against 102 (8448 x 8960 x 1536
+// with a small second product); for the others their staging buffers would cost a ring stage.
+__host__ __device__ constexpr int epi_warps(int bn) { return bn > 128 ? 8 : 4 * (bn / 64); }
 
 struct Args {
   int M, N, K;
@@ -49,7 +60,7 @@ struct Args {
   __nv_bfloat16* out;         // row pitch ldo
   int64_t ldr, ldo;
   int tma_out;      // whether `out` suits a TMA store
-  int vec_res;      // whether res may be read 16 bytes at a time
+  int tma_res;      // whether `res` suits a TMA load
   uint8_t* hcodes;  // kGeluMx
   uint8_t* hscales;
   int64_t hpitch, htiles;
@@ -57,30 +68,33 @@ struct Args {
 
 template <int FMT, int BN, int EPI, bool PAIR>
 struct Shape {
-  static constexpr int kEpiWarps = epi_warps(EPI);
+  static constexpr int kEpiWarps = epi_warps(BN);
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
-  static constexpr int kOutBytes = EPI == kGeluMx ? 0 : kEpiWarps * kStageOut;
-  static constexpr int kColBytes = 3 * BN * 4;  // the tile's column scales, biases and gates
+  static constexpr int kOut = EPI == kGeluMx ? kStageCodes : kStageOut;
+  static constexpr int kOutBytes = kEpiWarps * kOut;
+  static constexpr int kColBytes = 2 * 2 * BN * 4;  // two tiles' column scales (fp32), biases and gates (bf16)
   static constexpr int kTilesK = FMT == FVB_FP4_NV ? 4 : 2;  // scale tiles per K block
-  static constexpr int kGroups = kTilesK / 2;                // TMEM groups of two scale tiles
-  static constexpr int kMmas = 4 / kGroups;                  // MMAs (K = 64) per group
+  static constexpr int kMmas = 4 / kTilesK;                  // MMAs (K = 64) per scale tile
   static constexpr int kRowsB = PAIR ? BN / 2 : BN;          // W rows this CTA stages
-  static constexpr int kSfTilesB = BN > 128 ? BN / 128 : 1;  // 128-row tiles of W's scales
+  static constexpr int kSfTilesB = BN > 128 ? 2 : 1;  // 128-row scale tiles a tile's columns lie in
   static constexpr int kBytesA = BM * kRowBytes;
   static constexpr int kBytesB = kRowsB * kRowBytes;
-  static constexpr int kBytesSfA = kGroups * 1024;
-  static constexpr int kBytesSfB = kGroups * kSfTilesB * 1024;
+  static constexpr int kBytesSfA = kTilesK * 512;
+  static constexpr int kBytesSfB = kTilesK * kSfTilesB * 512;
   static constexpr int kBytes = kBytesA + kBytesB + kBytesSfA + kBytesSfB;
-  static constexpr int kFixed = kOutBytes + kColBytes + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int kFixed = kOutBytes + kColBytes + 1024 /*align*/ + 384 /*barriers*/;
   static constexpr int kFit = (227 * 1024 - kFixed) / kBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr size_t kSmem = (size_t)kStages * kBytes + kFixed;
   // TMEM columns
-  static constexpr int kAcc1 = BN == 256 ? 192 : BN;  // start of the second accumulator
   static constexpr bool kOverlap = BN == 256;
-  static constexpr int kSf = kAcc1 + BN;                    // start of the scale columns
-  static constexpr int kSfCols = 8 + 8 * kSfTilesB;         // one group's
-  static_assert(kSf + 2 * kSfCols <= 512, "TMEM columns");
+  static constexpr int kAcc1 = kOverlap ? 128 : BN;   // start of the second accumulator
+  static constexpr int kSf = kAcc1 + BN;              // start of the scale buffers
+  static constexpr int kSfA = 4 * kTilesK, kSfB = 4 * kTilesK * kSfTilesB;  // columns of one
+  static constexpr int kFitSf = (512 - kSf) / (kSfA + kSfB);
+  static constexpr int kSfBufs = kFitSf > kStages ? kStages : kFitSf;
+  static_assert(kSfBufs >= 2, "TMEM columns");
+  static_assert(BN % 64 == 0 && BN <= 256, "a tile's columns start on half a scale tile");
   static_assert(kStages >= 3, "ring");
 };
 
@@ -120,6 +134,59 @@ __device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
                  : "memory");
 }
 
+// 16 lanes x 64 columns of 32-bit TMEM: register 4 g + 2 h + e of lane l is row l / 4 + 8 h,
+// column 8 g + 2 (l % 4) + e
+__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// four 8 x 8 matrices of 16-bit values: lane l names row l % 8 of matrix l / 8, and register m
+// holds row l / 4, columns 2 (l % 4) + {0, 1} of matrix m
+__device__ __forceinline__ void stmatrix_x4(uint32_t saddr, const uint32_t* r) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(saddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t* r, uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// into this CTA's shared memory, counted on the barrier at shared::cluster address bar_caddr
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map,
+                                                 uint32_t bar_caddr, int32_t x, int32_t y,
+                                                 int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_caddr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// arrive on a barrier of the pair without releasing this thread's earlier stores: what it
+// signals is TMEM that has been read (tcgen05.wait::ld), and a release at cluster scope waits
+// for the thread's global stores in flight (1300 clocks a tile in the GELU epilogue)
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t caddr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
+}
+
 // instruction descriptor: E2M1 operands, scale type, M x N; the scale ids (byte of the 4-byte
 // scale column an mx MMA starts at) are added per MMA
 template <int FMT>
@@ -129,40 +196,121 @@ __host__ __device__ constexpr uint32_t idesc4(int M, int N) {
 }
 
 // GELU(tanh) of two values in fp32: x * sigmoid(2 u) = x / (1 + 2^v), u = sqrt(2/pi) (x + c x^3),
-// v = -2 u log2(e).  One reciprocal of the product serves both: 1 / a = b / (a b).  v is held
-// at 60 so the product stays finite; x / 2^60 is then already far below any step of the codes
-// next to it, and 0.5 x (1 + tanh u) in fp32 has long been 0.
-__device__ __forceinline__ void gelu2(float& x0, float& x1) {
+// v = -2 u log2(e).  One reciprocal of the product serves both, 1 / a = b / (a b): the
+// special-function unit (16 a clock per SM) would bound the epilogue with two for each value.
+// v is held at 60 so that the product stays finite; x / 2^60 is far below any code next to it,
+// and 0.5 x (1 + tanh u) in fp32 has long been 0 there.
+__device__ __forceinline__ uint64_t gelu2(uint64_t x) {
   const float k1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, k3 = k1 * 0.044715f;
-  const uint64_t x = f2_pack(x0, x1);
   const uint64_t v = f2_mul(x, f2_fma(f2_mul(x, x), f2_pack(k3, k3), f2_pack(k1, k1)));
-  float v0, v1;
+  float v0, v1, a, b;
   f2_unpack(v, v0, v1);
-  const float a = 1.0f + ex2_approx(fminf(v0, 60.0f)), b = 1.0f + ex2_approx(fminf(v1, 60.0f));
+  f2_unpack(f2_add(f2_pack(ex2_approx(fminf(v0, 60.0f)), ex2_approx(fminf(v1, 60.0f))),
+                   f2_pack(1.0f, 1.0f)),
+            a, b);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
-  f2_unpack(f2_mul(f2_mul(x, f2_pack(r, r)), f2_pack(b, a)), x0, x1);
+  return f2_mul(x, f2_pack(b * r, a * r));
 }
-__device__ __forceinline__ float max_nan(float a, float b) {  // keeps a NaN
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// max(m, |x.lo|, |x.hi|), a NaN if one is
+__device__ __forceinline__ float max_abs_nan(float m, uint64_t x) {
+  float a, b, r;
+  f2_unpack(x, a, b);
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
   return r;
 }
 
-__device__ __forceinline__ void load_cols8(const __nv_bfloat16* p, int c, int N, bool vec, float* v) {
-  if (vec && c + 8 <= N) {
-    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(p + c)), v);
-  } else {
+// GELU and mx quantisation of an epilogue chunk (32 rows x 64 columns, v as in the kernel): the
+// codes into the staging buffer at shared address `stg` (32 rows x 32 bytes, 32-byte swizzle),
+// the two scale bytes of row lr + 8 k returned in sb[k] by every lane of the row.
+// A row's block lies in four neighbouring lanes: its exponent is the maximum of theirs, and the
+// code bytes (one per pair of columns) are transposed within the four, so that lane j ends up
+// with columns 8 j .. 8 j + 7 of the block as one word.
+__device__ __forceinline__ void gelu_mx(uint64_t (&v)[4][8], int col0, int N, int lane, uint32_t stg,
+                                        uint32_t* sb) {
+  const int lr = lane >> 2, lq = lane & 3;
+  if (col0 + 64 > N) {  // columns past N carry whatever scales lie past W's rows
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < N ? __bfloat162float(p[c + i]) : 0.f;
+    for (int g = 0; g < 8; ++g) {
+      const int left = N - (col0 + g * 8 + 2 * lq);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (left < 1) v[k][g] &= 0xFFFFFFFF00000000ull;
+        if (left < 2) v[k][g] &= 0x00000000FFFFFFFFull;
+      }
+    }
   }
+  // the exponent fields of the 4 rows x 2 blocks, two to a word (255: not finite)
+  uint32_t ex[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float m[2] = {0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      v[k][g] = gelu2(v[k][g]);
+      m[g >> 2] = max_abs_nan(m[g >> 2], v[k][g]);
+    }
+    ex[k] = __byte_perm(__float_as_uint(m[0]) >> 23, __float_as_uint(m[1]) >> 23, 0x5410);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) ex[k] = __vmaxu2(ex[k], __shfl_xor_sync(0xffffffffu, ex[k], 1));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) ex[k] = __vmaxu2(ex[k], __shfl_xor_sync(0xffffffffu, ex[k], 2));
+  uint32_t w[2][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    sb[k] = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t e = h ? ex[k] >> 16 : ex[k] & 0xFFFFu;
+      // scale byte: amax's exponent field - 2, at least 0; 1 / scale = 2^(127 - byte)
+      const uint32_t byte = e > 2u ? e - 2u : 0u;
+      const bool bad = e == 255u;
+      sb[k] |= (bad ? 255u : byte) << (8 * h);
+      const float rs = __uint_as_float((254u - byte) << 23);
+      const uint64_t rs2 = f2_pack(rs, rs);
+      float x[8];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) f2_unpack(f2_mul(v[k][4 * h + g], rs2), x[2 * g], x[2 * g + 1]);
+      w[h][k] = bad ? 0u : fp4::e2m1x8(x);
+    }
+  }
+  // 4 x 4 byte transposes in each group of four lanes, two words (rows k, k + 1) per exchange:
+  // lane bit 0 trades odd for even bytes, lane bit 1 the upper for the lower pair
+  const bool o = lane & 1, u = lane & 2;
+  const uint32_t give1 = o ? 0x6420u : 0x7531u, keep1p = o ? 0x3514u : 0x5240u,
+                 keep1q = o ? 0x3716u : 0x7260u, give2 = u ? 0x5410u : 0x7632u,
+                 keep2p = u ? 0x3254u : 0x5410u, keep2q = u ? 0x3276u : 0x7610u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      uint32_t p = w[h][k], q = w[h][k + 1];
+      uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(p, q, give1), 1);
+      p = __byte_perm(p, got, keep1p);
+      q = __byte_perm(q, got, keep1q);
+      got = __shfl_xor_sync(0xffffffffu, __byte_perm(p, q, give2), 2);
+      w[h][k] = __byte_perm(p, got, keep2p);
+      w[h][k + 1] = __byte_perm(q, got, keep2q);
+    }
+  }
+  // 16-byte chunk h of row l lies at chunk h ^ (l / 4 % 2)
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t at = stg + (lr + 8 * k) * 32 + ((h ^ ((lr >> 2) & 1)) << 4) + lq * 4;
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w[h][k]) : "memory");
+    }
 }
+
 template <int FMT, int BN, int EPI, bool PAIR>
-__global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
+__global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSfA,
                     const __grid_constant__ CUtensorMap tmSfB,
-                    const __grid_constant__ CUtensorMap tmOut, const Args args) {
+                    const __grid_constant__ CUtensorMap tmOut,
+                    const __grid_constant__ CUtensorMap tmRes, const Args args) {
   using S = Shape<FMT, BN, EPI, PAIR>;
   constexpr int STAGES = S::kStages;
   constexpr int TM = PAIR ? 2 * BM : BM;
@@ -174,14 +322,14 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
   uint8_t* sSfA = sB + STAGES * S::kBytesB;
   uint8_t* sSfB = sSfA + STAGES * S::kBytesSfA;
   uint8_t* sOut = sSfB + STAGES * S::kBytesSfB;
-  float* sCol = reinterpret_cast<float*>(sOut + S::kOutBytes);  // [3][BN]
+  float* sCol = reinterpret_cast<float*>(sOut + S::kOutBytes);  // [2 tiles][2][BN]
   uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::kOutBytes + S::kColBytes);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;   // [2] accumulator finished
-  uint64_t* tempty = tfull + 2;       // [2] accumulator (its shared columns) read
-  uint64_t* sfree = tempty + 2;       // [2] the MMAs of a scale buffer finished
-  uint64_t* drain = sfree + 2;        // every MMA this CTA issued finished
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* tempty = tfull + 2;       // [2] accumulator read
+  uint64_t* drain = tempty + 2;       // every MMA this CTA issued finished
+  uint64_t* rfull = drain + 1;        // [epilogue warps] residual arrived
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + S::kEpiWarps);
   uint32_t* pair_ok = tmem_slot + 1;
 
   const int warp = warp_id_uniform();
@@ -202,9 +350,9 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], PAIR ? 2 * S::kEpiWarps : S::kEpiWarps);
-      mbar_init(&sfree[b], 1);
     }
     mbar_init(drain, 1);
+    for (int w = 0; w < S::kEpiWarps; ++w) mbar_init(&rfull[w], 1);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -241,60 +389,56 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
     // straight to the teardown
   } else if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      int64_t issued = 0;
-      for (int tile = unit; tile < num_tiles && ok; tile += units) {
-        const int m0 = (tile / n_tiles) * TM + (int)rank * BM;
-        const int nt = (tile % n_tiles) * BN;
-        const int n0 = nt + (int)rank * (PAIR ? S::kRowsB : 0);
-        for (int kb = 0; kb < kblocks; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, 0x401u)) {
-            ok = false;
-            break;
-          }
+    // like the MMA issuer below, the whole warp walks the loop and one elected lane issues
+    const bool leader = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int64_t issued = 0;
+    for (int tile = unit; tile < num_tiles && ok; tile += units) {
+      const int m0 = (tile / n_tiles) * TM + (int)rank * BM;
+      const int nt = (tile % n_tiles) * BN;
+      const int n0 = nt + (int)rank * (PAIR ? S::kRowsB : 0);
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, 0x401u))) {
+          ok = false;
+          break;
+        }
+        if (leader) {
           uint8_t* a = sA + stage * S::kBytesA;
           uint8_t* b = sB + stage * S::kBytesB;
           uint8_t* fa = sSfA + stage * S::kBytesSfA;
           uint8_t* fb = sSfB + stage * S::kBytesSfB;
+          // scale tiles past the last of a row are filled with zeros
           if (PAIR) {
+            // the even CTA arms its barrier for both CTAs' bytes
             const uint32_t bar = full0_c + 8u * stage;
             if (rank == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)(2 * S::kBytes));
             tma_load_2d_pair(a, &tmA, bar, kb * kRowBytes, m0);
             tma_load_2d_pair(b, &tmB, bar, kb * kRowBytes, n0);
-#pragma unroll
-            for (int g = 0; g < S::kGroups; ++g) {
-              // two scale tiles = 256 words; past the last tile of a row TMA fills zeros
-              const int x = (kb * S::kTilesK + 2 * g) * 128;
-              tma_load_2d_pair(fa + g * 1024, &tmSfA, bar, x, m0 >> 7);
-              tma_load_2d_pair(fb + g * S::kSfTilesB * 1024, &tmSfB, bar, x, nt >> 7);
-            }
+            tma_load_3d_pair(fa, &tmSfA, bar, 0, kb * S::kTilesK, m0 >> 7);
+            tma_load_3d_pair(fb, &tmSfB, bar, 0, kb * S::kTilesK, nt >> 7);
           } else {
             mbar_arrive_expect_tx(&full[stage], (uint32_t)S::kBytes);
             tma_load_2d(a, &tmA, &full[stage], kb * kRowBytes, m0);
             tma_load_2d(b, &tmB, &full[stage], kb * kRowBytes, n0);
-#pragma unroll
-            for (int g = 0; g < S::kGroups; ++g) {
-              const int x = (kb * S::kTilesK + 2 * g) * 128;
-              tma_load_2d(fa + g * 1024, &tmSfA, &full[stage], x, m0 >> 7);
-              tma_load_2d(fb + g * S::kSfTilesB * 1024, &tmSfB, &full[stage], x, nt >> 7);
-            }
-          }
-          ++issued;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+            tma_load_3d(fa, &tmSfA, &full[stage], 0, kb * S::kTilesK, m0 >> 7);
+            tma_load_3d(fb, &tmSfB, &full[stage], 0, kb * S::kTilesK, nt >> 7);
           }
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
-      // no load may still be writing shared memory when its CTA exits: the last STAGES loads
-      // are the newest phase of their stages' full barriers (a pair's are the even CTA's)
-      if (!PAIR || rank == 0)
-        for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
-          mbar_wait(&full[i % STAGES], (uint32_t)((i / STAGES) & 1), 0x40Au);
     }
+    // no load may still be writing shared memory when its CTA exits: the last STAGES loads
+    // are the newest phase of their stages' full barriers (a pair's are the even CTA's)
+    if (!PAIR || rank == 0)
+      for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+        mbar_wait(&full[i % STAGES], (uint32_t)((i / STAGES) & 1), 0x40Au);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp walks the loop, so addresses and descriptors stay warp-uniform (the form
@@ -310,21 +454,24 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
       int stage = 0;
       uint32_t phase = 0;
       int t = 0;
-      uint32_t grp = 0;  // scale groups issued
+      int sbuf = 0;  // scale buffer, and the stage and parity of the K block that had it last
+      int old_stage = 0;
+      uint32_t old_phase = 0;
+      bool reuse = false;
       bool ok = true, any = false;
       for (int tile = unit; tile < num_tiles && ok; tile += units, ++t) {
         const int buf = t & 1;
-        // shared columns: wait until the previous tile's were read; else until this
-        // accumulator's last tile was
+        // separate accumulators: until this one's last tile was read.  Shared columns: until the
+        // previous tile's were; its other warps arrive there having read the tile before it
         const bool clear =
             S::kOverlap
                 ? (t == 0 || mbar_wait(&tempty[buf ^ 1], (uint32_t)((t - 1) >> 1) & 1u, 0x402u))
                 : mbar_wait(&tempty[buf], ((uint32_t)(t >> 1) & 1u) ^ 1u, 0x402u);
         if (!__all_sync(0xffffffffu, clear)) break;
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(buf ? S::kAcc1 : 0);
-        const int nt = (tile % n_tiles) * BN;
-        const uint32_t shift = BN < 128 ? (uint32_t)((nt & 127) >> 5) : 0u;
+        const uint32_t d = tmem + (uint32_t)(buf * S::kAcc1);
+        // a tile may start half way into a 128-row scale tile: two 32-row scale columns on
+        const uint32_t shift = BN % 128 == 0 ? 0u : (uint32_t)((((tile % n_tiles) * BN) & 127) >> 5);
         for (int kb = 0; kb < kblocks && ok; ++kb) {
           if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, 0x403u))) {
             ok = false;
@@ -336,44 +483,42 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
           const uint64_t fa = descFA + (uint32_t)(stage * (S::kBytesSfA >> 4));
           const uint64_t fb = descFB + (uint32_t)(stage * (S::kBytesSfB >> 4));
           const int left = ksteps - kb * 4;  // K steps from this block on
-#pragma unroll
-          for (int g = 0; g < S::kGroups; ++g) {
-            if (g * S::kMmas < left) {
-              const uint32_t sb = grp & 1u;
-              if (!__all_sync(0xffffffffu, mbar_wait(&sfree[sb], ((grp >> 1) & 1u) ^ 1u, 0x405u))) {
-                ok = false;
-                break;
-              }
-              const uint32_t sfa = tmem + (uint32_t)S::kSf + sb * (uint32_t)S::kSfCols;
-              const uint32_t sfb = sfa + 8u;
-              if (leader) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  cp_scales<PAIR>(sfa + 4u * i, fa + (g * 1024 + i * 512) / 16);
-#pragma unroll
-                  for (int r = 0; r < S::kSfTilesB; ++r)
-                    cp_scales<PAIR>(sfb + (uint32_t)(4 * S::kSfTilesB * i + 4 * r),
-                                    fb + ((g * S::kSfTilesB + r) * 1024 + i * 512) / 16);
-                }
-#pragma unroll
-                for (int i = 0; i < S::kMmas; ++i) {
-                  const int ks = g * S::kMmas + i;  // K step inside the block
-                  if (ks < left) {
-                    const int ti = FMT == FVB_FP4_NV ? i : i >> 1;            // scale tile
-                    const uint32_t id = FMT == FVB_FP4_NV ? 0u : (i & 1) * 2u;  // byte in its column
-                    mma_fp4<FMT, PAIR>(d, da + 2 * ks, db + 2 * ks, idesc | (id << 4) | (id << 29),
-                                       sfa + 4u * ti, sfb + (uint32_t)(4 * S::kSfTilesB * ti) + shift,
-                                       (kb | ks) != 0 ? 1u : 0u);
-                  }
-                }
-                if (PAIR) tc_commit_pair(&sfree[sb]);
-                else tc_commit(&sfree[sb]);
-              }
-              ++grp;
-              any = true;
+          if (reuse && S::kSfBufs < STAGES) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[old_stage], old_phase, 0x405u))) {
+              ok = false;
+              break;
+            }
+            if (++old_stage == STAGES) {
+              old_stage = 0;
+              old_phase ^= 1u;
             }
           }
-          if (!ok) break;
+          const uint32_t sfa = tmem + (uint32_t)(S::kSf + sbuf * (S::kSfA + S::kSfB));
+          const uint32_t sfb = sfa + (uint32_t)S::kSfA;
+          if (leader) {
+#pragma unroll
+            for (int i = 0; i < S::kTilesK; ++i) {
+              cp_scales<PAIR>(sfa + 4u * i, fa + i * 512 / 16);
+#pragma unroll
+              for (int r = 0; r < S::kSfTilesB; ++r)
+                cp_scales<PAIR>(sfb + (uint32_t)(4 * (S::kSfTilesB * i + r)),
+                                fb + (r * S::kTilesK + i) * 512 / 16);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              // an mx MMA takes two bytes of the four in a scale column
+              const uint32_t i = ks / S::kMmas, id = 2u * (ks % S::kMmas);
+              if (ks < left)
+                mma_fp4<FMT, PAIR>(d, da + 2 * ks, db + 2 * ks, idesc | (id << 4) | (id << 29),
+                                   sfa + 4u * i, sfb + 4u * S::kSfTilesB * i + shift,
+                                   (kb | ks) != 0 ? 1u : 0u);
+            }
+          }
+          any = true;
+          if (++sbuf == S::kSfBufs) {
+            sbuf = 0;
+            reuse = true;
+          }
           if (leader) {
             if (PAIR) tc_commit_pair_both(&empty[stage], 0x3);
             else tc_commit(&empty[stage]);
@@ -402,164 +547,217 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(EPI), 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    // G warps per TMEM lane quarter (warp % 4) take the tile's 64-column chunks in turn, each
-    // thread one row of a chunk
-    constexpr int G = S::kEpiWarps / 4;
+    constexpr int G = S::kEpiWarps / 4;  // warps per TMEM lane quarter
     constexpr int kChunks = BN / 64;
-    const int q = warp & 3;
-    const int sub = (warp - 2) >> 2;
+    const int q = warp & 3;              // TMEM lane quarter this warp may access
+    const int sub = (warp - 2) >> 2;     // its first chunk
     const int et = (int)threadIdx.x - 64;
-    uint8_t* stg = sOut + (size_t)(warp - 2) * kStageOut;
-    auto release = [&](int b) {
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (PAIR) mbar_arrive_remote(tempty0_c + 8u * b);
-        else mbar_arrive(&tempty[b]);
-      }
-    };
+    const int lr = lane >> 2, lc = 2 * (lane & 3);  // this thread's rows lr + 8 k, columns 8 g + lc + {0, 1}
+    uint8_t* stg = sOut + (size_t)(warp - 2) * S::kOut;
+    uint64_t* rbar = &rfull[warp - 2];
     // the tile's column vectors go through shared memory: read from global one tile ahead,
     // so that no thread waits for them between the accumulator and the store
-    float cs = 1.f, cb = 0.f, cg = 1.f;
+    float cs = 1.f;
+    __nv_bfloat16 cb = __float2bfloat16_rn(0.f), cg = __float2bfloat16_rn(1.f);
     auto columns = [&](int tile) {
       const int c = (tile % n_tiles) * BN + et;
       if (tile < num_tiles && et < BN && c < args.N) {
         if (args.sw) cs = __ldg(args.sw + (args.sw_row ? c : 0));
-        if (args.bias) cb = __bfloat162float(args.bias[c]);
-        if (EPI == kResidual && args.gate) cg = __bfloat162float(args.gate[c]);
+        if (args.bias) cb = args.bias[c];
+        if (EPI == kResidual && args.gate) cg = args.gate[c];
       }
     };
     columns(unit);
+    auto release = [&](int b) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_remote_relaxed(tempty0_c + 8u * b);
+        else mbar_arrive(&tempty[b]);
+      }
+    };
+    const bool tma_res = EPI == kResidual && args.tma_res;
     bool ok = true;
     int t = 0;
+    uint32_t rphase = 0;
     for (int tile = unit; tile < num_tiles; tile += units, ++t) {
       const int buf = t & 1;
-      const int m0 = (tile / n_tiles) * TM + (int)rank * BM;
+      const int m0 = (tile / n_tiles) * TM + (int)rank * BM + q * 32;
       const int n0 = (tile % n_tiles) * BN;
-      const int row = m0 + q * 32 + lane;
-      const bool row_ok = row < args.M;
-      float sa = 1.0f;
-      if (args.sa) sa = args.sa_row ? (row_ok ? __ldg(args.sa + row) : 0.f) : __ldg(args.sa);
-      asm volatile("bar.sync 1, %0;" ::"r"(S::kEpiWarps * 32) : "memory");  // last tile's readers
+      // chunk order: the columns shared with the other accumulator first (the first
+      // accumulator's last two chunks, the second's first two)
+      const int first = S::kOverlap && buf == 0 ? 2 : 0;  // kChunks is 4 then
+      auto residual = [&](int c) {  // the chunk's residual on its way into the staging buffer
+        if (lane == 0) {
+          tma_store_wait_read<0>();  // the last store has left the buffer
+          mbar_arrive_expect_tx(rbar, kStageOut);
+          tma_load_2d(stg, &tmRes, rbar, n0 + c * 64, m0);
+        }
+      };
+      bool coming = false;  // a residual load of this warp is in flight
+      if (tma_res && ok && sub < kChunks && n0 + ((S::kOverlap ? (sub + first) & 3 : sub)) * 64 < args.N) {
+        residual((S::kOverlap ? (sub + first) & 3 : sub));
+        coming = true;
+      }
+      uint64_t sa2[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = m0 + lr + 8 * k;
+        float sa = 1.f;
+        if (args.sa) sa = args.sa_row ? (row < args.M ? __ldg(args.sa + row) : 0.f) : __ldg(args.sa);
+        sa2[k] = f2_pack(sa, sa);
+      }
+      // two tiles' vectors: whoever passes this tile's barrier has read the last but one's
+      float* sScale = sCol + buf * 2 * BN;
+      __nv_bfloat162* sBias = reinterpret_cast<__nv_bfloat162*>(sScale + BN);
+      __nv_bfloat162* sGate = sBias + BN / 2;
       if (et < BN) {
-        sCol[et] = cs;
-        sCol[BN + et] = cb;
-        if (EPI == kResidual) sCol[2 * BN + et] = cg;
+        sScale[et] = cs;
+        reinterpret_cast<__nv_bfloat16*>(sBias)[et] = cb;
+        if (EPI == kResidual) reinterpret_cast<__nv_bfloat16*>(sGate)[et] = cg;
       }
       asm volatile("bar.sync 1, %0;" ::"r"(S::kEpiWarps * 32) : "memory");
       columns(tile + units);
       // a warp whose wait ran out goes on to the barriers above, which its neighbours may be at,
-      // and does nothing else
+      // and to the end of its own load, and does nothing else
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&tfull[buf], (uint32_t)(t >> 1) & 1u, 0x404u));
-      if (!ok) continue;
+      if (!ok) {
+        if (coming) mbar_wait(rbar, rphase, 0x406u);
+        continue;
+      }
       tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf ? S::kAcc1 : 0);
-      const uint64_t sa2 = f2_pack(sa, sa);
-      // chunk order: the columns shared with the other accumulator first (the first
-      // accumulator's last chunk, the second's first)
-      const int first = S::kOverlap && buf == 0 ? kChunks - 1 : 0;
-      if (sub >= kChunks || (S::kOverlap && sub != 0)) release(buf);  // reads no shared column
+      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * S::kAcc1);
 #pragma unroll 1
       for (int i = sub; i < kChunks; i += G) {
-        const int c = (i + first) & (kChunks - 1);
+        const int c = S::kOverlap ? (i + first) & 3 : i;
         const int col0 = n0 + c * 64;
+        const bool cols_ok = col0 < args.N;  // warp-uniform
         uint32_t r[64];
-        tmem_ld_32x32b_x32(acc + (uint32_t)(c * 64), r);
-        tmem_ld_32x32b_x32(acc + (uint32_t)(c * 64 + 32), r + 32);
+        // v[k][g]: row lr + 8 k, columns 8 g + lc and the next, as an fp32 pair
+        tmem_ld_16x256b_x8(acc + (uint32_t)(c * 64), r);
+        tmem_ld_16x256b_x8(acc + (uint32_t)(c * 64) + (16u << 16), r + 32);
         tmem_ld_wait();
-        if (S::kOverlap ? i == 0 : i + G >= kChunks) release(buf);
-        float* v = reinterpret_cast<float*>(r);
-        if (col0 < args.N) {  // warp-uniform
-          const float4* s4 = reinterpret_cast<const float4*>(sCol + c * 64);
-          const float4* b4 = reinterpret_cast<const float4*>(sCol + BN + c * 64);
+        if (S::kOverlap ? i < 2 : i + G >= kChunks) release(buf);
+        uint64_t v[4][8];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float4 s = s4[j], b = b4[j];
-            f2_unpack(f2_fma(f2_pack(v[4 * j], v[4 * j + 1]), f2_mul(sa2, f2_pack(s.x, s.y)),
-                             f2_pack(b.x, b.y)),
-                      v[4 * j], v[4 * j + 1]);
-            f2_unpack(f2_fma(f2_pack(v[4 * j + 2], v[4 * j + 3]), f2_mul(sa2, f2_pack(s.z, s.w)),
-                             f2_pack(b.z, b.w)),
-                      v[4 * j + 2], v[4 * j + 3]);
-          }
-        }
-        if (EPI == kGeluMx) {
-          // two mx blocks of this row
-          uint32_t byte[2] = {0u, 0u};
-          uint4 code[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            code[h] = make_uint4(0u, 0u, 0u, 0u);
-            const int cb0 = col0 + h * 32;
-            if (cb0 >= args.N) continue;  // past the last block: a zero scale
-            float* x = v + h * 32;
-            float am = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              gelu2(x[j], x[j + 1]);
-              if (cb0 + 32 > args.N) {  // columns past N carry whatever scales lie past W's rows
-                if (cb0 + j >= args.N) x[j] = 0.f;
-                if (cb0 + j + 1 >= args.N) x[j + 1] = 0.f;
-              }
-              am = max_nan(max_nan(am, fabsf(x[j])), fabsf(x[j + 1]));
-            }
-            if (am < INFINITY) {
-              const int e = fp4::mx_exponent(am);
-              byte[h] = (uint32_t)(e + 127);
-              const uint2 lo = fp4::mx_codes16(x, e), hi = fp4::mx_codes16(x + 16, e);
-              code[h] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            } else {
-              byte[h] = 0xFFu;
-            }
-          }
-          if (row_ok && (col0 >> 5) < args.htiles * 4) {
-            uint8_t* hp = args.hcodes + (int64_t)row * args.hpitch + (col0 >> 1);
-            if (col0 < args.N) *reinterpret_cast<uint4*>(hp) = code[0];
-            if (col0 + 32 < args.N) *reinterpret_cast<uint4*>(hp + 16) = code[1];
-            *reinterpret_cast<uint16_t*>(args.hscales + fp4::scale_at(row, col0 >> 5, args.htiles)) =
-                (uint16_t)(byte[0] | (byte[1] << 8));
-          }
-          continue;
-        }
-        if (col0 >= args.N) continue;
-        if (EPI == kResidual) {
-          const __nv_bfloat16* rp = args.res + (int64_t)row * args.ldr;
-          const float4* g4 = reinterpret_cast<const float4*>(sCol + 2 * BN + c * 64);
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
-            float x[8];
-            load_cols8(rp, row_ok ? col0 + g * 8 : args.N, args.N, args.vec_res, x);
-            const float4 ga = g4[2 * g], gb = g4[2 * g + 1];
-            float* y = v + g * 8;
-            y[0] = __fmaf_rn(ga.x, y[0], x[0]);
-            y[1] = __fmaf_rn(ga.y, y[1], x[1]);
-            y[2] = __fmaf_rn(ga.z, y[2], x[2]);
-            y[3] = __fmaf_rn(ga.w, y[3], x[3]);
-            y[4] = __fmaf_rn(gb.x, y[4], x[4]);
-            y[5] = __fmaf_rn(gb.y, y[5], x[5]);
-            y[6] = __fmaf_rn(gb.z, y[6], x[6]);
-            y[7] = __fmaf_rn(gb.w, y[7], x[7]);
+            const int i0 = (k >> 1) * 32 + g * 4 + (k & 1) * 2;
+            v[k][g] = f2_pack(__uint_as_float(r[i0]), __uint_as_float(r[i0 + 1]));
+          }
+        if (cols_ok) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const float2 b = __bfloat1622float2(sBias[(c * 64 + g * 8 + lc) >> 1]);
+            const uint64_t b2 = f2_pack(b.x, b.y);
+            if (args.sw) {
+              const float2 s = *reinterpret_cast<const float2*>(sScale + c * 64 + g * 8 + lc);
+              const uint64_t s2 = f2_pack(s.x, s.y);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k][g] = f2_fma(v[k][g], f2_mul(sa2[k], s2), b2);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k][g] = f2_fma(v[k][g], sa2[k], b2);
+            }
+          }
+        }
+        if constexpr (EPI == kGeluMx) {
+          uint32_t sb[4] = {0u, 0u, 0u, 0u};  // past the last block: the next product reads whole tiles
+          if (cols_ok) {
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+            gelu_mx(v, col0, args.N, lane, smem_u32(stg), sb);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {  // ends at the rows' pitch
+              tma_store_2d(&tmOut, stg, col0 >> 1, m0);
+              tma_store_commit();
+            }
+          }
+          // scale_at(row, col0 / 32): the warp's rows are one 4-byte column of their tile; lane
+          // lq of a row's four stores row lr + 8 lq
+          const int k = lane & 3;
+          const uint32_t b = k == 0 ? sb[0] : k == 1 ? sb[1] : k == 2 ? sb[2] : sb[3];
+          if (m0 + lr + 8 * k < args.M && (col0 >> 7) < args.htiles)
+            *reinterpret_cast<uint16_t*>(args.hscales + ((m0 >> 7) * args.htiles + (col0 >> 7)) * 512 +
+                                         (lr + 8 * k) * 16 + q * 4 + ((col0 >> 5) & 3)) = (uint16_t)b;
+          continue;
+        }
+        if (!cols_ok) continue;
+        // 128-byte swizzle of the staging rows: 16-byte chunk g of row l lies at chunk g ^ (l % 8);
+        // lane l names row l of a group's 32 rows x 8 columns
+        const uint32_t srow = smem_u32(stg) + lane * 128;
+        if (EPI == kResidual) {
+          if (tma_res) {
+            if (i != sub) residual(c);
+            ok = __all_sync(0xffffffffu, mbar_wait(rbar, rphase, 0x406u));
+            if (!ok) break;
+            rphase ^= 1u;
+          }
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            uint32_t x[4];
+            if (tma_res) {
+              ldmatrix_x4(x, srow + ((g ^ (lane & 7)) << 4));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int row = m0 + lr + 8 * k, col = col0 + g * 8 + lc;
+                const __nv_bfloat16* rp = args.res + (int64_t)row * args.ldr + col;
+                __nv_bfloat162 p = __float2bfloat162_rn(0.f);
+                if (row < args.M && col < args.N) p.x = rp[0];
+                if (row < args.M && col + 1 < args.N) p.y = rp[1];
+                x[k] = *reinterpret_cast<uint32_t*>(&p);
+              }
+            }
+            const float2 gt = __bfloat1622float2(sGate[(c * 64 + g * 8 + lc) >> 1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 xf = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[k]));
+              v[k][g] = f2_fma(f2_pack(gt.x, gt.y), v[k][g], f2_pack(xf.x, xf.y));
+            }
           }
         }
         if (args.tma_out) {
-          if (lane == 0) tma_store_wait_read<0>();
+          if (!tma_res && lane == 0) tma_store_wait_read<0>();
           __syncwarp();
-          // 128-byte swizzle: 16-byte chunk g of row l lands at chunk g ^ (l % 8)
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            *reinterpret_cast<uint4*>(stg + lane * 128 + ((g ^ (lane & 7)) << 4)) =
-                f32_to_bf16x8(v + g * 8);
+          for (int g = 0; g < 8; ++g) {
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float v0, v1;
+              f2_unpack(v[k][g], v0, v1);
+              const __nv_bfloat162 p = __floats2bfloat162_rn(v0, v1);
+              o[k] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+            stmatrix_x4(srow + ((g ^ (lane & 7)) << 4), o);
+          }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmOut, stg, col0, m0 + q * 32);
+            tma_store_2d(&tmOut, stg, col0, m0);
             tma_store_commit();
           }
-        } else if (row_ok) {
-          __nv_bfloat16* op = args.out + (int64_t)row * args.ldo;
+        } else {
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (col0 + j < args.N) op[col0 + j] = __float2bfloat16_rn(v[j]);
+          for (int k = 0; k < 4; ++k) {
+            const int row = m0 + lr + 8 * k;
+            __nv_bfloat16* op = args.out + (int64_t)row * args.ldo + col0;
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              float v0, v1;
+              f2_unpack(v[k][g], v0, v1);
+              const int col = col0 + g * 8 + lc;
+              if (row < args.M && col < args.N) op[g * 8 + lc] = __float2bfloat16_rn(v0);
+              if (row < args.M && col + 1 < args.N) op[g * 8 + lc + 1] = __float2bfloat16_rn(v1);
+            }
+          }
+          if (tma_res) {  // the next residual load writes what this warp has read
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
         }
       }
     }
@@ -591,26 +789,35 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   using S = Shape<FMT, BN, EPI, PAIR>;
   const int64_t pitch = fp4::code_pitch(a.K);
   const int64_t tiles = fp4::scale_tiles(a.K, FMT);
-  CUtensorMap tmA, tmB, tmSfA, tmSfB, tmO;
+  CUtensorMap tmA, tmB, tmSfA, tmSfB, tmO, tmR;
   int rc = make_tmap_2d(&tmA, A.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)pitch,
                         (uint64_t)a.M, (uint64_t)pitch, kRowBytes, BM, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   rc = make_tmap_2d(&tmB, W.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)pitch, (uint64_t)a.N,
                     (uint64_t)pitch, kRowBytes, S::kRowsB, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  // scales as 32-bit words: a row of the map is one 128-row band, two tiles are 256 words
-  rc = make_tmap_2d(&tmSfA, A.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (uint64_t)tiles * 128,
-                    (uint64_t)((a.M + 127) / 128), (uint64_t)tiles * 512, 256, 1,
-                    CU_TENSOR_MAP_SWIZZLE_NONE);
+  // scales as 32-bit words of [band of 128 rows][tile][128 words]
+  rc = make_tmap_3d(&tmSfA, A.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 128, (uint64_t)tiles,
+                    (uint64_t)((a.M + 127) / 128), 512, (uint64_t)tiles * 512, 128, S::kTilesK, 1);
   if (rc) return rc;
-  rc = make_tmap_2d(&tmSfB, W.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (uint64_t)tiles * 128,
-                    (uint64_t)((a.N + 127) / 128), (uint64_t)tiles * 512, 256, S::kSfTilesB,
-                    CU_TENSOR_MAP_SWIZZLE_NONE);
+  rc = make_tmap_3d(&tmSfB, W.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 128, (uint64_t)tiles,
+                    (uint64_t)((a.N + 127) / 128), 512, (uint64_t)tiles * 512, 128, S::kTilesK,
+                    S::kSfTilesB);
   if (rc) return rc;
   tmO = tmA;  // unused unless tma_out
-  if (a.tma_out) {
+  if (EPI == kGeluMx) {
+    rc = make_tmap_2d(&tmO, a.hcodes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.hpitch,
+                      (uint64_t)a.M, (uint64_t)a.hpitch, 32, 32, CU_TENSOR_MAP_SWIZZLE_32B);
+    if (rc) return rc;
+  } else if (a.tma_out) {
     rc = make_tmap_2d(&tmO, a.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.N,
                       (uint64_t)a.M, (uint64_t)a.ldo * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  tmR = tmA;  // unused unless tma_res
+  if (a.tma_res) {
+    rc = make_tmap_2d(&tmR, a.res, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.N,
+                      (uint64_t)a.M, (uint64_t)a.ldr * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
   auto kern = fp4_gemm_kernel<FMT, BN, EPI, PAIR>;
@@ -657,7 +864,8 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   else
     grid = num < sm_count() ? num : sm_count();
   cfg.gridDim = dim3(grid);
-  FVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmSfA, tmSfB, tmO, a), "fp4 gemm launch");
+  FVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmSfA, tmSfB, tmO, tmR, a),
+               "fp4 gemm launch");
   return check_launch("fp4 gemm");
 }
 
@@ -729,7 +937,7 @@ int fvb_fp4_gemm(const void* A, const void* sfA, const float* rsA, int a_mode, c
   a.out = (__nv_bfloat16*)out;
   a.ldo = N;
   a.tma_out = aligned16(out) && N % 8 == 0;
-  a.vec_res = residual && aligned16(residual) && ldr % 8 == 0;
+  a.tma_res = residual && aligned16(residual) && ldr % 8 == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (residual) return gemm4::dispatch_fmt<gemm4::kResidual>(fmt, a, oa, ow, st);
   return gemm4::dispatch_fmt<gemm4::kPlain>(fmt, a, oa, ow, st);
