@@ -40,6 +40,14 @@ __device__ __forceinline__ int64_t scale_at(int64_t m, int64_t j, int64_t tiles)
   return ((m >> 7) * tiles + (j >> 2)) * 512 + (m & 31) * 16 + ((m & 127) >> 5) * 4 + (j & 3);
 }
 
+// max(m, |x.lo|, |x.hi|), a NaN if one is
+__device__ __forceinline__ float max_abs_nan(float m, uint64_t x) {
+  float a, b, r;
+  f2_unpack(x, a, b);
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
 // 8 fp32 -> 8 E2M1 codes (nearest even, saturating), element 0 in the low nibble
 __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
   uint32_t r;

@@ -212,14 +212,6 @@ __device__ __forceinline__ uint64_t gelu2(uint64_t x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
   return f2_mul(x, f2_pack(b * r, a * r));
 }
-// max(m, |x.lo|, |x.hi|), a NaN if one is
-__device__ __forceinline__ float max_abs_nan(float m, uint64_t x) {
-  float a, b, r;
-  f2_unpack(x, a, b);
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
-  return r;
-}
-
 // GELU and mx quantisation of an epilogue chunk (32 rows x 64 columns, v as in the kernel): the
 // codes into the staging buffer at shared address `stg` (32 rows x 32 bytes, 32-byte swizzle),
 // the two scale bytes of row lr + 8 k returned in sb[k] by every lane of the row.
@@ -248,7 +240,7 @@ __device__ __forceinline__ void gelu_mx(uint64_t (&v)[4][8], int col0, int N, in
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
       v[k][g] = gelu2(v[k][g]);
-      m[g >> 2] = max_abs_nan(m[g >> 2], v[k][g]);
+      m[g >> 2] = fp4::max_abs_nan(m[g >> 2], v[k][g]);
     }
     ex[k] = __byte_perm(__float_as_uint(m[0]) >> 23, __float_as_uint(m[1]) >> 23, 0x5410);
   }

@@ -8,9 +8,17 @@
 // loads and the stores is fp32: h is normed from x' before its rounding to bf16, and the codes
 // are those of h before its rounding, so nothing is rounded twice.
 //
-// HBM bounds it: x and y are read once, x' and h (or its codes) written once.  WPR warps own a
-// row and hold it in registers, thread t the 16-byte vectors t, t + 32 WPR, ...; statistics are
-// two-pass in registers (mean, then centred squares).
+// HBM bounds it: x and y are read once, x' and h (or its codes) written once, so what is spent
+// on an element has to stay near 15 instructions.  A block works on rows of one batch item and
+// folds the per-column operands into fp32 vectors in shared memory first:
+//   x' = rs * x + n1 * A1      A1 = gate * pw,  n1 = post norm of y
+//   h  = n2 * A2 + B2          A2 = w * (1 + scale), B2 = b * (1 + scale) + shift
+// (with a gate per row or a post-norm bias, A1 = pw and the other two are read as they are).
+// WPR warps own a row and hold it in registers as fp32 pairs, thread t the 16-byte vectors
+// t, t + 32 WPR, ...; statistics are two-pass in registers (mean, then centred squares); the
+// next row's loads go out as soon as the current row's registers are free.  Measured on
+// 2 x 8448 x 1536 (207 MB moved): 60 us with every operand unpacked for every row, see the
+// launch below for the present figure.
 #include "fp4.cuh"
 
 namespace fvb {
@@ -38,230 +46,331 @@ struct Args {
   uint8_t* scales;
   float* row_scale;
   int64_t pitch, tiles;
+  int64_t chunk;               // rows of a block
+  int blocks;                  // blocks of a batch item
 };
 
+// The row's threads: a warp, or WPR warps of the block meeting at named barrier 1 + team.
 template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  v = warp_sum(v);
-  if (WPR > 1) {
-    __syncthreads();  // the last reduction's readers are done with red
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < WPR; ++i) v += red[i];
-  }
-  return v;
+__device__ __forceinline__ void team_sync(int team) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * WPR) : "memory");
 }
-template <int WPR>
-__device__ __forceinline__ float row_max(float v, float* red) {
-  v = warp_max(v);
-  if (WPR > 1) {
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
+template <int WPR, typename Op>
+__device__ __forceinline__ float team_reduce(float v, float* red, int team, Op op) {
 #pragma unroll
-    for (int i = 0; i < WPR; ++i) v = fmaxf(v, red[i]);
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (WPR > 1) {
+    const int w = (threadIdx.x >> 5) % WPR;
+    team_sync<WPR>(team);  // the last reduction's readers are done
+    if ((threadIdx.x & 31) == 0) red[w] = v;
+    team_sync<WPR>(team);
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < WPR; ++i) v = op(v, red[i]);
   }
   return v;
 }
 
-__device__ __forceinline__ void ld8(const __nv_bfloat16* p, int v, float* f) {
-  bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(p) + v), f);
+__device__ __forceinline__ void unpack8(const uint4& u, uint64_t* f) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    f[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint4 pack8(const uint64_t* f) {
+  uint4 u;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    f2_unpack(f[i], a, b);
+    h[i] = __floats2bfloat162_rn(a, b);
+  }
+  return u;
 }
 
-// f <- the row normed: (f - mean) * rsqrt(mean of squares + eps); kRms: no mean.
-// Vectors past the row hold zeros and stay zeros.
-template <int NV, int WPR>
-__device__ __forceinline__ void norm_row(float (*f)[8], int t, int nvec, int D, int kind, float eps,
-                                         float* red) {
+// normed = f * scale + off (a pair each, the same in both halves): (f - mean) * rstd.  kRms has
+// mean 0, kNone is the identity.  Vectors past the row hold zeros and count for nothing.
+template <int NV, int WPR, bool FULL>
+__device__ __forceinline__ void row_norm(const uint64_t (*f)[4], int t, int nvec, float dim, int kind,
+                                         float eps, float* red, int team, uint64_t& scale,
+                                         uint64_t& off) {
+  const auto add = [](float a, float b) { return a + b; };
+  float a, b, mean = 0.f;
+  if (kind == kNone) {
+    scale = f2_pack(1.f, 1.f);
+    off = f2_pack(0.f, 0.f);
+    return;
+  }
   if (kind == kLayer) {
-    float s = 0.f;
+    uint64_t s2 = f2_pack(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += f[j][i];
+      for (int i = 0; i < 4; ++i) s2 = f2_add(s2, f[j][i]);
+    f2_unpack(s2, a, b);
     // a true quotient: the mean of a constant row is that constant, so its variance is 0
-    const float mean = __fdiv_rn(row_sum<WPR>(s, red), (float)D);
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (t + j * 32 * WPR < nvec) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] -= mean;
-      }
+    mean = __fdiv_rn(team_reduce<WPR>(a + b, red, team, add), dim);
   }
-  float q = 0.f;
+  const uint64_t nm = f2_pack(-mean, -mean);
+  uint64_t q2 = f2_pack(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
+    if (FULL || t + j * 32 * WPR < nvec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q = __fmaf_rn(f[j][i], f[j][i], q);
-  const float r = rsqrtf(__fdiv_rn(row_sum<WPR>(q, red), (float)D) + eps);
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[j][i] *= r;
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t d = f2_add(f[j][i], nm);
+        q2 = f2_fma(d, d, q2);
+      }
+    }
+  f2_unpack(q2, a, b);
+  const float r = rsqrtf(__fdiv_rn(team_reduce<WPR>(a + b, red, team, add), dim) + eps);
+  scale = f2_pack(r, r);
+  off = nm;
 }
 
-template <int NV, int WPR>
-__global__ void __launch_bounds__(WPR == 1 ? 256 : 32 * WPR) residual_norm_kernel(const Args a) {
-  constexpr int T = 32 * WPR;
-  __shared__ float red[WPR];
-  const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-  if (row >= a.rows) return;  // whole warps; with WPR > 1 the grid has exactly the rows
-  const int t = WPR == 1 ? threadIdx.x & 31 : threadIdx.x;
+// EXTRA: a gate per row or a post-norm bias.  FMT: format of the emitted codes, 0 for none.
+// FULL: the row fills every thread's NV vectors.
+template <int NV, int WPR, bool FULL, bool EXTRA, int FMT>
+__global__ void __launch_bounds__(256, NV == 8 ? 1 : 2) residual_norm_kernel(const Args a) {
+  constexpr int T = 32 * WPR, TEAMS = 8 / WPR;
+  // A1, A2, B2: for each first the lower, then the upper four floats of every vector, so that a
+  // warp's 16-byte reads fall on all banks
+  extern __shared__ float4 cols[];
+  __shared__ float red_all[8];
+  const int team = WPR == 1 ? threadIdx.x >> 5 : threadIdx.x / T;
+  const int t = threadIdx.x % T;
+  float* red = red_all + team * WPR;
   const int nvec = a.D >> 3;
-  const int64_t bi = row / a.L;
-  const uint4* xr = reinterpret_cast<const uint4*>(a.x + row * a.D);
-  const uint4* yr = reinterpret_cast<const uint4*>(a.y + row * a.D);
+  // the block's rows: [first, last) of batch item bi, dealt to the teams in turn
+  const int64_t bi = blockIdx.x / a.blocks;
+  const int64_t first = bi * a.L + (int64_t)(blockIdx.x % a.blocks) * a.chunk;
+  const int64_t end = (bi + 1) * a.L;
+  const int64_t last = first + a.chunk < end ? first + a.chunk : end;
+  int64_t row = first + team;
+
   uint4 xv[NV], yv[NV];
+  auto load = [&](uint4* v, const __nv_bfloat16* p, int64_t r) {
+    const uint4* src = reinterpret_cast<const uint4*>(p + r * a.D);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = t + j * T;
-    yv[j] = v < nvec ? ld_stream(yr + v) : make_uint4(0u, 0u, 0u, 0u);
-  }
+    for (int j = 0; j < NV; ++j)
+      v[j] = r < last && (FULL || t + j * T < nvec) ? ld_stream(src + t + j * T)
+                                                    : make_uint4(0u, 0u, 0u, 0u);
+  };
+  load(yv, a.y, row);
+  load(xv, a.x, row);
+
+  for (int v = threadIdx.x; v < nvec; v += 256) {
+    float p[8], q[8], s[8], sh[8];
+    auto get = [&](const __nv_bfloat16* src, float* d, float fill) {
+      if (src) {
+        bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(src) + v), d);
+      } else {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = t + j * T;
-    xv[j] = v < nvec ? ld_stream(xr + v) : make_uint4(0u, 0u, 0u, 0u);
-  }
-  float f[NV][8];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) bf16x8_to_f32(yv[j], f[j]);
-  if (a.post != kNone) norm_row<NV, WPR>(f, t, nvec, a.D, a.post, a.post_eps, red);
-  const __nv_bfloat16* gate = a.gate ? a.gate + (a.gate_rows ? row : bi) * a.D : nullptr;
-  uint4* xo = reinterpret_cast<uint4*>(a.x_out + row * a.D);
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = t + j * T;
-    if (v < nvec) {
-      float p[8], x[8];
-      if (a.pw) {
-        ld8(a.pw, v, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] *= p[i];
+        for (int i = 0; i < 8; ++i) d[i] = fill;
       }
-      if (a.pb) {
-        ld8(a.pb, v, p);
+    };
+    auto put = [&](int k, const float* d) {
+      cols[2 * k * nvec + v] = make_float4(d[0], d[1], d[2], d[3]);
+      cols[(2 * k + 1) * nvec + v] = make_float4(d[4], d[5], d[6], d[7]);
+    };
+    get(!EXTRA && a.gate ? a.gate + bi * a.D : nullptr, s, 1.f);
+    get(a.pw, p, 1.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] += p[i];
-      }
-      if (gate) {
-        ld8(gate, v, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] *= p[i];
-      }
-      bf16x8_to_f32(xv[j], x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[j][i] = __fmaf_rn(a.rs, x[i], f[j][i]);
-      xo[v] = f32_to_bf16x8(f[j]);
-    }
-  }
-  norm_row<NV, WPR>(f, t, nvec, a.D, a.norm, a.eps, red);
-  const __nv_bfloat16* scale = a.scale ? a.scale + bi * a.D : nullptr;
-  const __nv_bfloat16* shift = a.shift ? a.shift + bi * a.D : nullptr;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = t + j * T;
-    if (v < nvec) {
-      float p[8];
-      if (a.w) {
-        ld8(a.w, v, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] *= p[i];
-      }
-      if (a.b) {
-        ld8(a.b, v, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] += p[i];
-      }
-      if (scale) {
-        ld8(scale, v, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] *= 1.0f + p[i];
-      }
-      if (shift) {
-        ld8(shift, v, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] += p[i];
-      }
-      if (a.out) reinterpret_cast<uint4*>(a.out + row * a.D)[v] = f32_to_bf16x8(f[j]);
-    }
-  }
-  if (a.fmt == 0) return;
-  // 4-bit codes: a block is 2 (nv) or 4 (mx) neighbouring lanes' vectors
-  float am[NV];
-  uint32_t bad = 0u;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    float m = 0.f;
-    bool nf = false;
+    for (int i = 0; i < 8; ++i) p[i] *= s[i];
+    put(0, p);
+    get(a.scale ? a.scale + bi * a.D : nullptr, s, 0.f);
+    get(a.w, p, 1.f);
+    get(a.b, q, 0.f);
+    get(a.shift ? a.shift + bi * a.D : nullptr, sh, 0.f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float v = fabsf(f[j][i]);
-      nf |= !(v < INFINITY);
-      if (v < INFINITY) m = fmaxf(m, v);
+      const float m = 1.0f + s[i];
+      p[i] *= m;
+      q[i] = __fmaf_rn(q[i], m, sh[i]);
     }
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    nf = __shfl_xor_sync(0xffffffffu, (int)nf, 1) || nf;
-    if (a.fmt == FVB_FP4_MX) {
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      nf = __shfl_xor_sync(0xffffffffu, (int)nf, 2) || nf;
-    }
-    am[j] = m;
-    bad |= (uint32_t)nf << j;
+    put(1, p);
+    put(2, q);
   }
-  float rs = 1.f, ik = 1.f;
-  if (a.fmt == FVB_FP4_NV) {
-    float top = 0.f;
+  __syncthreads();
+  auto column = [&](int k, int v, uint64_t* d) {  // vector v of column operand k, as pairs
+    const float4 u = cols[2 * k * nvec + v], w = cols[(2 * k + 1) * nvec + v];
+    d[0] = f2_pack(u.x, u.y);
+    d[1] = f2_pack(u.z, u.w);
+    d[2] = f2_pack(w.x, w.y);
+    d[3] = f2_pack(w.z, w.w);
+  };
+
+  const uint64_t rs2 = f2_pack(a.rs, a.rs);
+  const float dim = (float)a.D;
+  for (; row < last; row += TEAMS) {
+    uint64_t f[NV][4], sc, of;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) top = fmaxf(top, am[j]);
-    const int k = fp4::row_exponent(row_max<WPR>(top, red));
-    rs = fp4::pow2i(k);
-    ik = fp4::pow2i(-k);
-    if (t == 0) a.row_scale[row] = rs;
-  }
-  const int npad = (int)(a.tiles * (a.fmt == FVB_FP4_NV ? 8 : 16));  // vectors under the scale tiles
+    for (int j = 0; j < NV; ++j) unpack8(yv[j], f[j]);
+    load(yv, a.y, row + TEAMS);
+    row_norm<NV, WPR, FULL>(f, t, nvec, dim, a.post, a.post_eps, red, team, sc, of);
+    uint4* xo = reinterpret_cast<uint4*>(a.x_out + row * a.D);
 #pragma unroll
-  for (int j = 0; j < NV + 1; ++j) {
-    // one more turn than the registers hold: the padding of the last scale tile may start
-    // past the row's last vector
-    const int v = t + j * T;
-    if (v >= npad) break;
-    const bool nf = j < NV && ((bad >> j) & 1u);
-    float q[8];
-    uint32_t byte;
-    if (a.fmt == FVB_FP4_NV) {
-      byte = j < NV ? fp4::nv_scale(am[j < NV ? j : 0], ik) : 0u;
-      const float d = fp4::e4m3_value(byte) * rs;
-      const float r = __frcp_rn(d);
+    for (int j = 0; j < NV; ++j) {
+      const int v = t + j * T;
+      if (FULL || v < nvec) {
+        uint64_t x[4], c[4], pb[4], g[4];
+        unpack8(xv[j], x);
+        column(0, v, c);
+        if (EXTRA) {
+          const int64_t gr = a.gate_rows ? row : bi;
+          if (a.pb) unpack8(__ldg(reinterpret_cast<const uint4*>(a.pb) + v), pb);
+          if (a.gate) unpack8(__ldg(reinterpret_cast<const uint4*>(a.gate + gr * a.D) + v), g);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float h = j < NV ? f[j < NV ? j : 0][i] : 0.f;
-        q[i] = byte == 0u ? 0.f * h : fp4::quotient(h, d, r);
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t n = f2_mul(f2_add(f[j][i], of), sc);
+          if (EXTRA) {
+            const uint64_t z = a.pb ? f2_fma(n, c[i], pb[i]) : f2_mul(n, c[i]);
+            const uint64_t y = f2_mul(rs2, x[i]);
+            f[j][i] = a.gate ? f2_fma(z, g[i], y) : f2_add(z, y);
+          } else {
+            f[j][i] = f2_fma(n, c[i], f2_mul(rs2, x[i]));
+          }
+        }
+        xo[v] = pack8(f[j]);
       }
-    } else {
-      const int e = j < NV ? fp4::mx_exponent(am[j < NV ? j : 0]) : -127;
-      byte = (uint32_t)(e + 127);
-      const float r = fp4::pow2i(-e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = (j < NV ? f[j < NV ? j : 0][i] : 0.f) * r;
     }
-    if (v * 4 < a.pitch)
-      *reinterpret_cast<uint32_t*>(a.codes + row * a.pitch + v * 4) = nf ? 0u : fp4::e2m1x8(q);
-    if (a.fmt == FVB_FP4_NV) {
-      if ((t & 1) == 0) a.scales[fp4::scale_at(row, v >> 1, a.tiles)] = (uint8_t)(nf ? 0x7Fu : byte);
-    } else {
-      if ((t & 3) == 0) a.scales[fp4::scale_at(row, v >> 2, a.tiles)] = (uint8_t)(nf ? 0xFFu : byte);
+    load(xv, a.x, row + TEAMS);
+    row_norm<NV, WPR, FULL>(f, t, nvec, dim, a.norm, a.eps, red, team, sc, of);
+    uint4* ho = reinterpret_cast<uint4*>(a.out + row * a.D);
+    float am[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int v = t + j * T;
+      am[j] = 0.f;
+      if (FULL || v < nvec) {
+        uint64_t c1[4], c2[4];
+        column(1, v, c1);
+        column(2, v, c2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[j][i] = f2_fma(f2_mul(f2_add(f[j][i], of), sc), c1[i], c2[i]);
+          if (FMT) am[j] = fp4::max_abs_nan(am[j], f[j][i]);
+        }
+        if (a.out) ho[v] = pack8(f[j]);
+      }
+    }
+    if (FMT == 0) continue;
+    // 4-bit codes: a block is 2 (nv) or 4 (mx) neighbouring lanes' vectors.  The whole warp
+    // takes every turn (shuffles); one more than the registers hold, since the padding of the
+    // last scale tile may start past the row's last vector
+    const auto mx = [](float x, float y) { return fmaxf(x, y); };
+    uint32_t bad = 0u;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint32_t any = __ballot_sync(0xffffffffu, !(am[j] < INFINITY));
+      if (any) {  // a block with a non-finite value: NaN scale, its finite values still count
+        const uint32_t mine = FMT == FVB_FP4_NV ? 3u << (t & 30) : 15u << (t & 28);
+        if (any & mine) bad |= 1u << j;
+        if (!(am[j] < INFINITY)) {
+          am[j] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float u, w;
+            f2_unpack(f[j][i], u, w);
+            if (fabsf(u) < INFINITY) am[j] = fmaxf(am[j], fabsf(u));
+            if (fabsf(w) < INFINITY) am[j] = fmaxf(am[j], fabsf(w));
+          }
+        }
+      }
+      am[j] = fmaxf(am[j], __shfl_xor_sync(0xffffffffu, am[j], 1));
+      if (FMT == FVB_FP4_MX) am[j] = fmaxf(am[j], __shfl_xor_sync(0xffffffffu, am[j], 2));
+    }
+    float rs = 1.f, ik = 1.f;
+    if (FMT == FVB_FP4_NV) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) top = fmaxf(top, am[j]);
+      const int k = fp4::row_exponent(team_reduce<WPR>(top, red, team, mx));
+      rs = fp4::pow2i(k);
+      ik = fp4::pow2i(-k);
+      if (t == 0) a.row_scale[row] = rs;
+    }
+    const int npad = (int)(a.tiles * (FMT == FVB_FP4_NV ? 8 : 16));  // vectors under the scale tiles
+    uint32_t* cp = reinterpret_cast<uint32_t*>(a.codes + row * a.pitch);
+    // scale_at(row, j): a thread's blocks of successive turns are whole tiles apart
+    constexpr int PER = FMT == FVB_FP4_NV ? 2 : 4;  // vectors per block
+    uint8_t* sp = a.scales + fp4::scale_at(row, t / PER, a.tiles);
+#pragma unroll
+    for (int j = 0; j < NV + 1; ++j) {
+      const int v = t + j * T;
+      if (v >= npad) break;
+      uint32_t byte = 0u, code = 0u;
+      if (j < NV) {
+        constexpr int last_j = NV - 1;
+        const int jj = j < NV ? j : last_j;
+        float r;
+        if (FMT == FVB_FP4_NV) {
+          byte = fp4::nv_scale(am[jj], ik);
+          // the codes are h's to the last bit of its own fp32 rounding: a product will do
+          r = byte == 0u ? 0.f : __frcp_rn(fp4::e4m3_value(byte) * rs);
+        } else {
+          const int e = fp4::mx_exponent(am[jj]);
+          byte = (uint32_t)(e + 127);
+          r = fp4::pow2i(-e);
+        }
+        const uint64_t r2 = f2_pack(r, r);
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f[jj][i], r2), q[2 * i], q[2 * i + 1]);
+        code = fp4::e2m1x8(q);
+        if ((bad >> jj) & 1u) {
+          code = 0u;
+          byte = FMT == FVB_FP4_NV ? 0x7Fu : 0xFFu;
+        }
+        if (!FULL && v >= nvec) code = byte = 0u;
+      }
+      if (v * 4 < a.pitch) cp[v] = code;
+      if (t % PER == 0) sp[(int64_t)j * (T / PER / 4) * 512] = (uint8_t)byte;
     }
   }
 }
 
-template <int NV, int WPR>
-static int launch(const Args& a, cudaStream_t st) {
-  const unsigned grid = (unsigned)(WPR == 1 ? (a.rows + 7) / 8 : a.rows);
-  residual_norm_kernel<NV, WPR><<<grid, WPR == 1 ? 256 : 32 * WPR, 0, st>>>(a);
+template <int NV, int WPR, bool FULL, bool EXTRA, int FMT>
+static int launch_as(Args a, int64_t B, cudaStream_t st) {
+  auto kern = residual_norm_kernel<NV, WPR, FULL, EXTRA, FMT>;
+  const size_t smem = (size_t)3 * a.D * 4;
+  static size_t set[64] = {0};
+  int dev = 0;
+  FVB_CUDA_TRY(cudaGetDevice(&dev), "fvb_residual_norm device");
+  FVB_REQUIRE(dev >= 0 && dev < 64, "fvb_residual_norm: device ordinal %d", dev);
+  if (smem > 48 * 1024 && smem > set[dev]) {
+    FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                 "fvb_residual_norm smem attribute");
+    set[dev] = smem;
+  }
+  // two blocks per SM, rows split evenly; no block without a row for each of its teams if
+  // there are enough
+  constexpr int TEAMS = 8 / WPR;
+  int64_t blocks = (2 * (int64_t)sm_count() + B - 1) / B;
+  const int64_t most = (a.L + TEAMS - 1) / TEAMS;
+  if (blocks > most) blocks = most;
+  a.chunk = (a.L + blocks - 1) / blocks;
+  blocks = (a.L + a.chunk - 1) / a.chunk;
+  a.blocks = (int)blocks;
+  FVB_REQUIRE(blocks * B < (1ll << 31), "fvb_residual_norm: batch");
+  kern<<<(unsigned)(blocks * B), 256, smem, st>>>(a);
   return check_launch("fvb_residual_norm");
+}
+
+template <int NV, int WPR>
+static int launch(const Args& a, int64_t B, cudaStream_t st) {
+  const bool full = a.D == NV * WPR * 256, extra = a.gate_rows || a.pb;
+#define FVB_RN(FULL, EXTRA)                                                     \
+  return a.fmt == 0 ? launch_as<NV, WPR, FULL, EXTRA, 0>(a, B, st)              \
+                    : a.fmt == FVB_FP4_NV ? launch_as<NV, WPR, FULL, EXTRA, FVB_FP4_NV>(a, B, st) \
+                                          : launch_as<NV, WPR, FULL, EXTRA, FVB_FP4_MX>(a, B, st)
+  if (full && extra) FVB_RN(true, true);
+  if (full) FVB_RN(true, false);
+  if (extra) FVB_RN(false, true);
+  FVB_RN(false, false);
+#undef FVB_RN
 }
 
 }  // namespace resnorm
@@ -294,7 +403,7 @@ extern "C" int fvb_residual_norm(const void* x, const void* y, const void* gate,
   a.x = (const __nv_bfloat16*)x;
   a.y = (const __nv_bfloat16*)y;
   a.gate = (const __nv_bfloat16*)gate;
-  a.gate_rows = gate_rows;
+  a.gate_rows = gate && gate_rows;
   a.pw = (const __nv_bfloat16*)post_w;
   a.pb = (const __nv_bfloat16*)post_b;
   a.w = (const __nv_bfloat16*)w;
@@ -318,12 +427,12 @@ extern "C" int fvb_residual_norm(const void* x, const void* y, const void* gate,
   a.pitch = fp4::code_pitch(D);
   a.tiles = fmt ? fp4::scale_tiles(D, fmt) : 0;
   cudaStream_t st = (cudaStream_t)stream;
-  if (D <= 256) return resnorm::launch<1, 1>(a, st);
-  if (D <= 512) return resnorm::launch<2, 1>(a, st);
-  if (D <= 1024) return resnorm::launch<4, 1>(a, st);
-  if (D <= 1536) return resnorm::launch<6, 1>(a, st);
-  if (D <= 2048) return resnorm::launch<2, 4>(a, st);
-  if (D <= 4096) return resnorm::launch<4, 4>(a, st);
-  if (D <= 8192) return resnorm::launch<4, 8>(a, st);
-  return resnorm::launch<8, 8>(a, st);
+  if (D <= 256) return resnorm::launch<1, 1>(a, B, st);
+  if (D <= 512) return resnorm::launch<2, 1>(a, B, st);
+  if (D <= 1024) return resnorm::launch<4, 1>(a, B, st);
+  if (D <= 1536) return resnorm::launch<6, 1>(a, B, st);
+  if (D <= 2048) return resnorm::launch<4, 2>(a, B, st);
+  if (D <= 4096) return resnorm::launch<4, 4>(a, B, st);
+  if (D <= 8192) return resnorm::launch<4, 8>(a, B, st);
+  return resnorm::launch<8, 8>(a, B, st);
 }
