@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .fp4_quant import _FMTS, FP4Tensor, fp4_format, quantize_fp4
+from .fp4_quant import _FMTS, FP4Tensor, fp4_format, quantize_fp4, require_cuda
 
 
 def _vector(t, n, what, device):
@@ -62,15 +62,15 @@ def fp4_mm(a: FP4Tensor, w: FP4Tensor, bias: torch.Tensor | None = None,
     a [M, K] and w [N, K] of the same format; bias and gate [N], residual [M, N].  fp32 sums
     and epilogue, one rounding.  out (contiguous [M, N]) may be the residual.
     """
-    _lib.require_cuda(a.codes, w.codes)
+    require_cuda(a)
     M, K = a.shape
     N = w.shape[0]
-    dev = a.codes.device
+    dev = a.device
     if a.fmt != w.fmt:
         raise ValueError(f"fp4_mm: formats differ ({a.fmt} x {w.fmt})")
     if w.shape[1] != K:
         raise ValueError(f"fp4_mm: K mismatch {a.shape} x {w.shape}")
-    if w.codes.device != dev:
+    if w.device != dev:
         raise ValueError("fp4_mm: operands are on different devices")
     if gate is not None and residual is None:
         raise ValueError("fp4_mm: gate needs a residual")
@@ -78,10 +78,10 @@ def fp4_mm(a: FP4Tensor, w: FP4Tensor, bias: torch.Tensor | None = None,
     gate = _vector(gate, N, "fp4_mm: gate", dev)
     residual, ldr = _residual(residual, M, N, "fp4_mm", dev)
     out = _out(out, M, N, "fp4_mm", dev)
-    _lib.call("fvb_fp4_gemm", a.codes.data_ptr(), a.scales.data_ptr(), _lib.ptr(a.row_scale),
-              a.row_mode(), w.codes.data_ptr(), w.scales.data_ptr(), _lib.ptr(w.row_scale),
-              w.row_mode(), _FMTS[a.fmt], _lib.ptr(bias), _lib.ptr(residual), ldr, _lib.ptr(gate),
-              M, N, K, out.data_ptr(), _lib.stream_of(out))
+    ptr = _lib.ptr
+    _lib.call("fvb_fp4_gemm", a.codes_ptr, a.scales_ptr, a.row_scale_ptr, a._row_mode, w.codes_ptr,
+              w.scales_ptr, w.row_scale_ptr, w._row_mode, _FMTS[a.fmt], ptr(bias), ptr(residual),
+              ldr, ptr(gate), M, N, K, out.data_ptr(), _lib.stream_of(out))
     return out
 
 
@@ -96,17 +96,17 @@ def ffn_fp4(a: FP4Tensor, w0: FP4Tensor, b0: torch.Tensor | None, w2: FP4Tensor,
     blocks need nothing of the rest of their row, so the first product writes them itself).
     workspace: uint8, at least fvb_fp4_ffn_workspace_bytes(M, F), 256-byte aligned.
     """
-    _lib.require_cuda(a.codes, w0.codes, w2.codes)
+    require_cuda(a)
     M, D = a.shape
     F, N = w0.shape[0], w2.shape[0]
-    dev = a.codes.device
+    dev = a.device
     if a.fmt != w0.fmt:
         raise ValueError(f"ffn_fp4: formats differ ({a.fmt} x {w0.fmt})")
     if w2.fmt != "mx":
         raise ValueError("ffn_fp4: w2 must be mx, the hidden state's format")
     if w0.shape[1] != D or w2.shape[1] != F:
         raise ValueError(f"ffn_fp4: shapes {a.shape}, {w0.shape}, {w2.shape} do not chain")
-    if w0.codes.device != dev or w2.codes.device != dev:
+    if w0.device != dev or w2.device != dev:
         raise ValueError("ffn_fp4: operands are on different devices")
     if gate is not None and residual is None:
         raise ValueError("ffn_fp4: gate needs a residual")
@@ -120,10 +120,10 @@ def ffn_fp4(a: FP4Tensor, w0: FP4Tensor, b0: torch.Tensor | None, w2: FP4Tensor,
         workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
     elif workspace.numel() * workspace.element_size() < need or workspace.device != dev:
         raise ValueError(f"ffn_fp4: workspace needs {need} bytes on {dev}")
-    _lib.call("fvb_fp4_ffn", a.codes.data_ptr(), a.scales.data_ptr(), _lib.ptr(a.row_scale),
-              a.row_mode(), w0.codes.data_ptr(), w0.scales.data_ptr(), _lib.ptr(w0.row_scale),
-              w0.row_mode(), _FMTS[a.fmt], _lib.ptr(b0), w2.codes.data_ptr(), w2.scales.data_ptr(),
-              _lib.ptr(b2), _lib.ptr(residual), ldr, _lib.ptr(gate), M, D, F, N, out.data_ptr(),
+    ptr = _lib.ptr
+    _lib.call("fvb_fp4_ffn", a.codes_ptr, a.scales_ptr, a.row_scale_ptr, a._row_mode, w0.codes_ptr,
+              w0.scales_ptr, w0.row_scale_ptr, w0._row_mode, _FMTS[a.fmt], ptr(b0), w2.codes_ptr,
+              w2.scales_ptr, ptr(b2), ptr(residual), ldr, ptr(gate), M, D, F, N, out.data_ptr(),
               workspace.data_ptr(), _lib.stream_of(out))
     return out
 
@@ -138,9 +138,10 @@ class FP4Linear(nn.Module):
         self.in_features = linear.in_features
         self.out_features = linear.out_features
         q = quantize_fp4(linear.weight.detach(), fmt)
-        self.weight = nn.Parameter(q.codes, requires_grad=False)
-        self.register_buffer("w_scales", q.scales, persistent=False)
-        self.register_buffer("w_row_scale", q.row_scale, persistent=False)
+        self.weight = nn.Parameter(q.codes.clone(), requires_grad=False)
+        self.register_buffer("w_scales", q.scales.clone(), persistent=False)
+        self.register_buffer("w_row_scale", None if fmt == "mx" else q.row_scale.clone(),
+                             persistent=False)
         if linear.bias is not None:
             self.bias = nn.Parameter(linear.bias.detach().to(torch.bfloat16).clone(),
                                      requires_grad=False)

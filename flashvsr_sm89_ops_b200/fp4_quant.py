@@ -48,7 +48,8 @@ class FP4Tensor:
     shape      (M, K);  fmt  "nv" or "mx"
     """
 
-    __slots__ = ("codes", "scales", "row_scale", "shape", "fmt")
+    __slots__ = ("shape", "fmt", "device", "_row_mode", "codes_ptr", "scales_ptr", "row_scale_ptr",
+                 "_buf", "_codes", "_scales", "_row_scale")
 
     def __init__(self, codes, scales, row_scale, shape, fmt):
         code = fp4_format(fmt)
@@ -62,46 +63,84 @@ class FP4Tensor:
         if scales.dtype != torch.uint8 or scales.numel() != tiles * 512 or not scales.is_contiguous():
             raise ValueError(f"FP4Tensor: scales must be contiguous uint8 of {tiles * 512} bytes, "
                              f"got {scales.dtype} {tuple(scales.shape)}")
+        device = codes.device
+        rows = 0
         if code == _lib.FVB_FP4_MX:
             if row_scale is not None:
                 raise ValueError("FP4Tensor: mx has no row_scale")
-        elif row_scale is not None and (row_scale.dtype != torch.float32
-                                        or row_scale.numel() not in (1, M)
-                                        or not row_scale.is_contiguous()):
-            raise ValueError("FP4Tensor: row_scale must be contiguous fp32 with 1 or M entries")
-        if scales.device != codes.device or (row_scale is not None
-                                             and row_scale.device != codes.device):
+        elif row_scale is not None:
+            rows = row_scale.numel()
+            if row_scale.dtype != torch.float32 or rows not in (1, M) \
+                    or not row_scale.is_contiguous():
+                raise ValueError("FP4Tensor: row_scale must be contiguous fp32 with 1 or M entries")
+            if row_scale.device != device:
+                raise ValueError("FP4Tensor: codes, scales and row_scale must be on one device")
+        if scales.device != device:
             raise ValueError("FP4Tensor: codes, scales and row_scale must be on one device")
-        self.codes = codes
-        self.scales = scales
-        self.row_scale = row_scale
+        self._codes, self._scales, self._row_scale, self._buf = codes, scales, row_scale, None
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+        self.row_scale_ptr = None if row_scale is None else row_scale.data_ptr()
+        self._row_mode = _lib.FVB_SCALE_ROW if rows and rows == M else _lib.FVB_SCALE_TENSOR
         self.shape = (M, K)
         self.fmt = fmt
+        self.device = device
+
+    # the buffers of a tensor the library made lie in one allocation and become tensors when
+    # they are asked for
+    @property
+    def codes(self):
+        if self._codes is None:
+            M, K = self.shape
+            pitch = (K + 31) // 32 * 16
+            self._codes = self._buf[:M * pitch].view(M, pitch)
+        return self._codes
 
     @property
-    def device(self):
-        return self.codes.device
+    def scales(self):
+        if self._scales is None:
+            a = self.scales_ptr - self._buf.data_ptr()
+            per = 4 * _BLOCK[self.fmt]
+            n = (self.shape[0] + 127) // 128 * ((self.shape[1] + per - 1) // per) * 512
+            self._scales = self._buf[a:a + n]
+        return self._scales
+
+    @property
+    def row_scale(self):
+        if self._row_scale is None and self._buf is not None and self.fmt == "nv":
+            a = self.row_scale_ptr - self._buf.data_ptr()
+            self._row_scale = self._buf[a:a + 4 * self.shape[0]].view(torch.float32)
+        return self._row_scale
 
     def row_mode(self) -> int:
-        rs = self.row_scale
-        return _lib.FVB_SCALE_ROW if rs is not None and rs.numel() == self.shape[0] \
-            else _lib.FVB_SCALE_TENSOR
+        """FVB_SCALE_ROW for one row scale a row, else FVB_SCALE_TENSOR."""
+        return self._row_mode
 
     def __repr__(self):
-        return f"FP4Tensor({self.fmt}, shape={self.shape}, device={self.codes.device})"
+        return f"FP4Tensor({self.fmt}, shape={self.shape}, device={self.device})"
 
 
 def _empty(M: int, K: int, fmt: str, device) -> FP4Tensor:
-    """An FP4Tensor of uninitialised buffers."""
+    """An FP4Tensor of uninitialised buffers in one allocation (three cost 5 us more)."""
     t = FP4Tensor.__new__(FP4Tensor)
     per = 4 * _BLOCK[fmt]
-    t.codes = torch.empty((M, (K + 31) // 32 * 16), dtype=torch.uint8, device=device)
-    t.scales = torch.empty((M + 127) // 128 * ((K + per - 1) // per) * 512, dtype=torch.uint8,
-                           device=device)
-    t.row_scale = torch.empty(M, dtype=torch.float32, device=device) if fmt == "nv" else None
+    scales = (M * ((K + 31) // 32 * 16) + 511) // 512 * 512
+    rows = scales + (M + 127) // 128 * ((K + per - 1) // per) * 512
+    nv = fmt == "nv"
+    buf = torch.empty(rows + 4 * M if nv else rows, dtype=torch.uint8, device=device)
+    base = buf.data_ptr()
+    t._buf, t._codes, t._scales, t._row_scale = buf, None, None, None
+    t.codes_ptr, t.scales_ptr = base, base + scales
+    t.row_scale_ptr = base + rows if nv else None
+    t._row_mode = _lib.FVB_SCALE_ROW if nv and M else _lib.FVB_SCALE_TENSOR
     t.shape = (M, K)
     t.fmt = fmt
+    t.device = buf.device
     return t
+
+
+def require_cuda(q: FP4Tensor):
+    if q.device.type != "cuda":
+        _lib.require_cuda(q.codes)
 
 
 def quantize_fp4(x2: torch.Tensor, fmt: str = "nv") -> FP4Tensor:
@@ -120,17 +159,17 @@ def quantize_fp4(x2: torch.Tensor, fmt: str = "nv") -> FP4Tensor:
         x2 = x2.contiguous()
     q = _empty(M, K, fmt, x2.device)
     _lib.call("fvb_quant_fp4", x2.data_ptr(), dt, x2.stride(0) if M > 1 else K, M, K, code,
-              q.codes.data_ptr(), q.scales.data_ptr(), _lib.ptr(q.row_scale), _lib.stream_of(x2))
+              q.codes_ptr, q.scales_ptr, q.row_scale_ptr, _lib.stream_of(x2))
     return q
 
 
 def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values an FP4Tensor stands for, [M, K]; one rounding to `dtype` (none for codes of
     quantize_fp4 in bf16 or fp32: they hold a code times a scale exactly)."""
-    _lib.require_cuda(q.codes)
+    require_cuda(q)
     dt = _dtype_code(dtype, "dequantize_fp4")
     M, K = q.shape
-    out = torch.empty((M, K), dtype=dtype, device=q.codes.device)
-    _lib.call("fvb_dequant_fp4", q.codes.data_ptr(), q.scales.data_ptr(), _lib.ptr(q.row_scale),
-              q.row_mode(), M, K, _FMTS[q.fmt], dt, out.data_ptr(), _lib.stream_of(out))
+    out = torch.empty((M, K), dtype=dtype, device=q.device)
+    _lib.call("fvb_dequant_fp4", q.codes_ptr, q.scales_ptr, q.row_scale_ptr, q._row_mode, M, K,
+              _FMTS[q.fmt], dt, out.data_ptr(), _lib.stream_of(out))
     return out

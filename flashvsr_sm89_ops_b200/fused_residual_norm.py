@@ -83,6 +83,6 @@ def fused_residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor 
               _NORMS[post_norm], p(post_weight), p(post_bias),
               float(eps if post_eps is None else post_eps), _NORMS[norm], p(weight), p(bias),
               p(scale), p(shift), float(eps), B, L, D, p(x_new), p(h), fmt,
-              p(q.codes) if fmt else None, p(q.scales) if fmt else None,
-              p(q.row_scale) if fmt else None, _lib.stream_of(x))
+              q.codes_ptr if fmt else None, q.scales_ptr if fmt else None,
+              q.row_scale_ptr if fmt else None, _lib.stream_of(x))
     return (x_new, h, q) if fmt else (x_new, h)
