@@ -4,11 +4,18 @@
 // them.  A thread's unit is 16 elements of one row: one nv block, or half an mx block whose
 // other half is the neighbouring lane's.  nv needs the row's amax before its first code, so
 // the row waits in registers (one warp up to 2048 elements, four warps up to 16384); longer
-// rows are read twice.  mx blocks are independent and are dealt to threads flat.
+// rows are read twice.  mx blocks and the way back need nothing of the rest of their row.
+// Measured at 8448 x 8960 (193 MB read and written): mx 32.1 us from fp16 (6.0 TB/s, 93% of
+// a plain copy), nv 39 us from bf16, the way back 35 us; 8448 x 1536: nv 7.9 us, back 6.9 us.
 #include "fp4.cuh"
 
 namespace fvb {
 namespace fp4 {
+
+// Units of a row that a warp takes (mx), and the order of a grid of 8-row blocks: reading, the
+// row blocks of one segment follow each other (32 us against 33 the other way round); writing,
+// the segments of one row block do, or DRAM's pages are written in pieces (35 us against 44)
+constexpr int kSegUnits = 128;
 
 template <typename T>
 struct Raw {
@@ -20,14 +27,33 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162flo
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(float x) { return x; }
 
-// elements [k0, k0 + 16) of a row of K; zeros past its end.  vec: the row is 16-byte aligned
-template <typename T>
+// 32 bytes at once (one whole sector per lane), p 32-byte aligned
+__device__ __forceinline__ void ld32(const uint4* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p));
+}
+__device__ __forceinline__ void st32(uint4* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y),
+               "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// elements [k0, k0 + 16) of a row of K; zeros past its end.  vec: the row is 32-byte aligned
+template <typename T, bool WIDE = false>
 __device__ __forceinline__ void load16(Raw<T>& r, const T* __restrict__ row, int64_t k0, int64_t K,
                                        bool vec) {
   if (vec && k0 + 16 <= K) {
     const uint4* p = reinterpret_cast<const uint4*>(row + k0);
 #pragma unroll
-    for (int i = 0; i < Raw<T>::kVec; ++i) r.v[i] = ld_stream(p + i);
+    for (int i = 0; i < Raw<T>::kVec; i += 2) {
+      if (WIDE) {
+        ld32(p + i, r.v[i], r.v[i + 1]);
+      } else {
+        r.v[i] = ld_stream(p + i);
+        r.v[i + 1] = ld_stream(p + i + 1);
+      }
+    }
   } else {
     T* e = reinterpret_cast<T*>(r.v);
 #pragma unroll
@@ -89,6 +115,7 @@ struct QuantArgs {
   int64_t pitch;  // bytes of one row of codes
   int64_t tiles;  // scale tiles along a row
   bool vec;
+  unsigned row_blocks;  // of 8 rows (mx)
 };
 
 // codes and scale of one nv unit
@@ -116,7 +143,8 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : 32 * WPR) quant_nv_kernel(con
   const int units = (int)(a.tiles * 4);
   Raw<T> r[NB];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) load16(r[i], row, (int64_t)(t + i * T_ROW) * 16, a.K, a.vec);
+  for (int i = 0; i < NB; ++i)  // 32 bytes a load: 7.9 us against 9.0 at 8448 x 1536, 40.7 against 39.2 at x 8960
+    load16<T, WPR == 1>(r[i], row, (int64_t)(t + i * T_ROW) * 16, a.K, a.vec);
   float am[NB], top = 0.f;
   uint32_t bad = 0u;
 #pragma unroll
@@ -176,33 +204,34 @@ __global__ void __launch_bounds__(256) quant_nv_long_kernel(const QuantArgs<T> a
   }
 }
 
-// mx: units dealt flat, lanes 2i and 2i + 1 share a block
+// mx: lanes 2i and 2i + 1 share a block; a block of threads is 8 rows x 32 units
 template <typename T>
 __global__ void __launch_bounds__(256) quant_mx_kernel(const QuantArgs<T> a) {
-  const int64_t units = a.tiles * 8;  // per row; a multiple of 8, so a block's lanes are neighbours
-  const int64_t total = a.M * units;
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  // whole warps run every turn of the loop (the shuffle needs both lanes)
-  for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x; i0 < total; i0 += stride) {
-    const int64_t i = i0 + threadIdx.x;
-    const int64_t m = i < total ? i / units : a.M - 1;
-    const int64_t u = i < total ? i - m * units : 0;
+  const int64_t m = (int64_t)(blockIdx.x % a.row_blocks) * 8 + (threadIdx.x >> 5);
+  if (m >= a.M) return;  // whole warps
+  const int lane = threadIdx.x & 31;
+  const int64_t units = a.tiles * 8;  // a multiple of 8, so both lanes of a block are in or out
+  const T* row = a.x + m * a.ld;
+  uint8_t* codes = a.codes + m * a.pitch;
+  const int64_t u1 = (int64_t)(blockIdx.x / a.row_blocks) * kSegUnits;
+#pragma unroll 2
+  for (int64_t u0 = u1; u0 < units && u0 < u1 + kSegUnits; u0 += 32) {
+    const int64_t u = u0 + lane;
     Raw<T> r;
-    load16(r, a.x + m * a.ld, u * 16, a.K, a.vec);
+    load16(r, row, u * 16, a.K, a.vec);
     bool bad;
     float am = amax16(r, bad);
     am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
     const bool other = __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;  // by every lane
     bad = bad || other;
-    if (i >= total) continue;
+    if (u >= units) continue;
     const int e = mx_exponent(am);
     if (u * 8 < a.pitch) {
       float f[16];
       unpack16(r, f);
-      *reinterpret_cast<uint2*>(a.codes + m * a.pitch + u * 8) =
-          bad ? make_uint2(0u, 0u) : mx_codes16(f, e);
+      *reinterpret_cast<uint2*>(codes + u * 8) = bad ? make_uint2(0u, 0u) : mx_codes16(f, e);
     }
-    // scales past the last block are 0, not the exponent of an empty block (also byte 0)
+    // scales past the last block are 0, the exponent byte of an empty block
     if ((u & 1) == 0) a.scales[scale_at(m, u >> 1, a.tiles)] = (uint8_t)(bad ? 0xFF : e + 127);
   }
 }
@@ -222,18 +251,18 @@ __device__ __forceinline__ float from_f32<float>(float v) {
   return v;
 }
 
-// the values that codes stand for; one thread per 16 elements
+// the values that codes stand for; one thread per 16 elements, 8 rows x 32 units a block
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict__ codes,
                                                       const uint8_t* __restrict__ scales,
                                                       const float* __restrict__ row_scale,
                                                       int rs_row, int64_t M, int64_t K,
-                                                      int64_t pitch, int64_t tiles,
-                                                      T* __restrict__ out) {
-  const int64_t units = (K + 15) / 16, total = M * units;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t m = i / units, u = i - m * units;
+                                                      int64_t pitch, int64_t tiles, bool vec,
+                                                      unsigned segs, T* __restrict__ out) {
+  const int64_t m = (int64_t)(blockIdx.x / segs) * 8 + (threadIdx.x >> 5);
+  if (m >= M) return;
+  const int64_t u = (int64_t)(blockIdx.x % segs) * 32 + (threadIdx.x & 31);
+  if (u < (K + 15) / 16) {
     const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + m * pitch + u * 8));
     const uint32_t b = __ldg(scales + scale_at(m, FMT == FVB_FP4_NV ? u : u >> 1, tiles));
     float s;
@@ -253,20 +282,15 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
       e[2 * j + 1] = from_f32<T>(f.y * s);
     }
     T* p = out + m * K + u * 16;
-    if (K % (16 / (int)sizeof(T)) == 0 && u * 16 + 16 <= K) {
+    if (vec && u * 16 + 16 <= K) {
 #pragma unroll
-      for (int j = 0; j < Raw<T>::kVec; ++j) reinterpret_cast<uint4*>(p)[j] = o.v[j];
+      for (int j = 0; j < Raw<T>::kVec; j += 2) st32(reinterpret_cast<uint4*>(p) + j, o.v[j], o.v[j + 1]);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (u * 16 + j < K) p[j] = e[j];
     }
   }
-}
-
-static unsigned flat_grid(int64_t total) {
-  const int64_t blocks = (total + 255) / 256, most = (int64_t)sm_count() * 64;
-  return (unsigned)(blocks < most ? blocks : most);
 }
 
 template <typename T>
@@ -282,9 +306,12 @@ static int quant(const void* x, int64_t ld, int64_t M, int64_t K, int fmt, void*
   a.row_scale = row_scale;
   a.pitch = code_pitch(K);
   a.tiles = scale_tiles(K, fmt);
-  a.vec = aligned16(x) && (ld * (int64_t)sizeof(T)) % 16 == 0;
+  a.vec = (reinterpret_cast<uintptr_t>(x) & 31u) == 0 && (ld * (int64_t)sizeof(T)) % 32 == 0;
   if (fmt == FVB_FP4_MX) {
-    quant_mx_kernel<T><<<flat_grid(M * a.tiles * 8), 256, 0, st>>>(a);
+    const int64_t segs = (a.tiles * 8 + kSegUnits - 1) / kSegUnits, blocks = (M + 7) / 8 * segs;
+    FVB_REQUIRE(blocks < (1ll << 31), "fvb_quant_fp4: size");
+    a.row_blocks = (unsigned)((M + 7) / 8);
+    quant_mx_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
     return check_launch("fvb_quant_fp4");
   }
   const int64_t units = a.tiles * 4;
@@ -311,16 +338,19 @@ static int quant(const void* x, int64_t ld, int64_t M, int64_t K, int fmt, void*
 template <typename T>
 static int dequant(const void* codes, const void* scales, const float* row_scale, int rs_row,
                    int64_t M, int64_t K, int fmt, void* out, cudaStream_t st) {
-  const unsigned grid = flat_grid(M * ((K + 15) / 16));
+  const int64_t segs64 = ((K + 15) / 16 + 31) / 32, blocks = (M + 7) / 8 * segs64;
+  FVB_REQUIRE(blocks < (1ll << 31), "fvb_dequant_fp4: size");
+  const unsigned grid = (unsigned)blocks, segs = (unsigned)segs64;
   const int64_t pitch = code_pitch(K), tiles = scale_tiles(K, fmt);
+  const bool vec = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && K * (int64_t)sizeof(T) % 32 == 0;
   if (fmt == FVB_FP4_NV)
     dequant_kernel<T, FVB_FP4_NV><<<grid, 256, 0, st>>>((const uint8_t*)codes,
                                                         (const uint8_t*)scales, row_scale, rs_row,
-                                                        M, K, pitch, tiles, (T*)out);
+                                                        M, K, pitch, tiles, vec, segs, (T*)out);
   else
     dequant_kernel<T, FVB_FP4_MX><<<grid, 256, 0, st>>>((const uint8_t*)codes,
                                                         (const uint8_t*)scales, nullptr, 0, M, K,
-                                                        pitch, tiles, (T*)out);
+                                                        pitch, tiles, vec, segs, (T*)out);
   return check_launch("fvb_dequant_fp4");
 }
 
