@@ -769,6 +769,302 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few output tiles: a 128 x 128 tile for each cluster of Z CTAs, each CTA a part of K.
+//
+// What bounds such a product is not a rate but how many SMs read the weight and how long one of
+// them is in its K loop: 129 x 1536 x 8960 has 6 pair tiles, 12 of 148 SMs for 16.6 us.  The
+// CTAs of a cluster leave their fp32 partial tiles in their own shared memory (the ring's, which
+// is free by then) and each adds up and finishes a share of the rows, reading the others' over
+// the cluster in the order of their ranks, so the sums do not depend on timing.  No workspace.
+// ---------------------------------------------------------------------------------------------
+template <int FMT>
+struct Split {
+  static constexpr int BN = 128;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kTilesK = FMT == FVB_FP4_NV ? 4 : 2;
+  static constexpr int kMmas = 4 / kTilesK;
+  static constexpr int kBytesA = BM * kRowBytes, kBytesB = BN * kRowBytes, kBytesSf = kTilesK * 512;
+  static constexpr int kBytes = kBytesA + kBytesB + 2 * kBytesSf;
+  static constexpr int kStages = 6;
+  static constexpr size_t kSmem = (size_t)kStages * kBytes + BM * 4 /*row scales*/ + 1024 + 256;
+  static constexpr int kSf = BN;             // TMEM: accumulator, then a scale buffer per stage
+  static constexpr int kSfCols = 8 * kTilesK;
+  static_assert(kSf + kStages * kSfCols <= 512, "TMEM columns");
+  static_assert(kStages * (kBytesA + kBytesB) >= BM * BN * 4, "partial tile");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t caddr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(caddr));
+  return v;
+}
+
+// SPLIT: Z > 1
+template <int FMT, int EPI, bool SPLIT>
+__global__ void __launch_bounds__(Split<FMT>::kThreads, 1)
+    fp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tmA,
+                          const __grid_constant__ CUtensorMap tmB,
+                          const __grid_constant__ CUtensorMap tmSfA,
+                          const __grid_constant__ CUtensorMap tmSfB, const Args args, const int Z) {
+  using S = Split<FMT>;
+  constexpr int STAGES = S::kStages, BN = S::BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  uint8_t* sA = base;
+  uint8_t* sB = sA + STAGES * S::kBytesA;
+  uint8_t* sSfA = sB + STAGES * S::kBytesB;
+  uint8_t* sSfB = sSfA + STAGES * S::kBytesSf;
+  float* sRow = reinterpret_cast<float*>(sSfB + STAGES * S::kBytesSf);  // the tile's row scales
+  uint64_t* full = reinterpret_cast<uint64_t*>(sRow + BM);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+
+  const int warp = warp_id_uniform();
+  const int lane = threadIdx.x & 31;
+  const uint32_t z = SPLIT ? cluster_ctarank() : 0u;
+  const int tile = (int)(blockIdx.x >> (31 - __clz(Z)));
+  const int n_tiles = (args.N + BN - 1) / BN;
+  const int m0 = tile / n_tiles * BM, n0 = tile % n_tiles * BN;
+  const int kblocks = (args.K + 255) / 256;
+  // Z is 1, 2, 4 or 8
+  const int zs = 31 - __clz(Z), k0 = (kblocks * (int)z) >> zs, k1 = (kblocks * ((int)z + 1)) >> zs;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(tfull, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    prefetch_tmap(&tmSfA);
+    prefetch_tmap(&tmSfB);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const bool leader = elect_one();
+    int issued = 0, stage = 0;
+    uint32_t phase = 0;
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, 0x421u))) break;
+      if (leader) {
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)S::kBytes);
+        tma_load_2d(sA + stage * S::kBytesA, &tmA, &full[stage], kb * kRowBytes, m0);
+        tma_load_2d(sB + stage * S::kBytesB, &tmB, &full[stage], kb * kRowBytes, n0);
+        tma_load_3d(sSfA + stage * S::kBytesSf, &tmSfA, &full[stage], 0, kb * S::kTilesK, m0 >> 7);
+        tma_load_3d(sSfB + stage * S::kBytesSf, &tmSfB, &full[stage], 0, kb * S::kTilesK, n0 >> 7);
+      }
+      __syncwarp();
+      ++issued;
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // no load may still be writing shared memory when the partial tile goes there or the CTA exits
+    for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+      mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u, 0x42Au);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t idesc = idesc4<FMT>(BM, BN);
+    const bool leader = elect_one();
+    const uint64_t descA = smem_desc_sw128(smem_u32(sA), 16, 1024);
+    const uint64_t descB = smem_desc_sw128(smem_u32(sB), 16, 1024);
+    const uint64_t descFA = scale_desc(smem_u32(sSfA));
+    const uint64_t descFB = scale_desc(smem_u32(sSfB));
+    const int ksteps = (args.K + 63) / 64;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, 0x423u))) break;
+      tc_fence_after();
+      const uint64_t da = descA + (uint32_t)(stage * (S::kBytesA >> 4));
+      const uint64_t db = descB + (uint32_t)(stage * (S::kBytesB >> 4));
+      const uint64_t fa = descFA + (uint32_t)(stage * (S::kBytesSf >> 4));
+      const uint64_t fb = descFB + (uint32_t)(stage * (S::kBytesSf >> 4));
+      const int left = ksteps - kb * 4;
+      // the stage's own scale columns: its last MMAs are done, or the stage were not full again
+      const uint32_t sfa = tmem + (uint32_t)(S::kSf + stage * S::kSfCols);
+      const uint32_t sfb = sfa + (uint32_t)(4 * S::kTilesK);
+      if (leader) {
+#pragma unroll
+        for (int i = 0; i < S::kTilesK; ++i) {
+          cp_scales<false>(sfa + 4u * i, fa + i * 512 / 16);
+          cp_scales<false>(sfb + 4u * i, fb + i * 512 / 16);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const uint32_t i = ks / S::kMmas, id = 2u * (ks % S::kMmas);
+          if (ks < left)
+            mma_fp4<FMT, false>(tmem, da + 2 * ks, db + 2 * ks, idesc | (id << 4) | (id << 29),
+                                sfa + 4u * i, sfb + 4u * i, kb != k0 || ks != 0 ? 1u : 0u);
+        }
+        tc_commit(&empty[stage]);
+      }
+      __syncwarp();
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // every MMA issued above has finished when this arrives
+    if (leader) tc_commit(tfull);
+    __syncwarp();
+    mbar_wait(tfull, 0, 0x42Bu);
+  }
+
+  // ------------------------------------------------------------ partial tiles, sum, epilogue
+  const int et = (int)threadIdx.x - 64;
+  const int u = et & 15;  // this thread's 8 columns of every row it finishes
+  const int col = n0 + u * 8;
+  float sw[8], bias[8], gate[8];
+  bool ok = true;
+  if (warp >= 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = col + i < args.N;
+      sw[i] = args.sw ? (args.sw_row ? (in ? __ldg(args.sw + col + i) : 0.f) : __ldg(args.sw)) : 1.f;
+      bias[i] = args.bias && in ? __bfloat162float(args.bias[col + i]) : 0.f;
+      gate[i] = EPI == kResidual && args.gate && in ? __bfloat162float(args.gate[col + i]) : 1.f;
+    }
+    if (et < BM)
+      sRow[et] = args.sa && m0 + et < args.M ? __ldg(args.sa + (args.sa_row ? m0 + et : 0)) : 1.f;
+    ok = __all_sync(0xffffffffu, mbar_wait(tfull, 0, 0x424u));
+    tc_fence_after();
+    const int q = warp & 3, c = (warp - 2) >> 2;
+    uint32_t r[64];
+    const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(c * 64);
+    tmem_ld_16x256b_x8(acc, r);
+    tmem_ld_16x256b_x8(acc + (16u << 16), r + 32);
+    tmem_ld_wait();
+    // row pitch 512 bytes, 32-byte units of 8 columns: unit w of row l at w ^ (l % 8)
+    const int lr = lane >> 2, lq = lane & 3;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const int row = q * 32 + lr + 8 * k, w = (c * 8 + g) ^ (row & 7);
+        const int i0 = (k >> 1) * 32 + g * 4 + (k & 1) * 2;
+        *reinterpret_cast<uint2*>(base + row * 512 + w * 32 + lq * 8) = make_uint2(r[i0], r[i0 + 1]);
+      }
+  }
+  tc_fence_before();
+  if (SPLIT) cluster_sync_all();
+  else __syncthreads();
+  if (warp >= 2) {
+    const int rows = args.M - m0 < BM ? args.M - m0 : BM;
+    const uint32_t base_u = smem_u32(base);
+    // whole warps go round (the GELU form shuffles); two rows a warp
+#pragma unroll 4
+    for (int it = (int)z * 16 + (et >> 4); (it & ~1) < rows; it += Z * 16) {
+      const int rl = it, row = m0 + rl;
+      const bool in = rl < rows && ok;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      if (in) {
+        const uint32_t at = base_u + rl * 512 + ((u ^ (rl & 7)) << 5);
+        if (!SPLIT) {
+          const float4* own = reinterpret_cast<const float4*>(base + (at - base_u));
+          const float4 a = own[0], b = own[1];
+          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+          v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        }
+        // four ranks' values on their way at once (one at a time, eight cost 3 us)
+        for (int p0 = 0; SPLIT && p0 < Z; p0 += 4) {
+          float4 a[4], b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p0 + j < Z) {
+              const uint32_t ca = mapa_shared(at, (uint32_t)(p0 + j));
+              a[j] = ld_cluster_f4(ca);
+              b[j] = ld_cluster_f4(ca + 16);
+            }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p0 + j < Z) {
+              v[0] += a[j].x; v[1] += a[j].y; v[2] += a[j].z; v[3] += a[j].w;
+              v[4] += b[j].x; v[5] += b[j].y; v[6] += b[j].z; v[7] += b[j].w;
+            }
+        }
+      }
+      const float sa = sRow[rl & (BM - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __fmaf_rn(v[i], sa * sw[i], bias[i]);
+      if constexpr (EPI == kGeluMx) {
+        uint64_t p[4];
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (col + 2 * i >= args.N) v[2 * i] = 0.f;
+          if (col + 2 * i + 1 >= args.N) v[2 * i + 1] = 0.f;
+          p[i] = gelu2(f2_pack(v[2 * i], v[2 * i + 1]));
+          m = fp4::max_abs_nan(m, p[i]);
+        }
+        uint32_t e = __float_as_uint(m) >> 23;  // amax's exponent field over the block's four lanes
+        e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+        e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+        const uint32_t byte = e > 2u ? e - 2u : 0u;
+        const float rs = __uint_as_float((254u - byte) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(p[i], f2_pack(rs, rs)), v[2 * i], v[2 * i + 1]);
+        if (in) {
+          if ((col >> 1) < args.hpitch)
+            *reinterpret_cast<uint32_t*>(args.hcodes + (int64_t)row * args.hpitch + (col >> 1)) =
+                e == 255u ? 0u : fp4::e2m1x8(v);
+          if ((u & 3) == 0)
+            args.hscales[fp4::scale_at(row, col >> 5, args.htiles)] = (uint8_t)(e == 255u ? 255u : byte);
+        }
+      } else if (in && col < args.N) {
+        if (EPI == kResidual) {
+          const __nv_bfloat16* rp = args.res + (int64_t)row * args.ldr + col;
+          float x[8];
+          if (args.tma_res && col + 8 <= args.N) {  // 16-byte aligned rows
+            bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(rp)), x);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = col + i < args.N ? __bfloat162float(rp[i]) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __fmaf_rn(gate[i], v[i], x[i]);
+        }
+        __nv_bfloat16* op = args.out + (int64_t)row * args.ldo + col;
+        if (args.tma_out && col + 8 <= args.N) {
+          *reinterpret_cast<uint4*>(op) = f32_to_bf16x8(v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < args.N) op[i] = __float2bfloat16_rn(v[i]);
+        }
+      }
+    }
+  }
+  // neither shared memory that a peer reads nor TMEM goes before everybody is done
+  if (SPLIT) cluster_sync_all();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 struct Operand {
   const void* codes;
   const void* scales;
@@ -776,25 +1072,34 @@ struct Operand {
   int rs_row;
 };
 
-template <int FMT, int BN, int EPI, bool PAIR>
-static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_t st) {
-  using S = Shape<FMT, BN, EPI, PAIR>;
+// codes of A in boxes of 128 rows and of W in boxes of `rows_b`, a K block wide; the scale tiles
+// of a K block for one 128-row band of A and for `bands_b` of W
+template <int FMT>
+static int operand_maps(const Args& a, const Operand& A, const Operand& W, int rows_b, int bands_b,
+                        CUtensorMap& tmA, CUtensorMap& tmB, CUtensorMap& tmSfA, CUtensorMap& tmSfB) {
   const int64_t pitch = fp4::code_pitch(a.K);
   const int64_t tiles = fp4::scale_tiles(a.K, FMT);
-  CUtensorMap tmA, tmB, tmSfA, tmSfB, tmO, tmR;
+  constexpr int kTilesK = FMT == FVB_FP4_NV ? 4 : 2;
   int rc = make_tmap_2d(&tmA, A.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)pitch,
                         (uint64_t)a.M, (uint64_t)pitch, kRowBytes, BM, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   rc = make_tmap_2d(&tmB, W.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)pitch, (uint64_t)a.N,
-                    (uint64_t)pitch, kRowBytes, S::kRowsB, CU_TENSOR_MAP_SWIZZLE_128B);
+                    (uint64_t)pitch, kRowBytes, (uint32_t)rows_b, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   // scales as 32-bit words of [band of 128 rows][tile][128 words]
   rc = make_tmap_3d(&tmSfA, A.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 128, (uint64_t)tiles,
-                    (uint64_t)((a.M + 127) / 128), 512, (uint64_t)tiles * 512, 128, S::kTilesK, 1);
+                    (uint64_t)((a.M + 127) / 128), 512, (uint64_t)tiles * 512, 128, kTilesK, 1);
   if (rc) return rc;
-  rc = make_tmap_3d(&tmSfB, W.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 128, (uint64_t)tiles,
-                    (uint64_t)((a.N + 127) / 128), 512, (uint64_t)tiles * 512, 128, S::kTilesK,
-                    S::kSfTilesB);
+  return make_tmap_3d(&tmSfB, W.scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, 128, (uint64_t)tiles,
+                      (uint64_t)((a.N + 127) / 128), 512, (uint64_t)tiles * 512, 128, kTilesK,
+                      (uint32_t)bands_b);
+}
+
+template <int FMT, int BN, int EPI, bool PAIR>
+static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_t st) {
+  using S = Shape<FMT, BN, EPI, PAIR>;
+  CUtensorMap tmA, tmB, tmSfA, tmSfB, tmO, tmR;
+  int rc = operand_maps<FMT>(a, A, W, S::kRowsB, S::kSfTilesB, tmA, tmB, tmSfA, tmSfB);
   if (rc) return rc;
   tmO = tmA;  // unused unless tma_out
   if (EPI == kGeluMx) {
@@ -861,10 +1166,68 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   return check_launch("fp4 gemm");
 }
 
+template <int FMT, int EPI, bool SPLIT>
+static int launch_split(const Args& a, const Operand& A, const Operand& W, int Z, cudaStream_t st) {
+  using S = Split<FMT>;
+  CUtensorMap tmA, tmB, tmSfA, tmSfB;
+  int rc = operand_maps<FMT>(a, A, W, S::BN, 1, tmA, tmB, tmSfA, tmSfB);
+  if (rc) return rc;
+  auto kern = fp4_gemm_split_kernel<FMT, EPI, SPLIT>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  FVB_CUDA_TRY(cudaGetDevice(&dev), "fp4 gemm device");
+  FVB_REQUIRE(dev >= 0 && dev < 64, "fp4 gemm: device ordinal %d", dev);
+  if (!configured[dev]) {
+    FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem),
+                 "fp4 gemm smem attribute");
+    configured[dev] = true;
+  }
+  const int64_t tiles = (int64_t)((a.M + BM - 1) / BM) * ((a.N + S::BN - 1) / S::BN);
+  FVB_REQUIRE(tiles * Z < (1ll << 31), "fp4 gemm: too many output tiles");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.gridDim = dim3((unsigned)(tiles * Z));
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  if (SPLIT) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = Z;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  FVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmSfA, tmSfB, a, Z), "fp4 gemm launch");
+  return check_launch("fp4 gemm");
+}
+
+// Pair tiles for products that fill the machine with them, split tiles for the rest: whichever
+// the fitted times (in 10 ns) call shorter.  A K block takes a pair tile 0.37 us and a split tile
+// 0.25, a wave 1.3 and 3.0 us besides (fill and epilogue, which split tiles do not overlap), and
+// Z parts of K cost their exchange.  Measured (us), pair / Z = 1 / 2 / 4:
+//   129 x 1536 x 8960  16.6 / 11.9 / 10.6 / 10.0     16 x 1536 x 8960    16.0 / 10.6 / 8.5 / 7.4
+//   1024 x 1536 x 1536  8.1 /  6.3 / 14.1 / 24.7     517 x 1544 x 1000    7.6 /  5.5 / 7.6 / 15.9
+//   2048 x 1536 x 1536  8.5 / 10.8                   1024 x 1536 x 8960  18.1 / 12.9
+// Clusters that do not all fit at once (more than about 128 CTAs) lose more than they give.
 template <int FMT, int EPI>
 static int dispatch(const Args& a, const Operand& A, const Operand& W, cudaStream_t st) {
-  if (a.M > BM && a.N > 128) return launch<FMT, 256, EPI, true>(a, A, W, st);
-  return launch<FMT, 128, EPI, false>(a, A, W, st);
+  const int64_t kb = (a.K + 255) / 256, sms = sm_count();
+  const int64_t pairs = (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256);
+  const int64_t tiles = (int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128);
+  const int64_t pair_cost = (pairs + sms / 2 - 1) / (sms / 2) * (37 * kb + 130) + 500;
+  int best = 1;
+  int64_t split_cost = (tiles + sms - 1) / sms * (25 * kb + 300) + 50;
+  for (int z = 2; z <= 8 && z <= kb && tiles * z <= 128; z *= 2) {
+    const int64_t cost = 25 * ((kb + z - 1) / z) + 470 + 60 * z;
+    if (cost < split_cost) {
+      split_cost = cost;
+      best = z;
+    }
+  }
+  if (pair_cost <= split_cost) return launch<FMT, 256, EPI, true>(a, A, W, st);
+  return best > 1 ? launch_split<FMT, EPI, true>(a, A, W, best, st)
+                  : launch_split<FMT, EPI, false>(a, A, W, 1, st);
 }
 
 template <int EPI>

@@ -228,6 +228,53 @@ def test_product_many_tiles(fmt):
         check(fp4_mm(a, w, bias), y, BF16 * y.abs() + (steps(K) + 2.0 ** -22) * S + 2.0 ** -22 * y.abs())
 
 
+@pytest.mark.parametrize("M,N,K", [(2500, 2056, 300), (2305, 2001, 1000), (4000, 1544, 64), (3000, 1536, 1600),
+                                   (2049, 2600, 2300), (4100, 4000, 520)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product_pair_tiles(M, N, K, fmt):
+    """Sizes that run on CTA pairs: rows and columns that end inside a tile or leave a pair's
+    second CTA without rows, K that ends inside a block, odd N (no TMA for the output)."""
+    from flashvsr_sm89_ops_b200 import _lib, fp4_mm
+    a, w, bias, res, gate = mm_case(M, N, K, fmt)
+    y, S = mm_ref(a, w)
+    acc = steps(K) * S
+    check(fp4_mm(a, w), y, BF16 * y.abs() + acc)
+    yb = y + bias.double()
+    o = res.double() + gate.double() * yb
+    mag = res.double().abs() + gate.double().abs() * (yb.abs() + S)
+    tol = BF16 * o.abs() + gate.double().abs() * acc + 2.0 ** -22 * mag
+    check(fp4_mm(a, w, bias, residual=res, gate=gate), o, tol)
+    wide = torch.zeros(M, N + 3, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1:N + 1] = res
+    check(fp4_mm(a, w, bias, residual=wide[:, 1:N + 1], gate=gate), o, tol)
+    out = res.clone()
+    fp4_mm(a, w, bias, residual=out, gate=gate, out=out)
+    check(out, o, tol)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 128, 512), (3, 300, 2048), (128, 1536, 4096), (129, 1536, 8960),
+                                   (40, 130, 9000), (200, 520, 2100), (256, 256, 20000)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product_parts_of_k(M, N, K, fmt):
+    """Sizes whose K is divided among the CTAs of a cluster: the same bits every time."""
+    from flashvsr_sm89_ops_b200 import _lib, fp4_mm
+    a, w, bias, res, gate = mm_case(M, N, K, fmt)
+    y, S = mm_ref(a, w)
+    yb = y + bias.double()
+    out = fp4_mm(a, w, bias)
+    check(out, yb, BF16 * yb.abs() + steps(K) * S + 2.0 ** -21 * (yb.abs() + S))
+    for _ in range(3):
+        assert torch.equal(fp4_mm(a, w, bias), out)
+    o = res.double() + gate.double() * yb
+    mag = res.double().abs() + gate.double().abs() * (yb.abs() + S)
+    check(fp4_mm(a, w, bias, residual=res, gate=gate), o,
+          BF16 * o.abs() + gate.double().abs() * steps(K) * S + 2.0 ** -21 * mag)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+
+
 @pytest.mark.parametrize("M", [1, 3, 200])
 def test_product_row_scale_forms(M):
     """nv operands whose second scale is one number or missing, as checkpoints ship them."""
@@ -330,7 +377,8 @@ def spread(h, e, fmt):
 
 @pytest.mark.parametrize("M,D,F,N", [(1, 64, 32, 64), (3, 256, 500, 96), (13, 1000, 1000, 136),
                                      (100, 136, 1544, 137), (128, 256, 256, 256), (129, 264, 4096, 264),
-                                     (300, 1536, 8960, 1536), (700, 72, 2056, 512)])
+                                     (300, 1536, 8960, 1536), (700, 72, 2056, 512),
+                                     (2500, 264, 2056, 1500), (2309, 200, 2001, 2003), (5000, 100, 1040, 72)])
 @pytest.mark.parametrize("fmt", FMTS)
 def test_ffn(M, D, F, N, fmt):
     from flashvsr_sm89_ops_b200 import _lib, ffn_fp4, quantize_fp4
