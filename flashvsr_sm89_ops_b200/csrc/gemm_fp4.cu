@@ -5,7 +5,9 @@
 //   y = acc * sa[m] * sw[n] + bias[n]      sa, sw: the nv formats' row scales (mx: 1)
 //   out = bf16(y)  or  bf16(res + gate[n] * y)  or  mx codes of GELU(tanh)(y)
 //
-// One persistent CTA per SM, or one CTA pair per two SMs, warp-specialised:
+// Two kernels.  Products with many output tiles run on persistent CTA pairs (cta_group::2, one
+// CTA per SM, 256 x 256 tiles of which each CTA holds 128 rows), warp-specialised; those with few
+// on a tile per cluster of CTAs that share its K loop (further down).
 //   warp 0      TMA producer: 256-element (128-byte) K blocks of A and W and their scale tiles
 //               into a ring of shared-memory stages
 //   warp 1      MMA issuer: copies a K block's scale tiles into TMEM (tcgen05.cp), then issues
@@ -14,11 +16,12 @@
 //               turn; bf16 through a swizzled staging buffer and a TMA store, a residual into
 //               the same buffer by TMA while the tile is still being multiplied
 //
-// TMEM (512 columns): two accumulators of BN columns, so that a tile's epilogue runs under the
-// next tile's MMAs, and at least two buffers of a K block's scales.  With BN = 256 that is
-// more than 512, so the second accumulator starts at column 128: the two share half their
-// columns, the epilogue's warps read those first, and the next tile's MMAs start when they have
-// been read.
+// TMEM (512 columns): two accumulators of 256 columns, so that a tile's epilogue runs under the
+// next tile's MMAs, and two or more buffers of a K block's scales.  That is more than 512, so
+// the second accumulator starts at column 128: the two share half their columns, the epilogue's
+// warps read those first, and the next tile's MMAs start when they have been read.  Tiles 192
+// wide with separate accumulators move more operands for each flop and measured 39.8 us against
+// 36.4 on 8448 x 4608 x 1536 and 62 against 50 on 8448 x 1536 x 8960.
 //
 // A scale buffer is overwritten after a wait for the MMAs that read it: the issue order puts a
 // copy before the MMAs after it, but nothing puts an MMA before a copy after it.  The wait is on
@@ -44,10 +47,10 @@ constexpr int kStageCodes = 32 * 32;  // with GELU: 32 rows x 64 codes
 
 enum { kPlain = 0, kResidual = 1, kGeluMx = 2 };
 
-// epilogue warps: one per TMEM lane quarter and 64-column chunk, at most 8.  16 for BN = 256 left
+// epilogue warps: two per TMEM lane quarter.  Four, one for each 64-column chunk, left
 // the GELU epilogue 96 registers a thread and measured 119 us against 102 (8448 x 8960 x 1536
 // with a small second product); for the others their staging buffers would cost a ring stage.
-__host__ __device__ constexpr int epi_warps(int bn) { return bn > 128 ? 8 : 4 * (bn / 64); }
+constexpr int kEpiWarps = 8;
 
 struct Args {
   int M, N, K;
@@ -66,17 +69,17 @@ struct Args {
   int64_t hpitch, htiles;
 };
 
-template <int FMT, int BN, int EPI, bool PAIR>
+template <int FMT, int EPI>
 struct Shape {
-  static constexpr int kEpiWarps = epi_warps(BN);
+  static constexpr int BN = 256;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kOut = EPI == kGeluMx ? kStageCodes : kStageOut;
   static constexpr int kOutBytes = kEpiWarps * kOut;
   static constexpr int kColBytes = 2 * 2 * BN * 4;  // two tiles' column scales (fp32), biases and gates (bf16)
   static constexpr int kTilesK = FMT == FVB_FP4_NV ? 4 : 2;  // scale tiles per K block
   static constexpr int kMmas = 4 / kTilesK;                  // MMAs (K = 64) per scale tile
-  static constexpr int kRowsB = PAIR ? BN / 2 : BN;          // W rows this CTA stages
-  static constexpr int kSfTilesB = BN > 128 ? 2 : 1;  // 128-row scale tiles a tile's columns lie in
+  static constexpr int kRowsB = BN / 2;                      // W rows a CTA of the pair stages
+  static constexpr int kSfTilesB = BN / 128;                 // 128-row scale tiles of W
   static constexpr int kBytesA = BM * kRowBytes;
   static constexpr int kBytesB = kRowsB * kRowBytes;
   static constexpr int kBytesSfA = kTilesK * 512;
@@ -87,14 +90,12 @@ struct Shape {
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr size_t kSmem = (size_t)kStages * kBytes + kFixed;
   // TMEM columns
-  static constexpr bool kOverlap = BN == 256;
-  static constexpr int kAcc1 = kOverlap ? 128 : BN;   // start of the second accumulator
+  static constexpr int kAcc1 = BN / 2;                // start of the second accumulator
   static constexpr int kSf = kAcc1 + BN;              // start of the scale buffers
   static constexpr int kSfA = 4 * kTilesK, kSfB = 4 * kTilesK * kSfTilesB;  // columns of one
   static constexpr int kFitSf = (512 - kSf) / (kSfA + kSfB);
   static constexpr int kSfBufs = kFitSf > kStages ? kStages : kFitSf;
   static_assert(kSfBufs >= 2, "TMEM columns");
-  static_assert(BN % 64 == 0 && BN <= 256, "a tile's columns start on half a scale tile");
   static_assert(kStages >= 3, "ring");
 };
 
@@ -296,16 +297,17 @@ __device__ __forceinline__ void gelu_mx(uint64_t (&v)[4][8], int col0, int N, in
     }
 }
 
-template <int FMT, int BN, int EPI, bool PAIR>
-__global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
+template <int FMT, int EPI>
+__global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSfA,
                     const __grid_constant__ CUtensorMap tmSfB,
                     const __grid_constant__ CUtensorMap tmOut,
                     const __grid_constant__ CUtensorMap tmRes, const Args args) {
-  using S = Shape<FMT, BN, EPI, PAIR>;
+  using S = Shape<FMT, EPI>;
+  constexpr int BN = S::BN;
   constexpr int STAGES = S::kStages;
-  constexpr int TM = PAIR ? 2 * BM : BM;
+  constexpr int TM = 2 * BM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
@@ -321,14 +323,14 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
   uint64_t* tempty = tfull + 2;       // [2] accumulator read
   uint64_t* drain = tempty + 2;       // every MMA this CTA issued finished
   uint64_t* rfull = drain + 1;        // [epilogue warps] residual arrived
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + S::kEpiWarps);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + kEpiWarps);
   uint32_t* pair_ok = tmem_slot + 1;
 
   const int warp = warp_id_uniform();
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
-  const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
-  const int units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const uint32_t rank = cluster_ctarank();
+  const int unit = (int)(blockIdx.x >> 1);
+  const int units = (int)(gridDim.x >> 1);
   const int m_tiles = (args.M + TM - 1) / TM;
   const int n_tiles = (args.N + BN - 1) / BN;
   const int num_tiles = m_tiles * n_tiles;
@@ -341,10 +343,10 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], PAIR ? 2 * S::kEpiWarps : S::kEpiWarps);
+      mbar_init(&tempty[b], 2 * kEpiWarps);
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < S::kEpiWarps; ++w) mbar_init(&rfull[w], 1);
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(&rfull[w], 1);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -352,30 +354,21 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     prefetch_tmap(&tmSfB);
   }
   if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(tmem_slot, 512);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(tmem_slot, 512);
-      tmem_relinquish();
-    }
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
-  if (PAIR) {
-    cluster_sync_all();
-    if (threadIdx.x == 0)
-      *pair_ok = ld_shared_cluster_u32(mapa_shared(smem_u32(tmem_slot), rank ^ 1u)) == *tmem_slot;
-    __syncthreads();
-  } else {
-    __syncthreads();
-  }
+  cluster_sync_all();
+  if (threadIdx.x == 0)
+    *pair_ok = ld_shared_cluster_u32(mapa_shared(smem_u32(tmem_slot), rank ^ 1u)) == *tmem_slot;
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // a pair whose TMEM addresses differ (never expected) does no work and reports it
-  const bool run = !PAIR || *pair_ok != 0u;
+  const bool run = *pair_ok != 0u;
   if (!run && threadIdx.x == 0 && rank == 0) atomicCAS(&g_device_error, 0u, 0x40Cu);
-  const uint32_t full0_c = PAIR ? mapa_shared(smem_u32(full), 0u) : 0u;
-  const uint32_t tempty0_c = PAIR ? mapa_shared(smem_u32(tempty), 0u) : 0u;
+  const uint32_t full0_c = mapa_shared(smem_u32(full), 0u);
+  const uint32_t tempty0_c = mapa_shared(smem_u32(tempty), 0u);
 
   if (!run) {
     // straight to the teardown
@@ -390,7 +383,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     for (int tile = unit; tile < num_tiles && ok; tile += units) {
       const int m0 = (tile / n_tiles) * TM + (int)rank * BM;
       const int nt = (tile % n_tiles) * BN;
-      const int n0 = nt + (int)rank * (PAIR ? S::kRowsB : 0);
+      const int n0 = nt + (int)rank * S::kRowsB;
       for (int kb = 0; kb < kblocks; ++kb) {
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, 0x401u))) {
           ok = false;
@@ -402,21 +395,13 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
           uint8_t* fa = sSfA + stage * S::kBytesSfA;
           uint8_t* fb = sSfB + stage * S::kBytesSfB;
           // scale tiles past the last of a row are filled with zeros
-          if (PAIR) {
-            // the even CTA arms its barrier for both CTAs' bytes
-            const uint32_t bar = full0_c + 8u * stage;
-            if (rank == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)(2 * S::kBytes));
-            tma_load_2d_pair(a, &tmA, bar, kb * kRowBytes, m0);
-            tma_load_2d_pair(b, &tmB, bar, kb * kRowBytes, n0);
-            tma_load_3d_pair(fa, &tmSfA, bar, 0, kb * S::kTilesK, m0 >> 7);
-            tma_load_3d_pair(fb, &tmSfB, bar, 0, kb * S::kTilesK, nt >> 7);
-          } else {
-            mbar_arrive_expect_tx(&full[stage], (uint32_t)S::kBytes);
-            tma_load_2d(a, &tmA, &full[stage], kb * kRowBytes, m0);
-            tma_load_2d(b, &tmB, &full[stage], kb * kRowBytes, n0);
-            tma_load_3d(fa, &tmSfA, &full[stage], 0, kb * S::kTilesK, m0 >> 7);
-            tma_load_3d(fb, &tmSfB, &full[stage], 0, kb * S::kTilesK, nt >> 7);
-          }
+          // the even CTA arms its barrier for both CTAs' bytes
+          const uint32_t bar = full0_c + 8u * stage;
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)(2 * S::kBytes));
+          tma_load_2d_pair(a, &tmA, bar, kb * kRowBytes, m0);
+          tma_load_2d_pair(b, &tmB, bar, kb * kRowBytes, n0);
+          tma_load_3d_pair(fa, &tmSfA, bar, 0, kb * S::kTilesK, m0 >> 7);
+          tma_load_3d_pair(fb, &tmSfB, bar, 0, kb * S::kTilesK, nt >> 7);
         }
         __syncwarp();
         ++issued;
@@ -428,7 +413,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     }
     // no load may still be writing shared memory when its CTA exits: the last STAGES loads
     // are the newest phase of their stages' full barriers (a pair's are the even CTA's)
-    if (!PAIR || rank == 0)
+    if (rank == 0)
       for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
         mbar_wait(&full[i % STAGES], (uint32_t)((i / STAGES) & 1), 0x40Au);
   } else if (warp == 1) {
@@ -453,17 +438,12 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
       bool ok = true, any = false;
       for (int tile = unit; tile < num_tiles && ok; tile += units, ++t) {
         const int buf = t & 1;
-        // separate accumulators: until this one's last tile was read.  Shared columns: until the
-        // previous tile's were; its other warps arrive there having read the tile before it
-        const bool clear =
-            S::kOverlap
-                ? (t == 0 || mbar_wait(&tempty[buf ^ 1], (uint32_t)((t - 1) >> 1) & 1u, 0x402u))
-                : mbar_wait(&tempty[buf], ((uint32_t)(t >> 1) & 1u) ^ 1u, 0x402u);
+        // until the columns shared with the previous tile were read; the warps that arrive there
+        // have read all of the tile before it
+        const bool clear = t == 0 || mbar_wait(&tempty[buf ^ 1], (uint32_t)((t - 1) >> 1) & 1u, 0x402u);
         if (!__all_sync(0xffffffffu, clear)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * S::kAcc1);
-        // a tile may start half way into a 128-row scale tile: two 32-row scale columns on
-        const uint32_t shift = BN % 128 == 0 ? 0u : (uint32_t)((((tile % n_tiles) * BN) & 127) >> 5);
         for (int kb = 0; kb < kblocks && ok; ++kb) {
           if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, 0x403u))) {
             ok = false;
@@ -490,10 +470,10 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
           if (leader) {
 #pragma unroll
             for (int i = 0; i < S::kTilesK; ++i) {
-              cp_scales<PAIR>(sfa + 4u * i, fa + i * 512 / 16);
+              cp_scales<true>(sfa + 4u * i, fa + i * 512 / 16);
 #pragma unroll
               for (int r = 0; r < S::kSfTilesB; ++r)
-                cp_scales<PAIR>(sfb + (uint32_t)(4 * (S::kSfTilesB * i + r)),
+                cp_scales<true>(sfb + (uint32_t)(4 * (S::kSfTilesB * i + r)),
                                 fb + (r * S::kTilesK + i) * 512 / 16);
             }
 #pragma unroll
@@ -501,8 +481,8 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
               // an mx MMA takes two bytes of the four in a scale column
               const uint32_t i = ks / S::kMmas, id = 2u * (ks % S::kMmas);
               if (ks < left)
-                mma_fp4<FMT, PAIR>(d, da + 2 * ks, db + 2 * ks, idesc | (id << 4) | (id << 29),
-                                   sfa + 4u * i, sfb + 4u * S::kSfTilesB * i + shift,
+                mma_fp4<FMT, true>(d, da + 2 * ks, db + 2 * ks, idesc | (id << 4) | (id << 29),
+                                   sfa + 4u * i, sfb + 4u * S::kSfTilesB * i,
                                    (kb | ks) != 0 ? 1u : 0u);
             }
           }
@@ -511,35 +491,26 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
             sbuf = 0;
             reuse = true;
           }
-          if (leader) {
-            if (PAIR) tc_commit_pair_both(&empty[stage], 0x3);
-            else tc_commit(&empty[stage]);
-          }
+          if (leader) tc_commit_pair_both(&empty[stage], 0x3);
           __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok && leader) {
-          if (PAIR) tc_commit_pair_both(&tfull[buf], 0x3);
-          else tc_commit(&tfull[buf]);
-        }
+        if (ok && leader) tc_commit_pair_both(&tfull[buf], 0x3);
         __syncwarp();
       }
       // every MMA issued above completes before TMEM is freed
       if (any) {
-        if (leader) {
-          if (PAIR) tc_commit_pair(drain);
-          else tc_commit(drain);
-        }
+        if (leader) tc_commit_pair(drain);
         __syncwarp();
         mbar_wait(drain, 0, 0x40Bu);
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    constexpr int G = S::kEpiWarps / 4;  // warps per TMEM lane quarter
+    constexpr int G = kEpiWarps / 4;  // warps per TMEM lane quarter
     constexpr int kChunks = BN / 64;
     const int q = warp & 3;              // TMEM lane quarter this warp may access
     const int sub = (warp - 2) >> 2;     // its first chunk
@@ -563,10 +534,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     auto release = [&](int b) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (PAIR) mbar_arrive_remote_relaxed(tempty0_c + 8u * b);
-        else mbar_arrive(&tempty[b]);
-      }
+      if (lane == 0) mbar_arrive_remote_relaxed(tempty0_c + 8u * b);
     };
     const bool tma_res = EPI == kResidual && args.tma_res;
     bool ok = true;
@@ -578,7 +546,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
       const int n0 = (tile % n_tiles) * BN;
       // chunk order: the columns shared with the other accumulator first (the first
       // accumulator's last two chunks, the second's first two)
-      const int first = S::kOverlap && buf == 0 ? 2 : 0;  // kChunks is 4 then
+      const int first = buf == 0 ? 2 : 0;
       auto residual = [&](int c) {  // the chunk's residual on its way into the staging buffer
         if (lane == 0) {
           tma_store_wait_read<0>();  // the last store has left the buffer
@@ -587,8 +555,8 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
         }
       };
       bool coming = false;  // a residual load of this warp is in flight
-      if (tma_res && ok && sub < kChunks && n0 + ((S::kOverlap ? (sub + first) & 3 : sub)) * 64 < args.N) {
-        residual((S::kOverlap ? (sub + first) & 3 : sub));
+      if (tma_res && ok && n0 + (sub + first) * 64 < args.N) {
+        residual(sub + first);
         coming = true;
       }
       uint64_t sa2[4];
@@ -608,7 +576,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
         reinterpret_cast<__nv_bfloat16*>(sBias)[et] = cb;
         if (EPI == kResidual) reinterpret_cast<__nv_bfloat16*>(sGate)[et] = cg;
       }
-      asm volatile("bar.sync 1, %0;" ::"r"(S::kEpiWarps * 32) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"r"(kEpiWarps * 32) : "memory");
       columns(tile + units);
       // a warp whose wait ran out goes on to the barriers above, which its neighbours may be at,
       // and to the end of its own load, and does nothing else
@@ -621,7 +589,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * S::kAcc1);
 #pragma unroll 1
       for (int i = sub; i < kChunks; i += G) {
-        const int c = S::kOverlap ? (i + first) & 3 : i;
+        const int c = (i + first) & 3;
         const int col0 = n0 + c * 64;
         const bool cols_ok = col0 < args.N;  // warp-uniform
         uint32_t r[64];
@@ -629,7 +597,7 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
         tmem_ld_16x256b_x8(acc + (uint32_t)(c * 64), r);
         tmem_ld_16x256b_x8(acc + (uint32_t)(c * 64) + (16u << 16), r + 32);
         tmem_ld_wait();
-        if (S::kOverlap ? i < 2 : i + G >= kChunks) release(buf);
+        if (i == sub) release(buf);
         uint64_t v[4][8];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -756,16 +724,10 @@ __global__ void __launch_bounds__(64 + 32 * epi_warps(BN), 1)
     if (lane == 0) tma_store_wait0();
   }
   tc_fence_before();
-  if (PAIR)
-    cluster_sync_all();
-  else
-    __syncthreads();
+  cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    if (PAIR)
-      tmem_dealloc_pair(tmem, 512);
-    else
-      tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -1095,9 +1057,9 @@ static int operand_maps(const Args& a, const Operand& A, const Operand& W, int r
                       (uint32_t)bands_b);
 }
 
-template <int FMT, int BN, int EPI, bool PAIR>
+template <int FMT, int EPI>
 static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_t st) {
-  using S = Shape<FMT, BN, EPI, PAIR>;
+  using S = Shape<FMT, EPI>;
   CUtensorMap tmA, tmB, tmSfA, tmSfB, tmO, tmR;
   int rc = operand_maps<FMT>(a, A, W, S::kRowsB, S::kSfTilesB, tmA, tmB, tmSfA, tmSfB);
   if (rc) return rc;
@@ -1117,7 +1079,7 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
                       (uint64_t)a.M, (uint64_t)a.ldr * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
-  auto kern = fp4_gemm_kernel<FMT, BN, EPI, PAIR>;
+  auto kern = fp4_gemm_kernel<FMT, EPI>;
   constexpr size_t smem = S::kSmem;
   static_assert(smem <= 227 * 1024, "fp4 gemm: shared memory");
   static bool configured[64] = {false};
@@ -1125,8 +1087,8 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   int dev = 0;
   FVB_CUDA_TRY(cudaGetDevice(&dev), "fp4 gemm device");
   FVB_REQUIRE(dev >= 0 && dev < 64, "fp4 gemm: device ordinal %d", dev);
-  constexpr int TM = PAIR ? 2 * BM : BM;
-  const int64_t n_tiles64 = (int64_t)((a.M + TM - 1) / TM) * ((a.N + BN - 1) / BN);
+  constexpr int TM = 2 * BM;
+  const int64_t n_tiles64 = (int64_t)((a.M + TM - 1) / TM) * ((a.N + S::BN - 1) / S::BN);
   FVB_REQUIRE(n_tiles64 < (1ll << 31) - 4096, "fp4 gemm: too many output tiles");
   const int num = (int)n_tiles64;
   cudaLaunchConfig_t cfg = {};
@@ -1134,33 +1096,23 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  if (PAIR) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (!configured[dev]) {
     FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                  "fp4 gemm smem attribute");
-    if (PAIR) {
-      int clusters = 0;
-      cfg.gridDim = dim3(2 * (sm_count() / 2));
-      FVB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg),
-                   "fp4 gemm cluster occupancy");
-      FVB_REQUIRE(clusters > 0, "fp4 gemm: no 2-CTA cluster fits on this device");
-      pair_slots[dev] = clusters;
-    }
+    int clusters = 0;
+    cfg.gridDim = dim3(2 * (sm_count() / 2));
+    FVB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg), "fp4 gemm cluster occupancy");
+    FVB_REQUIRE(clusters > 0, "fp4 gemm: no 2-CTA cluster fits on this device");
+    pair_slots[dev] = clusters;
     configured[dev] = true;
   }
-  int grid;
-  if (PAIR)
-    grid = 2 * (num < pair_slots[dev] ? num : pair_slots[dev]);
-  else
-    grid = num < sm_count() ? num : sm_count();
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = dim3(2 * (num < pair_slots[dev] ? num : pair_slots[dev]));
   FVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmSfA, tmSfB, tmO, tmR, a),
                "fp4 gemm launch");
   return check_launch("fp4 gemm");
@@ -1225,7 +1177,7 @@ static int dispatch(const Args& a, const Operand& A, const Operand& W, cudaStrea
       best = z;
     }
   }
-  if (pair_cost <= split_cost) return launch<FMT, 256, EPI, true>(a, A, W, st);
+  if (pair_cost <= split_cost) return launch<FMT, EPI>(a, A, W, st);
   return best > 1 ? launch_split<FMT, EPI, true>(a, A, W, best, st)
                   : launch_split<FMT, EPI, false>(a, A, W, 1, st);
 }
