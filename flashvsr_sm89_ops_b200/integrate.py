@@ -19,7 +19,11 @@ B200 fast path taken when every op of the block is on this pack:
 
 Extra flags of this pack: FS89_FP8_SCALE=token|tensor (activation granularity;
 ``tensor`` reproduces the reference's per-tensor numerics), FS89_FUSED_MASK=1
-(device keep-mask builder instead of upstream generate_draft_block_mask).
+(device keep-mask builder instead of upstream generate_draft_block_mask),
+FS89_FP4=ffn[,self,cross] (those parts in microscaled 4 bits instead of FP8; off by
+default) and FS89_FP4_FMT=nv|mx (the format of their inputs).  With FS89_FP4=ffn the
+block's FFN half runs as: cross-attention add + LN-mod emitting 4-bit codes -> 4-bit
+product with GELU and a 4-bit hidden state -> 4-bit product with the gated residual.
 """
 from __future__ import annotations
 
@@ -30,11 +34,13 @@ import torch
 
 from . import lcsa
 from .compat_bsa import active_backend, ensure_bsa_available
+from .fp4_linear import FP4FFN, convert_linears_fp4
 from .fp8_ffn import FP8FFN, convert_ffn_fp8, ffn_fp8
 from .fp8_linear import FP8Linear, convert_linears_fp8, fp8_mm
 from .fp8_quant import default_act_mode, quantize_fp8
 from .fused_adaln import (fused_gate_add, fused_ln_modulate, fused_ln_modulate_adaln,
                           gate_add_layer_norm, gate_add_ln_modulate, layer_norm)
+from .fused_residual_norm import fused_residual_norm
 from .fused_rms_rope import freqs_cos_sin, fused_rms_rope, qkv_rope_window, rms_rope_rows
 
 
@@ -420,7 +426,15 @@ def _make_dit_block_forward(dit):
             x = x + self.cross_attn(self.norm3(x), context, is_stream=is_stream)
         if fa is not None:
             ffn = self.ffn
-            if ca_out is not None and token and isinstance(ffn, FP8FFN) \
+            if ca_out is not None and isinstance(ffn, FP4FFN):
+                # cross-attention add and norm2 in one pass that emits the FFN's 4-bit input,
+                # then the FFN with the block's closing gated residual add
+                x, _, x4 = fused_residual_norm(x, ca_out, norm="layer", scale=scale_mlp,
+                                               shift=shift_mlp, eps=_module_eps(self.norm2),
+                                               emit_fp4=ffn.lin0.fmt, want_out=False)
+                x = ffn.ffn(x4, residual=x, gate=gate_mlp).view(x.shape)
+                y = None
+            elif ca_out is not None and token and isinstance(ffn, FP8FFN) \
                     and ffn.lin0.mode == "token":
                 # cross-attention add and norm2 in one pass; the FFN reads only the FP8 codes
                 x, _, x8, s8 = gate_add_ln_modulate(x, None, ca_out, scale_mlp, shift_mlp,
@@ -493,15 +507,20 @@ def _patch_dit(dit, fused_rope, fused_adaln):
     dit._FS89_PATCHED = True
 
 
-def enable(pipe, dit_module=None, parts=None, compile_memblocks=None, verbose=True):
+def enable(pipe, dit_module=None, parts=None, compile_memblocks=None, verbose=True,
+           fp4_parts=None):
     """Apply the B200 operator pack to a FlashVSR Tiny pipeline (integrate.py:229-292).
 
-    Call once after ``pipe.enable_vram_management(...)`` and before
+    fp4_parts (default: FS89_FP4, empty): parts that run in microscaled 4 bits, taken out of
+    `parts`.  Call once after ``pipe.enable_vram_management(...)`` and before
     ``pipe.init_cross_kv()``.  Returns a dict of what was enabled.  Re-running it on
     an already patched pipeline is safe.
     """
     if parts is None:
         parts = [p for p in os.environ.get("FS89_FP8", "ffn,self,cross").split(",") if p]
+    if fp4_parts is None:
+        fp4_parts = [p for p in os.environ.get("FS89_FP4", "").split(",") if p]
+    parts = [p for p in parts if p not in fp4_parts]
     if compile_memblocks is None:
         compile_memblocks = _FLAG("FS89_TCDEC_COMPILE", "0")
     applied = {}
@@ -530,6 +549,10 @@ def enable(pipe, dit_module=None, parts=None, compile_memblocks=None, verbose=Tr
                 n += 1
         applied["tcdec_compiled_memblocks"] = n
 
+    if fp4_parts:
+        fmt = os.environ.get("FS89_FP4_FMT", "nv")
+        applied["fp4_linears"] = convert_linears_fp4(pipe.denoising_model(), parts=fp4_parts, fmt=fmt)
+        applied["fp4_format"] = fmt
     if parts:
         mode = default_act_mode()
         model = pipe.denoising_model()

@@ -620,3 +620,64 @@ def test_refusals():
             f()
             pytest.fail(f"case {i} was accepted")
     torch.cuda.synchronize()
+
+
+# ----------------------------------------------------------------------------- the model's path
+@pytest.mark.parametrize("fmt", FMTS)
+def test_block_with_a_4bit_ffn(fmt, monkeypatch):
+    """enable() with FS89_FP4=ffn: the block's FFN half equals its definition in 64 bits on the
+    tensors that reached it, and the FP8 half before it is untouched."""
+    from flashvsr_sm89_ops_b200 import FP4FFN, _lib, integrate
+    from flashvsr_sm89_ops_b200 import wan_video_dit as W
+    from oracle import wan as OW
+    f, h, w = 2, 16, 24
+    P, x, t_mod, ctx, cache = OW.block_case(seed=4, f=f, h=h, w=w)
+    W.MASK_RULE = "causal"
+    state = OW.standin_state_dict(P)
+
+    def block(fp4):
+        dit = W.WanDiT(num_layers=1).to(torch.bfloat16)
+        dit.blocks[0].load_state_dict(state, strict=True)
+        dit = dit.to(DEV)
+        monkeypatch.setenv("FS89_FP4", "ffn" if fp4 else "")
+        monkeypatch.setenv("FS89_FP4_FMT", fmt)
+        applied = integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False)
+        assert applied.get("fp4_linears") == (2 if fp4 else None)
+        assert integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False).get("fp4_linears", 0) == 0
+        dit.init_cross_kv(ctx.to(DEV))
+        return dit
+
+    def run(dit):
+        fr = W.grid_freqs(dit.freqs, f, h, w, f0=6).to(DEV)
+        with torch.no_grad():
+            return dit.blocks[0](x.to(DEV), None, t_mod.to(DEV), fr, f, h, w, kv_len=3, is_stream=True,
+                                 pre_cache_k=cache[0].to(DEV), pre_cache_v=cache[1].to(DEV))
+
+    y8, k8, v8 = run(block(False))
+    dit = block(True)
+    ffn = dit.blocks[0].ffn
+    assert isinstance(ffn, FP4FFN) and ffn.lin0.fmt == fmt and ffn.lin2.fmt == "mx"
+    seen = {}
+    seam = integrate.fused_residual_norm
+
+    def spy(xx, yy, **kw):
+        seen.update(x=xx.clone(), y=yy.clone(), kw=kw)
+        return seam(xx, yy, **kw)
+
+    monkeypatch.setattr(integrate, "fused_residual_norm", spy)
+    y4, k4, v4 = run(dit)
+    assert torch.equal(k4, k8) and torch.equal(v4, v8)
+    kw = seen["kw"]
+    D = x.shape[-1]
+    xn, hn = R.residual_norm(seen["x"], seen["y"], norm_kind="layer", scale=kw["scale"], shift=kw["shift"],
+                             eps=kw["eps"])
+    a = R.quantize(hn.reshape(-1, D), fmt)[0]
+    u = a @ R.quantize(state["ffn.0.weight"].to(DEV), fmt)[0].t() + state["ffn.0.bias"].to(DEV).double()
+    hq = R.quantize(R.gelu_tanh(u), "mx")[0]
+    o = hq @ R.quantize(state["ffn.2.weight"].to(DEV), "mx")[0].t() + state["ffn.2.bias"].to(DEV).double()
+    mod = dit.blocks[0].modulation.double() + t_mod.to(DEV).double()
+    want = xn.reshape(-1, D).to(torch.bfloat16).double() + mod[:, 5] * o
+    err = ((y4.double().reshape(-1, D) - want).norm() / want.norm()).item()
+    # bf16 modulation and result: a few 2^-9 relative
+    assert err < 4 * 2.0 ** -9, err
+    assert _lib.device_error() == 0
