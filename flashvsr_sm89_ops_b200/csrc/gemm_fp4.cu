@@ -33,7 +33,8 @@
 // reads 32 KB and writes 38 KB per CTA in the 512 clocks of its MMAs.  So the epilogue reads
 // TMEM in the 16x256b shape, where a thread holds 2 columns of every 8 for 4 rows: a 64-column
 // chunk's scales and biases then cost a warp 24 wavefronts of shared memory, where a thread
-// that holds a whole row reads all 64 columns' and costs it 128.
+// that holds a whole row reads all 64 columns' and costs it 128.  They travel by shuffles, each
+// warp with the two columns a lane that it read one chunk ahead: no barrier between the warps.
 #include "fp4.cuh"
 
 namespace fvb {
@@ -47,10 +48,13 @@ constexpr int kStageCodes = 32 * 32;  // with GELU: 32 rows x 64 codes
 
 enum { kPlain = 0, kResidual = 1, kGeluMx = 2 };
 
-// epilogue warps: two per TMEM lane quarter.  Four, one for each 64-column chunk, left
-// the GELU epilogue 96 registers a thread and measured 119 us against 102 (8448 x 8960 x 1536
-// with a small second product); for the others their staging buffers would cost a ring stage.
-constexpr int kEpiWarps = 8;
+// Epilogue warps per TMEM lane quarter.  The GELU epilogue is the longer part of its product
+// (two special functions and the codes for every element), so it has three: they take the
+// 64-column chunks of successive tiles in turn and drift out of step, so that one's special
+// functions run beside another's sums and conversions.  Four left 96 registers a thread and
+// spilled; two measured 102 us (8448 x 8960 x 1536 and a small second product).  The others
+// need a 4 KB staging buffer a warp, and a third would cost them a ring stage.
+__host__ __device__ constexpr int epi_per_quarter(int epi) { return epi == kGeluMx ? 3 : 2; }
 
 struct Args {
   int M, N, K;
@@ -72,10 +76,10 @@ struct Args {
 template <int FMT, int EPI>
 struct Shape {
   static constexpr int BN = 256;
+  static constexpr int kEpiWarps = 4 * epi_per_quarter(EPI);
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kOut = EPI == kGeluMx ? kStageCodes : kStageOut;
   static constexpr int kOutBytes = kEpiWarps * kOut;
-  static constexpr int kColBytes = 2 * 2 * BN * 4;  // two tiles' column scales (fp32), biases and gates (bf16)
   static constexpr int kTilesK = FMT == FVB_FP4_NV ? 4 : 2;  // scale tiles per K block
   static constexpr int kMmas = 4 / kTilesK;                  // MMAs (K = 64) per scale tile
   static constexpr int kRowsB = BN / 2;                      // W rows a CTA of the pair stages
@@ -85,7 +89,7 @@ struct Shape {
   static constexpr int kBytesSfA = kTilesK * 512;
   static constexpr int kBytesSfB = kTilesK * kSfTilesB * 512;
   static constexpr int kBytes = kBytesA + kBytesB + kBytesSfA + kBytesSfB;
-  static constexpr int kFixed = kOutBytes + kColBytes + 1024 /*align*/ + 384 /*barriers*/;
+  static constexpr int kFixed = kOutBytes + 1024 /*align*/ + 384 /*barriers*/;
   static constexpr int kFit = (227 * 1024 - kFixed) / kBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr size_t kSmem = (size_t)kStages * kBytes + kFixed;
@@ -298,7 +302,7 @@ __device__ __forceinline__ void gelu_mx(uint64_t (&v)[4][8], int col0, int N, in
 }
 
 template <int FMT, int EPI>
-__global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
+__global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSfA,
                     const __grid_constant__ CUtensorMap tmSfB,
@@ -316,14 +320,14 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
   uint8_t* sSfA = sB + STAGES * S::kBytesB;
   uint8_t* sSfB = sSfA + STAGES * S::kBytesSfA;
   uint8_t* sOut = sSfB + STAGES * S::kBytesSfB;
-  float* sCol = reinterpret_cast<float*>(sOut + S::kOutBytes);  // [2 tiles][2][BN]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::kOutBytes + S::kColBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + S::kOutBytes);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;   // [2] accumulator finished
-  uint64_t* tempty = tfull + 2;       // [2] accumulator read
-  uint64_t* drain = tempty + 2;       // every MMA this CTA issued finished
+  uint64_t* tempty = tfull + 2;       // [2] the columns shared with the other accumulator read
+  uint64_t* tdone = tempty + 2;       // [2] the other columns read
+  uint64_t* drain = tdone + 2;        // every MMA this CTA issued finished
   uint64_t* rfull = drain + 1;        // [epilogue warps] residual arrived
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + kEpiWarps);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + S::kEpiWarps);
   uint32_t* pair_ok = tmem_slot + 1;
 
   const int warp = warp_id_uniform();
@@ -343,10 +347,11 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 2 * kEpiWarps);
+      mbar_init(&tempty[b], 16);  // 2 CTAs x 4 lane quarters x 2 chunks
+      mbar_init(&tdone[b], 16);
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < kEpiWarps; ++w) mbar_init(&rfull[w], 1);
+    for (int w = 0; w < S::kEpiWarps; ++w) mbar_init(&rfull[w], 1);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -438,9 +443,11 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
       bool ok = true, any = false;
       for (int tile = unit; tile < num_tiles && ok; tile += units, ++t) {
         const int buf = t & 1;
-        // until the columns shared with the previous tile were read; the warps that arrive there
-        // have read all of the tile before it
-        const bool clear = t == 0 || mbar_wait(&tempty[buf ^ 1], (uint32_t)((t - 1) >> 1) & 1u, 0x402u);
+        // until the columns shared with the previous tile were read, and the others of the tile
+        // before it, whose accumulator this is
+        const bool clear =
+            (t < 1 || mbar_wait(&tempty[buf ^ 1], (uint32_t)((t - 1) >> 1) & 1u, 0x402u)) &&
+            (t < 2 || mbar_wait(&tdone[buf], (uint32_t)((t - 2) >> 1) & 1u, 0x407u));
         if (!__all_sync(0xffffffffu, clear)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * S::kAcc1);
@@ -510,94 +517,89 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    constexpr int G = kEpiWarps / 4;  // warps per TMEM lane quarter
-    constexpr int kChunks = BN / 64;
-    const int q = warp & 3;              // TMEM lane quarter this warp may access
-    const int sub = (warp - 2) >> 2;     // its first chunk
-    const int et = (int)threadIdx.x - 64;
+    // A tile is four 64-column chunks; chunk n = 4 * (tile's number) + position goes to the warp
+    // n % G of its lane quarter.  Positions 0 and 1 are the columns shared with the other
+    // accumulator (the first accumulator's last two chunks, the second's first two).
+    constexpr int G = epi_per_quarter(EPI);
+    const int q = warp & 3;  // TMEM lane quarter this warp may access
     const int lr = lane >> 2, lc = 2 * (lane & 3);  // this thread's rows lr + 8 k, columns 8 g + lc + {0, 1}
     uint8_t* stg = sOut + (size_t)(warp - 2) * S::kOut;
     uint64_t* rbar = &rfull[warp - 2];
-    // the tile's column vectors go through shared memory: read from global one tile ahead,
-    // so that no thread waits for them between the accumulator and the store
-    float cs = 1.f;
-    __nv_bfloat16 cb = __float2bfloat16_rn(0.f), cg = __float2bfloat16_rn(1.f);
-    auto columns = [&](int tile) {
-      const int c = (tile % n_tiles) * BN + et;
-      if (tile < num_tiles && et < BN && c < args.N) {
-        if (args.sw) cs = __ldg(args.sw + (args.sw_row ? c : 0));
-        if (args.bias) cb = args.bias[c];
-        if (EPI == kResidual && args.gate) cg = args.gate[c];
-      }
-    };
-    columns(unit);
-    auto release = [&](int b) {
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote_relaxed(tempty0_c + 8u * b);
-    };
+    const uint32_t tdone0_c = mapa_shared(smem_u32(tdone), 0u);
     const bool tma_res = EPI == kResidual && args.tma_res;
-    bool ok = true;
-    int t = 0;
-    uint32_t rphase = 0;
-    for (int tile = unit; tile < num_tiles; tile += units, ++t) {
-      const int buf = t & 1;
-      const int m0 = (tile / n_tiles) * TM + (int)rank * BM + q * 32;
-      const int n0 = (tile % n_tiles) * BN;
-      // chunk order: the columns shared with the other accumulator first (the first
-      // accumulator's last two chunks, the second's first two)
-      const int first = buf == 0 ? 2 : 0;
-      auto residual = [&](int c) {  // the chunk's residual on its way into the staging buffer
-        if (lane == 0) {
-          tma_store_wait_read<0>();  // the last store has left the buffer
-          mbar_arrive_expect_tx(rbar, kStageOut);
-          tma_load_2d(stg, &tmRes, rbar, n0 + c * 64, m0);
+    // the column vectors of a chunk, two columns a lane, read one chunk ahead; the lanes that
+    // need them get them by shuffles
+    struct Columns {
+      float s0, s1;
+      uint32_t b, g;  // bf16 pairs
+    };
+    auto place = [&](int n, int& m0, int& col0) {  // false past the last tile
+      const int tile = unit + (n >> 2) * units;
+      if (tile >= num_tiles) return false;
+      m0 = (tile / n_tiles) * TM + (int)rank * BM + q * 32;
+      col0 = (tile % n_tiles) * BN + (((n & 3) + (n & 4 ? 0 : 2)) & 3) * 64;
+      return true;
+    };
+    auto columns = [&](int n) {
+      Columns c = {1.f, 1.f, 0u, 0x3F803F80u};
+      int m0, col0;
+      if (place(n, m0, col0)) {
+        const int col = col0 + 2 * lane;
+        if (args.sw) {
+          if (col < args.N) c.s0 = __ldg(args.sw + (args.sw_row ? col : 0));
+          if (col + 1 < args.N) c.s1 = __ldg(args.sw + (args.sw_row ? col + 1 : 0));
         }
-      };
-      bool coming = false;  // a residual load of this warp is in flight
-      if (tma_res && ok && n0 + (sub + first) * 64 < args.N) {
-        residual(sub + first);
-        coming = true;
+        auto pair = [&](const __nv_bfloat16* p, uint32_t& d) {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(p) + col;
+          if (col < args.N) d = (d & 0xFFFF0000u) | __ldg(u);
+          if (col + 1 < args.N) d = (d & 0xFFFFu) | ((uint32_t)__ldg(u + 1) << 16);
+        };
+        if (args.bias) pair(args.bias, c.b);
+        if (EPI == kResidual && args.gate) pair(args.gate, c.g);
       }
-      uint64_t sa2[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = m0 + lr + 8 * k;
-        float sa = 1.f;
-        if (args.sa) sa = args.sa_row ? (row < args.M ? __ldg(args.sa + row) : 0.f) : __ldg(args.sa);
-        sa2[k] = f2_pack(sa, sa);
-      }
-      // two tiles' vectors: whoever passes this tile's barrier has read the last but one's
-      float* sScale = sCol + buf * 2 * BN;
-      __nv_bfloat162* sBias = reinterpret_cast<__nv_bfloat162*>(sScale + BN);
-      __nv_bfloat162* sGate = sBias + BN / 2;
-      if (et < BN) {
-        sScale[et] = cs;
-        reinterpret_cast<__nv_bfloat16*>(sBias)[et] = cb;
-        if (EPI == kResidual) reinterpret_cast<__nv_bfloat16*>(sGate)[et] = cg;
-      }
-      asm volatile("bar.sync 1, %0;" ::"r"(kEpiWarps * 32) : "memory");
-      columns(tile + units);
-      // a warp whose wait ran out goes on to the barriers above, which its neighbours may be at,
-      // and to the end of its own load, and does nothing else
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&tfull[buf], (uint32_t)(t >> 1) & 1u, 0x404u));
-      if (!ok) {
-        if (coming) mbar_wait(rbar, rphase, 0x406u);
-        continue;
-      }
-      tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * S::kAcc1);
+      return c;
+    };
+    auto unpack = [](uint32_t w) {
+      return f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    };
+    int n = (warp - 2) >> 2, m0, col0;
+    Columns ahead = columns(n);
+    uint32_t rphase = 0;
 #pragma unroll 1
-      for (int i = sub; i < kChunks; i += G) {
-        const int c = (i + first) & 3;
-        const int col0 = n0 + c * 64;
-        const bool cols_ok = col0 < args.N;  // warp-uniform
+    for (; place(n, m0, col0); n += G) {
+      const int t = n >> 2, buf = t & 1;
+      const bool cols_ok = col0 < args.N;  // warp-uniform
+      {
+        if (tma_res && cols_ok && lane == 0) {  // the chunk's residual into the staging buffer
+          tma_store_wait_read<0>();               // which the last store has left
+          mbar_arrive_expect_tx(rbar, kStageOut);
+          tma_load_2d(stg, &tmRes, rbar, col0, m0);
+        }
+        const Columns cols = ahead;
+        ahead = columns(n + G);
+        uint64_t sa2[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = m0 + lr + 8 * k;
+          float sa = 1.f;
+          if (args.sa) sa = args.sa_row ? (row < args.M ? __ldg(args.sa + row) : 0.f) : __ldg(args.sa);
+          sa2[k] = f2_pack(sa, sa);
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&tfull[buf], (uint32_t)(t >> 1) & 1u, 0x404u))) {
+          if (tma_res && cols_ok) mbar_wait(rbar, rphase, 0x406u);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) +
+                             (uint32_t)(buf * S::kAcc1 + (((n & 3) + (n & 4 ? 0 : 2)) & 3) * 64);
         uint32_t r[64];
         // v[k][g]: row lr + 8 k, columns 8 g + lc and the next, as an fp32 pair
-        tmem_ld_16x256b_x8(acc + (uint32_t)(c * 64), r);
-        tmem_ld_16x256b_x8(acc + (uint32_t)(c * 64) + (16u << 16), r + 32);
+        tmem_ld_16x256b_x8(acc, r);
+        tmem_ld_16x256b_x8(acc + (16u << 16), r + 32);
         tmem_ld_wait();
-        if (i == sub) release(buf);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote_relaxed(((n & 3) < 2 ? tempty0_c : tdone0_c) + 8u * buf);
         uint64_t v[4][8];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -609,11 +611,11 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
         if (cols_ok) {
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
-            const float2 b = __bfloat1622float2(sBias[(c * 64 + g * 8 + lc) >> 1]);
-            const uint64_t b2 = f2_pack(b.x, b.y);
+            const int from = 4 * g + (lane & 3);
+            const uint64_t b2 = unpack(__shfl_sync(0xffffffffu, cols.b, from));
             if (args.sw) {
-              const float2 s = *reinterpret_cast<const float2*>(sScale + c * 64 + g * 8 + lc);
-              const uint64_t s2 = f2_pack(s.x, s.y);
+              const uint64_t s2 = f2_pack(__shfl_sync(0xffffffffu, cols.s0, from),
+                                          __shfl_sync(0xffffffffu, cols.s1, from));
 #pragma unroll
               for (int k = 0; k < 4; ++k) v[k][g] = f2_fma(v[k][g], f2_mul(sa2[k], s2), b2);
             } else {
@@ -650,9 +652,7 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
         const uint32_t srow = smem_u32(stg) + lane * 128;
         if (EPI == kResidual) {
           if (tma_res) {
-            if (i != sub) residual(c);
-            ok = __all_sync(0xffffffffu, mbar_wait(rbar, rphase, 0x406u));
-            if (!ok) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(rbar, rphase, 0x406u))) break;
             rphase ^= 1u;
           }
 #pragma unroll
@@ -671,11 +671,10 @@ __global__ void __launch_bounds__(64 + 32 * kEpiWarps, 1)
                 x[k] = *reinterpret_cast<uint32_t*>(&p);
               }
             }
-            const float2 gt = __bfloat1622float2(sGate[(c * 64 + g * 8 + lc) >> 1]);
+            const uint64_t g2 = unpack(__shfl_sync(0xffffffffu, cols.g, 4 * g + (lane & 3)));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const float2 xf = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[k]));
-              v[k][g] = f2_fma(f2_pack(gt.x, gt.y), v[k][g], f2_pack(xf.x, xf.y));
+              v[k][g] = f2_fma(g2, v[k][g], unpack(x[k]));
             }
           }
         }
