@@ -527,11 +527,12 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
     uint64_t* rbar = &rfull[warp - 2];
     const uint32_t tdone0_c = mapa_shared(smem_u32(tdone), 0u);
     const bool tma_res = EPI == kResidual && args.tma_res;
-    // the column vectors of a chunk, two columns a lane, read one chunk ahead; the lanes that
-    // need them get them by shuffles
-    struct Columns {
-      float s0, s1;
-      uint32_t b, g;  // bf16 pairs
+    // A chunk's vectors, two columns and four rows a lane, loaded one chunk ahead and left as they
+    // arrive (any arithmetic on them here would wait for the loads); the lanes that need a column
+    // get it by shuffles
+    struct Vectors {
+      float s0, s1, sa[4];
+      uint16_t b0, b1, g0, g1;
     };
     auto place = [&](int n, int& m0, int& col0) {  // false past the last tile
       const int tile = unit + (n >> 2) * units;
@@ -540,22 +541,27 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
       col0 = (tile % n_tiles) * BN + (((n & 3) + (n & 4 ? 0 : 2)) & 3) * 64;
       return true;
     };
-    auto columns = [&](int n) {
-      Columns c = {1.f, 1.f, 0u, 0x3F803F80u};
+    auto vectors = [&](int n) {
+      Vectors c = {1.f, 1.f, {1.f, 1.f, 1.f, 1.f}, 0, 0, 0x3F80, 0x3F80};
       int m0, col0;
       if (place(n, m0, col0)) {
         const int col = col0 + 2 * lane;
-        if (args.sw) {
-          if (col < args.N) c.s0 = __ldg(args.sw + (args.sw_row ? col : 0));
-          if (col + 1 < args.N) c.s1 = __ldg(args.sw + (args.sw_row ? col + 1 : 0));
+        const bool in0 = col < args.N, in1 = col + 1 < args.N;
+        const uint16_t* bias = reinterpret_cast<const uint16_t*>(args.bias) + col;
+        const uint16_t* gate = reinterpret_cast<const uint16_t*>(args.gate) + col;
+        if (args.sw && in0) c.s0 = __ldg(args.sw + (args.sw_row ? col : 0));
+        if (args.sw && in1) c.s1 = __ldg(args.sw + (args.sw_row ? col + 1 : 0));
+        if (args.bias && in0) c.b0 = __ldg(bias);
+        if (args.bias && in1) c.b1 = __ldg(bias + 1);
+        if (EPI == kResidual && args.gate && in0) c.g0 = __ldg(gate);
+        if (EPI == kResidual && args.gate && in1) c.g1 = __ldg(gate + 1);
+        if (args.sa) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = m0 + lr + 8 * k;
+            if (row < args.M) c.sa[k] = __ldg(args.sa + (args.sa_row ? row : 0));
+          }
         }
-        auto pair = [&](const __nv_bfloat16* p, uint32_t& d) {
-          const uint16_t* u = reinterpret_cast<const uint16_t*>(p) + col;
-          if (col < args.N) d = (d & 0xFFFF0000u) | __ldg(u);
-          if (col + 1 < args.N) d = (d & 0xFFFFu) | ((uint32_t)__ldg(u + 1) << 16);
-        };
-        if (args.bias) pair(args.bias, c.b);
-        if (EPI == kResidual && args.gate) pair(args.gate, c.g);
       }
       return c;
     };
@@ -563,7 +569,7 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
       return f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     };
     int n = (warp - 2) >> 2, m0, col0;
-    Columns ahead = columns(n);
+    Vectors ahead = vectors(n);
     uint32_t rphase = 0;
 #pragma unroll 1
     for (; place(n, m0, col0); n += G) {
@@ -575,16 +581,12 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
           mbar_arrive_expect_tx(rbar, kStageOut);
           tma_load_2d(stg, &tmRes, rbar, col0, m0);
         }
-        const Columns cols = ahead;
-        ahead = columns(n + G);
+        const Vectors vec = ahead;
+        ahead = vectors(n + G);
+        const uint32_t bias = __byte_perm(vec.b0, vec.b1, 0x5410);
         uint64_t sa2[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = m0 + lr + 8 * k;
-          float sa = 1.f;
-          if (args.sa) sa = args.sa_row ? (row < args.M ? __ldg(args.sa + row) : 0.f) : __ldg(args.sa);
-          sa2[k] = f2_pack(sa, sa);
-        }
+        for (int k = 0; k < 4; ++k) sa2[k] = f2_pack(vec.sa[k], vec.sa[k]);
         if (!__all_sync(0xffffffffu, mbar_wait(&tfull[buf], (uint32_t)(t >> 1) & 1u, 0x404u))) {
           if (tma_res && cols_ok) mbar_wait(rbar, rphase, 0x406u);
           break;
@@ -612,10 +614,10 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             const int from = 4 * g + (lane & 3);
-            const uint64_t b2 = unpack(__shfl_sync(0xffffffffu, cols.b, from));
+            const uint64_t b2 = unpack(__shfl_sync(0xffffffffu, bias, from));
             if (args.sw) {
-              const uint64_t s2 = f2_pack(__shfl_sync(0xffffffffu, cols.s0, from),
-                                          __shfl_sync(0xffffffffu, cols.s1, from));
+              const uint64_t s2 = f2_pack(__shfl_sync(0xffffffffu, vec.s0, from),
+                                          __shfl_sync(0xffffffffu, vec.s1, from));
 #pragma unroll
               for (int k = 0; k < 4; ++k) v[k][g] = f2_fma(v[k][g], f2_mul(sa2[k], s2), b2);
             } else {
@@ -655,6 +657,7 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
             if (!__all_sync(0xffffffffu, mbar_wait(rbar, rphase, 0x406u))) break;
             rphase ^= 1u;
           }
+          const uint32_t gate = __byte_perm(vec.g0, vec.g1, 0x5410);
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             uint32_t x[4];
@@ -671,7 +674,7 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
                 x[k] = *reinterpret_cast<uint32_t*>(&p);
               }
             }
-            const uint64_t g2 = unpack(__shfl_sync(0xffffffffu, cols.g, 4 * g + (lane & 3)));
+            const uint64_t g2 = unpack(__shfl_sync(0xffffffffu, gate, 4 * g + (lane & 3)));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               v[k][g] = f2_fma(g2, v[k][g], unpack(x[k]));
