@@ -7,7 +7,9 @@
 //
 // Two kernels.  Products with many output tiles run on persistent CTA pairs (cta_group::2, one
 // CTA per SM, 256 x 256 tiles of which each CTA holds 128 rows), warp-specialised; those with few
-// on a tile per cluster of CTAs that share its K loop (further down).
+// on a tile per cluster of CTAs that share its K loop (further down).  Measured: 8448 x 4608 x 1536
+// nv 33 us (3.6 PFLOP/s), mx 28.5; 8448 x 1536 x 8960 nv 46 us (5.0 PFLOP/s), with the gated
+// residual 50; the MMAs of the latter alone 36.5.
 //   warp 0      TMA producer: 256-element (128-byte) K blocks of A and W and their scale tiles
 //               into a ring of shared-memory stages
 //   warp 1      MMA issuer: copies a K block's scale tiles into TMEM (tcgen05.cp), then issues
@@ -26,7 +28,7 @@
 // A scale buffer is overwritten after a wait for the MMAs that read it: the issue order puts a
 // copy before the MMAs after it, but nothing puts an MMA before a copy after it.  The wait is on
 // the ring stage's own barrier; a commit and a wait for every scale tile measured 84.6 us on
-// 8448 x 1536 x 8960, where one for every K block takes 49.
+// 8448 x 1536 x 8960, where one for every K block took 49.
 //
 // Shared-memory bandwidth (128 bytes a clock per SM) is what the operands, their TMA writes and
 // the epilogue share, and it is nearly used up: a 256-element K block of a 256 x 256 pair tile
@@ -49,11 +51,11 @@ constexpr int kStageCodes = 32 * 32;  // with GELU: 32 rows x 64 codes
 enum { kPlain = 0, kResidual = 1, kGeluMx = 2 };
 
 // Epilogue warps per TMEM lane quarter.  The GELU epilogue is the longer part of its product
-// (two special functions and the codes for every element), so it has three: they take the
+// (1.5 special functions and the codes for every element), so it has three: they take the
 // 64-column chunks of successive tiles in turn and drift out of step, so that one's special
-// functions run beside another's sums and conversions.  Four left 96 registers a thread and
-// spilled; two measured 102 us (8448 x 8960 x 1536 and a small second product).  The others
-// need a 4 KB staging buffer a warp, and a third would cost them a ring stage.
+// functions run beside another's sums and conversions.  8448 x 8960 x 1536 (nv) measured 75 us
+// with three, 87 with two; four leave 96 registers a thread and spill.  The others need a 4 KB
+// staging buffer a warp, and a third would cost them a ring stage.
 __host__ __device__ constexpr int epi_per_quarter(int epi) { return epi == kGeluMx ? 3 : 2; }
 
 struct Args {

@@ -17,8 +17,8 @@
 // WPR warps own a row and hold it in registers as fp32 pairs, thread t the 16-byte vectors
 // t, t + 32 WPR, ...; statistics are two-pass in registers (mean, then centred squares); the
 // next row's loads go out as soon as the current row's registers are free.  Measured on
-// 2 x 8448 x 1536 (207 MB moved): 60 us with every operand unpacked for every row, see the
-// launch below for the present figure.
+// 2 x 8448 x 1536 (208 MB moved): 38.7 us, 5.4 TB/s (60 us with every operand unpacked for every
+// row, 45 instructions an element); 8448 x 1536 with nv codes for h: 20.6 us.
 #include "fp4.cuh"
 
 namespace fvb {

@@ -112,3 +112,14 @@ def test_values_reads_the_documented_layout():
     assert v[129, 78] == -6 and v[129, 79] == -0.5 and v[70, 0] == 2.0
     assert v.abs().sum() == 8.5
     assert not R.padding(FP4Tensor(codes, scales, None, (M, K), "nv")).any()
+
+
+def test_conversion_refuses_what_it_does_not_know():
+    import torch.nn as nn
+    from flashvsr_sm89_ops_b200 import convert_linears_fp4
+    model = nn.Sequential(nn.Linear(8, 8))
+    with pytest.raises(ValueError, match="unknown parts"):
+        convert_linears_fp4(model, parts=("ffn", "mlp"))
+    with pytest.raises(ValueError, match="format"):
+        convert_linears_fp4(model, fmt="int4")
+    assert convert_linears_fp4(model) == 0 and type(model[0]) is nn.Linear
