@@ -174,9 +174,15 @@ def stop_launch_count() -> int:
     return n
 
 
+_fns: dict = {}
+
+
 def call(name: str, *args):
     global _count
-    rc = getattr(load(), name)(*args)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != FVB_OK:
         _raise(rc, name)
     if _count is not None:

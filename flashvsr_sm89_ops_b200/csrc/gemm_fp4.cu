@@ -494,21 +494,20 @@ __global__ void __launch_bounds__(64 + 128 * epi_per_quarter(EPI), 1)
                                    sfa + 4u * i, sfb + 4u * S::kSfTilesB * i,
                                    (kb | ks) != 0 ? 1u : 0u);
             }
+            tc_commit_pair_both(&empty[stage], 0x3);
+            if (kb + 1 == kblocks) tc_commit_pair_both(&tfull[buf], 0x3);
           }
+          __syncwarp();
           any = true;
           if (++sbuf == S::kSfBufs) {
             sbuf = 0;
             reuse = true;
           }
-          if (leader) tc_commit_pair_both(&empty[stage], 0x3);
-          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok && leader) tc_commit_pair_both(&tfull[buf], 0x3);
-        __syncwarp();
       }
       // every MMA issued above completes before TMEM is freed
       if (any) {

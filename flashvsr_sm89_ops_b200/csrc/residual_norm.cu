@@ -17,7 +17,7 @@
 // WPR warps own a row and hold it in registers as fp32 pairs, thread t the 16-byte vectors
 // t, t + 32 WPR, ...; statistics are two-pass in registers (mean, then centred squares); the
 // next row's loads go out as soon as the current row's registers are free.  Measured on
-// 2 x 8448 x 1536 (208 MB moved): 38.7 us, 5.4 TB/s (60 us with every operand unpacked for every
+// 2 x 8448 x 1536 (208 MB moved): 37.4 us, 5.6 TB/s (60 us with every operand unpacked for every
 // row, 45 instructions an element); 8448 x 1536 with nv codes for h: 20.6 us.
 #include "fp4.cuh"
 
@@ -430,7 +430,9 @@ extern "C" int fvb_residual_norm(const void* x, const void* y, const void* gate,
   if (D <= 256) return resnorm::launch<1, 1>(a, B, st);
   if (D <= 512) return resnorm::launch<2, 1>(a, B, st);
   if (D <= 1024) return resnorm::launch<4, 1>(a, B, st);
-  if (D <= 1536) return resnorm::launch<6, 1>(a, B, st);
+  // one warp a row or two: 39.0 us against 37.4 on 2 x 8448 x 1536, with codes 20.9 against 22.8
+  // on 8448 x 1536 (nv)
+  if (D <= 1536) return fmt ? resnorm::launch<6, 1>(a, B, st) : resnorm::launch<3, 2>(a, B, st);
   if (D <= 2048) return resnorm::launch<4, 2>(a, B, st);
   if (D <= 4096) return resnorm::launch<4, 4>(a, B, st);
   if (D <= 8192) return resnorm::launch<4, 8>(a, B, st);

@@ -21,6 +21,8 @@ def _vector(t, n, what, device):
     """A bf16 vector of n entries for the kernel (None stays None)."""
     if t is None:
         return None
+    if t.dtype is torch.bfloat16 and t.shape == (n,) and t.device == device and t.is_contiguous():
+        return t
     if t.numel() != n:
         raise ValueError(f"{what} must have {n} entries, got {tuple(t.shape)}")
     if t.device != device:
@@ -34,6 +36,8 @@ def _residual(r, M, N, what, device):
     """(residual as [M, N] with unit column stride, its row pitch)."""
     if r is None:
         return None, 0
+    if r.dtype is torch.bfloat16 and r.shape == (M, N) and r.device == device and r.is_contiguous():
+        return r, N
     if r.dtype != torch.bfloat16 or r.numel() != M * N or r.shape[-1] != N:
         raise ValueError(f"{what}: residual must be bf16 [{M}, {N}], got {r.dtype} {tuple(r.shape)}")
     if r.device != device:
