@@ -6,7 +6,9 @@
 // the row waits in registers (one warp up to 2048 elements, four warps up to 16384); longer
 // rows are read twice.  mx blocks and the way back need nothing of the rest of their row.
 // Measured at 8448 x 8960 (193 MB read and written): mx 32.1 us from fp16 (6.0 TB/s, 93% of
-// a plain copy), nv 39 us from bf16, the way back 35 us; 8448 x 1536: nv 7.9 us, back 6.9 us.
+// a plain copy), nv 39 us from bf16, the way back 35 us; 8448 x 1536: nv 7.9 us, back 6.9 us;
+// rows of an odd length, 4000 x 7001: mx 19.8 us, nv 25.7, back 17.5 (159 when each thread wrote
+// its 16 elements one by one).
 #include "fp4.cuh"
 
 namespace fvb {
@@ -39,15 +41,21 @@ __device__ __forceinline__ void st32(uint4* p, const uint4& a, const uint4& b) {
                : "memory");
 }
 
-// elements [k0, k0 + 16) of a row of K; zeros past its end.  vec: the row is 32-byte aligned
+// How a matrix's rows are aligned: 2 = 32 bytes, 1 = 16, 0 = less
+__host__ __forceinline__ int row_alignment(const void* p, int64_t pitch_bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes;
+  return (a & 31u) == 0 ? 2 : (a & 15u) == 0 ? 1 : 0;
+}
+
+// elements [k0, k0 + 16) of a row of K; zeros past its end
 template <typename T, bool WIDE = false>
 __device__ __forceinline__ void load16(Raw<T>& r, const T* __restrict__ row, int64_t k0, int64_t K,
-                                       bool vec) {
-  if (vec && k0 + 16 <= K) {
+                                       int align) {
+  if (align && k0 + 16 <= K) {
     const uint4* p = reinterpret_cast<const uint4*>(row + k0);
 #pragma unroll
     for (int i = 0; i < Raw<T>::kVec; i += 2) {
-      if (WIDE) {
+      if (WIDE && align == 2) {
         ld32(p + i, r.v[i], r.v[i + 1]);
       } else {
         r.v[i] = ld_stream(p + i);
@@ -62,6 +70,34 @@ __device__ __forceinline__ void load16(Raw<T>& r, const T* __restrict__ row, int
     for (int i = 0; i < 16; ++i)
       if (k0 + i < K) e[i] = row[k0 + i];
   }
+}
+
+// The same for a whole warp, lane l the unit u0 + l.  Rows that are not 16-byte aligned go
+// through the warp's 512 elements of shared memory: element by element in row order (a lane
+// that read its own 16 one by one would touch 32 sectors with each load).  STAGED: they do; a
+// kernel of its own, since the branch and its buffer cost the aligned one 8 of 32 us (mx).
+template <typename T, bool WIDE, bool STAGED>
+__device__ __forceinline__ void load_units(Raw<T>& r, const T* __restrict__ row, int64_t u0, int64_t K,
+                                           int align, T* stage) {
+  const int lane = threadIdx.x & 31;
+  if (!STAGED) {
+    load16<T, WIDE>(r, row, (u0 + lane) * 16, K, align);
+    return;
+  }
+  using U = typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type;
+  const U* src = reinterpret_cast<const U*>(row) + u0 * 16;
+  U* st = reinterpret_cast<U*>(stage);
+  const int64_t left = K - u0 * 16;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int i = j * 32 + lane;
+    st[i] = i < left ? __ldg(src + i) : (U)0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < Raw<T>::kVec; ++i)
+    r.v[i] = reinterpret_cast<const uint4*>(stage)[lane * Raw<T>::kVec + i];
+  __syncwarp();
 }
 
 template <typename T>
@@ -114,7 +150,7 @@ struct QuantArgs {
   float* row_scale;
   int64_t pitch;  // bytes of one row of codes
   int64_t tiles;  // scale tiles along a row
-  bool vec;
+  int align;  // row_alignment of x
   unsigned row_blocks;  // of 8 rows (mx)
 };
 
@@ -133,7 +169,7 @@ __device__ __forceinline__ void nv_store(const QuantArgs<T>& a, int64_t m, int64
 }
 
 // nv, the row held in registers: WPR warps a row, NB units a thread
-template <typename T, int NB, int WPR>
+template <typename T, int NB, int WPR, bool STAGED>
 __global__ void __launch_bounds__(WPR == 1 ? 256 : 32 * WPR) quant_nv_kernel(const QuantArgs<T> a) {
   constexpr int T_ROW = 32 * WPR;
   const int64_t m = WPR == 1 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -142,9 +178,12 @@ __global__ void __launch_bounds__(WPR == 1 ? 256 : 32 * WPR) quant_nv_kernel(con
   const T* row = a.x + m * a.ld;
   const int units = (int)(a.tiles * 4);
   Raw<T> r[NB];
+  __shared__ __align__(16) T stage[WPR == 1 ? 8 : WPR][STAGED ? 512 : 1];
+  const int64_t w0 = t & ~31;  // the warp's first unit
 #pragma unroll
-  for (int i = 0; i < NB; ++i)  // 32 bytes a load: 7.9 us against 9.0 at 8448 x 1536, 40.7 against 39.2 at x 8960
-    load16<T, WPR == 1>(r[i], row, (int64_t)(t + i * T_ROW) * 16, a.K, a.vec);
+  for (int i = 0; i < NB; ++i)
+    // 32 bytes a load: 7.9 us against 9.0 at 8448 x 1536, but 40.7 against 39.2 at 8448 x 8960
+    load_units<T, WPR == 1, STAGED>(r[i], row, w0 + i * T_ROW, a.K, a.align, stage[threadIdx.x >> 5]);
   float am[NB], top = 0.f;
   uint32_t bad = 0u;
 #pragma unroll
@@ -183,7 +222,7 @@ __global__ void __launch_bounds__(256) quant_nv_long_kernel(const QuantArgs<T> a
   for (int64_t u = threadIdx.x; u < units; u += 256) {
     Raw<T> r;
     bool b;
-    load16(r, row, u * 16, a.K, a.vec);
+    load16(r, row, u * 16, a.K, a.align);
     top = fmaxf(top, amax16(r, b));
   }
   __shared__ float red[8];
@@ -198,14 +237,14 @@ __global__ void __launch_bounds__(256) quant_nv_long_kernel(const QuantArgs<T> a
   for (int64_t u = threadIdx.x; u < units; u += 256) {
     Raw<T> r;
     bool b;
-    load16(r, row, u * 16, a.K, a.vec);
+    load16(r, row, u * 16, a.K, a.align);
     const float am = amax16(r, b);
     nv_store(a, m, u, r, am, b, rs, ik);
   }
 }
 
 // mx: lanes 2i and 2i + 1 share a block; a block of threads is 8 rows x 32 units
-template <typename T>
+template <typename T, bool STAGED>
 __global__ void __launch_bounds__(256) quant_mx_kernel(const QuantArgs<T> a) {
   const int64_t m = (int64_t)(blockIdx.x % a.row_blocks) * 8 + (threadIdx.x >> 5);
   if (m >= a.M) return;  // whole warps
@@ -213,12 +252,13 @@ __global__ void __launch_bounds__(256) quant_mx_kernel(const QuantArgs<T> a) {
   const int64_t units = a.tiles * 8;  // a multiple of 8, so both lanes of a block are in or out
   const T* row = a.x + m * a.ld;
   uint8_t* codes = a.codes + m * a.pitch;
+  __shared__ __align__(16) T stage[8][STAGED ? 512 : 1];
   const int64_t u1 = (int64_t)(blockIdx.x / a.row_blocks) * kSegUnits;
 #pragma unroll 2
   for (int64_t u0 = u1; u0 < units && u0 < u1 + kSegUnits; u0 += 32) {
     const int64_t u = u0 + lane;
     Raw<T> r;
-    load16(r, row, u * 16, a.K, a.vec);
+    load_units<T, false, STAGED>(r, row, u0, a.K, a.align, stage[threadIdx.x >> 5]);
     bool bad;
     float am = amax16(r, bad);
     am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
@@ -252,16 +292,19 @@ __device__ __forceinline__ float from_f32<float>(float v) {
 }
 
 // the values that codes stand for; one thread per 16 elements, 8 rows x 32 units a block
-template <typename T, int FMT>
+template <typename T, int FMT, bool STAGED>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict__ codes,
                                                       const uint8_t* __restrict__ scales,
                                                       const float* __restrict__ row_scale,
                                                       int rs_row, int64_t M, int64_t K,
-                                                      int64_t pitch, int64_t tiles, bool vec,
+                                                      int64_t pitch, int64_t tiles, int align,
                                                       unsigned segs, T* __restrict__ out) {
   const int64_t m = (int64_t)(blockIdx.x / segs) * 8 + (threadIdx.x >> 5);
   if (m >= M) return;
-  const int64_t u = (int64_t)(blockIdx.x % segs) * 32 + (threadIdx.x & 31);
+  const int lane = threadIdx.x & 31;
+  const int64_t u0 = (int64_t)(blockIdx.x % segs) * 32, u = u0 + lane;
+  __shared__ __align__(16) T stage[8][STAGED ? 512 : 1];
+  T* st = stage[threadIdx.x >> 5];
   if (u < (K + 15) / 16) {
     const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + m * pitch + u * 8));
     const uint32_t b = __ldg(scales + scale_at(m, FMT == FVB_FP4_NV ? u : u >> 1, tiles));
@@ -282,15 +325,48 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
       e[2 * j + 1] = from_f32<T>(f.y * s);
     }
     T* p = out + m * K + u * 16;
-    if (vec && u * 16 + 16 <= K) {
+    if (!STAGED && align == 2 && u * 16 + 16 <= K) {
 #pragma unroll
       for (int j = 0; j < Raw<T>::kVec; j += 2) st32(reinterpret_cast<uint4*>(p) + j, o.v[j], o.v[j + 1]);
-    } else {
+    } else if (!STAGED && u * 16 + 16 <= K) {
+#pragma unroll
+      for (int j = 0; j < Raw<T>::kVec; ++j) reinterpret_cast<uint4*>(p)[j] = o.v[j];
+    } else if (!STAGED) {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (u * 16 + j < K) p[j] = e[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < Raw<T>::kVec; ++j) reinterpret_cast<uint4*>(st)[lane * Raw<T>::kVec + j] = o.v[j];
     }
   }
+  if (!STAGED) return;
+  // rows that are not 16-byte aligned: element by element in row order
+  __syncwarp();
+  T* p = out + m * K + u0 * 16;
+  const int64_t left = K - u0 * 16;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j * 32 + lane < left) p[j * 32 + lane] = st[j * 32 + lane];
+}
+
+template <typename T, bool STAGED>
+static void quant_nv(const QuantArgs<T>& a, int64_t units, cudaStream_t st) {
+  const unsigned g8 = (unsigned)((a.M + 7) / 8), g1 = (unsigned)a.M;
+  if (units <= 32)
+    quant_nv_kernel<T, 1, 1, STAGED><<<g8, 256, 0, st>>>(a);
+  else if (units <= 64)
+    quant_nv_kernel<T, 2, 1, STAGED><<<g8, 256, 0, st>>>(a);
+  else if (units <= 96)
+    quant_nv_kernel<T, 3, 1, STAGED><<<g8, 256, 0, st>>>(a);
+  else if (units <= 128)
+    quant_nv_kernel<T, 4, 1, STAGED><<<g8, 256, 0, st>>>(a);
+  else if (units <= 256)
+    quant_nv_kernel<T, 2, 4, STAGED><<<g1, 128, 0, st>>>(a);
+  else if (units <= 640)
+    quant_nv_kernel<T, 5, 4, STAGED><<<g1, 128, 0, st>>>(a);
+  else
+    quant_nv_kernel<T, 8, 4, STAGED><<<g1, 128, 0, st>>>(a);
 }
 
 template <typename T>
@@ -306,32 +382,23 @@ static int quant(const void* x, int64_t ld, int64_t M, int64_t K, int fmt, void*
   a.row_scale = row_scale;
   a.pitch = code_pitch(K);
   a.tiles = scale_tiles(K, fmt);
-  a.vec = (reinterpret_cast<uintptr_t>(x) & 31u) == 0 && (ld * (int64_t)sizeof(T)) % 32 == 0;
+  a.align = row_alignment(x, ld * (int64_t)sizeof(T));
   if (fmt == FVB_FP4_MX) {
     const int64_t segs = (a.tiles * 8 + kSegUnits - 1) / kSegUnits, blocks = (M + 7) / 8 * segs;
     FVB_REQUIRE(blocks < (1ll << 31), "fvb_quant_fp4: size");
     a.row_blocks = (unsigned)((M + 7) / 8);
-    quant_mx_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
+    if (a.align) quant_mx_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+    else quant_mx_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(a);
     return check_launch("fvb_quant_fp4");
   }
   const int64_t units = a.tiles * 4;
-  const unsigned g8 = (unsigned)((M + 7) / 8), g1 = (unsigned)M;
-  if (units <= 32)
-    quant_nv_kernel<T, 1, 1><<<g8, 256, 0, st>>>(a);
-  else if (units <= 64)
-    quant_nv_kernel<T, 2, 1><<<g8, 256, 0, st>>>(a);
-  else if (units <= 96)
-    quant_nv_kernel<T, 3, 1><<<g8, 256, 0, st>>>(a);
-  else if (units <= 128)
-    quant_nv_kernel<T, 4, 1><<<g8, 256, 0, st>>>(a);
-  else if (units <= 256)
-    quant_nv_kernel<T, 2, 4><<<g1, 128, 0, st>>>(a);
-  else if (units <= 640)
-    quant_nv_kernel<T, 5, 4><<<g1, 128, 0, st>>>(a);
-  else if (units <= 1024)
-    quant_nv_kernel<T, 8, 4><<<g1, 128, 0, st>>>(a);
-  else
+  const unsigned g1 = (unsigned)M;
+  if (units > 1024)
     quant_nv_long_kernel<T><<<g1, 256, 0, st>>>(a);
+  else if (a.align)
+    quant_nv<T, false>(a, units, st);
+  else
+    quant_nv<T, true>(a, units, st);
   return check_launch("fvb_quant_fp4");
 }
 
@@ -342,15 +409,20 @@ static int dequant(const void* codes, const void* scales, const float* row_scale
   FVB_REQUIRE(blocks < (1ll << 31), "fvb_dequant_fp4: size");
   const unsigned grid = (unsigned)blocks, segs = (unsigned)segs64;
   const int64_t pitch = code_pitch(K), tiles = scale_tiles(K, fmt);
-  const bool vec = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && K * (int64_t)sizeof(T) % 32 == 0;
-  if (fmt == FVB_FP4_NV)
-    dequant_kernel<T, FVB_FP4_NV><<<grid, 256, 0, st>>>((const uint8_t*)codes,
-                                                        (const uint8_t*)scales, row_scale, rs_row,
-                                                        M, K, pitch, tiles, vec, segs, (T*)out);
-  else
-    dequant_kernel<T, FVB_FP4_MX><<<grid, 256, 0, st>>>((const uint8_t*)codes,
-                                                        (const uint8_t*)scales, nullptr, 0, M, K,
-                                                        pitch, tiles, vec, segs, (T*)out);
+  const int align = row_alignment(out, K * (int64_t)sizeof(T));
+  const auto c = (const uint8_t*)codes;
+  const auto f = (const uint8_t*)scales;
+#define FVB_DQ(FMT, STAGED)                                                                      \
+  dequant_kernel<T, FMT, STAGED><<<grid, 256, 0, st>>>(c, f, row_scale, rs_row, M, K, pitch, tiles, \
+                                                       align, segs, (T*)out)
+  if (fmt == FVB_FP4_NV) {
+    if (align) FVB_DQ(FVB_FP4_NV, false);
+    else FVB_DQ(FVB_FP4_NV, true);
+  } else {
+    if (align) FVB_DQ(FVB_FP4_MX, false);
+    else FVB_DQ(FVB_FP4_MX, true);
+  }
+#undef FVB_DQ
   return check_launch("fvb_dequant_fp4");
 }
 
