@@ -18,7 +18,8 @@
 // t, t + 32 WPR, ...; statistics are two-pass in registers (mean, then centred squares); the
 // next row's loads go out as soon as the current row's registers are free.  Measured on
 // 2 x 8448 x 1536 (208 MB moved): 37.4 us, 5.6 TB/s (60 us with every operand unpacked for every
-// row, 45 instructions an element); 8448 x 1536 with nv codes for h: 20.6 us.
+// row, 45 instructions an element); 8448 x 1536 with nv codes for h: 21.7 us (20.9 with a
+// bare product in place of the quotient, which put some midpoints on their wrong side).
 #include "fp4.cuh"
 
 namespace fvb {
@@ -305,20 +306,24 @@ __global__ void __launch_bounds__(256, NV == 8 ? 1 : 2) residual_norm_kernel(con
       if (j < NV) {
         constexpr int last_j = NV - 1;
         const int jj = j < NV ? j : last_j;
-        float r;
+        float q[8];
         if (FMT == FVB_FP4_NV) {
           byte = fp4::nv_scale(am[jj], ik);
-          // the codes are h's to the last bit of its own fp32 rounding: a product will do
-          r = byte == 0u ? 0.f : __frcp_rn(fp4::e4m3_value(byte) * rs);
+          const float d = fp4::e4m3_value(byte) * rs, r = byte == 0u ? 0.f : __frcp_rn(d);
+          const uint64_t r2 = f2_pack(r, r), nd2 = f2_pack(-d, -d);
+          // fp4::quotient on pairs: a bare product with r puts some midpoints on their wrong side
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t p = f2_mul(f[jj][i], r2);
+            f2_unpack(f2_fma(f2_fma(p, nd2, f[jj][i]), r2, p), q[2 * i], q[2 * i + 1]);
+          }
         } else {
           const int e = fp4::mx_exponent(am[jj]);
+          const float r = fp4::pow2i(-e);
           byte = (uint32_t)(e + 127);
-          r = fp4::pow2i(-e);
-        }
-        const uint64_t r2 = f2_pack(r, r);
-        float q[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f[jj][i], r2), q[2 * i], q[2 * i + 1]);
+          for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f[jj][i], f2_pack(r, r)), q[2 * i], q[2 * i + 1]);
+        }
         code = fp4::e2m1x8(q);
         if ((bad >> jj) & 1u) {
           code = 0u;

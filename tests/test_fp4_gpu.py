@@ -508,6 +508,23 @@ def test_residual_norm_emits_codes(B, L, D, emit):
     assert r[1] is None
 
 
+@pytest.mark.parametrize("emit", FMTS)
+def test_residual_norm_codes_on_midpoints(emit):
+    """An h that is exact in fp32 (scale -1 leaves the shift) gets the codes of its definition:
+    every midpoint of two codes under every E4M3 mantissa, on its even side."""
+    from flashvsr_sm89_ops_b200 import fused_residual_norm
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0])
+    exact = torch.cat([torch.cat((mids, -mids)) * (1 + j / 8) * 2.0 ** e for e in (-3, 0, 5) for j in range(8)])
+    h = exact.to(torch.bfloat16)
+    assert torch.equal(h.float(), exact)
+    D = h.numel()
+    z = torch.zeros(1, 3, D, dtype=torch.bfloat16, device=DEV)
+    minus = torch.full((1, 1, D), -1.0, dtype=torch.bfloat16, device=DEV)
+    _, out, q = fused_residual_norm(z, z, scale=minus, shift=h.view(1, 1, D).to(DEV), emit_fp4=emit)
+    assert torch.equal(out[0].cpu(), h.expand(3, D))
+    assert torch.equal(R.values(q), R.quantize(h.expand(3, D), emit)[0])
+
+
 def test_residual_norm_gate_forms():
     from flashvsr_sm89_ops_b200 import fused_residual_norm
     c = rn_case(2, 6, 264)
