@@ -54,8 +54,8 @@ enum { kPlain = 0, kResidual = 1, kGeluMx = 2 };
 // (1.5 special functions and the codes for every element), so it has three: they take the
 // 64-column chunks of successive tiles in turn and drift out of step, so that one's special
 // functions run beside another's sums and conversions.  8448 x 8960 x 1536 (nv) measured 75 us
-// with three, 87 with two; four leave 96 registers a thread and spill.  The others need a 4 KB
-// staging buffer a warp, and a third would cost them a ring stage.
+// with three (78 with gelu2's tail), 87 with two; four leave 96 registers a thread and spill.  The
+// others need a 4 KB staging buffer a warp, and a third would cost them a ring stage.
 __host__ __device__ constexpr int epi_per_quarter(int epi) { return epi == kGeluMx ? 3 : 2; }
 
 struct Args {
@@ -205,16 +205,19 @@ __host__ __device__ constexpr uint32_t idesc4(int M, int N) {
 // GELU(tanh) of two values in fp32: x * sigmoid(2 u) = x / (1 + 2^v), u = sqrt(2/pi) (x + c x^3),
 // v = -2 u log2(e).  One reciprocal of the product serves both, 1 / a = b / (a b): the
 // special-function unit (16 a clock per SM) would bound the epilogue with two for each value.
-// v is held at 60 so that the product stays finite; x / 2^60 is far below any code next to it,
-// and 0.5 x (1 + tanh u) in fp32 has long been 0 there.
+// So that the product stays finite, x below -7.5 (v = 60.7, GELU = -4e-18) counts as 0; -inf
+// becomes NaN there, as 0.5 x (1 + tanh u) has it.  Holding v at 60 instead (3 us of the FFN's 126
+// at 8448 x 1536 x 8960 less) leaves x / 2^60: -8.7e11 of -1e30, and a block of nothing but such
+// values would be scaled to them.  One minimum over a thread's 64 values and these selects behind a
+// branch measured 128 us.
 __device__ __forceinline__ uint64_t gelu2(uint64_t x) {
   const float k1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, k3 = k1 * 0.044715f;
-  const uint64_t v = f2_mul(x, f2_fma(f2_mul(x, x), f2_pack(k3, k3), f2_pack(k1, k1)));
-  float v0, v1, a, b;
-  f2_unpack(v, v0, v1);
-  f2_unpack(f2_add(f2_pack(ex2_approx(fminf(v0, 60.0f)), ex2_approx(fminf(v1, 60.0f))),
-                   f2_pack(1.0f, 1.0f)),
-            a, b);
+  float x0, x1, z0, z1, v0, v1, a, b;
+  f2_unpack(x, x0, x1);
+  f2_unpack(f2_mul(x, f2_pack(-0.0f, -0.0f)), z0, z1);
+  x = f2_pack(x0 < -7.5f ? z0 : x0, x1 < -7.5f ? z1 : x1);
+  f2_unpack(f2_mul(x, f2_fma(f2_mul(x, x), f2_pack(k3, k3), f2_pack(k1, k1))), v0, v1);
+  f2_unpack(f2_add(f2_pack(ex2_approx(v0), ex2_approx(v1)), f2_pack(1.0f, 1.0f)), a, b);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
   return f2_mul(x, f2_pack(b * r, a * r));

@@ -428,6 +428,46 @@ def test_ffn_hidden_extremes():
     check(y, ref, spread(h, e, "mx")[:, :64] + BF16 * ref.abs())
 
 
+@pytest.mark.parametrize("M,F", [(98, 64), (2500, 2080)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_ffn_hidden_deep_negative(fmt, M, F):
+    """Blocks of nothing but large negative hidden values, to -2^100, are exactly 0 (GELU of
+    -7.5 is -4e-18), on few tiles and on pairs; -inf makes its row NaN as the formula does."""
+    from flashvsr_sm89_ops_b200 import ffn_fp4, quantize_fp4
+    x = torch.zeros(M, 64, device=DEV)
+    x[:, 0] = -torch.pow(2.0, torch.arange(M, device=DEV) % 98 + 3)
+    w0 = torch.zeros(F, 64, device=DEV)
+    w0[:, 0] = 1.0
+    w2 = torch.zeros(40, F, device=DEV)
+    w2[torch.arange(40), torch.arange(40)] = 1.0
+    a, q0, q2 = quantize_fp4(x.to(torch.bfloat16), fmt), quantize_fp4(w0, fmt), quantize_fp4(w2, "mx")
+    assert mm_ref(a, q0)[0].max() < -7.5  # nv's scale of a lone 8 is within 1/16 of 8 / 6
+    assert not ffn_fp4(a, q0, None, q2, None).any()
+    b0 = torch.zeros(F, dtype=torch.bfloat16, device=DEV)
+    b0[35] = -math.inf
+    assert ffn_fp4(a, q0, b0, q2, None).isnan().all()
+
+
+def test_ffn_hidden_negative_tail():
+    """Hidden values -4, -4.25, ... -9, each a block of its own, so that its scale is theirs."""
+    from flashvsr_sm89_ops_b200 import ffn_fp4, quantize_fp4
+    n = 21
+    u = -(4 + torch.arange(n, device=DEV) / 4)
+    F = 32 * n
+    a = quantize_fp4(torch.zeros(5, 64, device=DEV), "nv")
+    q0 = quantize_fp4(torch.ones(F, 64, device=DEV), "nv")
+    w2 = torch.zeros(n, F, device=DEV)
+    w2[torch.arange(n), 32 * torch.arange(n)] = 1.0
+    y = ffn_fp4(a, q0, u.repeat_interleave(32).to(torch.bfloat16), quantize_fp4(w2, "mx"), None)
+    # in 64 bits 1 + tanh cancels: x / (1 + exp(-2 u)) is the same formula
+    x = u.double().repeat_interleave(32)
+    h = (x / (1 + torch.exp(-2 * math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)))).expand(5, F)
+    # v (61 at most) carries 6 roundings of 2^-24, so 2^v is within 2^-15; below -7.5 the value is 0
+    e = 2.0 ** -15 * h.abs() + 4.2e-18
+    ref = R.quantize(h, "mx")[0]
+    check(y, ref[:, ::32], (spread(h, e, "mx") + BF16 * ref.abs())[:, ::32])
+
+
 # ----------------------------------------------------------------------------- residual norm
 def rn_case(B, L, D, seed=0):
     g = gen(seed + B + L + D)
