@@ -291,6 +291,17 @@ __device__ __forceinline__ float from_f32<float>(float v) {
   return v;
 }
 
+// p * r for a p of few bits and any r, such that from_f32<T> of it is the product rounded once:
+// for a 16-bit T the fp32 product is cut off and its last bit holds whether anything was lost
+template <typename T>
+__device__ __forceinline__ float scaled(float p, float r) {
+  if (sizeof(T) == 4) return __fmul_rn(p, r);
+  const float a = fabsf(p), b = fabsf(r), t = __fmul_rz(a, b);
+  const uint32_t lost = __fmaf_ru(a, b, -t) > 0.f ? 1u : 0u;
+  const uint32_t sign = (__float_as_uint(p) ^ __float_as_uint(r)) & 0x80000000u;
+  return __uint_as_float(sign | __float_as_uint(t) | lost);
+}
+
 // the values that codes stand for; one thread per 16 elements, 8 rows x 32 units a block
 template <typename T, int FMT, bool STAGED>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict__ codes,
@@ -308,22 +319,37 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
   if (u < (K + 15) / 16) {
     const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + m * pitch + u * 8));
     const uint32_t b = __ldg(scales + scale_at(m, FMT == FVB_FP4_NV ? u : u >> 1, tiles));
-    float s;
-    if (FMT == FVB_FP4_NV)
-      s = e4m3_value(b) * (row_scale ? __ldg(row_scale + (rs_row ? m : 0)) : 1.0f);
-    else
+    // code times s is exact; so it stays with a row scale that is a power of two (quantisation
+    // makes no other), away from the ends of the range.  Any other multiplies last (warp-uniform).
+    float s, rs = 1.0f;
+    bool apart = false;
+    if (FMT == FVB_FP4_NV) {
+      s = e4m3_value(b);
+      if (row_scale) rs = __ldg(row_scale + (rs_row ? m : 0));
+      const uint32_t bits = __float_as_uint(rs);
+      apart = (bits & 0x7FFFFFu) != 0u || (bits >> 23) - 17u > 228u;  // 2^-110 .. 2^118
+      if (!apart) s *= rs;
+    } else {
       s = b == 0xFFu ? __uint_as_float(0x7FC00000u) : pow2i((int)b - 127);
+    }
     uint32_t h[8];
     e2m1x8_to_f16(c.x, h);
     e2m1x8_to_f16(c.y, h + 4);
-    Raw<T> o;
-    T* e = reinterpret_cast<T*>(o.v);
+    float v[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      e[2 * j] = from_f32<T>(f.x * s);
-      e[2 * j + 1] = from_f32<T>(f.y * s);
+      v[2 * j] = f.x * s;
+      v[2 * j + 1] = f.y * s;
     }
+    if (apart) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = scaled<T>(v[j], rs);
+    }
+    Raw<T> o;
+    T* e = reinterpret_cast<T*>(o.v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) e[j] = from_f32<T>(v[j]);
     T* p = out + m * K + u * 16;
     if (!STAGED && align == 2 && u * 16 + 16 <= K) {
 #pragma unroll

@@ -137,6 +137,34 @@ def test_quantize_extremes(fmt, dtype):
     assert v[5, :n].isnan().all() and not v[5, n:].isnan().any()
 
 
+@pytest.mark.parametrize("dtype,bits,low", [(torch.bfloat16, 8, -126), (torch.float16, 11, -14),
+                                            (torch.float32, 24, -126)])
+def test_dequantize_rounds_once(dtype, bits, low):
+    """Any fp32 row scale, chosen so that a code times its scales lies within an fp32 rounding of
+    the middle of two neighbours of the output type; and row scales at the ends of fp32's range."""
+    from flashvsr_sm89_ops_b200 import FP4Tensor, dequantize_fp4
+    g = torch.Generator().manual_seed(bits)
+    p = torch.tensor([c * (1 + j / 8) for c in (1.0, 1.5) for j in range(8)], dtype=torch.float64)
+    i = torch.randint(2 ** min(bits - 1, 20), (400,), generator=g).double()
+    mid = (2.0 ** (bits - 1) + i + 0.5) / 2.0 ** (bits - 1)
+    row = (mid[:, None] / p).float().reshape(-1)
+    row = torch.cat((row, -row[:64], torch.tensor([2.0 ** -149, 2.0 ** -126, 1.7e-38, 2.0 ** 119, 2.0 ** 127, 0.0])))
+    M = row.numel()
+    codes = torch.full((M, 16), 0x20, dtype=torch.uint8)  # codes 0 (value 0) and 2 (value 1)
+    codes[:, 1::2] = 0xB2  # 2 (1) and 11 (-1.5)
+    tiles = torch.zeros(-(-M // 128) * 512, dtype=torch.uint8)
+    m = torch.arange(M)
+    for j in (0, 1):  # E4M3 1 .. 1.875
+        tiles[m // 128 * 512 + m % 32 * 16 + m % 128 // 32 * 4 + j] = (0x38 + m % 8).to(torch.uint8)
+    q = FP4Tensor(codes.to(DEV), tiles.to(DEV), row.to(DEV), (M, 32), "nv")
+    v = R.values(q)
+    e = (torch.frexp(v)[1] - 1).clamp(min=low).double()
+    step = torch.pow(torch.full_like(v, 2.0), e - bits + 1)
+    want = torch.round(v / step) * step
+    want = torch.where(want.abs() > torch.finfo(dtype).max, want * math.inf, want)
+    assert torch.equal(dequantize_fp4(q, dtype).cpu().double(), want)
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_quantize_strides(fmt):
     """Row pitches, unaligned starts, a transposed view: all as their contiguous copy."""
