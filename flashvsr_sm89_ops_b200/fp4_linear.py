@@ -132,8 +132,20 @@ def ffn_fp4(a: FP4Tensor, w0: FP4Tensor, b0: torch.Tensor | None, w2: FP4Tensor,
     return out
 
 
+def _quantize_weight(w: torch.Tensor, fmt: str):
+    """(codes, scales, row scale) of a weight, in buffers of their own on the weight's device.  A
+    weight on the host (a model that is moved to the GPU after its conversion) goes through the
+    current CUDA device, since the quantiser has no other form."""
+    if not w.is_cuda and not torch.cuda.is_available():
+        raise ValueError("FP4Linear: quantising a weight takes a CUDA device (sm_100a)")
+    q = quantize_fp4(w if w.is_cuda else w.cuda(), fmt)
+    parts = (q.codes, q.scales, q.row_scale)
+    return tuple(None if t is None else t.clone() if w.is_cuda else t.to(w.device) for t in parts)
+
+
 class FP4Linear(nn.Module):
-    """nn.Linear replacement with 4-bit weights and activations (cf. FP8Linear)."""
+    """nn.Linear replacement with 4-bit weights and activations (cf. FP8Linear).  The weight is
+    quantised once, here; a linear on the host stays there."""
 
     def __init__(self, linear: nn.Linear, fmt: str = "nv"):
         super().__init__()
@@ -141,11 +153,10 @@ class FP4Linear(nn.Module):
         self.fmt = fmt
         self.in_features = linear.in_features
         self.out_features = linear.out_features
-        q = quantize_fp4(linear.weight.detach(), fmt)
-        self.weight = nn.Parameter(q.codes.clone(), requires_grad=False)
-        self.register_buffer("w_scales", q.scales.clone(), persistent=False)
-        self.register_buffer("w_row_scale", None if fmt == "mx" else q.row_scale.clone(),
-                             persistent=False)
+        codes, scales, row_scale = _quantize_weight(linear.weight.detach(), fmt)
+        self.weight = nn.Parameter(codes, requires_grad=False)
+        self.register_buffer("w_scales", scales, persistent=False)
+        self.register_buffer("w_row_scale", row_scale, persistent=False)
         if linear.bias is not None:
             self.bias = nn.Parameter(linear.bias.detach().to(torch.bfloat16).clone(),
                                      requires_grad=False)

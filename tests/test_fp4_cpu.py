@@ -123,3 +123,16 @@ def test_conversion_refuses_what_it_does_not_know():
     with pytest.raises(ValueError, match="format"):
         convert_linears_fp4(model, fmt="int4")
     assert convert_linears_fp4(model) == 0 and type(model[0]) is nn.Linear
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="needs a machine without a GPU")
+def test_conversion_without_a_gpu_says_so_and_converts_nothing():
+    import torch.nn as nn
+    from flashvsr_sm89_ops_b200 import FP4Linear, integrate
+    from flashvsr_sm89_ops_b200 import wan_video_dit as W
+    with pytest.raises(ValueError, match="CUDA device"):
+        FP4Linear(nn.Linear(64, 64))
+    dit = W.WanDiT(num_layers=1, dim=256, num_heads=2, ffn_dim=512)
+    with pytest.raises(ValueError, match="CUDA device"):
+        integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False, fp4_parts=["ffn", "self"])
+    assert all(type(m) is nn.Linear for n, m in dit.named_modules() if n.endswith((".q", ".o", ".ffn.0")))

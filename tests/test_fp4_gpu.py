@@ -708,6 +708,33 @@ def test_refusals():
 
 
 # ----------------------------------------------------------------------------- the model's path
+def small_dit(device, dtype=torch.bfloat16):
+    from flashvsr_sm89_ops_b200 import wan_video_dit as W
+    dit = W.WanDiT(num_layers=1, dim=256, num_heads=2, ffn_dim=512).init_random(seed=3)
+    return W, dit.to(dtype).to(device)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_enable_on_a_host_model(fmt, monkeypatch):
+    """enable() before the model is moved to the GPU gives the weights of enable() after it."""
+    from flashvsr_sm89_ops_b200 import integrate
+    monkeypatch.setenv("FS89_FP4_FMT", fmt)
+    made = []
+    for device in ("cpu", DEV):
+        W, dit = small_dit(device)
+        applied = integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False, fp4_parts=["ffn"])
+        assert applied["fp4_linears"] == 2
+        lin = dit.blocks[0].ffn.lin0
+        assert all(t.device.type == torch.device(device).type for t in (lin.weight, lin.w_scales, lin.bias))
+        made.append(dit.to(DEV).blocks[0].ffn)
+    x = randn(gen(2), 3, 5, 256).to(torch.bfloat16)
+    a, b = made
+    for s, t in ((a.lin0, b.lin0), (a.lin2, b.lin2)):
+        assert torch.equal(s.weight, t.weight)
+        assert torch.equal(R.values(s.weight_fp4()), R.values(t.weight_fp4()))
+    assert torch.equal(a(x), b(x))
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_block_with_a_4bit_ffn(fmt, monkeypatch):
     """enable() with FS89_FP4=ffn: the block's FFN half equals its definition in 64 bits on the
