@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from . import _lib
 from .fp4_quant import _FMTS, FP4Tensor, fp4_format, quantize_fp4, require_cuda
+from .fp8_linear import FP8Linear
 
 
 def _vector(t, n, what, device):
@@ -205,24 +206,31 @@ _PATTERNS = {"self": r"^blocks\.\d+\.self_attn\.[qkvo]$", "cross": r"^blocks\.\d
 def convert_linears_fp4(model: nn.Module, parts=("ffn",), fmt: str = "nv") -> int:
     """Swap the DiT blocks' Linears of `parts` (ffn, self, cross) for 4-bit ones; returns the
     count.  ``blocks.i.ffn`` becomes an FP4FFN whose first linear has `fmt`.  Same module names
-    as convert_linears_fp8 (fp8_linear.py:45-67)."""
+    as convert_linears_fp8 (fp8_linear.py:45-67).  What is 4-bit in `fmt` already stays; a part
+    that was converted to FP8 or to the other format, its full-precision weights gone, is refused
+    before anything is converted."""
     fp4_format(fmt)
     unknown = set(parts) - {"ffn", "self", "cross"}
     if unknown:
         raise ValueError(f"convert_linears_fp4: unknown parts {sorted(unknown)} (ffn|self|cross)")
-    n = 0
     pats = [re.compile(_PATTERNS[p]) for p in parts if p in _PATTERNS]
     ffn = re.compile(r"^blocks\.\d+\.ffn$") if "ffn" in parts else None
+    todo = []
     for name, mod in list(model.named_modules()):
-        parent_name, _, leaf = name.rpartition(".")
-        if ffn is not None and ffn.match(name) and isinstance(mod, nn.Sequential) \
-                and type(mod[0]) is nn.Linear and type(mod[2]) is nn.Linear:
-            new = FP4FFN(FP4Linear(mod[0], fmt), FP4Linear(mod[2], "mx"))
-            n += 2
-        elif type(mod) is nn.Linear and any(p.match(name) for p in pats):
-            new = FP4Linear(mod, fmt)
-            n += 1
-        else:
+        is_ffn = ffn is not None and ffn.match(name)
+        if not is_ffn and not any(p.match(name) for p in pats):
             continue
+        # the linear that an FFN, of whichever kind, begins with speaks for it
+        lin = mod if not is_ffn else mod[0] if isinstance(mod, nn.Sequential) else getattr(mod, "lin0", None)
+        if isinstance(lin, FP8Linear) or (isinstance(lin, FP4Linear) and lin.fmt != fmt):
+            kind = "FP8" if isinstance(lin, FP8Linear) else lin.fmt
+            raise ValueError(f"convert_linears_fp4: {name} is already {kind}, it cannot become {fmt}")
+        if type(lin) is nn.Linear and (not is_ffn or type(mod[2]) is nn.Linear):
+            todo.append((name, mod, is_ffn))
+    n = 0
+    for name, mod, is_ffn in todo:
+        parent_name, _, leaf = name.rpartition(".")
+        new = FP4FFN(FP4Linear(mod[0], fmt), FP4Linear(mod[2], "mx")) if is_ffn else FP4Linear(mod, fmt)
         setattr(model.get_submodule(parent_name) if parent_name else model, leaf, new)
+        n += 2 if is_ffn else 1
     return n

@@ -14,6 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .fp4_linear import FP4FFN
 from .fp8_linear import FP8Linear
 from .fp8_quant import fused_gelu_quant_fp8, mode_code, quantize_fp8  # noqa: F401 (re-export)
 
@@ -83,7 +84,7 @@ def convert_ffn_fp8(model: nn.Module) -> int:
     pat = re.compile(r"^blocks\.\d+\.ffn$")
     n = 0
     for name, mod in list(model.named_modules()):
-        if not pat.match(name) or isinstance(mod, FP8FFN):
+        if not pat.match(name) or isinstance(mod, (FP8FFN, FP4FFN)):
             continue  # already converted: re-running enable() is safe
         l0, l2 = mod[0], mod[2]
         if not (isinstance(l0, FP8Linear) and isinstance(l2, FP8Linear)):

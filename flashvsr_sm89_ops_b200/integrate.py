@@ -514,7 +514,9 @@ def enable(pipe, dit_module=None, parts=None, compile_memblocks=None, verbose=Tr
     fp4_parts (default: FS89_FP4, empty): parts that run in microscaled 4 bits, taken out of
     `parts`.  Call once after ``pipe.enable_vram_management(...)`` and before
     ``pipe.init_cross_kv()``.  Returns a dict of what was enabled.  Re-running it on
-    an already patched pipeline is safe.
+    an already patched pipeline is safe: what is converted stays as it is, whichever of the
+    two `parts` then name it, except that fp4_parts that run in FP8 already (or in the other
+    4-bit format) are a ValueError.
     """
     if parts is None:
         parts = [p for p in os.environ.get("FS89_FP8", "ffn,self,cross").split(",") if p]

@@ -136,3 +136,17 @@ def test_conversion_without_a_gpu_says_so_and_converts_nothing():
     with pytest.raises(ValueError, match="CUDA device"):
         integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False, fp4_parts=["ffn", "self"])
     assert all(type(m) is nn.Linear for n, m in dit.named_modules() if n.endswith((".q", ".o", ".ffn.0")))
+
+
+@pytest.mark.parametrize("fused", ["0", "1"])
+@pytest.mark.parametrize("part", ["ffn", "self", "cross"])
+def test_enable_refuses_4_bits_for_a_part_that_is_fp8(part, fused, monkeypatch):
+    from flashvsr_sm89_ops_b200 import integrate
+    from flashvsr_sm89_ops_b200 import wan_video_dit as W
+    monkeypatch.setenv("FS89_FP8_FFNFUSED", fused)
+    dit = W.WanDiT(num_layers=1, dim=256, num_heads=2, ffn_dim=512).to(torch.bfloat16)
+    assert integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False)["fp8_linears"] == 10
+    before = {n: type(m) for n, m in dit.named_modules()}
+    with pytest.raises(ValueError, match="already FP8"):
+        integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False, fp4_parts=[part])
+    assert {n: type(m) for n, m in dit.named_modules()} == before

@@ -735,6 +735,26 @@ def test_enable_on_a_host_model(fmt, monkeypatch):
     assert torch.equal(a(x), b(x))
 
 
+def test_enable_again_with_other_parts(monkeypatch):
+    """A second enable() without the 4-bit parts leaves them as they are and converts the rest;
+    one with them again too; the other format is refused."""
+    from flashvsr_sm89_ops_b200 import FP4FFN, FP8Linear, integrate
+    W, dit = small_dit(DEV)
+    monkeypatch.delenv("FS89_FP4", raising=False)
+    pipe = W.DiTPipe(dit)
+    assert integrate.enable(pipe, dit_module=W, parts=[], verbose=False, fp4_parts=["ffn"])["fp4_linears"] == 2
+    ffn = dit.blocks[0].ffn
+    for _ in range(2):
+        applied = integrate.enable(pipe, dit_module=W, verbose=False)
+        assert applied["fp8_ffn_blocks"] == 0 and dit.blocks[0].ffn is ffn and type(ffn) is FP4FFN
+        assert type(dit.blocks[0].self_attn.q) is FP8Linear
+    assert integrate.enable(pipe, dit_module=W, verbose=False, fp4_parts=["ffn"])["fp4_linears"] == 0
+    monkeypatch.setenv("FS89_FP4_FMT", "mx")
+    with pytest.raises(ValueError, match="already nv"):
+        integrate.enable(pipe, dit_module=W, verbose=False, fp4_parts=["ffn"])
+    assert dit.blocks[0].ffn is ffn
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_block_with_a_4bit_ffn(fmt, monkeypatch):
     """enable() with FS89_FP4=ffn: the block's FFN half equals its definition in 64 bits on the
