@@ -23,7 +23,9 @@ Extra flags of this pack: FS89_FP8_SCALE=token|tensor (activation granularity;
 FS89_FP4=ffn[,self,cross] (those parts in microscaled 4 bits instead of FP8; off by
 default) and FS89_FP4_FMT=nv|mx (the format of their inputs).  With FS89_FP4=ffn the
 block's FFN half runs as: cross-attention add + LN-mod emitting 4-bit codes -> 4-bit
-product with GELU and a 4-bit hidden state -> 4-bit product with the gated residual.
+product with GELU and a 4-bit hidden state -> 4-bit product with the gated residual.  With
+self or cross the attention paths stay what they are around 4-bit projections (q, k and v
+as one product).
 """
 from __future__ import annotations
 
@@ -34,7 +36,8 @@ import torch
 
 from . import lcsa
 from .compat_bsa import active_backend, ensure_bsa_available
-from .fp4_linear import FP4FFN, convert_linears_fp4
+from .fp4_linear import FP4FFN, FP4Linear, convert_linears_fp4, fp4_mm
+from .fp4_quant import FP4Tensor, quantize_fp4
 from .fp8_ffn import FP8FFN, convert_ffn_fp8, ffn_fp8
 from .fp8_linear import FP8Linear, convert_linears_fp8, fp8_mm
 from .fp8_quant import default_act_mode, quantize_fp8
@@ -100,6 +103,30 @@ def _qkv_pack(attn):
                     .to(torch.bfloat16) for l in (q, k, v)]).contiguous()
     pk = (q.weight, W.contiguous(), S, Bv, q.mode)
     attn._fvb_qkv = pk
+    return pk
+
+
+def _qkv_pack4(attn):
+    """(q.weight, q|k|v as one FP4Tensor, their biases) of 4-bit linears, built once per module.
+
+    Rows of whole 128-row scale tiles follow each other, so the three buffers are concatenated
+    as they are."""
+    q, k, v = attn.q, attn.k, attn.v
+    if not all(type(l) is FP4Linear for l in (q, k, v)) or len({q.fmt, k.fmt, v.fmt}) != 1 \
+            or any(l.out_features % 128 for l in (q, k, v)):
+        return None
+    pk = getattr(attn, "_fvb_qkv4", None)
+    if pk is not None and pk[0] is q.weight and pk[1].device == q.weight.device:
+        return pk
+    ws = [l.weight_fp4() for l in (q, k, v)]
+    rows = None if q.fmt == "mx" else torch.cat([w.row_scale for w in ws])
+    W = FP4Tensor(torch.cat([w.codes for w in ws]), torch.cat([w.scales for w in ws]), rows,
+                  (sum(w.shape[0] for w in ws), q.in_features), q.fmt)
+    Bv = torch.cat([l.bias if l.bias is not None else
+                    torch.zeros(l.out_features, dtype=torch.bfloat16, device=W.device)
+                    for l in (q, k, v)])
+    pk = (q.weight, W, Bv.to(torch.bfloat16))
+    attn._fvb_qkv4 = pk
     return pk
 
 
@@ -207,7 +234,8 @@ def _keep_mask(self, dit, q_w, k_w, nh, seqlen, h, w, topk, local_range, pre_cac
 
 def _fast_self_ok(self, x):
     return x.dim() == 3 and x.shape[0] == 1 and x.dtype == torch.bfloat16 and x.is_cuda \
-        and _qkv_pack(self) is not None and type(self.o) is FP8Linear
+        and (_qkv_pack(self) is not None or _qkv_pack4(self) is not None) \
+        and type(self.o) in (FP8Linear, FP4Linear)
 
 
 def _self_fast_path(dit, attn, x):
@@ -218,7 +246,8 @@ def _self_fast_path(dit, attn, x):
 def _cross_fast_path(dit, ca, x):
     """Whether the cross-attention forward takes the B200 fast path for input like x."""
     return getattr(dit, "FUSED_ROPE_FN", None) is fused_rms_rope and x.dim() == 3 \
-        and x.shape[0] == 1 and x.is_cuda and type(ca.q) is FP8Linear and type(ca.o) is FP8Linear
+        and x.shape[0] == 1 and x.is_cuda and type(ca.q) in (FP8Linear, FP4Linear) \
+        and type(ca.o) in (FP8Linear, FP4Linear)
 
 
 # ----------------------------------------------------------------------------- forwards
@@ -227,13 +256,15 @@ def _fast_self_attn(self, dit, x, freqs, f, h, w, topk, kv_len, pre_cache_k, pre
     _, L, D = x.shape
     nh = self.num_heads
     hd = D // nh
-    _, W, S, Bv, mode = _qkv_pack(self)
     pre = _take_stash(self, x)
-    if pre is None:
-        x8, s8 = quantize_fp8(x.reshape(L, D), mode)
+    pack = _qkv_pack(self)
+    if pack is None:
+        _, W, Bv = _qkv_pack4(self)
+        qkv = fp4_mm(quantize_fp4(x.reshape(L, D), W.fmt), W, Bv)
     else:
-        x8, s8 = pre
-    qkv = fp8_mm(x8, s8, W, S, Bv)  # [L, 3D]
+        _, W, S, Bv, mode = pack
+        x8, s8 = pre if pre is not None else quantize_fp8(x.reshape(L, D), mode)
+        qkv = fp8_mm(x8, s8, W, S, Bv)  # [L, 3D]
     cos, sin = freqs_cos_sin(freqs)
     if cos.device != x.device:
         cos, sin = cos.to(x.device), sin.to(x.device)

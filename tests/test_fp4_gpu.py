@@ -813,3 +813,108 @@ def test_block_with_a_4bit_ffn(fmt, monkeypatch):
     # bf16 modulation and result: a few 2^-9 relative
     assert err < 4 * 2.0 ** -9, err
     assert _lib.device_error() == 0
+
+
+class Captured:
+    """A 4-bit linear of the oracle's block: the output that the block's own linear gave.  Checks
+    that output against the linear's definition in 64 bits on the input that the linear had, and
+    that the oracle has come to the same input."""
+
+    def __init__(self, w, b, fmt):
+        self.w, self.s = R.quantize(w.to(DEV), fmt)[0], []
+        self.b, self.fmt = b.to(DEV).double(), fmt
+
+    def saw(self, x, y):
+        x2, y2 = x.reshape(-1, x.shape[-1]), y.reshape(-1, y.shape[-1])
+        a = R.quantize(x2, self.fmt)[0]
+        ref, S = a @ self.w.t() + self.b, a.abs() @ self.w.abs().t()
+        check(y2, ref, BF16 * ref.abs() + (steps(x2.shape[1]) + 2.0 ** -22) * S + 2.0 ** -22 * ref.abs())
+        self.s.append((x.cpu(), y.cpu()))
+
+    def __call__(self, x):
+        from oracle import wan as OW
+        xin, y = self.s.pop(0)
+        assert OW.rel_l2(x.reshape(xin.shape), xin) < 2e-2
+        return y
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_block_with_4bit_attention(fmt, monkeypatch):
+    """enable() with FS89_FP4=self,cross: the block against the oracle's (2e-2 relative L2, the bar
+    of the FP8 block's test) with the 4-bit linears' own outputs in it, each of them held against its
+    definition; and all of it on the fused paths."""
+    from flashvsr_sm89_ops_b200 import FP4Linear, _lib, integrate
+    from flashvsr_sm89_ops_b200 import wan_video_dit as W
+    from oracle import wan as OW
+    f, h, w, heads = 2, 16, 24, 12
+    P, x, t_mod, ctx, cache = OW.block_case(seed=6, f=f, h=h, w=w)
+    W.MASK_RULE = "causal"
+    monkeypatch.setenv("FS89_FP4", "self,cross")
+    monkeypatch.setenv("FS89_FP4_FMT", fmt)
+    monkeypatch.setenv("FS89_FP8_SCALE", "token")
+    dit = W.WanDiT(num_layers=1).to(torch.bfloat16)
+    dit.blocks[0].load_state_dict(OW.standin_state_dict(P), strict=True)
+    dit = dit.to(DEV)
+    applied = integrate.enable(W.DiTPipe(dit), dit_module=W, verbose=False)
+    assert applied["fp4_linears"] == 8 and applied["fp8_linears"] == 2
+    blk = dit.blocks[0]
+    Q = OW.quantize_block(P, "token")
+    sd = OW.to_bf16(P)
+    for part, mod in (("self", blk.self_attn), ("cross", blk.cross_attn)):
+        for n in ("q", "k", "v", "o"):
+            lin = getattr(mod, n)
+            assert type(lin) is FP4Linear and lin.fmt == fmt
+            Q[part][n] = cap = Captured(*sd[part][n], fmt)
+            lin.register_forward_hook(lambda m, i, o, cap=cap: cap.saw(i[0], o))
+    quant, mm = integrate.quantize_fp4, integrate.fp4_mm
+    fused = []
+
+    def spy_quant(t, f):
+        fused.append(t)
+        return quant(t, f)
+
+    def spy_mm(*a):
+        y = mm(*a)
+        for n, part in zip("qkv", y.chunk(3, 1)):
+            Q["self"][n].saw(fused[0][None], part[None])
+        return y
+
+    monkeypatch.setattr(integrate, "quantize_fp4", spy_quant)
+    monkeypatch.setattr(integrate, "fp4_mm", spy_mm)
+    with torch.no_grad():
+        dit.init_cross_kv(ctx.to(DEV))
+        fr = W.grid_freqs(dit.freqs, f, h, w, f0=6).to(DEV)
+        y, ck, cv = blk(x.to(DEV), None, t_mod.to(DEV), fr, f, h, w, kv_len=3, is_stream=True,
+                        pre_cache_k=cache[0].to(DEV), pre_cache_v=cache[1].to(DEV))
+    assert len(fused) == 1  # one product for q, k and v
+    assert hasattr(ck, "_fvb_arena") and hasattr(ck, "_fvb_kpool")  # the fused self-attention's caches
+    cos, sin = OW.O.freqs_cos_sin(OW.grid_freqs(f, h, w, f0=6))
+    ref, (rk, rv) = OW.block_forward(Q, x, t_mod, cos, sin, (f, h, w), OW.cross_kv(Q, ctx),
+                                     OW.causal_mask_fn(heads, 6, 0.25), heads, cache, 3)
+    e, ek, ev = OW.rel_l2(y.cpu(), ref), OW.rel_l2(ck.cpu(), rk), OW.rel_l2(cv.cpu(), rv)
+    assert e < 2e-2 and ek < 2e-2 and ev < 2e-2, (e, ek, ev)
+    assert all(not Q[p][n].s for p in ("self", "cross") for n in "qkvo")
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("parts", ["ffn", "self", "ffn,self,cross"])
+def test_streaming_step_in_4_bits_replays_from_a_graph(parts, monkeypatch):
+    """The f = 6 start chunk and the streaming step with 4-bit parts, eagerly and from a CUDA graph."""
+    from flashvsr_sm89_ops_b200 import _lib
+    from flashvsr_sm89_ops_b200.runner import StreamingDiT
+    monkeypatch.setenv("FS89_FP4", parts)
+    r = StreamingDiT(num_layers=2, height=256, width=384, device=DEV)
+    assert r.applied["fp4_linears"] == 2 * (2 * ("ffn" in parts) + 4 * ("self" in parts) + 4 * ("cross" in parts))
+    r.prime()
+    x = r.make_input(2)
+    eager = r.step(x).clone()
+    assert torch.isfinite(eager).all()
+    g, y = r.capture(x)
+    x.copy_(r.make_input(2, seed=9))
+    g.replay()
+    assert torch.equal(y, r.step(x)) and not torch.equal(y, eager)
+    x.copy_(r.make_input(2))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, eager)
+    assert _lib.device_error() == 0
