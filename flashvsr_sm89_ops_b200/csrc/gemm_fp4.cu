@@ -37,6 +37,8 @@
 // chunk's scales and biases then cost a warp 24 wavefronts of shared memory, where a thread
 // that holds a whole row reads all 64 columns' and costs it 128.  They travel by shuffles, each
 // warp with the two columns a lane that it read one chunk ahead: no barrier between the warps.
+#include <atomic>
+
 #include "fp4.cuh"
 
 namespace fvb {
@@ -1088,8 +1090,8 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   auto kern = fp4_gemm_kernel<FMT, EPI>;
   constexpr size_t smem = S::kSmem;
   static_assert(smem <= 227 * 1024, "fp4 gemm: shared memory");
-  static bool configured[64] = {false};
-  static int pair_slots[64] = {0};
+  static std::atomic<bool> configured[64];  // calls of several threads may meet here
+  static std::atomic<int> pair_slots[64];
   int dev = 0;
   FVB_CUDA_TRY(cudaGetDevice(&dev), "fp4 gemm device");
   FVB_REQUIRE(dev >= 0 && dev < 64, "fp4 gemm: device ordinal %d", dev);
@@ -1108,17 +1110,18 @@ static int launch(const Args& a, const Operand& A, const Operand& W, cudaStream_
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (!configured[dev]) {
+  if (!configured[dev].load(std::memory_order_acquire)) {
     FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                  "fp4 gemm smem attribute");
     int clusters = 0;
     cfg.gridDim = dim3(2 * (sm_count() / 2));
     FVB_CUDA_TRY(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg), "fp4 gemm cluster occupancy");
     FVB_REQUIRE(clusters > 0, "fp4 gemm: no 2-CTA cluster fits on this device");
-    pair_slots[dev] = clusters;
-    configured[dev] = true;
+    pair_slots[dev].store(clusters, std::memory_order_relaxed);
+    configured[dev].store(true, std::memory_order_release);
   }
-  cfg.gridDim = dim3(2 * (num < pair_slots[dev] ? num : pair_slots[dev]));
+  const int slots = pair_slots[dev].load(std::memory_order_relaxed);
+  cfg.gridDim = dim3(2 * (num < slots ? num : slots));
   FVB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmSfA, tmSfB, tmO, tmR, a),
                "fp4 gemm launch");
   return check_launch("fp4 gemm");
@@ -1131,14 +1134,14 @@ static int launch_split(const Args& a, const Operand& A, const Operand& W, int Z
   int rc = operand_maps<FMT>(a, A, W, S::BN, 1, tmA, tmB, tmSfA, tmSfB);
   if (rc) return rc;
   auto kern = fp4_gemm_split_kernel<FMT, EPI, SPLIT>;
-  static bool configured[64] = {false};
+  static std::atomic<bool> configured[64];  // calls of several threads may meet here
   int dev = 0;
   FVB_CUDA_TRY(cudaGetDevice(&dev), "fp4 gemm device");
   FVB_REQUIRE(dev >= 0 && dev < 64, "fp4 gemm: device ordinal %d", dev);
-  if (!configured[dev]) {
+  if (!configured[dev].load(std::memory_order_acquire)) {
     FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem),
                  "fp4 gemm smem attribute");
-    configured[dev] = true;
+    configured[dev].store(true, std::memory_order_release);
   }
   const int64_t tiles = (int64_t)((a.M + BM - 1) / BM) * ((a.N + S::BN - 1) / S::BN);
   FVB_REQUIRE(tiles * Z < (1ll << 31), "fp4 gemm: too many output tiles");

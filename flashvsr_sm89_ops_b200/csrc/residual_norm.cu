@@ -20,6 +20,8 @@
 // 2 x 8448 x 1536 (208 MB moved): 37.4 us, 5.6 TB/s (60 us with every operand unpacked for every
 // row, 45 instructions an element); 8448 x 1536 with nv codes for h: 21.7 us (20.9 with a
 // bare product in place of the quotient, which put some midpoints on their wrong side).
+#include <atomic>
+
 #include "fp4.cuh"
 
 namespace fvb {
@@ -341,14 +343,18 @@ template <int NV, int WPR, bool FULL, bool EXTRA, int FMT>
 static int launch_as(Args a, int64_t B, cudaStream_t st) {
   auto kern = residual_norm_kernel<NV, WPR, FULL, EXTRA, FMT>;
   const size_t smem = (size_t)3 * a.D * 4;
-  static size_t set[64] = {0};
-  int dev = 0;
-  FVB_CUDA_TRY(cudaGetDevice(&dev), "fvb_residual_norm device");
-  FVB_REQUIRE(dev >= 0 && dev < 64, "fvb_residual_norm: device ordinal %d", dev);
-  if (smem > 48 * 1024 && smem > set[dev]) {
-    FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                 "fvb_residual_norm smem attribute");
-    set[dev] = smem;
+  constexpr size_t most_smem = (size_t)3 * NV * WPR * 256 * 4;  // of the widest row it takes
+  if (most_smem > 48 * 1024) {
+    // the same limit whoever sets it: calls of several threads and widths may meet here
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    FVB_CUDA_TRY(cudaGetDevice(&dev), "fvb_residual_norm device");
+    FVB_REQUIRE(dev >= 0 && dev < 64, "fvb_residual_norm: device ordinal %d", dev);
+    if (!configured[dev].load(std::memory_order_acquire)) {
+      FVB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem),
+                   "fvb_residual_norm smem attribute");
+      configured[dev].store(true, std::memory_order_release);
+    }
   }
   // two blocks per SM, rows split evenly; no block without a row for each of its teams if
   // there are enough

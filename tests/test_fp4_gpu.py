@@ -627,6 +627,48 @@ def test_residual_norm_extremes():
             assert torch.equal(h[0, 1].float(), want)
 
 
+FIRST_CALLS = """
+import threading
+import torch
+from flashvsr_sm89_ops_b200 import _lib
+lib, bad = _lib.load(), []
+
+def go(d, p, rows, fmt, bar):
+    bar.wait()
+    for _ in range(3):
+        q = p[5:] if fmt else [None] * 3
+        rc = lib.fvb_residual_norm(p[0], p[1], p[2] if rows else None, rows, 1.0, 0, None, None, 1e-6, 2, None,
+                                   None, None, None, 1e-6, 1, 2, d, p[3], p[4], fmt, *q, None)
+        if rc:
+            bar.bad.append((d, rc, lib.fvb_last_error()))
+
+for fmt in (0, 1, 2):
+    for rows in (0, 1):
+        for dims in ((4104, 8184, 6000, 8184), (8200, 16376, 12000, 16376)):
+            bar = threading.Barrier(len(dims))
+            bar.bad = bad
+            bufs = [[torch.zeros(128 * d, dtype=torch.uint8, device="cuda") for _ in range(8)] for d in dims]
+            torch.cuda.synchronize()
+            ts = [threading.Thread(target=go, args=(d, [t.data_ptr() for t in b], rows, fmt, bar))
+                  for d, b in zip(dims, bufs)]
+            [t.start() for t in ts]
+            [t.join() for t in ts]
+            torch.cuda.synchronize()
+assert not bad, bad
+"""
+
+
+def test_residual_norm_first_calls_from_threads():
+    """Rows of different widths from several threads at once, in a process that has not launched
+    these kernels before: every call gets the shared memory of its own width."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_empty_batches():
     from flashvsr_sm89_ops_b200 import ffn_fp4, fp4_mm, fused_residual_norm, quantize_fp4
     x = torch.empty(2, 0, 64, dtype=torch.bfloat16, device=DEV)
