@@ -28,6 +28,14 @@ def _operand(t, n, what, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _per_item(t, B, D, what, device):
+    """An operand with a row for each batch item.  A 3-D one of as many entries in another shape,
+    [1, L, D] with L = B say, would mean something else and is refused."""
+    if t is not None and t.dim() == 3 and t.shape != (B, 1, D):
+        raise ValueError(f"fused_residual_norm: {what} must be [{B}, 1, {D}], got {tuple(t.shape)}")
+    return _operand(t, B * D, what, device)
+
+
 def fused_residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor | None = None,
                         residual_scale: float = 1.0, post_norm: str | None = None,
                         post_weight: torch.Tensor | None = None,
@@ -65,12 +73,13 @@ def fused_residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor 
     x = x if x.is_contiguous() else x.contiguous()
     y = y if y.is_contiguous() else y.contiguous()
     gate_rows = 0
-    if gate is not None:
-        if L > 1 and gate.numel() == B * L * D:
-            gate_rows = 1
-        gate = _operand(gate, B * L * D if gate_rows else B * D, "gate", dev)
-    scale = _operand(scale, B * D, "scale", dev)
-    shift = _operand(shift, B * D, "shift", dev)
+    if gate is not None and L > 1 and gate.numel() == B * L * D and (gate.dim() != 3 or gate.shape == x.shape):
+        gate_rows = 1
+        gate = _operand(gate, B * L * D, "gate", dev)
+    else:
+        gate = _per_item(gate, B, D, "gate", dev)
+    scale = _per_item(scale, B, D, "scale", dev)
+    shift = _per_item(shift, B, D, "shift", dev)
     post_weight = _operand(post_weight, D, "post_weight", dev)
     post_bias = _operand(post_bias, D, "post_bias", dev)
     weight = _operand(weight, D, "weight", dev)

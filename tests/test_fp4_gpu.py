@@ -607,6 +607,25 @@ def test_residual_norm_gate_forms():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_residual_norm_refuses_operands_of_another_shape():
+    """As many entries in another order: [1, L, D] with L = B is not a row for each batch item."""
+    from flashvsr_sm89_ops_b200 import fused_residual_norm
+    for B, L, D in ((2, 2, 64), (3, 2, 64)):
+        x = randn(gen(4), B, L, D).to(torch.bfloat16)
+        for name in ("gate", "scale", "shift"):
+            t = randn(gen(5), B, 1, D).to(torch.bfloat16)
+            a = fused_residual_norm(x, x, **{name: t})
+            b = fused_residual_norm(x, x, **{name: t.view(B, D)})
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+            for shape in ((1, B, D), (B, D, 1), (1, 1, B * D)):
+                with pytest.raises(ValueError, match=name):
+                    fused_residual_norm(x, x, **{name: t.reshape(shape)})
+        rows = randn(gen(6), B, L, D).to(torch.bfloat16)
+        for shape in ((1, B * L, D), (B, D, L)) + (((L, B, D),) if L != B else ()):
+            with pytest.raises(ValueError, match="gate"):
+                fused_residual_norm(x, x, gate=rows.reshape(shape))
+
+
 def test_residual_norm_extremes():
     """Constant and zero rows (a variance of 0), and a NaN that stays in its row."""
     from flashvsr_sm89_ops_b200 import dequantize_fp4, fused_residual_norm
