@@ -123,8 +123,9 @@ def ffn_fp4(a: FP4Tensor, w0: FP4Tensor, b0: torch.Tensor | None, w2: FP4Tensor,
     need = _lib.load().fvb_fp4_ffn_workspace_bytes(M, F)
     if workspace is None:
         workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
-    elif workspace.numel() * workspace.element_size() < need or workspace.device != dev:
-        raise ValueError(f"ffn_fp4: workspace needs {need} bytes on {dev}")
+    elif workspace.numel() * workspace.element_size() < need or workspace.device != dev \
+            or not workspace.is_contiguous():
+        raise ValueError(f"ffn_fp4: workspace needs {need} contiguous bytes on {dev}")
     ptr = _lib.ptr
     _lib.call("fvb_fp4_ffn", a.codes_ptr, a.scales_ptr, a.row_scale_ptr, a._row_mode, w0.codes_ptr,
               w0.scales_ptr, w0.row_scale_ptr, w0._row_mode, _FMTS[a.fmt], ptr(b0), w2.codes_ptr,

@@ -768,6 +768,18 @@ def test_refusals():
     torch.cuda.synchronize()
 
 
+def test_ffn_refuses_a_workspace_with_less_memory_than_entries():
+    from flashvsr_sm89_ops_b200 import _lib, ffn_fp4, quantize_fp4
+    a = quantize_fp4(torch.randn(200, 64, device=DEV), "mx")
+    w0, w2 = (quantize_fp4(torch.randn(s, device=DEV), "mx") for s in ((96, 64), (8, 96)))
+    need = _lib.load().fvb_fp4_ffn_workspace_bytes(200, 96)
+    wide = torch.empty(256, dtype=torch.uint8, device=DEV)[:1].expand(need)
+    with pytest.raises(ValueError, match="contiguous"):
+        ffn_fp4(a, w0, None, w2, None, workspace=wide)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    assert torch.equal(ffn_fp4(a, w0, None, w2, None, workspace=ws), ffn_fp4(a, w0, None, w2, None))
+
+
 # ----------------------------------------------------------------------------- the model's path
 def small_dit(device, dtype=torch.bfloat16):
     from flashvsr_sm89_ops_b200 import wan_video_dit as W
