@@ -158,7 +158,10 @@ class FP4Linear(nn.Module):
         codes, scales, row_scale = _quantize_weight(linear.weight.detach(), fmt)
         self.weight = nn.Parameter(codes, requires_grad=False)
         self.register_buffer("w_scales", scales, persistent=False)
-        self.register_buffer("w_row_scale", row_scale, persistent=False)
+        # the fp32 row scales' bits as integers: a cast of the whole model, to fp16 say, where 2^-25
+        # is 0, leaves them alone
+        bits = None if row_scale is None else row_scale.view(torch.int32)
+        self.register_buffer("w_row_scale_bits", bits, persistent=False)
         if linear.bias is not None:
             self.bias = nn.Parameter(linear.bias.detach().to(torch.bfloat16).clone(),
                                      requires_grad=False)
@@ -166,8 +169,9 @@ class FP4Linear(nn.Module):
             self.bias = None
 
     def weight_fp4(self) -> FP4Tensor:
-        rs = self.w_row_scale  # a model cast to bf16 casts it too: a power of two, so exactly
-        return FP4Tensor(self.weight.data, self.w_scales, None if rs is None else rs.float(),
+        bits = self.w_row_scale_bits
+        return FP4Tensor(self.weight.data, self.w_scales,
+                         None if bits is None else bits.view(torch.float32),
                          (self.out_features, self.in_features), self.fmt)
 
     def forward(self, x):

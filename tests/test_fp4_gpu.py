@@ -722,6 +722,22 @@ def test_linear_and_ffn_modules():
         FP4FFN(FP4Linear(l0, "nv"), FP4Linear(l2, "nv"))
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_linear_survives_a_cast_of_the_model(fmt):
+    """Row scales far outside fp16 (weights near 1e-9 and 1e9) after .to(fp16 / fp64)."""
+    import torch.nn as nn
+    from flashvsr_sm89_ops_b200 import FP4Linear
+    lin = nn.Linear(64, 48, bias=False).to(DEV)
+    with torch.no_grad():
+        lin.weight[:16] *= 1e-9
+        lin.weight[16:32] *= 1e9
+    x = randn(gen(1), 5, 64).to(torch.bfloat16)
+    y = FP4Linear(lin, fmt)(x)
+    assert y[:, :16].any() and torch.isfinite(y).all()
+    for dt in (torch.float16, torch.float64, torch.bfloat16):
+        assert torch.equal(FP4Linear(lin, fmt).to(dt)(x), y)
+
+
 def test_refusals():
     from flashvsr_sm89_ops_b200 import (FP4Tensor, dequantize_fp4, ffn_fp4, fp4_mm,
                                         fused_residual_norm, quantize_fp4)
