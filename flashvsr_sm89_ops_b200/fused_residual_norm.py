@@ -16,6 +16,12 @@ from .fp4_quant import _empty, fp4_format
 _NORMS = {None: _lib.FVB_NORM_NONE, "rms": _lib.FVB_NORM_RMS, "layer": _lib.FVB_NORM_LAYER}
 
 
+def _dense(t):
+    """t as the kernel reads it: contiguous, from a 16-byte boundary on."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _operand(t, n, what, device):
     if t is None:
         return None
@@ -25,7 +31,7 @@ def _operand(t, n, what, device):
         raise ValueError(f"fused_residual_norm: {what} is on {t.device}, x on {device}")
     if t.dtype != torch.bfloat16:
         t = t.to(torch.bfloat16)
-    return t if t.is_contiguous() else t.contiguous()
+    return _dense(t)
 
 
 def _per_item(t, B, D, what, device):
@@ -70,8 +76,7 @@ def fused_residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor 
     dev = x.device
     if y.device != dev:
         raise ValueError(f"fused_residual_norm: y is on {y.device}, x on {dev}")
-    x = x if x.is_contiguous() else x.contiguous()
-    y = y if y.is_contiguous() else y.contiguous()
+    x, y = _dense(x), _dense(y)
     gate_rows = 0
     if gate is not None and L > 1 and gate.numel() == B * L * D and (gate.dim() != 3 or gate.shape == x.shape):
         gate_rows = 1

@@ -344,8 +344,8 @@ FVB_API int fvb_dequant_fp4(const void* codes, const void* scales, const float* 
  *   y[m, n] = rsA[m] * rsW[n] * sum_k A[m, k] W[n, k] + bias[n]
  * A [M, K] and W [N, K] in 4 bits of the same format; rsA / rsW as in fvb_dequant_fp4 (a_mode,
  * w_mode; ignored for mx).  bias, gate [N] bf16 or NULL, residual [M, N] bf16 with row pitch
- * ldr (0 = N) or NULL, out [M, N] bf16 (may be the residual).  Any M, N, K: the sums are fp32
- * on the tcgen05 block-scaled tensor cores and out is rounded once. */
+ * ldr (0 = N) or NULL, out [M, N] bf16 (may be the residual).  Any M and N, K >= 1: the sums are
+ * fp32 on the tcgen05 block-scaled tensor cores and out is rounded once. */
 FVB_API int fvb_fp4_gemm(const void* A, const void* sfA, const float* rsA, int a_mode, const void* W,
                          const void* sfW, const float* rsW, int w_mode, int fmt, const void* bias,
                          const void* residual, int64_t ldr, const void* gate, int64_t M, int64_t N,
@@ -368,7 +368,8 @@ FVB_API int fvb_fp4_ffn(const void* A, const void* sfA, const float* rsA, int a_
  * [B, D]; post_w, post_b, w, b [D]; all bf16, any of them NULL.  post: FVB_NORM_NONE / RMS /
  * LAYER, norm: RMS / LAYER.  fp32 between loads and stores: h is normed from the unrounded sum.
  * out [B, L, D] bf16 (NULL with fmt != 0), and with fmt the 4-bit codes of the unrounded h
- * ([B * L, D]; codes, scales, row_scale).  D % 8 == 0, D <= 16384. */
+ * ([B * L, D]; codes, scales, row_scale).  D % 8 == 0, D <= 16384; all pointers but row_scale
+ * 16-byte aligned. */
 #define FVB_NORM_NONE 0
 #define FVB_NORM_RMS 1
 #define FVB_NORM_LAYER 2

@@ -607,6 +607,24 @@ def test_residual_norm_gate_forms():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_residual_norm_unaligned_views():
+    """Operands that start off a 16-byte boundary: as their aligned copies."""
+    from flashvsr_sm89_ops_b200 import fused_residual_norm
+    c = rn_case(2, 6, 264)
+
+    def off(t):
+        wide = torch.empty(t.numel() + 3, dtype=t.dtype, device=DEV)[3:].view(t.shape)
+        return wide.copy_(t)
+
+    for gate in ("gate", "rows"):
+        t = {k: c[v] for k, v in dict(FULL, gate=gate).items()}
+        a = fused_residual_norm(c["x"], c["y"], post_norm="layer", emit_fp4="nv", **t)
+        b = fused_residual_norm(off(c["x"]), off(c["y"]), post_norm="layer", emit_fp4="nv",
+                                **{k: off(v) for k, v in t.items()})
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        assert torch.equal(R.values(a[2]), R.values(b[2]))
+
+
 def test_residual_norm_refuses_operands_of_another_shape():
     """As many entries in another order: [1, L, D] with L = B is not a row for each batch item."""
     from flashvsr_sm89_ops_b200 import fused_residual_norm
