@@ -28,6 +28,7 @@ namespace fvb {
 namespace resnorm {
 
 enum { kNone = 0, kRms = 1, kLayer = 2 };
+constexpr size_t kStaticSmem = 8 * 4;  // red_all, which counts toward the 48 KB that need no asking
 
 struct Args {
   const __nv_bfloat16* x;
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(256, NV == 8 ? 1 : 2) residual_norm_kernel(con
   // A1, A2, B2: for each first the lower, then the upper four floats of every vector, so that a
   // warp's 16-byte reads fall on all banks
   extern __shared__ float4 cols[];
-  __shared__ float red_all[8];
+  __shared__ float red_all[kStaticSmem / 4];
   const int team = WPR == 1 ? threadIdx.x >> 5 : threadIdx.x / T;
   const int t = threadIdx.x % T;
   float* red = red_all + team * WPR;
@@ -344,7 +345,7 @@ static int launch_as(Args a, int64_t B, cudaStream_t st) {
   auto kern = residual_norm_kernel<NV, WPR, FULL, EXTRA, FMT>;
   const size_t smem = (size_t)3 * a.D * 4;
   constexpr size_t most_smem = (size_t)3 * NV * WPR * 256 * 4;  // of the widest row it takes
-  if (most_smem > 48 * 1024) {
+  if (most_smem + kStaticSmem > 48 * 1024) {
     // the same limit whoever sets it: calls of several threads and widths may meet here
     static std::atomic<bool> configured[64];
     int dev = 0;

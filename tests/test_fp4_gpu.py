@@ -593,6 +593,15 @@ def test_residual_norm_codes_on_midpoints(emit):
     assert torch.equal(R.values(q), R.quantize(h.expand(3, D), emit)[0])
 
 
+@pytest.mark.parametrize("emit", [None] + FMTS)
+@pytest.mark.parametrize("D", [256, 512, 1024, 2048, 4096, 8192])
+def test_residual_norm_widest_rows(D, emit):
+    """The widest row of each layout, whose column operands fill the layout's shared memory."""
+    c = rn_case(2, 5, D)
+    rn_check(c, {k: v for k, v in FULL.items() if k != "post_bias"}, emit=emit, post_norm="rms", norm="layer")
+    rn_check(c, FULL, emit=emit, post_norm="layer", norm="rms")
+
+
 def test_residual_norm_gate_forms():
     from flashvsr_sm89_ops_b200 import fused_residual_norm
     c = rn_case(2, 6, 264)
