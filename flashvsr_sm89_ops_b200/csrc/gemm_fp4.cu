@@ -1038,8 +1038,6 @@ __global__ void __launch_bounds__(Split<FMT>::kThreads, 1)
 struct Operand {
   const void* codes;
   const void* scales;
-  const float* rs;
-  int rs_row;
 };
 
 // codes of A in boxes of 128 rows and of W in boxes of `rows_b`, a K block wide; the scale tiles
@@ -1215,8 +1213,8 @@ static int operands(const char* who, const void* A, const void* sfA, const float
     g.sa_row = a_mode == FVB_SCALE_ROW;
     g.sw_row = w_mode == FVB_SCALE_ROW;
   }
-  oa = Operand{A, sfA, rsA, g.sa_row};
-  ow = Operand{W, sfW, rsW, g.sw_row};
+  oa = Operand{A, sfA};
+  ow = Operand{W, sfW};
   return FVB_OK;
 }
 

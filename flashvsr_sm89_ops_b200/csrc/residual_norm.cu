@@ -40,7 +40,7 @@ struct Args {
   const __nv_bfloat16* b;
   const __nv_bfloat16* scale;  // [B, D] or NULL
   const __nv_bfloat16* shift;
-  int64_t rows, L;
+  int64_t L;
   int D, post, norm, gate_rows;
   float rs, eps, post_eps;
   __nv_bfloat16* x_out;
@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(256, NV == 8 ? 1 : 2) residual_norm_kernel(con
     }
     if (FMT == 0) continue;
     // 4-bit codes: a block is 2 (nv) or 4 (mx) neighbouring lanes' vectors.  The whole warp
-    // takes every turn (shuffles); one more than the registers hold, since the padding of the
-    // last scale tile may start past the row's last vector
+    // takes every turn (shuffles).  The padding of the last scale tile ends within the turns: they
+    // cover whole tiles, 8 or 16 vectors
     const auto mx = [](float x, float y) { return fmaxf(x, y); };
     uint32_t bad = 0u;
 #pragma unroll
@@ -302,38 +302,34 @@ __global__ void __launch_bounds__(256, NV == 8 ? 1 : 2) residual_norm_kernel(con
     constexpr int PER = FMT == FVB_FP4_NV ? 2 : 4;  // vectors per block
     uint8_t* sp = a.scales + fp4::scale_at(row, t / PER, a.tiles);
 #pragma unroll
-    for (int j = 0; j < NV + 1; ++j) {
+    for (int j = 0; j < NV; ++j) {
       const int v = t + j * T;
       if (v >= npad) break;
-      uint32_t byte = 0u, code = 0u;
-      if (j < NV) {
-        constexpr int last_j = NV - 1;
-        const int jj = j < NV ? j : last_j;
-        float q[8];
-        if (FMT == FVB_FP4_NV) {
-          byte = fp4::nv_scale(am[jj], ik);
-          const float d = fp4::e4m3_value(byte) * rs, r = byte == 0u ? 0.f : __frcp_rn(d);
-          const uint64_t r2 = f2_pack(r, r), nd2 = f2_pack(-d, -d);
-          // fp4::quotient on pairs: a bare product with r puts some midpoints on their wrong side
+      uint32_t byte, code;
+      float q[8];
+      if (FMT == FVB_FP4_NV) {
+        byte = fp4::nv_scale(am[j], ik);
+        const float d = fp4::e4m3_value(byte) * rs, r = byte == 0u ? 0.f : __frcp_rn(d);
+        const uint64_t r2 = f2_pack(r, r), nd2 = f2_pack(-d, -d);
+        // fp4::quotient on pairs: a bare product with r puts some midpoints on their wrong side
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint64_t p = f2_mul(f[jj][i], r2);
-            f2_unpack(f2_fma(f2_fma(p, nd2, f[jj][i]), r2, p), q[2 * i], q[2 * i + 1]);
-          }
-        } else {
-          const int e = fp4::mx_exponent(am[jj]);
-          const float r = fp4::pow2i(-e);
-          byte = (uint32_t)(e + 127);
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t p = f2_mul(f[j][i], r2);
+          f2_unpack(f2_fma(f2_fma(p, nd2, f[j][i]), r2, p), q[2 * i], q[2 * i + 1]);
+        }
+      } else {
+        const int e = fp4::mx_exponent(am[j]);
+        const float r = fp4::pow2i(-e);
+        byte = (uint32_t)(e + 127);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f[jj][i], f2_pack(r, r)), q[2 * i], q[2 * i + 1]);
-        }
-        code = fp4::e2m1x8(q);
-        if ((bad >> jj) & 1u) {
-          code = 0u;
-          byte = FMT == FVB_FP4_NV ? 0x7Fu : 0xFFu;
-        }
-        if (!FULL && v >= nvec) code = byte = 0u;
+        for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f[j][i], f2_pack(r, r)), q[2 * i], q[2 * i + 1]);
       }
+      code = fp4::e2m1x8(q);
+      if ((bad >> j) & 1u) {
+        code = 0u;
+        byte = FMT == FVB_FP4_NV ? 0x7Fu : 0xFFu;
+      }
+      if (!FULL && v >= nvec) code = byte = 0u;
       if (v * 4 < a.pitch) cp[v] = code;
       if (t % PER == 0) sp[(int64_t)j * (T / PER / 4) * 512] = (uint8_t)byte;
     }
@@ -371,18 +367,24 @@ static int launch_as(Args a, int64_t B, cudaStream_t st) {
   return check_launch("fvb_residual_norm");
 }
 
+template <int NV, int WPR, int FMT>
+static int launch_fmt(const Args& a, int64_t B, cudaStream_t st) {
+  // without FULL's instances the widths that fill the registers take 5-13% longer: 8448 x 1536 18.3
+  // us against 17.4 (bf16), 23.3 against 21.4 (nv), 21.1 against 19.0 (mx); 25344 x 512 17.7 : 16.3
+  const bool full = a.D == NV * WPR * 256, extra = a.gate_rows || a.pb;
+  if (full && extra) return launch_as<NV, WPR, true, true, FMT>(a, B, st);
+  if (full) return launch_as<NV, WPR, true, false, FMT>(a, B, st);
+  if (extra) return launch_as<NV, WPR, false, true, FMT>(a, B, st);
+  return launch_as<NV, WPR, false, false, FMT>(a, B, st);
+}
+template <int NV, int WPR>
+static int launch_codes(const Args& a, int64_t B, cudaStream_t st) {
+  return a.fmt == FVB_FP4_NV ? launch_fmt<NV, WPR, FVB_FP4_NV>(a, B, st)
+                             : launch_fmt<NV, WPR, FVB_FP4_MX>(a, B, st);
+}
 template <int NV, int WPR>
 static int launch(const Args& a, int64_t B, cudaStream_t st) {
-  const bool full = a.D == NV * WPR * 256, extra = a.gate_rows || a.pb;
-#define FVB_RN(FULL, EXTRA)                                                     \
-  return a.fmt == 0 ? launch_as<NV, WPR, FULL, EXTRA, 0>(a, B, st)              \
-                    : a.fmt == FVB_FP4_NV ? launch_as<NV, WPR, FULL, EXTRA, FVB_FP4_NV>(a, B, st) \
-                                          : launch_as<NV, WPR, FULL, EXTRA, FVB_FP4_MX>(a, B, st)
-  if (full && extra) FVB_RN(true, true);
-  if (full) FVB_RN(true, false);
-  if (extra) FVB_RN(false, true);
-  FVB_RN(false, false);
-#undef FVB_RN
+  return a.fmt ? launch_codes<NV, WPR>(a, B, st) : launch_fmt<NV, WPR, 0>(a, B, st);
 }
 
 }  // namespace resnorm
@@ -422,7 +424,6 @@ extern "C" int fvb_residual_norm(const void* x, const void* y, const void* gate,
   a.b = (const __nv_bfloat16*)b;
   a.scale = (const __nv_bfloat16*)scale;
   a.shift = (const __nv_bfloat16*)shift;
-  a.rows = B * L;
   a.L = L;
   a.D = (int)D;
   a.post = post;
@@ -444,7 +445,8 @@ extern "C" int fvb_residual_norm(const void* x, const void* y, const void* gate,
   if (D <= 1024) return resnorm::launch<4, 1>(a, B, st);
   // one warp a row or two: 39.0 us against 37.4 on 2 x 8448 x 1536, with codes 20.9 against 22.8
   // on 8448 x 1536 (nv)
-  if (D <= 1536) return fmt ? resnorm::launch<6, 1>(a, B, st) : resnorm::launch<3, 2>(a, B, st);
+  if (D <= 1536)
+    return fmt ? resnorm::launch_codes<6, 1>(a, B, st) : resnorm::launch_fmt<3, 2, 0>(a, B, st);
   if (D <= 2048) return resnorm::launch<4, 2>(a, B, st);
   if (D <= 4096) return resnorm::launch<4, 4>(a, B, st);
   if (D <= 8192) return resnorm::launch<4, 8>(a, B, st);
