@@ -443,10 +443,15 @@ extern "C" int fvb_residual_norm(const void* x, const void* y, const void* gate,
   if (D <= 256) return resnorm::launch<1, 1>(a, B, st);
   if (D <= 512) return resnorm::launch<2, 1>(a, B, st);
   if (D <= 1024) return resnorm::launch<4, 1>(a, B, st);
-  // one warp a row or two: 39.0 us against 37.4 on 2 x 8448 x 1536, with codes 20.9 against 22.8
-  // on 8448 x 1536 (nv)
+  // One warp a row or two.  With codes one, which leaves their blocks and row maxima within a warp,
+  // once the rows give every SM a block of such warps; below that two.  us, one : two
+  //   nv   512 x 1032 5.1 : 4.1   512 x 1536 5.2 : 4.0   2112 x 1536 7.2 : 7.6   16896 x 1536 36.5 : 37.7
+  //   mx   512 x 1032 4.8 : 3.7   512 x 1536 4.7 : 3.6   2112 x 1536 6.4 : 6.6   16896 x 1536 32.0 : 31.9
+  // Without codes two: 512 x 1536 4.1 : 3.3, 16896 x 1536 37.5 : 36.8 (38.4 : 37.3 with a post-norm),
+  // though one is faster for narrow rows in numbers, 16896 x 1032 25.1 : 26.2
   if (D <= 1536)
-    return fmt ? resnorm::launch_codes<6, 1>(a, B, st) : resnorm::launch_fmt<3, 2, 0>(a, B, st);
+    return fmt && B * L > 8 * (int64_t)sm_count() ? resnorm::launch_codes<6, 1>(a, B, st)
+                                                  : resnorm::launch<3, 2>(a, B, st);
   if (D <= 2048) return resnorm::launch<4, 2>(a, B, st);
   if (D <= 4096) return resnorm::launch<4, 4>(a, B, st);
   if (D <= 8192) return resnorm::launch<4, 8>(a, B, st);

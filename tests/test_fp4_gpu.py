@@ -593,6 +593,15 @@ def test_residual_norm_codes_on_midpoints(emit):
     assert torch.equal(R.values(q), R.quantize(h.expand(3, D), emit)[0])
 
 
+@pytest.mark.parametrize("emit", FMTS)
+@pytest.mark.parametrize("B,L,D", [(1, 1200, 1536), (3, 401, 1040), (2, 600, 1032)])
+def test_residual_norm_emits_codes_for_many_rows(B, L, D, emit):
+    """Rows enough for one warp each."""
+    c = rn_case(B, L, D)
+    rn_check(c, {k: v for k, v in FULL.items() if k != "post_bias"}, emit=emit, post_norm="rms", norm="layer")
+    rn_check(c, dict(FULL, gate="rows"), emit=emit, post_norm="layer", norm="rms")
+
+
 @pytest.mark.parametrize("emit", [None] + FMTS)
 @pytest.mark.parametrize("D", [256, 512, 1024, 2048, 4096, 8192])
 def test_residual_norm_widest_rows(D, emit):
