@@ -385,6 +385,35 @@ def test_product_is_repeatable_and_graph_safe():
         assert torch.equal(back, dequantize_fp4(quantize_fp4(x, "nv")))
 
 
+@pytest.mark.parametrize("N", [8192, 8191])
+def test_product_offsets_past_32_bits(N):
+    """An output and a residual of more than 2^31 elements, with and without TMA for them."""
+    from flashvsr_sm89_ops_b200 import FP4Tensor, fp4_mm
+    M = 2 ** 31 // N + 300
+    a, w, bias, res, gate = mm_case(300, N, 64, "mx")
+    # the same 300 rows first and last, zero codes between
+    codes = torch.zeros(M, 32, dtype=torch.uint8, device=DEV)
+    codes[:300], codes[-300:] = a.codes, a.codes
+    last = torch.arange(M - 300, M, device=DEV)
+    scales = torch.zeros(-(-M // 128) * 512, dtype=torch.uint8, device=DEV)
+    for rows in (torch.arange(300, device=DEV), last):
+        for j in range(2):
+            at = rows // 128 * 512 + rows % 32 * 16 + rows % 128 // 32 * 4 + j
+            own = torch.arange(300, device=DEV)
+            scales[at] = a.scales[own // 128 * 512 + own % 32 * 16 + own % 128 // 32 * 4 + j]
+    big = FP4Tensor(codes, scales, None, (M, 64), "mx")
+    residual = torch.zeros(M, N, dtype=torch.bfloat16, device=DEV)
+    residual[:300], residual[-300:] = res, res
+    out = fp4_mm(big, w, bias, residual=residual, gate=gate, out=residual)
+    y, S = mm_ref(a, w)
+    yb = y + bias.double()
+    o = res.double() + gate.double() * yb
+    mag = res.double().abs() + gate.double().abs() * (yb.abs() + S)
+    tol = BF16 * o.abs() + gate.double().abs() * steps(64) * S + 2.0 ** -22 * mag
+    check(out[:300], o, tol)
+    check(out[-300:], o, tol)
+
+
 # ----------------------------------------------------------------------------- FFN
 def spread(h, e, fmt):
     """How far apart the quantised values of |h| - e and |h| + e are, elementwise: what an
@@ -609,6 +638,26 @@ def test_residual_norm_widest_rows(D, emit):
     c = rn_case(2, 5, D)
     rn_check(c, {k: v for k, v in FULL.items() if k != "post_bias"}, emit=emit, post_norm="rms", norm="layer")
     rn_check(c, FULL, emit=emit, post_norm="layer", norm="rms")
+
+
+@pytest.mark.parametrize("emit", FMTS)
+def test_residual_norm_offsets_past_32_bits(emit):
+    """More than 2^31 elements: the last rows get what they get alone."""
+    from flashvsr_sm89_ops_b200 import dequantize_fp4, fused_residual_norm
+    D = 8192
+    L = 2 ** 31 // D + 130
+    c = rn_case(1, 5, D)
+    x = torch.zeros(1, L, D, dtype=torch.bfloat16, device=DEV)
+    y = torch.zeros_like(x)
+    x[:, -5:], y[:, -5:] = c["x"], c["y"]
+    kw = dict(gate=c["gate"], scale=c["scale"], shift=c["shift"], post_norm="rms", emit_fp4=emit)
+    xn, h, q = fused_residual_norm(x, y, **kw)
+    xs, hs, qs = fused_residual_norm(c["x"], c["y"], **kw)
+    assert torch.equal(xn[:, -5:], xs) and torch.equal(h[:, -5:], hs)
+    assert not xn[:, :64].any() and torch.equal(h[:, L // 2], c["shift"][:, 0])
+    v = dequantize_fp4(q)
+    assert torch.equal(v[-5:], dequantize_fp4(qs))
+    assert torch.equal(v[:1], v[L // 2:L // 2 + 1]) and v[:1].any()
 
 
 def test_residual_norm_gate_forms():
