@@ -773,6 +773,30 @@ def test_residual_norm_first_calls_from_threads():
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+@pytest.mark.parametrize("emit", FMTS)
+@pytest.mark.parametrize("L,D", [(3, 40), (5, 256), (3, 1000), (2, 1536), (1200, 1536), (2, 4104)])
+def test_residual_norm_nonfinite_columns(L, D, emit):
+    """An infinity or NaN in one column of h makes that column's block NaN and no other; the
+    block's finite values still count in the row's maximum."""
+    from flashvsr_sm89_ops_b200 import fused_residual_norm
+    c = rn_case(1, L, D)
+    n = R.BLOCK[emit]
+    shift = c["shift"].clone()
+    hot = (D // 3) // n * n
+    shift[0, 0, hot] = 300.0  # the row's maximum, in the block that is then spoilt
+    _, _, ref = fused_residual_norm(c["x"], c["y"], scale=c["scale"], shift=shift, emit_fp4=emit)
+    for bad in (math.inf, -math.inf, math.nan):
+        spoilt = shift.clone()
+        spoilt[0, 0, hot + 5] = spoilt[0, 0, D - 1] = bad
+        _, h, q = fused_residual_norm(c["x"], c["y"], scale=c["scale"], shift=spoilt, emit_fp4=emit)
+        v, want = R.values(q), R.values(ref)
+        nan = torch.zeros(D, dtype=torch.bool)
+        nan[hot:hot + n] = nan[(D - 1) // n * n:] = True
+        assert torch.equal(v.isnan(), nan.expand(L, D))
+        assert torch.equal(v[:, ~nan], want[:, ~nan])
+        assert not R.padding(q).any()
+
+
 def test_empty_batches():
     from flashvsr_sm89_ops_b200 import ffn_fp4, fp4_mm, fused_residual_norm, quantize_fp4
     x = torch.empty(2, 0, 64, dtype=torch.bfloat16, device=DEV)
