@@ -16,30 +16,21 @@ from .fp4_quant import _empty, fp4_format
 _NORMS = {None: _lib.FVB_NORM_NONE, "rms": _lib.FVB_NORM_RMS, "layer": _lib.FVB_NORM_LAYER}
 
 
-def _dense(t):
-    """t as the kernel reads it: contiguous, from a 16-byte boundary on."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _operand(t, n, what, device):
+def _operand(t, n, what, device, items=0):
+    """t of n entries as the kernel takes it.  items: t has a row for each of so many batch items; a
+    3-D t of another shape, [1, L, D] with L = items say, would mean something else."""
     if t is None:
         return None
-    if t.numel() != n:
+    if items > 1 and t.dim() == 3:
+        if t.shape != (items, 1, n // items):
+            raise ValueError(f"fused_residual_norm: {what} must be [{items}, 1, {n // items}], got {tuple(t.shape)}")
+    elif t.numel() != n:
         raise ValueError(f"fused_residual_norm: {what} must have {n} entries, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"fused_residual_norm: {what} is on {t.device}, x on {device}")
     if t.dtype != torch.bfloat16:
         t = t.to(torch.bfloat16)
-    return _dense(t)
-
-
-def _per_item(t, B, D, what, device):
-    """An operand with a row for each batch item.  A 3-D one of as many entries in another shape,
-    [1, L, D] with L = B say, would mean something else and is refused."""
-    if t is not None and t.dim() == 3 and t.shape != (B, 1, D):
-        raise ValueError(f"fused_residual_norm: {what} must be [{B}, 1, {D}], got {tuple(t.shape)}")
-    return _operand(t, B * D, what, device)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def fused_residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor | None = None,
@@ -76,27 +67,40 @@ def fused_residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: torch.Tensor 
     dev = x.device
     if y.device != dev:
         raise ValueError(f"fused_residual_norm: y is on {y.device}, x on {dev}")
-    x, y = _dense(x), _dense(y)
+    x = x if x.is_contiguous() else x.contiguous()
+    y = y if y.is_contiguous() else y.contiguous()
     gate_rows = 0
-    if gate is not None and L > 1 and gate.numel() == B * L * D and (gate.dim() != 3 or gate.shape == x.shape):
-        gate_rows = 1
-        gate = _operand(gate, B * L * D, "gate", dev)
-    else:
-        gate = _per_item(gate, B, D, "gate", dev)
-    scale = _per_item(scale, B, D, "scale", dev)
-    shift = _per_item(shift, B, D, "shift", dev)
+    if gate is not None:
+        if L > 1 and gate.numel() == B * L * D and (gate.dim() != 3 or gate.shape == x.shape):
+            gate_rows = 1
+            gate = _operand(gate, B * L * D, "gate", dev)
+        else:
+            gate = _operand(gate, B * D, "gate", dev, B)
+    scale = _operand(scale, B * D, "scale", dev, B)
+    shift = _operand(shift, B * D, "shift", dev, B)
     post_weight = _operand(post_weight, D, "post_weight", dev)
     post_bias = _operand(post_bias, D, "post_bias", dev)
     weight = _operand(weight, D, "weight", dev)
     bias = _operand(bias, D, "bias", dev)
+    # NULL (0) for what is absent; the kernel reads 16-byte vectors
+    xp, yp = x.data_ptr(), y.data_ptr()
+    gp = gate.data_ptr() if gate is not None else 0
+    pwp = post_weight.data_ptr() if post_weight is not None else 0
+    pbp = post_bias.data_ptr() if post_bias is not None else 0
+    wp = weight.data_ptr() if weight is not None else 0
+    bp = bias.data_ptr() if bias is not None else 0
+    scp = scale.data_ptr() if scale is not None else 0
+    shp = shift.data_ptr() if shift is not None else 0
+    if (xp | yp | gp | pwp | pbp | wp | bp | scp | shp) & 15:
+        copies = [t.clone() if t is not None and t.data_ptr() & 15 else t
+                  for t in (x, y, gate, post_weight, post_bias, weight, bias, scale, shift)]
+        xp, yp, gp, pwp, pbp, wp, bp, scp, shp = (0 if t is None else t.data_ptr() for t in copies)
     x_new = torch.empty_like(x)
     h = torch.empty_like(x) if want_out else None
     q = _empty(B * L, D, emit_fp4, dev) if fmt else None
-    p = _lib.ptr
-    _lib.call("fvb_residual_norm", p(x), p(y), p(gate), gate_rows, float(residual_scale),
-              _NORMS[post_norm], p(post_weight), p(post_bias),
-              float(eps if post_eps is None else post_eps), _NORMS[norm], p(weight), p(bias),
-              p(scale), p(shift), float(eps), B, L, D, p(x_new), p(h), fmt,
+    _lib.call("fvb_residual_norm", xp, yp, gp, gate_rows, float(residual_scale), _NORMS[post_norm],
+              pwp, pbp, float(eps if post_eps is None else post_eps), _NORMS[norm], wp, bp, scp, shp,
+              float(eps), B, L, D, x_new.data_ptr(), h.data_ptr() if want_out else 0, fmt,
               q.codes_ptr if fmt else None, q.scales_ptr if fmt else None,
               q.row_scale_ptr if fmt else None, _lib.stream_of(x))
     return (x_new, h, q) if fmt else (x_new, h)
