@@ -1278,6 +1278,11 @@ int fvb_fp4_ffn(const void* A, const void* sfA, const float* rsA, int a_mode, co
   if (M == 0 || N == 0) return FVB_OK;
   FVB_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
               "fvb_fp4_ffn: workspace must be 256-byte aligned");
+  // what the second product would refuse, before the first is launched
+  FVB_REQUIRE(W2 && sfW2 && out, "fvb_fp4_ffn: NULL pointer");
+  FVB_REQUIRE(aligned16(W2) && aligned16(sfW2), "fvb_fp4_ffn: codes and scales must be 16-byte aligned");
+  FVB_REQUIRE(residual || !gate, "fvb_fp4_ffn: gate without a residual");
+  FVB_REQUIRE(!residual || ldr == 0 || ldr >= N || M == 1, "fvb_fp4_ffn: residual row pitch");
   gemm4::Args a;
   gemm4::Operand oa, ow;
   int rc = gemm4::operands("fvb_fp4_ffn", A, sfA, rsA, a_mode, W0, sfW0, rsW0, w_mode, fmt, M, F,

@@ -46,6 +46,17 @@ def test_entry_points_check_arguments_on_the_host():
     assert "fvb_residual_norm" in lib.fvb_last_error().decode()
 
 
+def test_ffn_entry_point_refuses_before_it_launches():
+    """What only the second product would refuse is refused at once."""
+    from flashvsr_sm89_ops_b200 import _lib
+    p = 4096
+    good = dict(A=p, sfA=p, rsA=None, am=0, W0=p, sfW0=p, rsW0=None, wm=0, fmt=1, b0=None, W2=p, sfW2=p,
+                b2=None, res=None, ldr=0, gate=None, M=4, D=64, F=32, N=8, out=p, ws=p, stream=None)
+    for bad in (dict(W2=None), dict(sfW2=None), dict(out=None), dict(W2=p + 8), dict(sfW2=p + 1),
+                dict(gate=p), dict(res=p, ldr=7)):
+        assert _lib.load().fvb_fp4_ffn(*{**good, **bad}.values()) == _lib.FVB_ERR_INVALID, bad
+
+
 def test_buffer_sizes():
     from flashvsr_sm89_ops_b200 import _lib
     lib = _lib.load()
