@@ -19,6 +19,8 @@ from .fp8_ffn import FP8FFN, convert_ffn_fp8  # noqa: E402
 from .fp4_quant import FP4_MAX, FP4Tensor, dequantize_fp4, quantize_fp4  # noqa: E402
 from .fp4_linear import FP4FFN, FP4Linear, convert_linears_fp4, ffn_fp4, fp4_mm  # noqa: E402
 from .fused_residual_norm import fused_residual_norm  # noqa: E402
+from .rope import Rope, fused_rope  # noqa: E402
+from .paged_kv import PagedKV, paged_attention  # noqa: E402
 from .integrate import enable  # noqa: E402
 from .tiling import auto_tile_limits, plan_tiles, render_tiled, tile_weight  # noqa: E402
 
@@ -43,6 +45,10 @@ __all__ = [
     "FP4FFN",
     "convert_linears_fp4",
     "fused_residual_norm",
+    "Rope",
+    "fused_rope",
+    "PagedKV",
+    "paged_attention",
     "plan_tiles",
     "render_tiled",
     "auto_tile_limits",

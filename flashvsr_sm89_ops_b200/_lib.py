@@ -94,6 +94,22 @@ _SIGS = {
     "fvb_residual_norm": (_int, [_vp, _vp, _vp, _int, _f32, _int, _vp, _vp, _f32, _int, _vp, _vp,
                                  _vp, _vp, _f32, _i64, _i64, _i64, _vp, _vp, _int, _vp, _vp, _vp,
                                  _vp]),
+    "fvb_rope": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
+                        _i64, _i64, _i64, _int, _int, _vp, _int, _i64, _vp, _vp, _f32, _int, _vp]),
+    "fvb_kv_append": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                             _i64, _i64, _i64, _i64, _int, _int, _vp, _int, _i64, _vp, _vp, _f32, _vp,
+                             _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "fvb_pages_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "fvb_pages_reserve": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "fvb_pages_fork": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64,
+                              _i64, _i64, _i64, _vp, _vp]),
+    "fvb_pages_release": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "fvb_pages_compact": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
+                                 _i64, _vp, _vp]),
+    "fvb_paged_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "fvb_paged_attn": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
+                              _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _f32, _int,
+                              _vp, _i64, _i64, _vp, _vp]),
 }
 
 
@@ -153,7 +169,7 @@ def _kernels_per_call(name: str, args) -> int:
         return 4
     if name == "fvb_causal_topk_mask":
         return 3
-    if name == "fvb_fp4_ffn":
+    if name in ("fvb_fp4_ffn", "fvb_pages_fork", "fvb_pages_compact", "fvb_paged_attn"):
         return 2
     if name in ("fvb_device_error", "fvb_abi_version", "fvb_last_error", "fvb_copy_window_h2d"):
         return 0  # no kernel (fvb_copy_window_h2d is a copy-engine transfer)
@@ -187,6 +203,15 @@ def call(name: str, *args):
         _raise(rc, name)
     if _count is not None:
         _count += _kernels_per_call(name, args)
+
+
+def call_on(device: int, name: str, *args):
+    """call() with `device` (an index) current: a launch belongs to the current device."""
+    if torch._C._cuda_getDevice() == device:
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 def ptr(t) -> int | None:

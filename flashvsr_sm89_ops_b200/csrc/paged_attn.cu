@@ -1,0 +1,1127 @@
+// Attention of a chunk of new tokens over a paged cache.
+//
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j,  j <= len - n + i (causal) or j < len
+// for the n new tokens i of each sequence, len its tokens in the cache (the new ones included),
+// query head h on key head h / g.  The g query heads of a key head are rows of one tile ("packed
+// row" i * g + h % g), so a key is read once for all of them.
+//
+// Work is cut the same way in both kernels.  An item is (sequence, key head, tile of packed
+// rows); its length is the number of key tiles that its last row sees.  The items of all
+// sequences lie end to end on one line of `total` key tiles, and CTA c takes tiles [c per,
+// (c+1) per): uneven sequences and causal triangles balance by themselves, few rows over a long
+// cache spread over the machine, and a last partial wave does not exist.  An item cut by a
+// boundary leaves unnormalised partial sums (fp32 O, row maximum and sum) that merge_kernel
+// joins in the order of the cut, so results do not depend on timing.  Lengths are read on the
+// device only: a captured graph follows them.
+//
+//   decode_kernel  up to 16 packed rows a tile: single tokens, a few drafted ones.  Bound by the
+//                  bytes of the cache.
+//   chunk_kernel   256 packed rows a tile on the tcgen05 tensor cores.  Bound by them and by the
+//                  exponentials.
+//
+// Keys past a sequence's end are never seen: their scores are -inf whatever the page holds, and
+// their values are zeros in shared memory, so NaNs left in a recycled page do not spread.  A
+// page number outside the pool reads as zeros.
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace fvb {
+namespace pattn {
+
+struct Args {
+  const void* q;
+  void* out;
+  int64_t q_token, q_head, o_token, o_head;  // strides, elements
+  const void *k, *v;
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+  const int32_t *table, *lens, *cu;  // cu NULL: one token a sequence
+  int64_t T, width, pages;
+  int B, Hk, g, page, causal, ctas;
+  float scale_log2;
+  float* part;    // [2 ctas][rows][D]: O of an item begun before the CTA, of one begun in it
+  float* part_ml; // [2 ctas][rows][2]
+  int32_t* rec;   // [ctas][8]: the item begun in the CTA that other CTAs end
+};
+
+struct Seq {
+  int n, len, off;  // new tokens, keys, keys before the first new token
+  int64_t t0;
+};
+
+__device__ __forceinline__ Seq get_seq(const Args& a, int b) {
+  Seq s;
+  int64_t c0 = b, c1 = b + 1;
+  if (a.cu) c0 = a.cu[b], c1 = a.cu[b + 1];
+  const int len = a.lens[b];
+  const int64_t most = a.width * a.page;
+  s.len = len < 0 ? 0 : (len < most ? len : (int)most);
+  s.off = (int)(len - (c1 - c0));
+  if (c1 > a.T) c1 = a.T;
+  s.n = c0 < 0 || c1 <= c0 ? 0 : (int)(c1 - c0);
+  s.t0 = c0;
+  return s;
+}
+
+// keys that token i of the sequence sees
+__device__ __forceinline__ int sees(const Args& a, const Seq& s, int i) {
+  if (!a.causal) return s.len;
+  const int v = s.off + i + 1;
+  return v < 0 ? 0 : (v < s.len ? v : s.len);
+}
+
+// key tiles of packed rows [r0, r1): 0 if there are no such rows
+template <int KT>
+__device__ __forceinline__ int tiles_of(const Args& a, const Seq& s, int64_t r0, int64_t r1) {
+  const int64_t rows = (int64_t)s.n * a.g;
+  if (r0 >= rows) return 0;
+  if (r1 > rows) r1 = rows;
+  return (sees(a, s, (int)((r1 - 1) / a.g)) + KT - 1) / KT;
+}
+
+struct Segment {  // key tiles [t0, t1) of an item's [0, tiles)
+  int b, h, rt, t0, t1, tiles;
+  Seq s;
+};
+
+// Walks over a CTA's segments.  Items with no key count as one tile, so that their rows (zeros)
+// have an owner.
+template <int R, int KT>
+struct Walk {
+  int64_t unit, end;
+  int b, h, rt, t0;
+  Seq s;
+
+  __device__ int item_tiles(const Args& a) const {
+    const int t = tiles_of<KT>(a, s, (int64_t)rt * R, (int64_t)rt * R + R);
+    return t > 0 ? t : 1;
+  }
+  __device__ bool next(const Args& a, Segment& g) {
+    if (unit >= end) return false;
+    const int tiles = item_tiles(a);
+    g.b = b, g.h = h, g.rt = rt, g.t0 = t0, g.tiles = tiles, g.s = s;
+    g.t1 = (int64_t)(tiles - t0) < end - unit ? tiles : t0 + (int)(end - unit);
+    unit += g.t1 - t0;
+    t0 = 0;
+    if (unit < end) {
+      if ((int64_t)(++rt) * R >= (int64_t)s.n * a.g) {
+        rt = 0;
+        if (++h == a.Hk) {
+          h = 0;
+          do s = get_seq(a, ++b); while (s.n == 0);
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// units of one key head of a sequence
+template <int R, int KT>
+__device__ int64_t head_units(const Args& a, const Seq& s) {
+  const int64_t rows = (int64_t)s.n * a.g;
+  if (!a.causal) {
+    const int64_t t = (s.len + KT - 1) / KT;
+    return ((rows + R - 1) / R) * (t > 0 ? t : 1);
+  }
+  int64_t u = 0;
+  for (int64_t r = 0; r < rows; r += R) {
+    const int t = tiles_of<KT>(a, s, r, r + R);
+    u += t > 0 ? t : 1;
+  }
+  return u;
+}
+
+struct Found {
+  int64_t total, rem;
+  int b;
+};
+
+// Every thread of the block; finds the walk of this CTA.  Returns the tiles a CTA takes.
+template <int R, int KT, int kThreads, int kLeast>
+__device__ int64_t start_walk(const Args& a, Walk<R, KT>& w, Found* sh, int64_t* sums) {
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t first = 0, mine = 0;
+  for (int64_t b = threadIdx.x; b < a.B; b += kThreads) {
+    const int64_t u = head_units<R, KT>(a, get_seq(a, (int)b)) * a.Hk;
+    if (b < kThreads) first = u;
+    mine += u;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums[warp] = mine;
+  if (threadIdx.x == 0) sh->b = -1;
+  __syncthreads();
+  int64_t total = 0;
+  for (int i = 0; i < kWarps; ++i) total += sums[i];
+  int64_t per = (total + a.ctas - 1) / a.ctas;
+  if (per < kLeast) per = kLeast;
+  const int64_t unit = (int64_t)blockIdx.x * per;
+  w.unit = unit;
+  w.end = unit + per < total ? unit + per : total;
+  if (unit >= total) return per;  // nothing here (the same for every thread)
+  int64_t base = 0;
+  for (int64_t at = 0; at < a.B; at += kThreads) {
+    const int64_t b = at + threadIdx.x;
+    int64_t u = at == 0 ? first : 0;
+    if (at && b < a.B) u = head_units<R, KT>(a, get_seq(a, (int)b)) * a.Hk;
+    int64_t x = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    int64_t before = base + x - u, all = 0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += sums[i];
+      all += sums[i];
+    }
+    if (u > 0 && before <= unit && unit < before + u) sh->b = (int)b, sh->rem = unit - before;
+    base += all;
+    __syncthreads();
+    if (base > unit) break;
+  }
+  w.b = sh->b;
+  int64_t rem = sh->rem;
+  w.s = get_seq(a, w.b);
+  const int64_t hu = head_units<R, KT>(a, w.s);
+  w.h = (int)(rem / hu);
+  rem -= w.h * hu;
+  w.rt = 0;
+  if (!a.causal) {
+    const int t = w.item_tiles(a);
+    w.rt = (int)(rem / t);
+    rem -= (int64_t)w.rt * t;
+  } else {
+    for (int t = w.item_tiles(a); rem >= t; t = w.item_tiles(a)) rem -= t, ++w.rt;
+  }
+  w.t0 = (int)rem;
+  return per;
+}
+
+// One thread: the record of an item that begins in this CTA and ends in another.
+template <int R, int KT>
+__device__ void write_rec(const Args& a, Walk<R, KT> w, int64_t per) {
+  int32_t* r = a.rec + (int64_t)blockIdx.x * 8;
+  Segment g;
+  int valid = 0;
+  int64_t at = w.unit;
+  while (w.next(a, g)) {
+    if (g.t0 == 0 && g.t1 < g.tiles) {
+      valid = 1;
+      r[1] = g.b, r[2] = g.h, r[3] = g.rt;
+      r[4] = (int32_t)((at + g.tiles - 1) / per);
+    }
+    at += g.t1 - g.t0;
+  }
+  r[0] = valid;
+}
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static constexpr uint32_t kFmt = 1;  // tcgen05 operand format
+  __device__ static uint32_t pack(float lo, float hi) {
+    __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&b);
+  }
+  __device__ static void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Pair<__half> {
+  static constexpr uint32_t kFmt = 0;
+  __device__ static uint32_t pack(float lo, float hi) {
+    __half2 b = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&b);
+  }
+  __device__ static void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+// ===========================================================================
+// Few rows: 16 packed rows against 64 keys a step, 16 of them a warp.
+//
+// Each warp streams its own 16-key strips (cp.async into its own ring, no block barrier in the
+// loop), multiplies them with mma.sync (a 128-row tensor-memory tile would be 7/8 empty, and at
+// these rates the cache's bytes bound the loop, not the products) and keeps its own maximum, sum
+// and O; the four warps join through shared memory at the end of a segment.
+// ===========================================================================
+namespace dec {
+
+constexpr int kThreads = 128, kRows = 16, kKeys = 64, kLeast = 2;
+constexpr int kRing = 96 * 1024;  // two CTAs an SM: 192 KB in flight
+
+template <int D>
+struct Shape {
+  static constexpr int kRowBytes = D * 2, kChunks = D / 8;
+  static constexpr int kStage = 2 * 16 * kRowBytes;           // K and V strip of a warp
+  static constexpr int kStages = kRing / (4 * kStage);
+  static constexpr int kPad = D + 4;                           // floats a row of the join
+};
+
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(take ? 16 : 0)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
+  using S = Shape<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Found found;
+  __shared__ int64_t sums[4];
+  __shared__ float s_ml[4][kRows][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  Walk<kRows, kKeys> w;
+  const int64_t per = start_walk<kRows, kKeys, kThreads, kLeast>(a, w, &found, sums);
+  if (threadIdx.x == 0) write_rec(a, w, per);
+
+  uint8_t* ring = smem + warp * (S::kStages * S::kStage);
+  const uint32_t ring_u = smem_u32(ring);
+  const T* const kp = reinterpret_cast<const T*>(a.k);
+  const T* const vp = reinterpret_cast<const T*>(a.v);
+  const int qrow = lane >> 2, qcol = (lane & 3) * 2;
+
+  Segment g;
+  while (w.next(a, g)) {
+    const int row0 = g.rt * kRows;
+    const int left = g.s.n * a.g - row0;
+    const int rows = left < kRows ? left : kRows;
+    // Q: fragments of the 16 x D tile
+    uint32_t qf[D / 16][4];
+    int lim[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int r = qrow + 8 * hh;
+      const bool ok = r < rows;
+      const int pr = row0 + (ok ? r : 0);
+      const int i = pr / a.g;
+      const T* qp = reinterpret_cast<const T*>(a.q) + (g.s.t0 + i) * a.q_token +
+                    (int64_t)(g.h * a.g + pr - i * a.g) * a.q_head + qcol;
+      lim[hh] = ok ? sees(a, g.s, i) : 0;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][hh] = ok ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
+        qf[kk][hh + 2] = ok ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
+      }
+    }
+    const int vis = sees(a, g.s, (row0 + rows - 1) / a.g);  // of the tile's last row
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    const int steps = g.t1 - g.t0;
+    const int32_t* row = a.table + (int64_t)g.b * a.width;
+    auto strip = [&](int j) { return (g.t0 + j) * kKeys + warp * 16; };
+    auto page_of = [&](int j) {  // page of a strip (pages are multiples of 16 rows)
+      const int key = strip(j);
+      return j < steps && key < vis ? __ldg(row + key / a.page) : -1;
+    };
+    auto load = [&](int j, int pid) {
+      const int key = strip(j);
+      if (j < steps && key < vis) {
+        const bool in = pid >= 0 && pid < a.pages;
+        const int slot = key % a.page;
+        const int64_t p = in ? pid : 0;
+        const T* ks = kp + p * a.k_page + (int64_t)slot * a.k_slot + g.h * a.k_head;
+        const T* vs = vp + p * a.v_page + (int64_t)slot * a.v_slot + g.h * a.v_head;
+        const uint32_t st = ring_u + (uint32_t)((j % S::kStages) * S::kStage);
+        const int c = lane % S::kChunks;
+#pragma unroll
+        for (int i = 0; i < S::kChunks / 2; ++i) {
+          const int r = i * (32 / S::kChunks) + lane / S::kChunks;
+          const uint32_t dst = st + (uint32_t)(r * S::kRowBytes + ((c ^ (r & 7)) << 4));
+          const bool take = in && key + r < g.s.len;
+          const int rr = take ? r : 0;
+          cp_async16_or_zero(dst, ks + rr * a.k_slot + c * 8, take);
+          cp_async16_or_zero(dst + S::kStage / 2, vs + rr * a.v_slot + c * 8, take);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // page numbers are fetched one strip ahead of the strip that needs them
+    int pid = page_of(0);
+#pragma unroll 1
+    for (int j = 0; j < S::kStages - 1; ++j) {
+      const int nx = page_of(j + 1);
+      load(j, pid);
+      pid = nx;
+    }
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+      const int nx = page_of(j + S::kStages);
+      cp_async_wait<S::kStages - 2>();
+      __syncwarp();  // strip j is there for every lane, strip j - 1 has been read by every lane
+      load(j + S::kStages - 1, pid);
+      pid = nx;
+      const int key0 = strip(j);
+      if (key0 >= vis) continue;
+      const uint32_t ks = ring_u + (uint32_t)((j % S::kStages) * S::kStage);
+      const uint32_t vs = ks + S::kStage / 2;
+      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      {
+        const int r = ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t b[4];
+          ldsm4(ks + (uint32_t)(r * S::kRowBytes + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4)), b);
+          Pair<T>::mma(sc[0], qf[kk], b[0], b[1]);
+          Pair<T>::mma(sc[1], qf[kk], b[2], b[3]);
+        }
+      }
+      float alpha[2];
+      bool grew = false;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = sc[t][hh * 2 + e];
+            x = key0 + t * 8 + qcol + e < lim[hh] ? x * a.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, x);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[hh], mx);
+        alpha[hh] = mn == -INFINITY ? 1.f : ex2_approx(m[hh] - mn);
+        grew |= mn > m[hh];
+        m[hh] = mn;
+        const float sub = mn == -INFINITY ? 0.f : mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = sc[t][hh * 2 + e];
+            x = ex2_approx(x - sub);
+            sum += x;
+          }
+        l[hh] = l[hh] * alpha[hh] + sum;  // this lane's four keys; the quad joins at the end
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= alpha[0], o[i][1] *= alpha[0];
+          o[i][2] *= alpha[1], o[i][3] *= alpha[1];
+        }
+      }
+      // P rounded to 16 bits, as the tensor cores take it: 2^-9 (bf16) or 2^-12 (fp16) a term
+      const uint32_t p[4] = {Pair<T>::pack(sc[0][0], sc[0][1]), Pair<T>::pack(sc[0][2], sc[0][3]),
+                             Pair<T>::pack(sc[1][0], sc[1][1]), Pair<T>::pack(sc[1][2], sc[1][3])};
+      const int r = (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t b[4];
+        ldsm4t(vs + (uint32_t)(r * S::kRowBytes + (((i * 2 + (lane >> 4)) ^ (r & 7)) << 4)), b);
+        Pair<T>::mma(o[2 * i], p, b[0], b[1]);
+        Pair<T>::mma(o[2 * i + 1], p, b[2], b[3]);
+      }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
+      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
+    }
+    __syncthreads();  // every warp is done with its ring: the join takes its place
+    float* const so = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int r = qrow + 8 * hh;
+      if (r < rows) {
+        float* dst = so + (warp * kRows + r) * S::kPad + qcol;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hh], o[i][2 * hh + 1]);
+        if ((lane & 3) == 0) s_ml[warp][r][0] = m[hh], s_ml[warp][r][1] = l[hh];
+      }
+    }
+    __syncthreads();
+    const bool whole = g.t0 == 0 && g.t1 == g.tiles;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (g.t0 == 0);
+    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
+      const int r = idx / (D / 4), c = (idx % (D / 4)) * 4;
+      float mm = s_ml[0][r][0];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) mm = fmaxf(mm, s_ml[i][r][0]);
+      const float sub = mm == -INFINITY ? 0.f : mm;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float ll = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = ex2_approx(s_ml[i][r][0] - sub);
+        const float4 v = *reinterpret_cast<const float4*>(so + (i * kRows + r) * S::kPad + c);
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+        ll = fmaf(f, s_ml[i][r][1], ll);
+      }
+      if (whole) {
+        const float inv = ll > 0.f ? 1.f / ll : 0.f;
+        // a row that sees no key is 0, whatever the values that other rows of its tile see
+        if (mm == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int pr = row0 + r, i = pr / a.g;
+        T* dst = reinterpret_cast<T*>(a.out) + (g.s.t0 + i) * a.o_token +
+                 (int64_t)(g.h * a.g + pr - i * a.g) * a.o_head + c;
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(a.part + (slot * kRows + r) * D + c) = acc;
+        if (c == 0)
+          *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(mm, ll);
+      }
+    }
+    __syncthreads();  // the ring is loaded again
+  }
+}
+
+}  // namespace dec
+
+// ===========================================================================
+// Many rows: 256 packed rows (two tiles of 128, "A" and "B") against 128 keys a step.
+//
+// Both tiles read the same key and value tiles from one ring, so a key crosses L2 once for 256
+// rows.  Per tile a warpgroup of softmax threads (a thread owns a row) and one MMA-issuing
+// thread; one warp loads.  Tensor memory: one score buffer that the tiles take in turn (a tile's
+// softmax copies its scores to registers, and the buffer is the other's), P_A, P_B as packed
+// 16-bit pairs, O_A, O_B.  O stays there for a whole segment; the running maximum is raised only
+// when a tile's exceeds it by more than 2^8, and O is rescaled in place then.
+// ===========================================================================
+namespace chunk {
+
+constexpr int kThreads = 384, kRows = 256, kKeys = 128, kLeast = 2;
+constexpr int kAtom = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzle
+constexpr float kLazy = 8.0f;
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
+
+template <int D>
+struct Shape {
+  static constexpr int kTile = D * 256;  // bytes of 128 rows
+  static constexpr int kSlots = D == 128 ? 2 : 4;  // of K and of V
+  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;
+};
+
+// p = 2^(s c - m) of 64 scores, packed; fp32 row sum into acc2
+template <typename T>
+__device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint64_t nm,
+                                           uint64_t& acc2, uint32_t* pk) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint64_t xv =
+        f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, nm);
+    float x0, x1;
+    f2_unpack(xv, x0, x1);
+    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+    acc2 = f2_add(acc2, f2_pack(p0, p1));
+    pk[i] = Pair<T>::pack(p0, p1);
+  }
+}
+
+// what both tiles of a segment do, the same for every thread
+struct Counts {
+  int c[2], all;
+};
+__device__ __forceinline__ Counts counts(const Args& a, const Segment& g) {
+  Counts r;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int64_t r0 = (int64_t)g.rt * kRows + x * 128;
+    const int t = tiles_of<kKeys>(a, g.s, r0, r0 + 128);
+    const int e = t < g.t1 ? t : g.t1;
+    r.c[x] = e > g.t0 ? e - g.t0 : 0;
+  }
+  r.all = r.c[0] > r.c[1] ? r.c[0] : r.c[1];
+  return r;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const int box, const Args a) {
+  using S = Shape<D>;
+  constexpr int kSlots = S::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  uint8_t* const sQ = base;
+  uint8_t* const sK = base + 2 * S::kTile;
+  uint8_t* const sV = sK + kSlots * S::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kSlots * S::kTile);
+  enum { Q_FULL = 0, S_FULL, S_FREE, P_FULL, PV_DONE, DRAIN, kNB };
+  auto BAR = [&](int x, int i) { return bars + x * kNB + i; };
+  uint64_t* const k_full = bars + 2 * kNB;
+  uint64_t* const k_empty = k_full + kSlots;
+  uint64_t* const v_full = k_empty + kSlots;
+  uint64_t* const v_empty = v_full + kSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + kSlots);
+  __shared__ Found found;
+  __shared__ int64_t sums[kThreads / 32];
+
+  const int warp = warp_id_uniform();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int x = 0; x < 2; ++x)
+      for (int b = 0; b < kNB; ++b)
+        mbar_init(BAR(x, b), (b == Q_FULL || b == S_FREE || b == P_FULL) ? 4u : 1u);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(k_full + i, 1);
+      mbar_init(v_full + i, 1);
+      mbar_init(k_empty + i, 2);
+      mbar_init(v_empty + i, 2);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 10) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  Walk<kRows, kKeys> w;
+  const int64_t per = start_walk<kRows, kKeys, kThreads, kLeast>(a, w, &found, sums);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Segment g = {};
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    const int boxes = kKeys / box;
+    bool ok = true;
+    int64_t nk = 0, nv = 0;  // tiles issued
+    // a tile is `boxes` boxes of `box` rows, each inside one page; lane i loads box i
+    auto tile = [&](uint8_t* ring, const CUtensorMap& tm, uint64_t* full, uint64_t* empty,
+                    int64_t& count, int j) {
+      const int s = (int)(count % kSlots);
+      const uint32_t ph = (uint32_t)(count / kSlots) & 1u;
+      const int key = (g.t0 + j) * kKeys + lane * box;
+      int pid = -1;  // past the end, and numbers outside the pool: zeros
+      if (lane < boxes && key < g.s.len) pid = __ldg(a.table + g.b * a.width + key / a.page);
+      if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ph ^ 1u, 0x901u))) return false;
+      if (lane == 0) mbar_arrive_expect_tx(full + s, S::kTile);
+      __syncwarp();
+      if (lane < boxes) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(ring + s * S::kTile + c * kAtom + lane * box * 128, &tm, full + s, c * 64, g.h,
+                      key % a.page, pid);
+      }
+      ++count;
+      return true;
+    };
+    while (ok && w.next(a, g)) {
+      const Counts n = counts(a, g);
+      // the MMA threads take K(0) K(1) V(0) K(2) V(1) ...
+      for (int j = 0; j <= n.all && ok; ++j) {
+        if (n.all == 0) break;
+        if (j < n.all) ok = tile(sK, tmK, k_full, k_empty, nk, j);
+        if (ok && j >= 1) ok = tile(sV, tmV, v_full, v_empty, nv, j - 1);
+      }
+    }
+    // no load may still be writing shared memory when the CTA exits
+    if (lane == 0) {
+      for (int64_t i = nk > kSlots ? nk - kSlots : 0; i < nk; ++i)
+        mbar_wait(k_full + i % kSlots, (uint32_t)(i / kSlots) & 1u, 0x902u);
+      for (int64_t i = nv > kSlots ? nv - kSlots : 0; i < nv; ++i)
+        mbar_wait(v_full + i % kSlots, (uint32_t)(i / kSlots) & 1u, 0x902u);
+    }
+  } else if (warp == 9) {
+    if (lane == 0) write_rec(a, w, per);
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------ MMA issuer of tile x
+    const int x = warp - 10;
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc(Pair<T>::kFmt, Pair<T>::kFmt, 0, 0, 128, 128);
+      constexpr uint32_t idesc_o = make_idesc(Pair<T>::kFmt, Pair<T>::kFmt, 0, 1, 128, D);
+      const uint32_t q0 = smem_u32(sQ + x * S::kTile);
+      const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV);
+      const uint32_t tP = tmem + kColP + (uint32_t)(x * 64);
+      const uint32_t tO = tmem + kColO + (uint32_t)(x * 128);
+      uint64_t* const free_mine = BAR(x, S_FREE);
+      uint64_t* const free_other = BAR(x ^ 1, S_FREE);
+      bool ok = true;
+      uint32_t kv = 0, mine = 0, other = 0, segs = 0;  // ring tiles, tiles of x, of the other, segments
+      auto wait = [&](uint64_t* bar, uint32_t index, unsigned code) {
+        if (ok && !mbar_wait(bar, index & 1u, code)) ok = false;
+      };
+      while (ok && w.next(a, g)) {
+        const Counts n = counts(a, g);
+        const int cm = n.c[x], co = n.c[x ^ 1];
+        if (cm > 0) wait(BAR(x, Q_FULL), segs, 0x903u);
+        // The score buffer holds S_A(0) S_B(0) S_A(1) S_B(1) ... (a tile past its count drops
+        // out); S_x(j) waits until the softmax of the occupant before it has copied it out.
+        auto issue_s = [&](int j) {
+          if (!ok || j >= cm) return;
+          if (j == 0 && (x == 0 || co == 0)) {
+            if (other) wait(free_other, other - 1, 0x904u);
+            if (mine) wait(free_mine, mine - 1, 0x904u);
+          } else if (x == 0) {
+            if (j - 1 < co) wait(free_other, other + j - 1, 0x904u);
+            else wait(free_mine, mine + j - 1, 0x904u);
+          } else {
+            if (j < co) wait(free_other, other + j, 0x904u);
+            else wait(free_mine, mine + j - 1, 0x904u);
+          }
+          const uint32_t s = (kv + j) % kSlots;
+          wait(k_full + s, (kv + j) / kSlots, 0x905u);
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (uint32_t)((kk >> 2) * kAtom + (kk & 3) * 32);
+            mma_f16(tmem + kColS, smem_desc_sw128(q0 + off, 16, 1024),
+                    smem_desc_sw128(k0 + s * S::kTile + off, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(BAR(x, S_FULL));
+          tc_commit(k_empty + s);
+        };
+        auto issue_pv = [&](int j) {
+          if (!ok) return;
+          wait(BAR(x, P_FULL), mine + j, 0x906u);
+          const uint32_t s = (kv + j) % kSlots;
+          wait(v_full + s, (kv + j) / kSlots, 0x907u);
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)  // keys [16 kk, 16 kk + 16) are P columns [8 kk, 8 kk + 8)
+            mma_f16_ts(tO, tP + (uint32_t)(kk * 8),
+                       smem_desc_sw128(v0 + s * S::kTile + (uint32_t)(kk * 16 * 128), (uint32_t)kAtom,
+                                       1024),
+                       idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(v_empty + s);
+          tc_commit(BAR(x, PV_DONE));
+        };
+        issue_s(0);
+        issue_s(1);
+        for (int j = 0; j < cm && ok; ++j) {
+          issue_pv(j);
+          issue_s(j + 2);
+        }
+        for (int j = cm; j < n.all && ok; ++j) {  // tiles that only the other one reads
+          const uint32_t s = (kv + j) % kSlots;
+          wait(k_full + s, (kv + j) / kSlots, 0x908u);
+          if (ok) mbar_arrive(k_empty + s);
+          wait(v_full + s, (kv + j) / kSlots, 0x908u);
+          if (ok) mbar_arrive(v_empty + s);
+        }
+        kv += n.all;
+        mine += cm;
+        other += co;
+        segs += cm > 0;
+      }
+      // every MMA issued above completes before tensor memory is freed
+      tc_commit(BAR(x, DRAIN));
+      mbar_wait(BAR(x, DRAIN), 0, 0x909u);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax of tile x
+    const int x = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + kColS + lane_addr;
+    const uint32_t tP = tmem + kColP + (uint32_t)(x * 64) + lane_addr;
+    const uint32_t tO = tmem + kColO + (uint32_t)(x * 128) + lane_addr;
+    const float c = a.scale_log2;
+    bool ok = true;
+    uint32_t kv = 0, mine = 0;
+    while (ok && w.next(a, g)) {
+      const Counts n = counts(a, g);
+      const int cnt = n.c[x];
+      const int64_t pr = (int64_t)g.rt * kRows + x * 128 + row;
+      const bool row_ok = pr < (int64_t)g.s.n * a.g;
+      const int tok = row_ok ? (int)(pr / a.g) : 0;
+      const int head = g.h * a.g + (row_ok ? (int)(pr - (int64_t)tok * a.g) : 0);
+      const int lim = row_ok ? sees(a, g.s, tok) : 0;
+      if (cnt > 0) {
+        // this row of Q, swizzled as TMA would (the MMAs of the last segment are done)
+        const uint4* src = reinterpret_cast<const uint4*>(
+            reinterpret_cast<const T*>(a.q) + (g.s.t0 + tok) * a.q_token + head * a.q_head);
+        uint8_t* dst = sQ + x * S::kTile + row * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (row_ok) v = __ldg(src + i);
+          *reinterpret_cast<uint4*>(dst + (i >> 3) * kAtom + (((i & 7) ^ (row & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(x, Q_FULL));
+      }
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < cnt; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(BAR(x, S_FULL), (mine + j) & 1u, 0x90au))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[128];
+        tmem_ld_32x32b_x32(tS, s);
+        tmem_ld_32x32b_x32(tS + 32, s + 32);
+        tmem_ld_32x32b_x32(tS + 64, s + 64);
+        tmem_ld_32x32b_x32(tS + 96, s + 96);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(x, S_FREE));
+        const int key0 = (g.t0 + j) * kKeys;
+        if (key0 + kKeys > lim) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (key0 + i >= lim) s[i] = __float_as_uint(-INFINITY);
+        }
+        float mx[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          mx[t] = fmax3(__uint_as_float(s[t]), __uint_as_float(s[4 + t]), __uint_as_float(s[8 + t]));
+#pragma unroll
+        for (int i = 12; i < 124; i += 8) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            mx[t] = fmax3(mx[t], __uint_as_float(s[i + t]), __uint_as_float(s[i + 4 + t]));
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) mx[t] = fmaxf(mx[t], __uint_as_float(s[124 + t]));
+        const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;  // log2 domain
+        float alpha = 1.f;
+        const bool raise = mb > m_used + kLazy;
+        if (raise) {
+          alpha = (m_used == -INFINITY) ? 0.f : ex2_approx(m_used - mb);
+          m_used = mb;
+        }
+        // tcgen05.ld / st are warp-wide: the warp rescales when any of its rows does
+        const bool rescale = __any_sync(0xffffffffu, raise);
+        const float msub = (m_used == -INFINITY) ? 0.f : m_used;
+        const uint64_t cc = f2_pack(c, c);
+        const uint64_t nm = f2_pack(-msub, -msub);
+        uint64_t acc2 = f2_pack(0.f, 0.f);
+        uint32_t pk[32];
+        exp_pack64<T>(s, cc, nm, acc2, pk);
+        if (j > 0) {
+          // P_x and O_x are free once the product of tile j - 1 is done
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait(BAR(x, PV_DONE), (mine + j - 1) & 1u, 0x90bu))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (rescale) {
+#pragma unroll 1
+            for (int hh = 0; hh < D / 32; ++hh) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(tO + (uint32_t)(hh * 32), o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32b_x32(tO + (uint32_t)(hh * 32), o);
+            }
+          }
+        }
+        tmem_st_32x32b_x32(tP, pk);
+        exp_pack64<T>(s + 64, cc, nm, acc2, pk);
+        tmem_st_32x32b_x32(tP + 32, pk);
+        float la, lb;
+        f2_unpack(acc2, la, lb);
+        l = l * alpha + (la + lb);
+        if (key0 + kKeys > g.s.len) {
+          // values past the sequence's end: what a recycled page holds there is replaced by
+          // zeros (0 * NaN is NaN).  Both tiles write the same zeros before their own product.
+          const uint32_t vs = (kv + j) % kSlots;
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait(v_full + vs, ((kv + j) / kSlots) & 1u, 0x90cu))) {
+            ok = false;
+            break;
+          }
+          if (key0 + row >= g.s.len) {
+            uint8_t* dst = sV + vs * S::kTile + row * 128;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<uint4*>(dst + (i >> 3) * kAtom + ((i & 7) << 4)) =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(x, P_FULL));
+      }
+      const bool have_o = __all_sync(
+          0xffffffffu,
+          ok && cnt > 0 && mbar_wait(BAR(x, PV_DONE), (mine + cnt - 1) & 1u, 0x90du));
+      if (have_o) tc_fence_after();
+      else if (cnt > 0) ok = false;
+      const bool whole = g.t0 == 0 && g.t1 == g.tiles;
+      const float inv = (have_o && l > 0.f) ? 1.0f / l : 0.f;
+      const int64_t prow = ((int64_t)blockIdx.x * 2 + (g.t0 == 0)) * kRows + x * 128 + row;
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) +
+                                            (g.s.t0 + tok) * a.o_token + head * a.o_head);
+      float4* pdst = reinterpret_cast<float4*>(a.part + prow * D);
+#pragma unroll 1
+      for (int hh = 0; hh < D / 32; ++hh) {
+        uint32_t o[32];
+        if (have_o) {
+          tmem_ld_32x32b_x32(tO + (uint32_t)(hh * 32), o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (row_ok && whole) {
+          // a row that sees no key is 0, whatever the values that other rows of its tile see
+          if (m_used == -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+#pragma unroll
+          for (int cch = 0; cch < 4; ++cch) {
+            uint4 v;
+            uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              vw[i] = Pair<T>::pack(__uint_as_float(o[8 * cch + 2 * i]) * inv,
+                                    __uint_as_float(o[8 * cch + 2 * i + 1]) * inv);
+            dst[hh * 4 + cch] = v;
+          }
+        } else if (row_ok && have_o) {  // without keys there is only the maximum (-inf) to say so
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            pdst[hh * 8 + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                           __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+        }
+      }
+      if (row_ok && !whole)
+        *reinterpret_cast<float2*>(a.part_ml + prow * 2) =
+            make_float2(have_o ? m_used : -INFINITY, have_o ? l : 0.f);
+      tc_fence_before();
+      kv += n.all;
+      mine += cnt;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace chunk
+
+// ===========================================================================
+// Joins the parts of an item that CTA boundaries cut, in their order.  WPR warps a row, each
+// taking every WPR-th part.
+// ===========================================================================
+template <typename T, int D, int R, int WPR>
+__global__ void __launch_bounds__(128) merge_kernel(const Args a) {
+  constexpr int kE = D / 32;  // channels a lane
+  __shared__ float s_o[WPR > 1 ? WPR : 1][D];
+  __shared__ float s_l[WPR > 1 ? WPR : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c0 = blockIdx.x;
+  const int32_t* r = a.rec + (int64_t)c0 * 8;
+  if (!r[0]) return;
+  const int sub = WPR > 1 ? warp : 0;
+  const int row = WPR > 1 ? blockIdx.y : blockIdx.y * 4 + warp;
+  const Seq s = get_seq(a, r[1]);
+  const int64_t pr = (int64_t)r[3] * R + row;
+  if (pr >= (int64_t)s.n * a.g) return;  // with WPR > 1 the same for the whole block
+  const int parts = r[4] - c0 + 1;
+  auto slot = [&](int p) { return ((int64_t)(c0 + p) * 2 + (p == 0)) * R + row; };
+  float mm = -INFINITY;
+  for (int p = lane; p < parts; p += 32) mm = fmaxf(mm, a.part_ml[slot(p) * 2]);
+  mm = warp_max(mm);
+  float acc[kE], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) acc[i] = 0.f;
+  for (int p = sub; p < parts; p += WPR) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(p) * 2);
+    if (ml.x == -INFINITY) continue;
+    const float f = ex2_approx(ml.x - mm);
+    const float* o = a.part + slot(p) * D + lane * kE;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) acc[i] = fmaf(f, o[i], acc[i]);
+    l = fmaf(f, ml.y, l);
+  }
+  if (WPR > 1) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) s_o[sub][lane * kE + i] = acc[i];
+    if (lane == 0) s_l[sub] = l;
+    __syncthreads();
+    if (sub) return;
+#pragma unroll
+    for (int q = 1; q < WPR; ++q) {
+      l += s_l[q];
+#pragma unroll
+      for (int i = 0; i < kE; ++i) acc[i] += s_o[q][lane * kE + i];
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int64_t i = pr / a.g;
+  T* dst = reinterpret_cast<T*>(a.out) + (s.t0 + i) * a.o_token +
+           ((int64_t)r[2] * a.g + pr - i * a.g) * a.o_head + lane * kE;
+#pragma unroll
+  for (int e = 0; e < kE; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = Pair<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+}
+
+// Whether the rows of the longest sequence fit the few-rows kernel.  Measured at 48 sequences of
+// about 9 k keys, 32 / 8 heads of 128: see the figures at the entry point.
+inline bool few_rows(int64_t max_new, int64_t g) { return max_new * g <= dec::kRows; }
+inline int ctas_of(bool few) { return sm_count() * (few ? 2 : 1); }
+
+template <typename T, int D>
+int launch(Args& a, bool few, cudaStream_t stream) {
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    FVB_CUDA_TRY(cudaFuncSetAttribute(dec::decode_kernel<T, D>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, dec::kRing),
+                 "fvb_paged_attn smem attribute");
+    FVB_CUDA_TRY(cudaFuncSetAttribute(chunk::chunk_kernel<T, D>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)chunk::Shape<D>::kSmem),
+                 "fvb_paged_attn smem attribute");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  if (few) {
+    dec::decode_kernel<T, D><<<a.ctas, dec::kThreads, dec::kRing, stream>>>(a);
+    int rc = check_launch("fvb_paged_attn");
+    if (rc) return rc;
+    merge_kernel<T, D, dec::kRows, 4><<<dim3(a.ctas, dec::kRows), 128, 0, stream>>>(a);
+    return check_launch("fvb_paged_attn");
+  }
+  // rows of a TMA box: a power of two that divides the page, at most a tile
+  int box = 16;
+  while (box < chunk::kKeys && a.page % (2 * box) == 0) box *= 2;
+  CUtensorMap tk, tv;
+  const CUtensorMapDataType dt = Pair<T>::kFmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)a.Hk, (uint64_t)a.page, (uint64_t)a.pages};
+  const uint64_t sk[3] = {(uint64_t)a.k_head * 2, (uint64_t)a.k_slot * 2, (uint64_t)a.k_page * 2};
+  const uint64_t sv[3] = {(uint64_t)a.v_head * 2, (uint64_t)a.v_slot * 2, (uint64_t)a.v_page * 2};
+  const uint32_t bx[4] = {64, 1, (uint32_t)box, 1};
+  int rc = make_tmap_4d(&tk, a.k, dt, dims, sk, bx);
+  if (rc) return rc;
+  rc = make_tmap_4d(&tv, a.v, dt, dims, sv, bx);
+  if (rc) return rc;
+  chunk::chunk_kernel<T, D><<<a.ctas, chunk::kThreads, chunk::Shape<D>::kSmem, stream>>>(tk, tv, box, a);
+  rc = check_launch("fvb_paged_attn");
+  if (rc) return rc;
+  merge_kernel<T, D, chunk::kRows, 1><<<dim3(a.ctas, chunk::kRows / 4), 128, 0, stream>>>(a);
+  return check_launch("fvb_paged_attn");
+}
+
+struct Workspace {
+  int64_t part, ml, rec, total;  // byte offsets
+};
+inline Workspace workspace(bool few, int64_t D) {
+  const int64_t n = ctas_of(few), rows = few ? dec::kRows : chunk::kRows;
+  Workspace w;
+  w.part = 0;
+  w.ml = w.part + 2 * n * rows * D * 4;
+  w.rec = w.ml + 2 * n * rows * 2 * 4;
+  w.total = w.rec + n * 8 * 4;
+  return w;
+}
+
+}  // namespace pattn
+}  // namespace fvb
+
+extern "C" size_t fvb_paged_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hk, int64_t D) {
+  if (max_new < 1 || Hk < 1 || Hq < Hk || D < 1) return 0;
+  return (size_t)fvb::pattn::workspace(fvb::pattn::few_rows(max_new, Hq / Hk), D).total;
+}
+
+extern "C" int fvb_paged_attn(const void* q, int64_t q_token, int64_t q_head, const void* k,
+                              int64_t k_page, int64_t k_slot, int64_t k_head, const void* v,
+                              int64_t v_page, int64_t v_slot, int64_t v_head, const int32_t* table,
+                              int64_t width, const int32_t* lens, const int32_t* cu, int64_t T,
+                              int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages,
+                              int64_t page, int64_t max_new, int causal, float scale, int dtype,
+                              void* out, int64_t o_token, int64_t o_head, void* ws,
+                              fvb_stream_t stream) {
+  using namespace fvb;
+  FVB_REQUIRE(dtype == FVB_BF16 || dtype == FVB_F16, "fvb_paged_attn: dtype %d", dtype);
+  if (D != 64 && D != 128)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attn: head_dim must be 64 or 128 (got %lld)", (long long)D);
+  FVB_REQUIRE(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq < (1 << 20),
+              "fvb_paged_attn: %lld query heads on %lld key heads", (long long)Hq, (long long)Hk);
+  FVB_REQUIRE(page > 0 && page % 16 == 0 && page < (1 << 24),
+              "fvb_paged_attn: pages must hold a multiple of 16 tokens (got %lld)", (long long)page);
+  FVB_REQUIRE(T >= 0 && B >= 0 && B < (1 << 30) && width >= 0 && pages > 0 && pages < (1ll << 31) &&
+                  width * page < (1ll << 31) && T < (1ll << 31) && T * Hq < (1ll << 31),
+              "fvb_paged_attn: shape");
+  FVB_REQUIRE(scale > 0.f && scale < INFINITY, "fvb_paged_attn: scale %g", (double)scale);
+  FVB_REQUIRE(max_new >= 1, "fvb_paged_attn: max_new %lld", (long long)max_new);
+  if (T == 0 || B == 0) return FVB_OK;
+  FVB_REQUIRE(cu || T == B, "fvb_paged_attn: %lld tokens of %lld sequences need cu_seqlens", (long long)T,
+              (long long)B);
+  FVB_REQUIRE(q && lens && out && ws && (width == 0 || table) && k && v,
+              "fvb_paged_attn: NULL pointer");
+  FVB_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(ws),
+              "fvb_paged_attn: pointers must be 16-byte aligned");
+  FVB_REQUIRE((q_token | q_head | k_page | k_slot | k_head | v_page | v_slot | v_head | o_token | o_head) % 8 == 0,
+              "fvb_paged_attn: strides must be multiples of 8 elements");
+  const bool few = pattn::few_rows(max_new, Hq / Hk);
+  const pattn::Workspace w = pattn::workspace(few, D);
+  pattn::Args a = {};
+  a.q = q;
+  a.out = out;
+  a.q_token = q_token, a.q_head = q_head, a.o_token = o_token, a.o_head = o_head;
+  a.k = k, a.v = v;
+  a.k_page = k_page, a.k_slot = k_slot, a.k_head = k_head;
+  a.v_page = v_page, a.v_slot = v_slot, a.v_head = v_head;
+  a.table = table, a.lens = lens, a.cu = cu;
+  a.T = T, a.width = width, a.pages = pages;
+  a.B = (int)B, a.Hk = (int)Hk, a.g = (int)(Hq / Hk), a.page = (int)page, a.causal = causal != 0;
+  a.ctas = pattn::ctas_of(few);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.part = (float*)((char*)ws + w.part);
+  a.part_ml = (float*)((char*)ws + w.ml);
+  a.rec = (int32_t*)((char*)ws + w.rec);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FVB_BF16)
+    return D == 128 ? pattn::launch<__nv_bfloat16, 128>(a, few, st)
+                    : pattn::launch<__nv_bfloat16, 64>(a, few, st);
+  return D == 128 ? pattn::launch<__half, 128>(a, few, st) : pattn::launch<__half, 64>(a, few, st);
+}

@@ -101,6 +101,22 @@ int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
   return FVB_OK;
 }
 
+int make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
+                 const uint64_t* dims_in, const uint64_t* strides_in, const uint32_t* box_in) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(FVB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if (!aligned16(base)) return fail(FVB_ERR_INVALID, "TMA base pointer not 16-byte aligned");
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) dims[i] = dims_in[i], box[i] = box_in[i];
+  for (int i = 0; i < 3; ++i) strides[i] = strides_in[i];
+  CUresult r = fn(map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FVB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FVB_OK;
+}
+
 }  // namespace fvb
 
 extern "C" {

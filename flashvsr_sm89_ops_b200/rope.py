@@ -1,0 +1,192 @@
+"""Rotary positions of q and k in one launch on the sm_100a library.
+
+``fused_rope(q, k, positions, rope)`` is the general form beside fused_rms_rope (which takes a
+table of complex numbers, interleaved pairs and whole heads, after its norm): a :class:`Rope`
+holds the frequencies, and the angles are formed in the kernel from integer positions.  The
+gradient is the inverse rotation; autograd takes it, and ``inverse=True`` is it.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .fp4_quant import _dtype_code
+
+_SCALINGS = (None, "linear", "ntk", "yarn")
+
+
+def _frequencies(d: int, theta: float, scaling, factor: float, original_len, beta_fast: float, beta_slow: float):
+    """Angles a position, of the d / 2 pairs of one axis."""
+    if scaling == "ntk" and d > 2:
+        theta = theta * factor ** (d / (d - 2))
+    w = [theta ** (-2 * i / d) for i in range(d // 2)]
+    if scaling == "linear":
+        w = [x / factor for x in w]
+    elif scaling == "yarn":
+        # pairs that turn more than beta_fast times over the original length keep their
+        # frequency, those below beta_slow turns are stretched by the factor, a ramp between
+        def pair(turns):
+            return d * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), d // 2 - 1)
+        ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(d // 2)]
+        w = [x * (1 - r) + x / factor * r for x, r in zip(w, ramp)]
+    return w
+
+
+class Rope:
+    """Frequencies of a rotary embedding of the first `rotary_dim` channels of a head.
+
+    layout   "interleaved": pair i is channels (2i, 2i + 1); "half": (i, i + rotary_dim / 2)
+    theta    base: pair i turns by theta^(-2 i / d) a position
+    scaling  for contexts `factor` times longer than trained: None; "linear" (positions divided
+             by the factor); "ntk" (theta times factor^(d / (d - 2))); "yarn" (by parts, between
+             beta_fast and beta_slow turns over `original_len` positions, and the rotated channels
+             multiplied by 0.1 ln(factor) + 1, or by attention_factor)
+    axes     channels of each axis for positions of several coordinates, (44, 42, 42) for the
+             frame, row and column of a 128-channel head; each axis has its own frequencies
+    """
+
+    def __init__(self, rotary_dim: int, *, theta: float = 10000.0, layout: str = "interleaved",
+                 scaling: str | None = None, factor: float = 1.0, original_len: int | None = None,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, attention_factor: float | None = None,
+                 axes=None, device="cuda"):
+        if rotary_dim < 0 or rotary_dim % 2:
+            raise ValueError(f"Rope: rotary_dim must be even, got {rotary_dim}")
+        if layout not in ("interleaved", "half"):
+            raise ValueError(f"Rope: unknown layout {layout!r} (interleaved|half)")
+        if scaling not in _SCALINGS:
+            raise ValueError(f"Rope: unknown scaling {scaling!r} (linear|ntk|yarn)")
+        if not theta > 1 or not math.isfinite(theta):
+            raise ValueError(f"Rope: theta must be above 1, got {theta}")
+        if scaling is not None and not (factor >= 1 and math.isfinite(factor)):
+            raise ValueError(f"Rope: factor must be at least 1, got {factor}")
+        if scaling == "yarn" and (not original_len or original_len < 1 or not 0 < beta_slow < beta_fast):
+            raise ValueError("Rope: yarn needs original_len and 0 < beta_slow < beta_fast")
+        dims = (rotary_dim,) if axes is None else tuple(int(d) for d in axes)
+        if not 1 <= len(dims) <= 16 or any(d < 0 or d % 2 for d in dims) or sum(dims) != rotary_dim:
+            raise ValueError(f"Rope: axes must be up to 16 even counts that add up to {rotary_dim}, got {dims}")
+        w = [x for d in dims for x in _frequencies(d, theta, scaling, factor, original_len, beta_fast, beta_slow)]
+        # turns a position as a fraction of 2^64
+        turns = [round(x / (2 * math.pi) * 2.0 ** 64) for x in w]
+        self.rotary_dim, self.layout, self.axes = rotary_dim, layout, len(dims)
+        self.half = layout == "half"
+        self.scale = 1.0
+        if scaling == "yarn":
+            self.scale = 0.1 * math.log(factor) + 1 if attention_factor is None else float(attention_factor)
+        self.freq = torch.tensor(turns, dtype=torch.int64, device=device)
+        self.axis = torch.tensor([a for a, d in enumerate(dims) for _ in range(d // 2)], dtype=torch.int32,
+                                 device=device)
+        self.device = self.freq.device
+        self._freq, self._axis = self.freq.data_ptr(), self.axis.data_ptr()
+
+    def __repr__(self):
+        return f"Rope({self.rotary_dim}, layout={self.layout!r}, axes={self.axes}, scale={self.scale})"
+
+
+def _rows(x, what, name):
+    """x as [T, H, D] with unit stride inside a head."""
+    if x.dim() == 4:
+        x = x.flatten(0, 1) if x.stride(0) == x.shape[1] * x.stride(1) else x.contiguous().flatten(0, 1)
+    if x.dim() != 3:
+        raise ValueError(f"{name}: {what} must be [T, H, D] or [B, L, H, D], got {tuple(x.shape)}")
+    return x if x.shape[2] < 2 or x.stride(2) == 1 else x.contiguous()
+
+
+def _positions(positions, rope, T, device, name):
+    if positions.device != device:
+        raise ValueError(f"{name}: positions are on {positions.device}, q on {device}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: positions must be int32 or int64, got {positions.dtype}")
+    if positions.numel() != T * rope.axes or (rope.axes > 1 and positions.shape[-1] != rope.axes):
+        raise ValueError(f"{name}: positions must be one of {rope.axes} coordinate(s) for each of {T} tokens, "
+                         f"got {tuple(positions.shape)}")
+    return positions if positions.is_contiguous() else positions.contiguous()
+
+
+def _out(out, x, what, name):
+    """The tensor that x's rotation goes to, and its rows."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{name}: {what} must be {x.dtype} {tuple(x.shape)} on {x.device}")
+    rows = out
+    if out.dim() == 4:
+        if out.stride(0) != out.shape[1] * out.stride(1):
+            raise ValueError(f"{name}: the items of {what} must follow each other")
+        rows = out.flatten(0, 1)
+    if rows.shape[2] > 1 and rows.stride(2) != 1:
+        raise ValueError(f"{name}: {what} must have unit stride inside a head")
+    return out, rows
+
+
+def _run(q, k, positions, rope, inverse, out_q, out_k):
+    name = "fused_rope"
+    dt = _dtype_code(q.dtype, name)
+    dev = q.device
+    q3 = _rows(q, "q", name)
+    T, Hq, D = q3.shape
+    if rope.rotary_dim > D:
+        raise ValueError(f"{name}: rotary_dim {rope.rotary_dim} of a head of {D}")
+    if rope.device != dev:
+        raise ValueError(f"{name}: the Rope is on {rope.device}, q on {dev}")
+    positions = _positions(positions, rope, T, dev, name)
+    oq, oq3 = _out(out_q, q, "out_q", name)
+    s, so = q3.stride(), oq3.stride()
+    if k is None:
+        if out_k is not None:
+            raise ValueError(f"{name}: out_k without k")
+        ok, kargs = None, (0, 0, 0, 0, 0, 0, 0)
+    else:
+        if k.dtype != q.dtype or k.device != dev:
+            raise ValueError(f"{name}: k is {k.dtype} on {k.device}, q {q.dtype} on {dev}")
+        k3 = _rows(k, "k", name)
+        if k3.shape[0] != T or k3.shape[2] != D:
+            raise ValueError(f"{name}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+        ok, ok3 = _out(out_k, k, "out_k", name)
+        t, to = k3.stride(), ok3.stride()
+        kargs = (k3.data_ptr(), t[0], t[1], k3.shape[1], ok3.data_ptr(), to[0], to[1])
+    _lib.call_on(dev.index, "fvb_rope", q3.data_ptr(), s[0], s[1], Hq, oq3.data_ptr(), so[0], so[1], *kargs,
+                 T, D, rope.rotary_dim, rope.half, dt, positions.data_ptr(), positions.dtype == torch.int64,
+                 rope.axes, rope._freq, rope._axis, rope.scale, inverse, _lib.stream_of(q))
+    return oq, ok
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, rope, inverse):
+        ctx.save_for_backward(positions)
+        ctx.rope, ctx.inverse = rope, inverse
+        oq, ok = _run(q, k, positions, rope, inverse, None, None)
+        return (oq, ok) if k is not None else oq
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk=None):
+        positions, = ctx.saved_tensors
+        if gk is None:
+            return _run(gq, None, positions, ctx.rope, not ctx.inverse, None, None)[0], None, None, None, None
+        gq, gk = _run(gq, gk, positions, ctx.rope, not ctx.inverse, None, None)
+        return gq, gk, None, None, None
+
+
+def fused_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rope: Rope, *,
+               inverse: bool = False, out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None):
+    """q and k (or None) with their heads turned by their tokens' positions: (q, k).
+
+    q [T, Hq, D] or [B, L, Hq, D], k the same with its own heads; bf16, fp16 or fp32; any strides
+    of tokens and heads (slices of a fused projection are read as they lie).  positions int32 or
+    int64, one a token ([T] or [B, L]), or [.., axes] with a Rope of several axes; negative ones
+    turn backwards.  fp32 between loads and stores, one rounding.  out_q / out_k may be q / k.
+    inverse turns back, which is the gradient; autograd (once) goes through the call unless
+    outputs are given.  D at most 256.
+    """
+    _lib.require_cuda(q, k, positions)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if out_q is not None or out_k is not None:
+            raise ValueError("fused_rope: out_q / out_k with inputs that require a gradient")
+        r = _Rotate.apply(q, k, positions, rope, bool(inverse))
+        return r if k is not None else (r, None)
+    return _run(q, k, positions, rope, bool(inverse), out_q, out_k)

@@ -380,6 +380,87 @@ FVB_API int fvb_residual_norm(const void* x, const void* y, const void* gate, in
                               int64_t B, int64_t L, int64_t D, void* x_out, void* out, int fmt,
                               void* codes, void* scales, float* row_scale, fvb_stream_t stream);
 
+/* ------------------------------------------------- rotary positions and paged caches
+ * The reference rotates with a table of complex numbers, whole heads, interleaved, after its
+ * RMSNorm (fused_rms_rope.py:58-83), and holds one contiguous cache a stream (integrate.py:81-83).
+ * These have no counterpart there.  Lengths, tables and lists are int32 device memory and read
+ * on the device only, so a captured graph follows them.
+ *
+ * Rotation: the first `rot` channels of a head are pairs, pair i at channels (2i, 2i + 1), or
+ * (i, i + rot / 2) with half = 1; pair i of a token at position p turns by p * freq[i] / 2^64 of
+ * a full turn and is multiplied by `scale`; inverse = 1 turns back (the gradient).  positions:
+ * int32 or (pos64) int64 [T] or [T, axes], pair i on axis[i].  Strides in elements, unit stride
+ * inside a head, any alignment (16-byte vectors where every pointer, stride and part allows).
+ * D <= 256.  Outputs may be the inputs. */
+FVB_API int fvb_rope(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, void* q_out,
+                     int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
+                     int64_t k_head, int64_t Hk, void* k_out, int64_t ko_token, int64_t ko_head,
+                     int64_t T, int64_t D, int64_t rot, int half, int dtype, const void* pos,
+                     int pos64, int64_t axes, const uint64_t* freq, const int32_t* axis, float scale,
+                     int inverse, fvb_stream_t stream);
+
+/* A paged cache: pools of pages [pages][page][Hk][D] (page stride in elements, a page contiguous),
+ * table [B][width] of page numbers (-1: none), lens [B] tokens a sequence.  cu [B + 1]: new tokens
+ * cu[b] .. cu[b + 1] are the last ones of sequence b's lens[b].
+ * Writes k (rotated, rot = 0: as it is) and v of T new tokens to their places, and q rotated to
+ * q_out (Hq = 0: no q).  pos NULL: a token's position is its place in the sequence.  Tokens
+ * outside cu, and places without a page, are left alone.  bf16 / fp16. */
+FVB_API int fvb_kv_append(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, void* q_out,
+                          int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
+                          int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int64_t Hk,
+                          int64_t T, int64_t D, int64_t rot, int half, int dtype, const void* pos,
+                          int pos64, int64_t axes, const uint64_t* freq, const int32_t* axis,
+                          float scale, const int32_t* cu, const int32_t* lens, const int32_t* table,
+                          int64_t B, int64_t width, int64_t pages, int64_t page, void* k_pool,
+                          void* v_pool, int64_t page_stride, fvb_stream_t stream);
+
+/* Pages.  refs [pages]: how many sequences hold a page (0: free).  Free pages are given out lowest
+ * first, in the order of sequences and of their pages.  A step that cannot be done changes nothing
+ * and sets a bit of *status: 1 no free pages, 2 a table row too short, 4 bad arguments (an index
+ * out of range or twice, a negative count, a branch that is not empty).
+ * workspace: fvb_pages_workspace_bytes(seqs, pages, n), 16-byte aligned; n branches of a fork.
+ *   reserve  room for more[b] tokens in every sequence; lens grow
+ *   fork     dst[i] becomes a branch of src[i]: full pages shared, the tokens of a partly filled
+ *            last page copied to a page of its own in every layer's k and v
+ *   release  all of rows[i]'s pages (drop NULL) or its drop[i] first ones; the rest moves forward
+ *   compact  pages in use move to the front of the pool, both in ascending order
+ * Pools: layer_stride, page_stride, row_bytes (a token in one layer) in bytes, multiples of 16. */
+FVB_API size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages, int64_t n);
+FVB_API int fvb_pages_reserve(const int32_t* more, int32_t* table, int32_t* lens, int32_t* refs,
+                              int32_t* status, int64_t seqs, int64_t width, int64_t pages,
+                              int64_t page, void* workspace, fvb_stream_t stream);
+FVB_API int fvb_pages_fork(const int32_t* src, const int32_t* dst, int64_t n, int32_t* table,
+                           int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
+                           int64_t width, int64_t pages, int64_t page, void* k, void* v,
+                           int64_t layers, int64_t layer_stride, int64_t page_stride,
+                           int64_t row_bytes, void* workspace, fvb_stream_t stream);
+FVB_API int fvb_pages_release(const int32_t* rows, const int32_t* drop, int64_t n, int32_t* table,
+                              int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
+                              int64_t width, int64_t pages, int64_t page, void* workspace,
+                              fvb_stream_t stream);
+FVB_API int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* status,
+                              int64_t seqs, int64_t width, int64_t pages, int64_t page, void* k,
+                              void* v, int64_t layers, int64_t layer_stride, int64_t page_stride,
+                              int64_t row_bytes, void* workspace, fvb_stream_t stream);
+
+/* Attention of new tokens over a paged cache.  q, out [T][Hq][D], k and v [pages][page][Hk][D], all
+ * with strides in elements (multiples of 8, 16-byte aligned pointers); query head h reads key head
+ * h / (Hq / Hk).  Token i of a sequence's n new ones sees keys 0 .. lens - n + i (causal), else all
+ * lens.  A row that sees no key is 0; rows outside cu are left as they were; what lies past lens in
+ * a page is not seen.  A page number outside the pool reads as zeros.  cu NULL: one token a sequence
+ * (T = B).  max_new: new tokens of the longest sequence; it picks the kernel and need not be exact
+ * for the result to be right.  bf16 / fp16, D 64 or 128, pages of a multiple of 16 tokens, scale
+ * positive.  fp32 scores, statistics and sums; the probabilities are rounded to the input's type
+ * for their product with v. */
+FVB_API size_t fvb_paged_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hk, int64_t D);
+FVB_API int fvb_paged_attn(const void* q, int64_t q_token, int64_t q_head, const void* k,
+                           int64_t k_page, int64_t k_slot, int64_t k_head, const void* v,
+                           int64_t v_page, int64_t v_slot, int64_t v_head, const int32_t* table,
+                           int64_t width, const int32_t* lens, const int32_t* cu, int64_t T,
+                           int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page,
+                           int64_t max_new, int causal, float scale, int dtype, void* out,
+                           int64_t o_token, int64_t o_head, void* workspace, fvb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
