@@ -553,6 +553,26 @@ __device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint6
   }
 }
 
+__device__ __forceinline__ void add_release(uint32_t* p, uint32_t v) {
+  asm volatile("red.release.cta.shared::cta.add.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+// Bounded wait, as mbar_wait, for a count in shared memory to reach `v`.
+__device__ __forceinline__ bool wait_count(uint32_t* p, uint32_t v, unsigned code) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    uint32_t x;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(x) : "r"(smem_u32(p)) : "memory");
+    if ((int32_t)(x - v) >= 0) return true;
+    if ((i & 255u) == 255u) {
+      const uint64_t t = globaltimer_ns();
+      if (!t0) t0 = t;
+      if (t - t0 > kWaitLimitNs) break;
+    }
+  }
+  atomicCAS(&g_device_error, 0u, code);
+  return false;
+}
+
 // what both tiles of a segment do, the same for every thread
 struct Counts {
   int c[2], all;
@@ -590,12 +610,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* const v_full = k_empty + kSlots;
   uint64_t* const v_empty = v_full + kSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + kSlots);
+  // Score tiles that each tile's softmax has copied out, counted at the end of a segment (four
+  // warps each).  A parity names a phase only to a waiter that is at most one behind, and a tile
+  // that sits out keys which the other one sees falls further behind than that.
+  __shared__ uint32_t s_copied[2];
   __shared__ Found found;
   __shared__ int64_t sums[kThreads / 32];
 
   const int warp = warp_id_uniform();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    s_copied[0] = s_copied[1] = 0;
     for (int x = 0; x < 2; ++x)
       for (int b = 0; b < kNB; ++b)
         mbar_init(BAR(x, b), (b == Q_FULL || b == S_FREE || b == P_FULL) ? 4u : 1u);
@@ -691,15 +716,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         // out); S_x(j) waits until the softmax of the occupant before it has copied it out.
         auto issue_s = [&](int j) {
           if (!ok || j >= cm) return;
-          if (j == 0 && (x == 0 || co == 0)) {
-            if (other) wait(free_other, other - 1, 0x904u);
-            if (mine) wait(free_mine, mine - 1, 0x904u);
-          } else if (x == 0) {
-            if (j - 1 < co) wait(free_other, other + j - 1, 0x904u);
-            else wait(free_mine, mine + j - 1, 0x904u);
+          if (j == 0) {  // the buffer is free of the last segment's scores
+            if (!wait_count(s_copied + (x ^ 1), 4 * other, 0x904u) ||
+                !wait_count(s_copied + x, 4 * mine, 0x904u))
+              ok = false;
+          }
+          if (x == 0) {
+            if (j >= 1) {
+              if (j - 1 < co) wait(free_other, other + j - 1, 0x904u);
+              else wait(free_mine, mine + j - 1, 0x904u);
+            }
           } else {
             if (j < co) wait(free_other, other + j, 0x904u);
-            else wait(free_mine, mine + j - 1, 0x904u);
+            else if (j >= 1) wait(free_mine, mine + j - 1, 0x904u);
           }
           const uint32_t s = (kv + j) % kSlots;
           wait(k_full + s, (kv + j) / kSlots, 0x905u);
@@ -883,6 +912,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(x, P_FULL));
+      }
+      if (ok && cnt > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) add_release(s_copied + x, (uint32_t)cnt);
       }
       const bool have_o = __all_sync(
           0xffffffffu,

@@ -539,6 +539,10 @@ SHAPES = [
     ([1, 640, 5], [2000, 64, 0], 7, 7, 128, 64),
     ([20, 30, 40] * 20, [5, 200, 64] * 20, 4, 2, 64, 32),
     ([1, 1, 1], [5, 300, 1000], 40, 1, 128, 16),                   # one token of a group of 40
+    # items of several segments whose two halves see different numbers of key tiles
+    ([1537, 600, 900], [100, 300, 7], 16, 4, 64, 16),
+    ([1100, 700], [3, 0], 12, 12, 128, 64),
+    ([1500, 2000, 900, 700], [0, 0, 0, 0], 8, 1, 64, 32),
 ]
 
 
