@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -94,11 +95,10 @@ _SIGS = {
     "fvb_residual_norm": (_int, [_vp, _vp, _vp, _int, _f32, _int, _vp, _vp, _f32, _int, _vp, _vp,
                                  _vp, _vp, _f32, _i64, _i64, _i64, _vp, _vp, _int, _vp, _vp, _vp,
                                  _vp]),
-    "fvb_rope": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
-                        _i64, _i64, _i64, _int, _int, _vp, _int, _i64, _vp, _vp, _f32, _int, _vp]),
-    "fvb_kv_append": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
-                             _i64, _i64, _i64, _i64, _int, _int, _vp, _int, _i64, _vp, _vp, _f32, _vp,
-                             _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    # these take their arguments in one piece (bytes, see ROPE_ARGS and its likes): converting 27
+    # of them one by one costs 2.7 us a call, packing them 0.3
+    "fvb_rope": (_int, [ctypes.c_char_p, _vp]),
+    "fvb_kv_append": (_int, [ctypes.c_char_p, _vp]),
     "fvb_pages_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "fvb_pages_reserve": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "fvb_pages_fork": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64,
@@ -107,10 +107,14 @@ _SIGS = {
     "fvb_pages_compact": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                  _i64, _vp, _vp]),
     "fvb_paged_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
-    "fvb_paged_attn": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
-                              _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _f32, _int,
-                              _vp, _i64, _i64, _vp, _vp]),
+    "fvb_paged_attn": (_int, [ctypes.c_char_p, _vp]),
 }
+
+
+# fvb_rope_args, fvb_kv_append_args and fvb_paged_attn_args: every member is 8 bytes
+ROPE_ARGS = struct.Struct("=24qdq").pack
+KV_APPEND_ARGS = struct.Struct("=24qd10q").pack
+PAGED_ATTN_ARGS = struct.Struct("=24qd5q").pack
 
 
 class FvbError(RuntimeError):

@@ -72,11 +72,11 @@ __device__ __forceinline__ int sees(const Args& a, const Seq& s, int i) {
 
 // key tiles of packed rows [r0, r1): 0 if there are no such rows
 template <int KT>
-__device__ __forceinline__ int tiles_of(const Args& a, const Seq& s, int64_t r0, int64_t r1) {
-  const int64_t rows = (int64_t)s.n * a.g;
+__device__ __forceinline__ int tiles_of(const Args& a, const Seq& s, int r0, int r1) {
+  const int rows = s.n * a.g;  // below 2^31: checked at the entry
   if (r0 >= rows) return 0;
   if (r1 > rows) r1 = rows;
-  return (sees(a, s, (int)((r1 - 1) / a.g)) + KT - 1) / KT;
+  return (int)(((uint32_t)sees(a, s, (r1 - 1) / a.g) + KT - 1) / KT);
 }
 
 struct Segment {  // key tiles [t0, t1) of an item's [0, tiles)
@@ -93,7 +93,7 @@ struct Walk {
   Seq s;
 
   __device__ int item_tiles(const Args& a) const {
-    const int t = tiles_of<KT>(a, s, (int64_t)rt * R, (int64_t)rt * R + R);
+    const int t = tiles_of<KT>(a, s, rt * R, rt * R + R);
     return t > 0 ? t : 1;
   }
   __device__ bool next(const Args& a, Segment& g) {
@@ -104,7 +104,7 @@ struct Walk {
     unit += g.t1 - t0;
     t0 = 0;
     if (unit < end) {
-      if ((int64_t)(++rt) * R >= (int64_t)s.n * a.g) {
+      if (++rt * R >= s.n * a.g) {
         rt = 0;
         if (++h == a.Hk) {
           h = 0;
@@ -119,13 +119,13 @@ struct Walk {
 // units of one key head of a sequence
 template <int R, int KT>
 __device__ int64_t head_units(const Args& a, const Seq& s) {
-  const int64_t rows = (int64_t)s.n * a.g;
+  const int rows = s.n * a.g;
   if (!a.causal) {
-    const int64_t t = (s.len + KT - 1) / KT;
-    return ((rows + R - 1) / R) * (t > 0 ? t : 1);
+    const int64_t t = ((int64_t)s.len + KT - 1) / KT;
+    return (int64_t)((rows + R - 1) / R) * (t > 0 ? t : 1);
   }
   int64_t u = 0;
-  for (int64_t r = 0; r < rows; r += R) {
+  for (int r = 0; r < rows; r += R) {
     const int t = tiles_of<KT>(a, s, r, r + R);
     u += t > 0 ? t : 1;
   }
@@ -534,23 +534,82 @@ template <int D>
 struct Shape {
   static constexpr int kTile = D * 256;  // bytes of 128 rows
   static constexpr int kSlots = D == 128 ? 2 : 4;  // of K and of V
-  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;
+  // Exponentials on the FMA pipe: a quarter of them takes the largest case (8448 over 33792 keys, D
+  // 128) from 2.12 to 1.95 million clocks and from 1390 to 1360 us (1620 to 1587 under a lasting
+  // load: the clock gives way); an eighth or three eighths gained less.
+  static constexpr uint32_t kFma = D == 128 ? 0x22u : 0u;
+  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // align, barriers
 };
 
-// p = 2^(s c - m) of 64 scores, packed; fp32 row sum into acc2
+// 2^x of two numbers without the special-function unit, which at 16 a clock and SM would need as
+// long for a tile's exponentials as the tensor cores for its products: x = n + f with f in
+// [-1/2, 1/2] (n by adding and subtracting 1.5 2^23), a polynomial in f, and n added to the
+// exponent.  The polynomials minimise the largest relative error (fitted by reweighted least
+// squares): 2^-13.7 with degree 3, for probabilities that are rounded to bf16 (2^-9), 2^-18.5
+// with degree 4 for fp16 (2^-12).  Below -126 the result is 2^-126, which counts as nothing.
 template <typename T>
+__device__ __forceinline__ void exp2_fma(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  x = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t t = f2_add(x, f2_pack(12582912.f, 12582912.f));
+  const uint64_t n = f2_add(t, f2_pack(-12582912.f, -12582912.f));
+  const uint64_t f = f2_fma(n, f2_pack(-1.f, -1.f), x);
+  uint64_t p;
+  if (Pair<T>::kFmt) {
+    p = f2_fma(f, f2_pack(0.0551716685f, 0.0551716685f), f2_pack(0.242611125f, 0.242611125f));
+    p = f2_fma(f, p, f2_pack(0.693260968f, 0.693260968f));
+    p = f2_fma(f, p, f2_pack(0.999928057f, 0.999928057f));
+  } else {
+    p = f2_fma(f, f2_pack(0.0095701022f, 0.0095701022f), f2_pack(0.0559178591f, 0.0559178591f));
+    p = f2_fma(f, p, f2_pack(0.240247443f, 0.240247443f));
+    p = f2_fma(f, p, f2_pack(0.693121791f, 0.693121791f));
+    p = f2_fma(f, p, f2_pack(0.999999285f, 0.999999285f));
+  }
+  float t0, t1;
+  f2_unpack(t, t0, t1);
+  f2_unpack(p, p0, p1);
+  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+
+// p = 2^(s c - m) of 64 scores, packed; fp32 row sum into acc2.  kFma: which pairs of each eight
+// take exp2_fma.
+template <typename T, uint32_t kFma>
 __device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint64_t nm,
                                            uint64_t& acc2, uint32_t* pk) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const uint64_t xv =
         f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, nm);
-    float x0, x1;
-    f2_unpack(xv, x0, x1);
-    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+    float p0, p1;
+    if (kFma >> (i & 7) & 1) {
+      exp2_fma<T>(xv, p0, p1);
+    } else {
+      float x0, x1;
+      f2_unpack(xv, x0, x1);
+      p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+    }
     acc2 = f2_add(acc2, f2_pack(p0, p1));
     pk[i] = Pair<T>::pack(p0, p1);
   }
+}
+
+// the largest of 64 scores
+__device__ __forceinline__ float max64(const uint32_t* s) {
+  float mx[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    mx[t] = fmax3(__uint_as_float(s[t]), __uint_as_float(s[4 + t]), __uint_as_float(s[8 + t]));
+#pragma unroll
+  for (int i = 12; i < 60; i += 8) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      mx[t] = fmax3(mx[t], __uint_as_float(s[i + t]), __uint_as_float(s[i + 4 + t]));
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) mx[t] = fmaxf(mx[t], __uint_as_float(s[60 + t]));
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
 __device__ __forceinline__ void add_release(uint32_t* p, uint32_t v) {
@@ -573,22 +632,15 @@ __device__ __forceinline__ bool wait_count(uint32_t* p, uint32_t v, unsigned cod
   return false;
 }
 
-// what both tiles of a segment do, the same for every thread
-struct Counts {
-  int c[2], all;
+// A segment as one warp works it out for the others.
+struct Desc {
+  int more;       // 0: there are no further segments
+  int cnt[2], all;  // key tiles of either half, and of the longer one
+  int key_t0, b, h, len;
+  int n, off, row0, whole;
+  int64_t t0;
 };
-__device__ __forceinline__ Counts counts(const Args& a, const Segment& g) {
-  Counts r;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int64_t r0 = (int64_t)g.rt * kRows + x * 128;
-    const int t = tiles_of<kKeys>(a, g.s, r0, r0 + 128);
-    const int e = t < g.t1 ? t : g.t1;
-    r.c[x] = e > g.t0 ? e - g.t0 : 0;
-  }
-  r.all = r.c[0] > r.c[1] ? r.c[0] : r.c[1];
-  return r;
-}
+constexpr int kDescs = 4;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -609,7 +661,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* const k_empty = k_full + kSlots;
   uint64_t* const v_full = k_empty + kSlots;
   uint64_t* const v_empty = v_full + kSlots;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + kSlots);
+  uint64_t* const d_full = v_empty + kSlots;  // segments: one writer, 11 readers
+  uint64_t* const d_empty = d_full + kDescs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + kDescs);
+  __shared__ Desc descs[kDescs];
   // Score tiles that each tile's softmax has copied out, counted at the end of a segment (four
   // warps each).  A parity names a phase only to a waiter that is at most one behind, and a tile
   // that sits out keys which the other one sees falls further behind than that.
@@ -630,6 +685,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(k_empty + i, 2);
       mbar_init(v_empty + i, 2);
     }
+    for (int i = 0; i < kDescs; ++i) {
+      mbar_init(d_full + i, 1);
+      mbar_init(d_empty + i, 11);
+    }
     fence_mbar_init();
   }
   if (warp == 10) {
@@ -642,7 +701,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Segment g = {};
+  uint32_t seg = 0;  // segments seen
+  auto DESC = [&]() -> const Desc& { return descs[seg % kDescs]; };
+  // the next segment; false at the end, or after a time-out
+  auto next_segment = [&]() {
+    return mbar_wait(d_full + seg % kDescs, (seg / kDescs) & 1u, 0x90eu) && DESC().more;
+  };
 
   if (warp == 8) {
     // ------------------------------------------------------------ loads
@@ -658,9 +722,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     int64_t& count, int j) {
       const int s = (int)(count % kSlots);
       const uint32_t ph = (uint32_t)(count / kSlots) & 1u;
-      const int key = (g.t0 + j) * kKeys + lane * box;
+      const Desc& g = DESC();
+      const int key = (g.key_t0 + j) * kKeys + lane * box;
       int pid = -1;  // past the end, and numbers outside the pool: zeros
-      if (lane < boxes && key < g.s.len) pid = __ldg(a.table + g.b * a.width + key / a.page);
+      if (lane < boxes && key < g.len) pid = __ldg(a.table + g.b * a.width + key / a.page);
       if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ph ^ 1u, 0x901u))) return false;
       if (lane == 0) mbar_arrive_expect_tx(full + s, S::kTile);
       __syncwarp();
@@ -673,14 +738,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++count;
       return true;
     };
-    while (ok && w.next(a, g)) {
-      const Counts n = counts(a, g);
+    while (ok && __all_sync(0xffffffffu, next_segment())) {
+      const int all = DESC().all;
       // the MMA threads take K(0) K(1) V(0) K(2) V(1) ...
-      for (int j = 0; j <= n.all && ok; ++j) {
-        if (n.all == 0) break;
-        if (j < n.all) ok = tile(sK, tmK, k_full, k_empty, nk, j);
+      for (int j = 0; j <= all && all > 0 && ok; ++j) {
+        if (j < all) ok = tile(sK, tmK, k_full, k_empty, nk, j);
         if (ok && j >= 1) ok = tile(sV, tmV, v_full, v_empty, nv, j - 1);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_empty + seg % kDescs);
+      ++seg;
     }
     // no load may still be writing shared memory when the CTA exits
     if (lane == 0) {
@@ -690,97 +757,140 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(v_full + i % kSlots, (uint32_t)(i / kSlots) & 1u, 0x902u);
     }
   } else if (warp == 9) {
-    if (lane == 0) write_rec(a, w, per);
+    // ------------------------------------------------------------ segments
+    if (lane == 0) {
+      const Walk<kRows, kKeys> start = w;
+      Segment g;
+      for (bool more = true; more; ++seg) {
+        more = w.next(a, g);
+        if (!mbar_wait(d_empty + seg % kDescs, ((seg / kDescs) & 1u) ^ 1u, 0x90fu)) break;
+        Desc& d = descs[seg % kDescs];
+        d.more = more;
+        if (more) {
+          const int row0 = g.rt * kRows;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int tl = tiles_of<kKeys>(a, g.s, row0 + x * 128, row0 + x * 128 + 128);
+            const int e = tl < g.t1 ? tl : g.t1;
+            d.cnt[x] = e > g.t0 ? e - g.t0 : 0;
+          }
+          d.all = d.cnt[0] > d.cnt[1] ? d.cnt[0] : d.cnt[1];
+          d.key_t0 = g.t0, d.b = g.b, d.h = g.h, d.len = g.s.len, d.n = g.s.n, d.off = g.s.off;
+          d.row0 = row0, d.whole = g.t0 == 0 && g.t1 == g.tiles, d.t0 = g.s.t0;
+        }
+        mbar_arrive(d_full + seg % kDescs);
+      }
+      write_rec(a, start, per);
+    }
   } else if (warp >= 10) {
     // ------------------------------------------------------------ MMA issuer of tile x
+    // The whole warp walks the loop, so that descriptors and addresses stay warp-uniform (the form
+    // the tensor instructions take them in), and one elected lane issues: from a branch of one
+    // lane the eight instructions of a product took 800 clocks to issue, 512 to run.
     const int x = warp - 10;
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc(Pair<T>::kFmt, Pair<T>::kFmt, 0, 0, 128, 128);
-      constexpr uint32_t idesc_o = make_idesc(Pair<T>::kFmt, Pair<T>::kFmt, 0, 1, 128, D);
-      const uint32_t q0 = smem_u32(sQ + x * S::kTile);
-      const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV);
-      const uint32_t tP = tmem + kColP + (uint32_t)(x * 64);
-      const uint32_t tO = tmem + kColO + (uint32_t)(x * 128);
-      uint64_t* const free_mine = BAR(x, S_FREE);
-      uint64_t* const free_other = BAR(x ^ 1, S_FREE);
-      bool ok = true;
-      uint32_t kv = 0, mine = 0, other = 0, segs = 0;  // ring tiles, tiles of x, of the other, segments
-      auto wait = [&](uint64_t* bar, uint32_t index, unsigned code) {
-        if (ok && !mbar_wait(bar, index & 1u, code)) ok = false;
-      };
-      while (ok && w.next(a, g)) {
-        const Counts n = counts(a, g);
-        const int cm = n.c[x], co = n.c[x ^ 1];
-        if (cm > 0) wait(BAR(x, Q_FULL), segs, 0x903u);
-        // The score buffer holds S_A(0) S_B(0) S_A(1) S_B(1) ... (a tile past its count drops
-        // out); S_x(j) waits until the softmax of the occupant before it has copied it out.
-        auto issue_s = [&](int j) {
-          if (!ok || j >= cm) return;
-          if (j == 0) {  // the buffer is free of the last segment's scores
-            if (!wait_count(s_copied + (x ^ 1), 4 * other, 0x904u) ||
-                !wait_count(s_copied + x, 4 * mine, 0x904u))
-              ok = false;
+    const bool leader = elect_one();
+    constexpr uint32_t idesc_s = make_idesc(Pair<T>::kFmt, Pair<T>::kFmt, 0, 0, 128, 128);
+    constexpr uint32_t idesc_o = make_idesc(Pair<T>::kFmt, Pair<T>::kFmt, 0, 1, 128, D);
+    const uint64_t dq = smem_desc_sw128(smem_u32(sQ + x * S::kTile), 16, 1024);
+    const uint64_t dk = smem_desc_sw128(smem_u32(sK), 16, 1024);
+    const uint64_t dv = smem_desc_sw128(smem_u32(sV), (uint32_t)kAtom, 1024);
+    const uint32_t tP = tmem + kColP + (uint32_t)(x * 64);
+    const uint32_t tO = tmem + kColO + (uint32_t)(x * 128);
+    uint64_t* const free_mine = BAR(x, S_FREE);
+    uint64_t* const free_other = BAR(x ^ 1, S_FREE);
+    bool ok = true;
+    uint32_t mine = 0, other = 0, segs = 0;  // tiles of x, of the other, segments
+    uint32_t ks = 0, kph = 0, vs = 0, vph = 0;  // ring slots and their parities
+    auto wait = [&](uint64_t* bar, uint32_t index, unsigned code) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, index & 1u, code))) ok = false;
+    };
+    auto step = [&](uint32_t& slot, uint32_t& parity) {
+      if (++slot == kSlots) slot = 0, parity ^= 1u;
+    };
+    while (ok && __all_sync(0xffffffffu, next_segment())) {
+      const int cm = __shfl_sync(0xffffffffu, DESC().cnt[x], 0);
+      const int co = __shfl_sync(0xffffffffu, DESC().cnt[x ^ 1], 0);
+      const int all = __shfl_sync(0xffffffffu, DESC().all, 0);
+      if (leader) mbar_arrive(d_empty + seg % kDescs);
+      ++seg;
+      if (cm > 0) wait(BAR(x, Q_FULL), segs, 0x903u);
+      // The score buffer holds S_A(0) S_B(0) S_A(1) S_B(1) ... (a tile past its count drops
+      // out); S_x(j) waits until the softmax of the occupant before it has copied it out.
+      auto issue_s = [&](int j) {
+        if (!ok || j >= cm) return;
+        if (j == 0) {  // the buffer is free of the last segment's scores
+          if (!__all_sync(0xffffffffu, wait_count(s_copied + (x ^ 1), 4 * other, 0x904u) &&
+                                           wait_count(s_copied + x, 4 * mine, 0x904u)))
+            ok = false;
+        }
+        if (x == 0) {
+          if (j >= 1) {
+            if (j - 1 < co) wait(free_other, other + j - 1, 0x904u);
+            else wait(free_mine, mine + j - 1, 0x904u);
           }
-          if (x == 0) {
-            if (j >= 1) {
-              if (j - 1 < co) wait(free_other, other + j - 1, 0x904u);
-              else wait(free_mine, mine + j - 1, 0x904u);
-            }
-          } else {
-            if (j < co) wait(free_other, other + j, 0x904u);
-            else if (j >= 1) wait(free_mine, mine + j - 1, 0x904u);
-          }
-          const uint32_t s = (kv + j) % kSlots;
-          wait(k_full + s, (kv + j) / kSlots, 0x905u);
-          if (!ok) return;
-          tc_fence_after();
+        } else {
+          if (j < co) wait(free_other, other + j, 0x904u);
+          else if (j >= 1) wait(free_mine, mine + j - 1, 0x904u);
+        }
+        wait(k_full + ks, kph, 0x905u);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t k0 = dk + ks * (uint32_t)(S::kTile >> 4);
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (uint32_t)((kk >> 2) * kAtom + (kk & 3) * 32);
-            mma_f16(tmem + kColS, smem_desc_sw128(q0 + off, 16, 1024),
-                    smem_desc_sw128(k0 + s * S::kTile + off, 16, 1024), idesc_s, kk > 0 ? 1u : 0u);
+            const uint32_t off = (uint32_t)((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
+            mma_f16(tmem + kColS, dq + off, k0 + off, idesc_s, kk > 0 ? 1u : 0u);
           }
           tc_commit(BAR(x, S_FULL));
-          tc_commit(k_empty + s);
-        };
-        auto issue_pv = [&](int j) {
-          if (!ok) return;
-          wait(BAR(x, P_FULL), mine + j, 0x906u);
-          const uint32_t s = (kv + j) % kSlots;
-          wait(v_full + s, (kv + j) / kSlots, 0x907u);
-          if (!ok) return;
-          tc_fence_after();
+          tc_commit(k_empty + ks);
+        }
+        __syncwarp();
+        step(ks, kph);
+      };
+      auto issue_pv = [&](int j) {
+        if (!ok) return;
+        wait(BAR(x, P_FULL), mine + j, 0x906u);
+        wait(v_full + vs, vph, 0x907u);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t v0 = dv + vs * (uint32_t)(S::kTile >> 4);
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // keys [16 kk, 16 kk + 16) are P columns [8 kk, 8 kk + 8)
-            mma_f16_ts(tO, tP + (uint32_t)(kk * 8),
-                       smem_desc_sw128(v0 + s * S::kTile + (uint32_t)(kk * 16 * 128), (uint32_t)kAtom,
-                                       1024),
-                       idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-          tc_commit(v_empty + s);
+            mma_f16_ts(tO, tP + (uint32_t)(kk * 8), v0 + (uint32_t)(kk * 16 * 128 >> 4), idesc_o,
+                       (j > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(v_empty + vs);
           tc_commit(BAR(x, PV_DONE));
-        };
-        issue_s(0);
-        issue_s(1);
-        for (int j = 0; j < cm && ok; ++j) {
-          issue_pv(j);
-          issue_s(j + 2);
         }
-        for (int j = cm; j < n.all && ok; ++j) {  // tiles that only the other one reads
-          const uint32_t s = (kv + j) % kSlots;
-          wait(k_full + s, (kv + j) / kSlots, 0x908u);
-          if (ok) mbar_arrive(k_empty + s);
-          wait(v_full + s, (kv + j) / kSlots, 0x908u);
-          if (ok) mbar_arrive(v_empty + s);
-        }
-        kv += n.all;
-        mine += cm;
-        other += co;
-        segs += cm > 0;
+        __syncwarp();
+        step(vs, vph);
+      };
+      issue_s(0);
+      issue_s(1);
+      for (int j = 0; j < cm && ok; ++j) {
+        issue_pv(j);
+        issue_s(j + 2);
       }
-      // every MMA issued above completes before tensor memory is freed
+      for (int j = cm; j < all && ok; ++j) {  // tiles that only the other one reads
+        wait(k_full + ks, kph, 0x908u);
+        if (ok && leader) mbar_arrive(k_empty + ks);
+        wait(v_full + vs, vph, 0x908u);
+        if (ok && leader) mbar_arrive(v_empty + vs);
+        __syncwarp();
+        step(ks, kph);
+        step(vs, vph);
+      }
+      mine += cm;
+      other += co;
+      segs += cm > 0;
+    }
+    // every MMA issued above completes before tensor memory is freed
+    if (leader) {
       tc_commit(BAR(x, DRAIN));
       mbar_wait(BAR(x, DRAIN), 0, 0x909u);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax of tile x
     const int x = warp >> 2;
@@ -792,18 +902,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float c = a.scale_log2;
     bool ok = true;
     uint32_t kv = 0, mine = 0;
-    while (ok && w.next(a, g)) {
-      const Counts n = counts(a, g);
-      const int cnt = n.c[x];
-      const int64_t pr = (int64_t)g.rt * kRows + x * 128 + row;
-      const bool row_ok = pr < (int64_t)g.s.n * a.g;
-      const int tok = row_ok ? (int)(pr / a.g) : 0;
-      const int head = g.h * a.g + (row_ok ? (int)(pr - (int64_t)tok * a.g) : 0);
-      const int lim = row_ok ? sees(a, g.s, tok) : 0;
+    while (ok && __all_sync(0xffffffffu, next_segment())) {
+      const int cnt = DESC().cnt[x], key_t0 = DESC().key_t0, len = DESC().len;
+      int lim = 0;  // keys that this row sees
       if (cnt > 0) {
+        const Desc& g = DESC();
+        const int pr = g.row0 + x * 128 + row;
+        const bool row_ok = pr < g.n * a.g;
+        const int tok = row_ok ? pr / a.g : 0;
+        const int head = g.h * a.g + (row_ok ? pr - tok * a.g : 0);
+        if (row_ok) {
+          const int v = a.causal ? min(g.off + tok + 1, len) : len;
+          lim = v > 0 ? v : 0;
+        }
         // this row of Q, swizzled as TMA would (the MMAs of the last segment are done)
         const uint4* src = reinterpret_cast<const uint4*>(
-            reinterpret_cast<const T*>(a.q) + (g.s.t0 + tok) * a.q_token + head * a.q_head);
+            reinterpret_cast<const T*>(a.q) + (g.t0 + tok) * a.q_token + head * a.q_head);
         uint8_t* dst = sQ + x * S::kTile + row * 128;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
@@ -831,25 +945,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(x, S_FREE));
-        const int key0 = (g.t0 + j) * kKeys;
+        const int key0 = (key_t0 + j) * kKeys;
         if (key0 + kKeys > lim) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (key0 + i >= lim) s[i] = __float_as_uint(-INFINITY);
         }
-        float mx[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          mx[t] = fmax3(__uint_as_float(s[t]), __uint_as_float(s[4 + t]), __uint_as_float(s[8 + t]));
-#pragma unroll
-        for (int i = 12; i < 124; i += 8) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            mx[t] = fmax3(mx[t], __uint_as_float(s[i + t]), __uint_as_float(s[i + 4 + t]));
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) mx[t] = fmaxf(mx[t], __uint_as_float(s[124 + t]));
-        const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;  // log2 domain
+        const float mb = fmaxf(max64(s), max64(s + 64)) * c;  // log2 domain
         float alpha = 1.f;
         const bool raise = mb > m_used + kLazy;
         if (raise) {
@@ -863,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t nm = f2_pack(-msub, -msub);
         uint64_t acc2 = f2_pack(0.f, 0.f);
         uint32_t pk[32];
-        exp_pack64<T>(s, cc, nm, acc2, pk);
+        exp_pack64<T, S::kFma>(s, cc, nm, acc2, pk);
         if (j > 0) {
           // P_x and O_x are free once the product of tile j - 1 is done
           if (!__all_sync(0xffffffffu,
@@ -885,12 +987,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tmem_st_32x32b_x32(tP, pk);
-        exp_pack64<T>(s + 64, cc, nm, acc2, pk);
+        exp_pack64<T, S::kFma>(s + 64, cc, nm, acc2, pk);
         tmem_st_32x32b_x32(tP + 32, pk);
         float la, lb;
         f2_unpack(acc2, la, lb);
         l = l * alpha + (la + lb);
-        if (key0 + kKeys > g.s.len) {
+        if (key0 + kKeys > len) {
           // values past the sequence's end: what a recycled page holds there is replaced by
           // zeros (0 * NaN is NaN).  Both tiles write the same zeros before their own product.
           const uint32_t vs = (kv + j) % kSlots;
@@ -899,7 +1001,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          if (key0 + row >= g.s.len) {
+          if (key0 + row >= len) {
             uint8_t* dst = sV + vs * S::kTile + row * 128;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
@@ -923,11 +1025,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok && cnt > 0 && mbar_wait(BAR(x, PV_DONE), (mine + cnt - 1) & 1u, 0x90du));
       if (have_o) tc_fence_after();
       else if (cnt > 0) ok = false;
-      const bool whole = g.t0 == 0 && g.t1 == g.tiles;
+      const Desc& g = DESC();
+      const int pr = g.row0 + x * 128 + row;
+      const bool row_ok = pr < g.n * a.g;
+      const bool whole = g.whole;
       const float inv = (have_o && l > 0.f) ? 1.0f / l : 0.f;
-      const int64_t prow = ((int64_t)blockIdx.x * 2 + (g.t0 == 0)) * kRows + x * 128 + row;
-      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) +
-                                            (g.s.t0 + tok) * a.o_token + head * a.o_head);
+      const int64_t prow = ((int64_t)blockIdx.x * 2 + (key_t0 == 0)) * kRows + x * 128 + row;
+      const int tok = pr / a.g;
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (g.t0 + tok) * a.o_token +
+                                            (int64_t)(g.h * a.g + pr - tok * a.g) * a.o_head);
       float4* pdst = reinterpret_cast<float4*>(a.part + prow * D);
 #pragma unroll 1
       for (int hh = 0; hh < D / 32; ++hh) {
@@ -966,8 +1072,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<float2*>(a.part_ml + prow * 2) =
             make_float2(have_o ? m_used : -INFINITY, have_o ? l : 0.f);
       tc_fence_before();
-      kv += n.all;
+      kv += g.all;
       mine += cnt;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_empty + seg % kDescs);
+      ++seg;
     }
   }
   tc_fence_before();
@@ -1106,56 +1215,55 @@ extern "C" size_t fvb_paged_attn_workspace_bytes(int64_t max_new, int64_t Hq, in
   return (size_t)fvb::pattn::workspace(fvb::pattn::few_rows(max_new, Hq / Hk), D).total;
 }
 
-extern "C" int fvb_paged_attn(const void* q, int64_t q_token, int64_t q_head, const void* k,
-                              int64_t k_page, int64_t k_slot, int64_t k_head, const void* v,
-                              int64_t v_page, int64_t v_slot, int64_t v_head, const int32_t* table,
-                              int64_t width, const int32_t* lens, const int32_t* cu, int64_t T,
-                              int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages,
-                              int64_t page, int64_t max_new, int causal, float scale, int dtype,
-                              void* out, int64_t o_token, int64_t o_head, void* ws,
-                              fvb_stream_t stream) {
+extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(dtype == FVB_BF16 || dtype == FVB_F16, "fvb_paged_attn: dtype %d", dtype);
-  if (D != 64 && D != 128)
-    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attn: head_dim must be 64 or 128 (got %lld)", (long long)D);
-  FVB_REQUIRE(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq < (1 << 20),
-              "fvb_paged_attn: %lld query heads on %lld key heads", (long long)Hq, (long long)Hk);
-  FVB_REQUIRE(page > 0 && page % 16 == 0 && page < (1 << 24),
-              "fvb_paged_attn: pages must hold a multiple of 16 tokens (got %lld)", (long long)page);
-  FVB_REQUIRE(T >= 0 && B >= 0 && B < (1 << 30) && width >= 0 && pages > 0 && pages < (1ll << 31) &&
-                  width * page < (1ll << 31) && T < (1ll << 31) && T * Hq < (1ll << 31),
+  FVB_REQUIRE(p, "fvb_paged_attn: NULL pointer");
+  FVB_REQUIRE(p->dtype == FVB_BF16 || p->dtype == FVB_F16, "fvb_paged_attn: dtype %d", (int)p->dtype);
+  if (p->D != 64 && p->D != 128)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attn: head_dim must be 64 or 128 (got %lld)", (long long)p->D);
+  FVB_REQUIRE(p->Hk > 0 && p->Hq > 0 && p->Hq % p->Hk == 0 && p->Hq < (1 << 20),
+              "fvb_paged_attn: %lld query heads on %lld key heads", (long long)p->Hq, (long long)p->Hk);
+  FVB_REQUIRE(p->page > 0 && p->page % 16 == 0 && p->page < (1 << 24),
+              "fvb_paged_attn: pages must hold a multiple of 16 tokens (got %lld)", (long long)p->page);
+  FVB_REQUIRE(p->T >= 0 && p->B >= 0 && p->B < (1 << 30) && p->width >= 0 && p->width < (1ll << 31) &&
+                  p->pages > 0 && p->pages < (1ll << 31) && p->width * p->page < (1ll << 31) &&
+                  p->T < (1ll << 30) && p->T * p->Hq < (1ll << 30),
               "fvb_paged_attn: shape");
-  FVB_REQUIRE(scale > 0.f && scale < INFINITY, "fvb_paged_attn: scale %g", (double)scale);
-  FVB_REQUIRE(max_new >= 1, "fvb_paged_attn: max_new %lld", (long long)max_new);
-  if (T == 0 || B == 0) return FVB_OK;
-  FVB_REQUIRE(cu || T == B, "fvb_paged_attn: %lld tokens of %lld sequences need cu_seqlens", (long long)T,
-              (long long)B);
-  FVB_REQUIRE(q && lens && out && ws && (width == 0 || table) && k && v,
+  FVB_REQUIRE(p->scale > 0 && p->scale < 1e30, "fvb_paged_attn: scale %g", p->scale);
+  FVB_REQUIRE(p->max_new >= 1, "fvb_paged_attn: max_new %lld", (long long)p->max_new);
+  if (p->T == 0 || p->B == 0) return FVB_OK;
+  FVB_REQUIRE(p->cu || p->T == p->B, "fvb_paged_attn: %lld tokens of %lld sequences need cu_seqlens",
+              (long long)p->T, (long long)p->B);
+  FVB_REQUIRE(p->q && p->lens && p->out && p->workspace && (p->width == 0 || p->table) && p->k && p->v,
               "fvb_paged_attn: NULL pointer");
-  FVB_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(ws),
+  FVB_REQUIRE(aligned16(p->q) && aligned16(p->k) && aligned16(p->v) && aligned16(p->out) &&
+                  aligned16(p->workspace),
               "fvb_paged_attn: pointers must be 16-byte aligned");
-  FVB_REQUIRE((q_token | q_head | k_page | k_slot | k_head | v_page | v_slot | v_head | o_token | o_head) % 8 == 0,
+  FVB_REQUIRE((p->q_token | p->q_head | p->k_page | p->k_slot | p->k_head | p->v_page | p->v_slot |
+               p->v_head | p->o_token | p->o_head) % 8 == 0,
               "fvb_paged_attn: strides must be multiples of 8 elements");
-  const bool few = pattn::few_rows(max_new, Hq / Hk);
-  const pattn::Workspace w = pattn::workspace(few, D);
+  const bool few = pattn::few_rows(p->max_new, p->Hq / p->Hk);
+  const pattn::Workspace w = pattn::workspace(few, p->D);
+  char* const ws = (char*)p->workspace;
   pattn::Args a = {};
-  a.q = q;
-  a.out = out;
-  a.q_token = q_token, a.q_head = q_head, a.o_token = o_token, a.o_head = o_head;
-  a.k = k, a.v = v;
-  a.k_page = k_page, a.k_slot = k_slot, a.k_head = k_head;
-  a.v_page = v_page, a.v_slot = v_slot, a.v_head = v_head;
-  a.table = table, a.lens = lens, a.cu = cu;
-  a.T = T, a.width = width, a.pages = pages;
-  a.B = (int)B, a.Hk = (int)Hk, a.g = (int)(Hq / Hk), a.page = (int)page, a.causal = causal != 0;
+  a.q = p->q;
+  a.out = p->out;
+  a.q_token = p->q_token, a.q_head = p->q_head, a.o_token = p->o_token, a.o_head = p->o_head;
+  a.k = p->k, a.v = p->v;
+  a.k_page = p->k_page, a.k_slot = p->k_slot, a.k_head = p->k_head;
+  a.v_page = p->v_page, a.v_slot = p->v_slot, a.v_head = p->v_head;
+  a.table = p->table, a.lens = p->lens, a.cu = p->cu;
+  a.T = p->T, a.width = p->width, a.pages = p->pages;
+  a.B = (int)p->B, a.Hk = (int)p->Hk, a.g = (int)(p->Hq / p->Hk), a.page = (int)p->page;
+  a.causal = p->causal != 0;
   a.ctas = pattn::ctas_of(few);
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.part = (float*)((char*)ws + w.part);
-  a.part_ml = (float*)((char*)ws + w.ml);
-  a.rec = (int32_t*)((char*)ws + w.rec);
+  a.scale_log2 = (float)(p->scale * 1.4426950408889634);
+  a.part = (float*)(ws + w.part);
+  a.part_ml = (float*)(ws + w.ml);
+  a.rec = (int32_t*)(ws + w.rec);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == FVB_BF16)
-    return D == 128 ? pattn::launch<__nv_bfloat16, 128>(a, few, st)
-                    : pattn::launch<__nv_bfloat16, 64>(a, few, st);
-  return D == 128 ? pattn::launch<__half, 128>(a, few, st) : pattn::launch<__half, 64>(a, few, st);
+  if (p->dtype == FVB_BF16)
+    return p->D == 128 ? pattn::launch<__nv_bfloat16, 128>(a, few, st)
+                       : pattn::launch<__nv_bfloat16, 64>(a, few, st);
+  return p->D == 128 ? pattn::launch<__half, 128>(a, few, st) : pattn::launch<__half, 64>(a, few, st);
 }

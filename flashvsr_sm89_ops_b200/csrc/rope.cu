@@ -300,88 +300,83 @@ int launch_dtype(Args& a, int dtype, bool half, cudaStream_t stream, const char*
 }  // namespace rope
 }  // namespace fvb
 
-extern "C" int fvb_rope(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, void* q_out,
-                        int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
-                        int64_t k_head, int64_t Hk, void* k_out, int64_t ko_token, int64_t ko_head,
-                        int64_t T, int64_t D, int64_t rot, int half, int dtype, const void* pos,
-                        int pos64, int64_t axes, const uint64_t* freq, const int32_t* axis,
-                        float scale, int inverse, fvb_stream_t stream) {
+extern "C" int fvb_rope(const fvb_rope_args* p, fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(dtype >= FVB_BF16 && dtype <= FVB_F32, "fvb_rope: dtype %d", dtype);
-  FVB_REQUIRE(T >= 0 && D > 0 && D <= rope::kMaxDim, "fvb_rope: T %lld, D %lld (1..%d)", (long long)T,
-              (long long)D, rope::kMaxDim);
-  FVB_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0, "fvb_rope: rot %lld of %lld channels",
-              (long long)rot, (long long)D);
-  FVB_REQUIRE(Hq >= 0 && Hk >= 0 && Hq + Hk <= 4096, "fvb_rope: %lld + %lld heads", (long long)Hq,
-              (long long)Hk);
-  FVB_REQUIRE(axes >= 1 && axes <= 16, "fvb_rope: %lld axes", (long long)axes);
-  if (T == 0 || Hq + Hk == 0) return FVB_OK;
-  FVB_REQUIRE((Hq == 0 || (q && q_out)) && (Hk == 0 || (k && k_out)), "fvb_rope: NULL pointer");
-  FVB_REQUIRE(rot == 0 || (pos && freq && (axes == 1 || axis)), "fvb_rope: NULL pointer");
+  FVB_REQUIRE(p, "fvb_rope: NULL pointer");
+  FVB_REQUIRE(p->dtype >= FVB_BF16 && p->dtype <= FVB_F32, "fvb_rope: dtype %d", (int)p->dtype);
+  FVB_REQUIRE(p->T >= 0 && p->D > 0 && p->D <= rope::kMaxDim, "fvb_rope: T %lld, D %lld (1..%d)",
+              (long long)p->T, (long long)p->D, rope::kMaxDim);
+  FVB_REQUIRE(p->rot >= 0 && p->rot <= p->D && p->rot % 2 == 0, "fvb_rope: rot %lld of %lld channels",
+              (long long)p->rot, (long long)p->D);
+  FVB_REQUIRE(p->Hq >= 0 && p->Hk >= 0 && p->Hq <= 4096 && p->Hk <= 4096 - p->Hq,
+              "fvb_rope: %lld + %lld heads", (long long)p->Hq, (long long)p->Hk);
+  FVB_REQUIRE(p->axes >= 1 && p->axes <= 16, "fvb_rope: %lld axes", (long long)p->axes);
+  if (p->T == 0 || p->Hq + p->Hk == 0) return FVB_OK;
+  FVB_REQUIRE((p->Hq == 0 || (p->q && p->q_out)) && (p->Hk == 0 || (p->k && p->k_out)),
+              "fvb_rope: NULL pointer");
+  FVB_REQUIRE(p->rot == 0 || (p->pos && p->freq && (p->axes == 1 || p->axis)), "fvb_rope: NULL pointer");
   rope::Args a = {};
-  if (Hq) a.part[a.parts++] = {q, q_token, q_head, q_out, qo_token, qo_head, (int)Hq, 0, 1};
-  if (Hk) a.part[a.parts++] = {k, k_token, k_head, k_out, ko_token, ko_head, (int)Hk, 0, 1};
-  a.heads = (int)(Hq + Hk);
-  a.T = T;
-  a.D = (int)D;
-  a.rot = (int)rot;
-  a.pos = pos;
-  a.pos64 = pos64;
-  a.axes = (int)axes;
-  a.freq = freq;
-  a.axis = axis;
-  a.scale = scale;
-  a.inverse = inverse;
-  return rope::launch_dtype(a, dtype, half != 0, (cudaStream_t)stream, "fvb_rope");
+  if (p->Hq)
+    a.part[a.parts++] = {p->q, p->q_token, p->q_head, p->q_out, p->qo_token, p->qo_head, (int)p->Hq, 0, 1};
+  if (p->Hk)
+    a.part[a.parts++] = {p->k, p->k_token, p->k_head, p->k_out, p->ko_token, p->ko_head, (int)p->Hk, 0, 1};
+  a.heads = (int)(p->Hq + p->Hk);
+  a.T = p->T;
+  a.D = (int)p->D;
+  a.rot = (int)p->rot;
+  a.pos = p->pos;
+  a.pos64 = p->pos64 != 0;
+  a.axes = (int)p->axes;
+  a.freq = p->freq;
+  a.axis = p->axis;
+  a.scale = (float)p->scale;
+  a.inverse = p->inverse != 0;
+  return rope::launch_dtype(a, (int)p->dtype, p->half != 0, (cudaStream_t)stream, "fvb_rope");
 }
 
-extern "C" int fvb_kv_append(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, void* q_out,
-                             int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
-                             int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
-                             int64_t Hk, int64_t T, int64_t D, int64_t rot, int half, int dtype,
-                             const void* pos, int pos64, int64_t axes, const uint64_t* freq,
-                             const int32_t* axis, float scale, const int32_t* cu,
-                             const int32_t* lens, const int32_t* table, int64_t B, int64_t width,
-                             int64_t pages, int64_t page, void* k_pool, void* v_pool,
-                             int64_t page_stride, fvb_stream_t stream) {
+extern "C" int fvb_kv_append(const fvb_kv_append_args* p, fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(dtype == FVB_BF16 || dtype == FVB_F16, "fvb_kv_append: dtype %d", dtype);
-  FVB_REQUIRE(T >= 0 && D > 0 && D <= rope::kMaxDim, "fvb_kv_append: T %lld, D %lld (1..%d)",
-              (long long)T, (long long)D, rope::kMaxDim);
-  FVB_REQUIRE(rot >= 0 && rot <= D && rot % 2 == 0, "fvb_kv_append: rot %lld of %lld channels",
-              (long long)rot, (long long)D);
-  FVB_REQUIRE(Hq >= 0 && Hk > 0 && Hq + 2 * Hk <= 4096, "fvb_kv_append: %lld + 2 x %lld heads",
-              (long long)Hq, (long long)Hk);
-  FVB_REQUIRE(B >= 0 && width >= 0 && pages >= 0 && page > 0 && page < (1 << 24),
+  FVB_REQUIRE(p, "fvb_kv_append: NULL pointer");
+  FVB_REQUIRE(p->dtype == FVB_BF16 || p->dtype == FVB_F16, "fvb_kv_append: dtype %d", (int)p->dtype);
+  FVB_REQUIRE(p->T >= 0 && p->D > 0 && p->D <= rope::kMaxDim, "fvb_kv_append: T %lld, D %lld (1..%d)",
+              (long long)p->T, (long long)p->D, rope::kMaxDim);
+  FVB_REQUIRE(p->rot >= 0 && p->rot <= p->D && p->rot % 2 == 0,
+              "fvb_kv_append: rot %lld of %lld channels", (long long)p->rot, (long long)p->D);
+  FVB_REQUIRE(p->Hq >= 0 && p->Hk > 0 && p->Hq <= 4096 && p->Hk <= 2048 && p->Hq + 2 * p->Hk <= 4096,
+              "fvb_kv_append: %lld + 2 x %lld heads", (long long)p->Hq, (long long)p->Hk);
+  FVB_REQUIRE(p->B >= 0 && p->width >= 0 && p->pages >= 0 && p->page > 0 && p->page < (1 << 24),
               "fvb_kv_append: cache shape");
-  FVB_REQUIRE(axes >= 1 && axes <= 16 && (axes == 1 || pos), "fvb_kv_append: %lld axes need positions",
-              (long long)axes);
-  if (T == 0 || B == 0) return FVB_OK;
-  FVB_REQUIRE((Hq == 0 || (q && q_out)) && k && v && cu && lens && table && k_pool && v_pool,
+  FVB_REQUIRE(p->axes >= 1 && p->axes <= 16 && (p->axes == 1 || p->pos),
+              "fvb_kv_append: %lld axes need positions", (long long)p->axes);
+  if (p->T == 0 || p->B == 0) return FVB_OK;
+  FVB_REQUIRE((p->Hq == 0 || (p->q && p->q_out)) && p->k && p->v && p->cu && p->lens && p->table &&
+                  p->k_pool && p->v_pool,
               "fvb_kv_append: NULL pointer");
-  FVB_REQUIRE(rot == 0 || (freq && (axes == 1 || axis)), "fvb_kv_append: NULL pointer");
+  FVB_REQUIRE(p->rot == 0 || (p->freq && (p->axes == 1 || p->axis)), "fvb_kv_append: NULL pointer");
+  const int turned = p->rot > 0;
   rope::Args a = {};
-  if (Hq) a.part[a.parts++] = {q, q_token, q_head, q_out, qo_token, qo_head, (int)Hq, 0, rot > 0};
-  a.part[a.parts++] = {k, k_token, k_head, k_pool, 0, D, (int)Hk, 1, rot > 0};
-  a.part[a.parts++] = {v, v_token, v_head, v_pool, 0, D, (int)Hk, 1, 0};
-  a.heads = (int)(Hq + 2 * Hk);
-  a.T = T;
-  a.D = (int)D;
-  a.rot = (int)rot;
-  a.pos = pos;
-  a.pos64 = pos64;
-  a.axes = (int)axes;
-  a.freq = freq;
-  a.axis = axis;
-  a.scale = scale;
-  a.cu = cu;
-  a.lens = lens;
-  a.table = table;
-  a.B = B;
-  a.width = width;
-  a.pages = pages;
-  a.page = (int)page;
-  a.page_stride = page_stride;
-  a.slot_stride = Hk * D;
-  return rope::launch_dtype(a, dtype, half != 0, (cudaStream_t)stream, "fvb_kv_append");
+  if (p->Hq)
+    a.part[a.parts++] = {p->q, p->q_token, p->q_head, p->q_out, p->qo_token, p->qo_head, (int)p->Hq, 0, turned};
+  a.part[a.parts++] = {p->k, p->k_token, p->k_head, p->k_pool, 0, p->D, (int)p->Hk, 1, turned};
+  a.part[a.parts++] = {p->v, p->v_token, p->v_head, p->v_pool, 0, p->D, (int)p->Hk, 1, 0};
+  a.heads = (int)(p->Hq + 2 * p->Hk);
+  a.T = p->T;
+  a.D = (int)p->D;
+  a.rot = (int)p->rot;
+  a.pos = p->pos;
+  a.pos64 = p->pos64 != 0;
+  a.axes = (int)p->axes;
+  a.freq = p->freq;
+  a.axis = p->axis;
+  a.scale = (float)p->scale;
+  a.cu = p->cu;
+  a.lens = p->lens;
+  a.table = p->table;
+  a.B = p->B;
+  a.width = p->width;
+  a.pages = p->pages;
+  a.page = (int)p->page;
+  a.page_stride = p->page_stride;
+  a.slot_stride = p->Hk * p->D;
+  return rope::launch_dtype(a, (int)p->dtype, p->half != 0, (cudaStream_t)stream, "fvb_kv_append");
 }

@@ -12,24 +12,73 @@ belong on one stream, or must be ordered by the caller.  Inference only.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
-from .rope import Rope, _out, _positions, _rows
+from .rope import _POS64, Rope, _out, _positions, _rows
 
 _DTYPES = {torch.bfloat16: _lib.FVB_BF16, torch.float16: _lib.FVB_F16}
 _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
            4: "bad arguments (an index out of range or twice, a negative count, a branch that was not empty)"}
 
 
-def _ints(t, n, what, name, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.numel() != n):
+def _ints(t, n, what, name, index):
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
         raise ValueError(f"{name}: {what} must be int32 [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name}: {what} is on {t.device}, the cache on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: {what} is on {t.device}, the cache on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal, sm_scale, max_new, out):
+    """The call itself.  pools: k, its three strides, v, its three strides; shape: Hk, D, P, page."""
+    index = q.get_device()
+    T, Hq, D = q.shape
+    Hk, _, P, page = shape
+    if cu_seqlens is not None:
+        cu = _ints(cu_seqlens, B + 1, "cu_seqlens", name, index).data_ptr()
+        max_new = max(T, 1) if max_new is None else max_new
+    elif T != B:
+        raise ValueError(f"{name}: {T} tokens of {B} sequences need cu_seqlens")
+    else:
+        cu = 0
+        max_new = 1 if max_new is None else max_new
+    if max_new < 1:
+        raise ValueError(f"{name}: max_new must be at least 1, got {max_new}")
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"{name}: {Hq} query heads on {Hk} key heads")
+    st, sh, sd = q.stride()
+    if sd != 1 or (st | sh) & 7 or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+        st, sh, _ = q.stride()
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ot, oh = Hq * D, D
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)} on {q.device}")
+        ot, oh, od = out.stride()
+        if od != 1 or (ot | oh) & 7 or out.data_ptr() & 15:
+            raise ValueError(f"{name}: out must be 16-byte aligned, with strides that are multiples of 8")
+        if out.data_ptr() == q.data_ptr():
+            raise ValueError(f"{name}: out cannot be q")
+    few = max_new * (Hq // Hk) <= 16
+    ws = torch.empty(_WS.get((few, D, index)) or _workspace_bytes(few, D, index), dtype=torch.uint8, device=q.device)
+    _lib.call_on(index, "fvb_paged_attn",
+                 _lib.PAGED_ATTN_ARGS(q.data_ptr(), st, sh, *pools, table, width, lens, cu, T, B, Hq, Hk, D, P, page,
+                                      max_new, causal, D ** -0.5 if sm_scale is None else sm_scale, dt,
+                                      out.data_ptr(), ot, oh, ws.data_ptr()), _lib.stream_of(q))
+    return out
+
+
+_WS: dict = {}
+
+
+def _workspace_bytes(few, D, index):
+    """fvb_paged_attn_workspace_bytes of few or many rows, asked for once a device."""
+    with torch.cuda.device(index):
+        n = _WS[(few, D, index)] = _lib.load().fvb_paged_attn_workspace_bytes(1 if few else 17, 1, 1, D)
+    return n
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -67,23 +116,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     dev = q.device
     if k_pages.device != dev or v_pages.device != dev:
         raise ValueError(f"{name}: q is on {dev}, the pages on {k_pages.device} and {v_pages.device}")
+    index = dev.index
     B = lens.numel()
-    lens = _ints(lens, B, "lens", name, dev)
+    lens = _ints(lens, B, "lens", name, index)
     if table.dim() != 2 or table.shape[0] != B or table.dtype != torch.int32 or table.device != dev:
         raise ValueError(f"{name}: table must be int32 [{B}, width] on {dev}, got {table.dtype} {tuple(table.shape)}")
     table = table if table.is_contiguous() else table.contiguous()
-    if cu_seqlens is not None:
-        cu_seqlens = _ints(cu_seqlens, B + 1, "cu_seqlens", name, dev)
-    elif T != B:
-        raise ValueError(f"{name}: {T} tokens of {B} sequences need cu_seqlens")
-    if max_new is None:
-        max_new = 1 if cu_seqlens is None else max(T, 1)
-    elif max_new < 1:
-        raise ValueError(f"{name}: max_new must be at least 1, got {max_new}")
-    if Hk == 0 or Hq == 0 or Hq % Hk:
-        raise ValueError(f"{name}: {Hq} query heads on {Hk} key heads")
-    if q.stride(2) != 1 or (q.stride(0) | q.stride(1)) & 7 or q.data_ptr() & 15:
-        q = q.clone(memory_format=torch.contiguous_format)
     # the stride of an axis of one is any number
     ks, vs = list(k_pages.stride()), list(v_pages.stride())
     for t, s in ((k_pages, ks), (v_pages, vs)):
@@ -94,36 +132,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                 s[i] = D
             elif s[i] & 7 or s[i] <= 0:
                 raise ValueError(f"{name}: strides of the pages must be positive multiples of 8, got {tuple(t.stride())}")
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
-            or (out.stride(0) | out.stride(1)) & 7 or out.data_ptr() & 15:
-        raise ValueError(f"{name}: out must be {q.dtype} [{T}, {Hq}, {D}] on {dev}, 16-byte aligned, strides "
-                         f"multiples of 8")
-    elif out.data_ptr() == q.data_ptr():
-        raise ValueError(f"{name}: out cannot be q")
-    nws = _workspace_bytes(max_new * (Hq // Hk) <= 16, D, dev.index)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-    _lib.call_on(dev.index, "fvb_paged_attn", q.data_ptr(), q.stride(0), q.stride(1),
-                 k_pages.data_ptr(), ks[0], ks[1], ks[2], v_pages.data_ptr(), vs[0], vs[1], vs[2],
-                 table.data_ptr(), table.shape[1], lens.data_ptr(),
-                 None if cu_seqlens is None else cu_seqlens.data_ptr(), T, B, Hq, Hk, D, P, page, max_new,
-                 causal, 1.0 / math.sqrt(D) if sm_scale is None else sm_scale, dt, out.data_ptr(),
-                 out.stride(0), out.stride(1), ws.data_ptr(), _lib.stream_of(q))
-    return out
-
-
-_WS: dict = {}
-
-
-def _workspace_bytes(few, D, device):
-    """fvb_paged_attn_workspace_bytes of few or many rows, asked for once a device."""
-    n = _WS.get((few, D, device))
-    if n is None:
-        with torch.cuda.device(device):
-            n = _lib.load().fvb_paged_attn_workspace_bytes(1 if few else 17, 1, 1, D)
-        _WS[(few, D, device)] = n
-    return n
+    return _attend(name, q, dt, (k_pages.data_ptr(), *ks[:3], v_pages.data_ptr(), *vs[:3]), (Hk, D, P, page),
+                   table.data_ptr(), table.shape[1], lens.data_ptr(), B, cu_seqlens, causal, sm_scale, max_new, out)
 
 
 class PagedKV:
@@ -171,10 +181,16 @@ class PagedKV:
         seqs, width = table.shape
         n = _lib.load().fvb_pages_workspace_bytes(seqs, P, seqs)
         self._ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        self._ws_ptr = self._ws.data_ptr()
         # what every step of the pages takes: the state, then its sizes
         self._state = (table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.status.data_ptr(), seqs, width, P,
                        page)
         self._pools = (k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0) * 2, k.stride(1) * 2, H * D * 2)
+        # what every append and attention takes
+        self._index, self._dt, self._dtype = k.get_device(), _DTYPES[k.dtype], k.dtype
+        self._shape = (H, D, P, page)
+        self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
+        self._tail = (table.data_ptr(), seqs, width, P, page)
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads: int, head_dim: int, seqs: int,
@@ -194,19 +210,19 @@ class PagedKV:
             raise RuntimeError("PagedKV: " + "; ".join(m for bit, m in _STATUS.items() if s & bit))
 
     def _call(self, name, *args):
-        _lib.call_on(self.device.index, name, *args, self._ws.data_ptr(), _lib.stream_of(self.table))
+        _lib.call_on(self._index, name, *args, self._ws_ptr, _lib.stream_of(self.table))
 
     def reserve(self, more: torch.Tensor):
         """Room for more[b] tokens (int32 [seqs]) behind every sequence; lens grow by them."""
-        more = _ints(more, self.lens.numel(), "more", "PagedKV.reserve", self.device)
+        more = _ints(more, self.lens.numel(), "more", "PagedKV.reserve", self._index)
         self._call("fvb_pages_reserve", more.data_ptr(), *self._state)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor):
         """Sequence dst[i] becomes a branch of src[i] (int32 [n]; a parent may come several times,
         the branches are empty, distinct and no parents).  Full pages are shared; the tokens in a
         partly filled last page are copied, in every layer."""
-        src = _ints(src, None, "src", "PagedKV.fork", self.device)
-        dst = _ints(dst, src.numel(), "dst", "PagedKV.fork", self.device)
+        src = _ints(src, None, "src", "PagedKV.fork", self._index)
+        dst = _ints(dst, src.numel(), "dst", "PagedKV.fork", self._index)
         if src.numel() > self.lens.numel():
             raise ValueError(f"PagedKV.fork: {src.numel()} branches of {self.lens.numel()} sequences")
         self._call("fvb_pages_fork", src.data_ptr(), dst.data_ptr(), src.numel(), *self._state, *self._pools)
@@ -215,9 +231,9 @@ class PagedKV:
         """Sequences (int32 [n], distinct) give back all their pages and become empty, or with
         `pages` (int32 [n]) that many of their first ones: a stream's oldest tokens.  Pages that
         other sequences hold stay."""
-        seqs = _ints(seqs, None, "seqs", "PagedKV.release", self.device)
+        seqs = _ints(seqs, None, "seqs", "PagedKV.release", self._index)
         if pages is not None:
-            pages = _ints(pages, seqs.numel(), "pages", "PagedKV.release", self.device)
+            pages = _ints(pages, seqs.numel(), "pages", "PagedKV.release", self._index)
         self._call("fvb_pages_release", seqs.data_ptr(), None if pages is None else pages.data_ptr(), seqs.numel(),
                    *self._state)
 
@@ -234,18 +250,20 @@ class PagedKV:
         returned; positions (as in fused_rope) default to the tokens' places in their sequences.
         Tokens past cu_seqlens[seqs] are ignored, and rows of out_q for them stay as they are."""
         name = "PagedKV.append"
-        _lib.require_cuda(k, v, cu_seqlens, q, positions)
-        H, D = self.k.shape[3:]
+        index, dt = self._index, self._dtype
+        H, D, P, page = self._shape
+        if not (k.is_cuda and v.is_cuda and cu_seqlens.is_cuda):
+            _lib.require_cuda(k, v, cu_seqlens)
         k, v = _rows(k, "k", name), _rows(v, "v", name)
-        T = k.shape[0]
-        if k.shape != (T, H, D) or v.shape != (T, H, D):
+        T, Hk, Dk = k.shape
+        if Hk != H or Dk != D or v.shape != k.shape:
             raise ValueError(f"{name}: k and v must be [T, {H}, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
-        dt = self.k.dtype
-        if k.dtype != dt or v.dtype != dt or k.device != self.device or v.device != self.device:
+        if k.dtype != dt or v.dtype != dt or k.get_device() != index or v.get_device() != index:
             raise ValueError(f"{name}: k and v must be {dt} on {self.device}")
-        if not 0 <= layer < self.k.shape[0]:
-            raise ValueError(f"{name}: layer {layer} of {self.k.shape[0]}")
-        cu = _ints(cu_seqlens, self.lens.numel() + 1, "cu_seqlens", name, self.device)
+        if not 0 <= layer < self._pools[2]:
+            raise ValueError(f"{name}: layer {layer} of {self._pools[2]}")
+        table, seqs, width, P, page = self._tail
+        cu = _ints(cu_seqlens, seqs + 1, "cu_seqlens", name, index)
         if q is None:
             if out_q is not None:
                 raise ValueError(f"{name}: out_q without q")
@@ -253,41 +271,54 @@ class PagedKV:
         else:
             if rope is None:
                 raise ValueError(f"{name}: q without a Rope has nothing to be done to it")
-            if q.dtype != dt or q.device != self.device:
+            if q.dtype != dt or q.get_device() != index:
                 raise ValueError(f"{name}: q must be {dt} on {self.device}")
             q3 = _rows(q, "q", name)
-            if q3.shape[0] != T or q3.shape[2] != D:
+            Tq, Hq, Dq = q3.shape
+            if Tq != T or Dq != D:
                 raise ValueError(f"{name}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
-            oq, oq3 = _out(out_q, q, "out_q", name)
-            s, so = q3.stride(), oq3.stride()
-            qargs = (q3.data_ptr(), s[0], s[1], q3.shape[1], oq3.data_ptr(), so[0], so[1])
+            oq, ot, oh = _out(out_q, q, "out_q", name)
+            st, sh, _ = q3.stride()
+            qargs = (q3.data_ptr(), st, sh, Hq, oq.data_ptr(), ot, oh)
         if rope is None:
             if positions is not None:
                 raise ValueError(f"{name}: positions without a Rope")
-            rargs = (0, False, _DTYPES[dt], None, False, 1, None, None, 1.0)
+            rargs = (0, 0, self._dt, 0, 0, 1, 0, 0, 1.0)
         else:
-            if rope.device != self.device or rope.rotary_dim > D:
+            if rope.index != index or rope.rotary_dim > D:
                 raise ValueError(f"{name}: {rope} on {rope.device} for heads of {D} on {self.device}")
-            if positions is not None:
-                positions = _positions(positions, rope, T, self.device, name)
-            elif rope.axes > 1:
-                raise ValueError(f"{name}: a Rope of {rope.axes} axes needs positions")
-            rargs = (rope.rotary_dim, rope.half, _DTYPES[dt], None if positions is None else positions.data_ptr(),
-                     positions is not None and positions.dtype == torch.int64, rope.axes, rope._freq, rope._axis,
-                     rope.scale)
-        ks, vs = k.stride(), v.stride()
-        at = layer * self._pools[3]
-        table, lens, _, _, seqs, width, pages, page = self._state
-        _lib.call_on(self.device.index, "fvb_kv_append", *qargs, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
-                     vs[1], H, T, D, *rargs, cu.data_ptr(), lens, table, seqs, width, pages, page,
-                     self._pools[0] + at, self._pools[1] + at, self.k.stride(1), _lib.stream_of(k))
+            if positions is None:
+                if rope.axes > 1:
+                    raise ValueError(f"{name}: a Rope of {rope.axes} axes needs positions")
+                pos, pos64 = 0, 0
+            else:
+                positions = _positions(positions, rope, T, index, name)
+                pos, pos64 = positions.data_ptr(), _POS64[positions.dtype]
+            rargs = (rope.rotary_dim, rope.half, self._dt, pos, pos64, rope.axes, rope._freq, rope._axis, rope.scale)
+        kt, kh, _ = k.stride()
+        vt, vh, _ = v.stride()
+        kp, vp, _, layer_bytes, _, _ = self._pools
+        at = layer * layer_bytes
+        _lib.call_on(index, "fvb_kv_append",
+                     _lib.KV_APPEND_ARGS(*qargs, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, H, T, D, *rargs,
+                                         cu.data_ptr(), self._state[1], table, seqs, width, P, page, kp + at, vp + at,
+                                         self._strides[0]), _lib.stream_of(k))
         return oq
 
     def attend(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, causal: bool = True,
                sm_scale: float | None = None, max_new: int | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """paged_attention of q over one layer of this cache."""
-        if not 0 <= layer < self.k.shape[0]:
-            raise ValueError(f"PagedKV.attend: layer {layer} of {self.k.shape[0]}")
-        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, cu_seqlens, causal=causal,
-                               sm_scale=sm_scale, max_new=max_new, out=out)
+        name = "PagedKV.attend"
+        if not 0 <= layer < self._pools[2]:
+            raise ValueError(f"{name}: layer {layer} of {self._pools[2]}")
+        if not q.is_cuda:
+            _lib.require_cuda(q)
+        if q.dtype != self._dtype or q.get_device() != self._index or q.dim() != 3 or q.shape[2] != self._shape[1]:
+            raise ValueError(f"{name}: q must be {self._dtype} [T, Hq, {self._shape[1]}] on {self.device}, got {q.dtype} "
+                             f"{tuple(q.shape)} on {q.device}")
+        kp, vp, _, layer_bytes, _, _ = self._pools
+        at, s = layer * layer_bytes, self._strides
+        table, seqs, width, _, _ = self._tail
+        return _attend(name, q, self._dt, (kp + at, *s, vp + at, *s), self._shape, table, width, self._state[1], seqs,
+                       cu_seqlens, causal, sm_scale, max_new, out)

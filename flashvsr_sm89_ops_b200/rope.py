@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from .fp4_quant import _dtype_code
 
+_POS64 = {torch.int32: 0, torch.int64: 1}
 _SCALINGS = (None, "linear", "ntk", "yarn")
 
 
@@ -80,6 +81,7 @@ class Rope:
         self.axis = torch.tensor([a for a, d in enumerate(dims) for _ in range(d // 2)], dtype=torch.int32,
                                  device=device)
         self.device = self.freq.device
+        self.index = self.freq.get_device()  # -1 on the host
         self._freq, self._axis = self.freq.data_ptr(), self.axis.data_ptr()
 
     def __repr__(self):
@@ -95,10 +97,10 @@ def _rows(x, what, name):
     return x if x.shape[2] < 2 or x.stride(2) == 1 else x.contiguous()
 
 
-def _positions(positions, rope, T, device, name):
-    if positions.device != device:
-        raise ValueError(f"{name}: positions are on {positions.device}, q on {device}")
-    if positions.dtype not in (torch.int32, torch.int64):
+def _positions(positions, rope, T, index, name):
+    if positions.get_device() != index:
+        raise ValueError(f"{name}: positions are on {positions.device}, q on cuda:{index}")
+    if positions.dtype not in _POS64:
         raise ValueError(f"{name}: positions must be int32 or int64, got {positions.dtype}")
     if positions.numel() != T * rope.axes or (rope.axes > 1 and positions.shape[-1] != rope.axes):
         raise ValueError(f"{name}: positions must be one of {rope.axes} coordinate(s) for each of {T} tokens, "
@@ -107,50 +109,50 @@ def _positions(positions, rope, T, device, name):
 
 
 def _out(out, x, what, name):
-    """The tensor that x's rotation goes to, and its rows."""
+    """The tensor that x's rotation goes to, and its rows' strides of tokens and heads."""
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{name}: {what} must be {x.dtype} {tuple(x.shape)} on {x.device}")
-    rows = out
-    if out.dim() == 4:
-        if out.stride(0) != out.shape[1] * out.stride(1):
-            raise ValueError(f"{name}: the items of {what} must follow each other")
-        rows = out.flatten(0, 1)
-    if rows.shape[2] > 1 and rows.stride(2) != 1:
+    s = out.stride()
+    if len(s) == 4 and s[0] != out.shape[1] * s[1] and out.shape[0] > 1:
+        raise ValueError(f"{name}: the items of {what} must follow each other")
+    if s[-1] != 1 and out.shape[-1] > 1:
         raise ValueError(f"{name}: {what} must have unit stride inside a head")
-    return out, rows
+    return out, s[-3], s[-2]
 
 
 def _run(q, k, positions, rope, inverse, out_q, out_k):
     name = "fused_rope"
     dt = _dtype_code(q.dtype, name)
-    dev = q.device
+    index = q.get_device()
     q3 = _rows(q, "q", name)
     T, Hq, D = q3.shape
     if rope.rotary_dim > D:
         raise ValueError(f"{name}: rotary_dim {rope.rotary_dim} of a head of {D}")
-    if rope.device != dev:
-        raise ValueError(f"{name}: the Rope is on {rope.device}, q on {dev}")
-    positions = _positions(positions, rope, T, dev, name)
-    oq, oq3 = _out(out_q, q, "out_q", name)
-    s, so = q3.stride(), oq3.stride()
+    if rope.index != index:
+        raise ValueError(f"{name}: the Rope is on {rope.device}, q on {q.device}")
+    positions = _positions(positions, rope, T, index, name)
+    oq, ot, oh = _out(out_q, q, "out_q", name)
+    st, sh, _ = q3.stride()
     if k is None:
         if out_k is not None:
             raise ValueError(f"{name}: out_k without k")
         ok, kargs = None, (0, 0, 0, 0, 0, 0, 0)
     else:
-        if k.dtype != q.dtype or k.device != dev:
-            raise ValueError(f"{name}: k is {k.dtype} on {k.device}, q {q.dtype} on {dev}")
+        if k.dtype != q.dtype or k.get_device() != index:
+            raise ValueError(f"{name}: k is {k.dtype} on {k.device}, q {q.dtype} on {q.device}")
         k3 = _rows(k, "k", name)
-        if k3.shape[0] != T or k3.shape[2] != D:
+        Tk, Hk, Dk = k3.shape
+        if Tk != T or Dk != D:
             raise ValueError(f"{name}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
-        ok, ok3 = _out(out_k, k, "out_k", name)
-        t, to = k3.stride(), ok3.stride()
-        kargs = (k3.data_ptr(), t[0], t[1], k3.shape[1], ok3.data_ptr(), to[0], to[1])
-    _lib.call_on(dev.index, "fvb_rope", q3.data_ptr(), s[0], s[1], Hq, oq3.data_ptr(), so[0], so[1], *kargs,
-                 T, D, rope.rotary_dim, rope.half, dt, positions.data_ptr(), positions.dtype == torch.int64,
-                 rope.axes, rope._freq, rope._axis, rope.scale, inverse, _lib.stream_of(q))
+        ok, kot, koh = _out(out_k, k, "out_k", name)
+        kt, kh, _ = k3.stride()
+        kargs = (k3.data_ptr(), kt, kh, Hk, ok.data_ptr(), kot, koh)
+    _lib.call_on(index, "fvb_rope",
+                 _lib.ROPE_ARGS(q3.data_ptr(), st, sh, Hq, oq.data_ptr(), ot, oh, *kargs, T, D, rope.rotary_dim,
+                                rope.half, dt, positions.data_ptr(), _POS64[positions.dtype], rope.axes, rope._freq,
+                                rope._axis, rope.scale, inverse), _lib.stream_of(q))
     return oq, ok
 
 
@@ -183,7 +185,8 @@ def fused_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     inverse turns back, which is the gradient; autograd (once) goes through the call unless
     outputs are given.  D at most 256.
     """
-    _lib.require_cuda(q, k, positions)
+    if not (q.is_cuda and positions.is_cuda and (k is None or k.is_cuda)):
+        _lib.require_cuda(q, k, positions)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out_q is not None or out_k is not None:
             raise ValueError("fused_rope: out_q / out_k with inputs that require a gradient")

@@ -392,12 +392,24 @@ FVB_API int fvb_residual_norm(const void* x, const void* y, const void* gate, in
  * int32 or (pos64) int64 [T] or [T, axes], pair i on axis[i].  Strides in elements, unit stride
  * inside a head, any alignment (16-byte vectors where every pointer, stride and part allows).
  * D <= 256.  Outputs may be the inputs. */
-FVB_API int fvb_rope(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, void* q_out,
-                     int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
-                     int64_t k_head, int64_t Hk, void* k_out, int64_t ko_token, int64_t ko_head,
-                     int64_t T, int64_t D, int64_t rot, int half, int dtype, const void* pos,
-                     int pos64, int64_t axes, const uint64_t* freq, const int32_t* axis, float scale,
-                     int inverse, fvb_stream_t stream);
+typedef struct {
+  const void* q;
+  int64_t q_token, q_head, Hq;
+  void* q_out;
+  int64_t qo_token, qo_head;
+  const void* k; /* Hk = 0: none */
+  int64_t k_token, k_head, Hk;
+  void* k_out;
+  int64_t ko_token, ko_head;
+  int64_t T, D, rot, half, dtype;
+  const void* pos;
+  int64_t pos64, axes;
+  const uint64_t* freq; /* [rot / 2] */
+  const int32_t* axis;  /* [rot / 2]; NULL with one axis */
+  double scale;
+  int64_t inverse;
+} fvb_rope_args;
+FVB_API int fvb_rope(const fvb_rope_args* args, fvb_stream_t stream);
 
 /* A paged cache: pools of pages [pages][page][Hk][D] (page stride in elements, a page contiguous),
  * table [B][width] of page numbers (-1: none), lens [B] tokens a sequence.  cu [B + 1]: new tokens
@@ -405,14 +417,27 @@ FVB_API int fvb_rope(const void* q, int64_t q_token, int64_t q_head, int64_t Hq,
  * Writes k (rotated, rot = 0: as it is) and v of T new tokens to their places, and q rotated to
  * q_out (Hq = 0: no q).  pos NULL: a token's position is its place in the sequence.  Tokens
  * outside cu, and places without a page, are left alone.  bf16 / fp16. */
-FVB_API int fvb_kv_append(const void* q, int64_t q_token, int64_t q_head, int64_t Hq, void* q_out,
-                          int64_t qo_token, int64_t qo_head, const void* k, int64_t k_token,
-                          int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int64_t Hk,
-                          int64_t T, int64_t D, int64_t rot, int half, int dtype, const void* pos,
-                          int pos64, int64_t axes, const uint64_t* freq, const int32_t* axis,
-                          float scale, const int32_t* cu, const int32_t* lens, const int32_t* table,
-                          int64_t B, int64_t width, int64_t pages, int64_t page, void* k_pool,
-                          void* v_pool, int64_t page_stride, fvb_stream_t stream);
+typedef struct {
+  const void* q;
+  int64_t q_token, q_head, Hq;
+  void* q_out;
+  int64_t qo_token, qo_head;
+  const void* k;
+  int64_t k_token, k_head;
+  const void* v;
+  int64_t v_token, v_head, Hk;
+  int64_t T, D, rot, half, dtype;
+  const void* pos;
+  int64_t pos64, axes;
+  const uint64_t* freq;
+  const int32_t* axis;
+  double scale;
+  const int32_t *cu, *lens, *table;
+  int64_t B, width, pages, page;
+  void *k_pool, *v_pool;
+  int64_t page_stride;
+} fvb_kv_append_args;
+FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
 
 /* Pages.  refs [pages]: how many sequences hold a page (0: free).  Free pages are given out lowest
  * first, in the order of sequences and of their pages.  A step that cannot be done changes nothing
@@ -453,13 +478,24 @@ FVB_API int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int3
  * positive.  fp32 scores, statistics and sums; the probabilities are rounded to the input's type
  * for their product with v. */
 FVB_API size_t fvb_paged_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hk, int64_t D);
-FVB_API int fvb_paged_attn(const void* q, int64_t q_token, int64_t q_head, const void* k,
-                           int64_t k_page, int64_t k_slot, int64_t k_head, const void* v,
-                           int64_t v_page, int64_t v_slot, int64_t v_head, const int32_t* table,
-                           int64_t width, const int32_t* lens, const int32_t* cu, int64_t T,
-                           int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page,
-                           int64_t max_new, int causal, float scale, int dtype, void* out,
-                           int64_t o_token, int64_t o_head, void* workspace, fvb_stream_t stream);
+typedef struct {
+  const void* q;
+  int64_t q_token, q_head;
+  const void* k;
+  int64_t k_page, k_slot, k_head;
+  const void* v;
+  int64_t v_page, v_slot, v_head;
+  const int32_t* table;
+  int64_t width;
+  const int32_t *lens, *cu;
+  int64_t T, B, Hq, Hk, D, pages, page, max_new, causal;
+  double scale;
+  int64_t dtype;
+  void* out;
+  int64_t o_token, o_head;
+  void* workspace; /* fvb_paged_attn_workspace_bytes, 16-byte aligned */
+} fvb_paged_attn_args;
+FVB_API int fvb_paged_attn(const fvb_paged_attn_args* args, fvb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -69,33 +69,35 @@ def test_c_arguments():
     bad, unsupported = _lib.FVB_ERR_INVALID, _lib.FVB_ERR_UNSUPPORTED
 
     def rope(T=4, D=64, rot=64, dtype=0, Hq=2, Hk=0, axes=1, q=16, pos=16, freq=16, axis=16):
-        return lib.fvb_rope(q, Hq * D, D, Hq, q, Hq * D, D, None, 0, 0, Hk, None, 0, 0, T, D, rot, 0, dtype, pos, 0,
-                            axes, freq, axis, 1.0, 0, None)
+        return lib.fvb_rope(_lib.ROPE_ARGS(q, Hq * D, D, Hq, q, Hq * D, D, 0, 0, 0, Hk, 0, 0, 0, T, D, rot, 0, dtype,
+                                           pos, 0, axes, freq, axis, 1.0, 0), None)
 
     for kw in ({"T": -1}, {"D": 257}, {"D": 0}, {"rot": 65}, {"rot": 66}, {"rot": -2}, {"dtype": 3}, {"Hq": 4097},
-               {"Hk": 1}, {"axes": 0}, {"axes": 17}, {"q": None}, {"pos": None}, {"freq": None},
-               {"axes": 2, "axis": None}):
+               {"Hk": 1}, {"axes": 0}, {"axes": 17}, {"q": 0}, {"pos": 0}, {"freq": 0},
+               {"axes": 2, "axis": 0}):
         assert rope(**kw) == bad, kw
     assert rope(T=0) == _lib.FVB_OK
+    assert lib.fvb_rope(None, None) == lib.fvb_kv_append(None, None) == lib.fvb_paged_attn(None, None) == bad
 
     def append(T=4, D=64, rot=0, dtype=0, Hk=2, B=2, page=16, pages=4, width=2, axes=1, k=16, cu=16, pool=16):
-        return lib.fvb_kv_append(None, 0, 0, 0, None, 0, 0, k, Hk * D, D, k, Hk * D, D, Hk, T, D, rot, 0, dtype, None,
-                                 0, axes, None, None, 1.0, cu, 16, 16, B, width, pages, page, pool, pool,
-                                 page * Hk * D, None)
+        return lib.fvb_kv_append(_lib.KV_APPEND_ARGS(0, 0, 0, 0, 0, 0, 0, k, Hk * D, D, k, Hk * D, D, Hk, T, D, rot, 0,
+                                                     dtype, 0, 0, axes, 0, 0, 1.0, cu, 16, 16, B, width, pages, page,
+                                                     pool, pool, page * Hk * D), None)
 
     for kw in ({"T": -1}, {"D": 300}, {"rot": 2}, {"dtype": 2}, {"Hk": 0}, {"page": 0}, {"pages": -1}, {"width": -1},
-               {"axes": 2}, {"k": None}, {"cu": None}, {"pool": None}, {"B": -1}):
+               {"axes": 2}, {"k": 0}, {"cu": 0}, {"pool": 0}, {"B": -1}):
         assert append(**kw) == bad, kw
     assert append(T=0) == _lib.FVB_OK
 
-    def attn(T=4, B=4, Hq=2, Hk=2, D=64, page=16, pages=4, width=2, max_new=1, scale=0.1, dtype=0, q=16, ws=16, cu=None,
+    def attn(T=4, B=4, Hq=2, Hk=2, D=64, page=16, pages=4, width=2, max_new=1, scale=0.1, dtype=0, q=16, ws=16, cu=0,
              stride=0):
-        return lib.fvb_paged_attn(q, Hq * D + stride, D, 16, 8, 8, 8, 16, 8, 8, 8, 16, width, 16, cu, T, B, Hq, Hk, D,
-                                  pages, page, max_new, 1, scale, dtype, 32, Hq * D, D, ws, None)
+        return lib.fvb_paged_attn(_lib.PAGED_ATTN_ARGS(q, Hq * D + stride, D, 16, 8, 8, 8, 16, 8, 8, 8, 16, width, 16,
+                                                       cu, T, B, Hq, Hk, D, pages, page, max_new, 1, scale, dtype, 32,
+                                                       Hq * D, D, ws), None)
 
     for kw in ({"Hk": 0}, {"Hq": 3}, {"Hq": 0}, {"page": 8}, {"page": 24}, {"page": 0}, {"pages": 0}, {"width": -1},
                {"width": 1 << 28}, {"max_new": 0}, {"scale": 0.0}, {"scale": -1.0}, {"scale": math.inf},
-               {"scale": math.nan}, {"dtype": 2}, {"q": None}, {"q": 24}, {"ws": None}, {"T": 5}, {"B": -1},
+               {"scale": math.nan}, {"dtype": 2}, {"q": 0}, {"q": 24}, {"ws": 0}, {"T": 5}, {"B": -1},
                {"stride": 4}):
         assert attn(**kw) == bad, kw
     assert attn(D=96) == unsupported and attn(D=256) == unsupported
