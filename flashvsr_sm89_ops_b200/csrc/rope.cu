@@ -12,8 +12,11 @@
 // memory, serves every head of q and k.
 //
 // Bound by memory: q and k are read and written once (append: q, k and v, with k and v written
-// to their pages).  A thread keeps one place of a head (one 16-byte vector, or two half a
-// rotation apart) and walks over (token, head) rows with kRopeBatch rows in flight.
+// to their pages).  Measured (B200, cold inputs): 8448 tokens of 12 + 12 heads of 128 in bf16 20.5 us
+// (104 MB at 5.1 TB/s), 16896 tokens appended 51 us (261 MB at 5.1 TB/s), 4099 tokens of 24 + 4 heads
+// of 80 in fp32 12.6 us (73 MB at 5.8 TB/s).  An earlier form that dealt rows of heads to threads
+// spent 63% of its issue slots on indexes (27, 54 and 21 us); one that kept blocks resident and
+// prefetched the next tokens' angles held too many registers to cover latency (34, 74 and 20 us).
 #include "common.cuh"
 
 #include <cuda_fp16.h>
@@ -21,10 +24,10 @@
 namespace fvb {
 namespace rope {
 
-constexpr int kThreads = 256;
-constexpr int kBatch = 4;       // rows in flight a thread
-constexpr int kMaxTokens = 8;   // tokens a block
-constexpr int kMaxDim = kThreads;  // a place of a head is one thread's at the narrowest
+constexpr int kThreads = 512;      // most threads of a block
+constexpr int kManyThreads = 192;  // where there are tokens enough for every SM
+constexpr int kMaxTokens = 32;     // tokens a block
+constexpr int kMaxDim = 256;
 
 struct Part {  // q, k or v: heads of a token, and where they go
   const void* src;
@@ -41,8 +44,8 @@ struct Args {
   int parts, heads;  // heads: of all parts together
   int64_t T;
   int D, rot, tokens;  // tokens: a block's share
-  uint32_t heads_inv;  // ceil(2^32 / heads)
-  int units, turned_units, rows_at_once;
+  int units, turned_units;  // places of a head, those that are turned
+  int lanes, side;          // threads of a token, tokens side by side
   const void* pos;  // NULL: the token's place in its sequence
   int pos64, axes;
   const uint64_t* freq;  // [rot / 2] turns a position, 2^64 to a turn
@@ -102,30 +105,100 @@ struct Elem<__half> {
   __device__ static __half put(float v) { return __float2half_rn(v); }
 };
 
-__device__ __forceinline__ void turn(float& a, float& b, float2 cs) {
-  const float x = a, y = b;
-  a = fmaf(x, cs.x, -(y * cs.y));
-  b = fmaf(y, cs.x, x * cs.y);
+// 16 bytes that are read once (not as read-only data: the output may be the input)
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
-// VEC: 16-byte vectors (strides, pointers, D and the rotated part are multiples of them), else
-// one pair or one untouched channel at a time.
+// two pairs at once: (a, b) -> (a c - b s, b c + a s)
+__device__ __forceinline__ void turn2(float& a0, float& a1, float& b0, float& b1, float c0, float c1,
+                                      float s0, float s1) {
+  const uint64_t a = f2_pack(a0, a1), b = f2_pack(b0, b1), c = f2_pack(c0, c1), s = f2_pack(s0, s1);
+  const uint64_t x = f2_fma(a, c, f2_mul(b, f2_pack(-s0, -s1)));
+  const uint64_t y = f2_fma(b, c, f2_mul(a, s));
+  f2_unpack(x, a0, a1);
+  f2_unpack(y, b0, b1);
+}
+
+// A token's work is `heads * units` places: a 16-byte vector (interleaved, or not turned) or two half
+// a rotation apart (VEC: strides, pointers, D and the rotated part are multiples of them), else one
+// pair or one untouched channel.  A thread keeps its place over the block's tokens, kBatch of them
+// in flight, so that a token costs it two additions of strides; the first ones are on their way
+// while the angles are formed.
 template <typename T, bool HALF, bool VEC>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
   constexpr int V = VEC ? Elem<T>::kV : 1;
-  extern __shared__ float2 cs_all[];  // [tokens][rot / 2] cos, sin
+  constexpr int kBatch = HALF ? 2 : 4;  // tokens in flight a thread: 64 bytes either way
+  extern __shared__ __align__(16) float cs_all[];  // [tokens][cos, sin][rot / 2]
   __shared__ int64_t s_pos[kMaxTokens];
-  __shared__ int64_t s_slot[kMaxTokens];  // offset of the token's row in the pools, -1: none
-  __shared__ int s_live[kMaxTokens];
+  __shared__ int64_t s_slot[kMaxTokens];  // offset of the token's row in the pools, -1: leave it
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int n = (int)min((int64_t)a.tokens, a.T - t0);
   const int half_rot = a.rot >> 1;
+  const int work = a.heads * a.units;
+  // tokens side by side when a token's work is smaller than the block
+  const int lane_token = threadIdx.x / a.lanes, first = threadIdx.x - lane_token * a.lanes;
+  const bool works = lane_token < a.side && first < work;
 
-  if (threadIdx.x < n) {
-    const int64_t t = t0 + threadIdx.x;
-    int64_t slot = -1, place = 0;
-    int live = 1;
-    if (a.cu) {
+  uint4 va[kBatch], vb[kBatch];
+  float fa[kBatch], fb[kBatch];
+  const T* src;
+  T* dst;
+  int64_t src_step, dst_step;
+  int u, ch2, paged;
+  bool two, tr;
+  // the place w of a token: which part, head and channels
+  auto place = [&](int w) {
+    int h = w / a.units;
+    u = w - h * a.units;
+    int i = 0;
+    if (h >= a.part[0].heads) {
+      h -= a.part[0].heads, i = 1;
+      if (a.parts > 2 && h >= a.part[1].heads) h -= a.part[1].heads, i = 2;
+    }
+    const Part& pt = a.part[i];
+    const bool rotates = u < a.turned_units;
+    int ch;
+    if (VEC)
+      ch = HALF ? (rotates ? u * V : a.rot + (u - a.turned_units) * V) : u * V;
+    else
+      ch = rotates ? (HALF ? u : 2 * u) : a.rot + (u - a.turned_units);
+    two = rotates && (HALF || !VEC);
+    ch2 = HALF ? half_rot : 1;  // how far on the second one is
+    tr = rotates && pt.turned;
+    paged = pt.paged;
+    src_step = a.side * pt.src_token;
+    dst_step = pt.paged ? 0 : a.side * pt.dst_token;
+    const int64_t t = t0 + lane_token;
+    src = reinterpret_cast<const T*>(pt.src) + t * pt.src_token + h * pt.src_head + ch;
+    dst = reinterpret_cast<T*>(pt.dst) + (pt.paged ? 0 : t * pt.dst_token) + h * pt.dst_head + ch;
+  };
+  auto load = [&](int tk) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (tk + i * a.side >= n) break;
+      if (VEC) {
+        va[i] = ld_once(src);
+        if (two) vb[i] = ld_once(src + ch2);
+      } else {
+        fa[i] = Elem<T>::get(src[0]);
+        if (two) fb[i] = Elem<T>::get(src[ch2]);
+      }
+      src += src_step;
+    }
+  };
+  if (works) {
+    place(first);
+    load(lane_token);
+  }
+
+  if (a.cu) {
+    if (threadIdx.x < n) {
+      const int64_t t = t0 + threadIdx.x;
       // last sequence that starts at or before t; tokens behind the last sequence are left alone
       int64_t lo = 0, hi = a.B;
       while (lo + 1 < hi) {
@@ -133,20 +206,20 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
         if (a.cu[mid] <= t) lo = mid; else hi = mid;
       }
       const int64_t c0 = a.cu[lo], c1 = a.cu[lo + 1];
-      live = c0 <= t && t < c1;
-      place = (int64_t)a.lens[lo] - (c1 - c0) + (t - c0);
-      if (live && place >= 0) {
-        const int64_t j = place / a.page;
+      const bool live = c0 <= t && t < c1;
+      const int64_t at = (int64_t)a.lens[lo] - (c1 - c0) + (t - c0);
+      int64_t slot = -1;
+      if (live && at >= 0) {
+        const int64_t j = at / a.page;
         const int32_t p = j < a.width ? a.table[lo * a.width + j] : -1;
-        if (p >= 0 && p < a.pages) slot = p * a.page_stride + (place - j * a.page) * a.slot_stride;
+        if (p >= 0 && p < a.pages) slot = p * a.page_stride + (at - j * a.page) * a.slot_stride;
       }
+      s_pos[threadIdx.x] = at;
+      s_slot[threadIdx.x] = live ? slot : -2;  // -1: no place in the pool, -2: no token at all
     }
-    s_pos[threadIdx.x] = place;
-    s_slot[threadIdx.x] = slot;
-    s_live[threadIdx.x] = live;
+    __syncthreads();
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n * half_rot; i += kThreads) {
+  for (int i = threadIdx.x; i < n * half_rot; i += blockDim.x) {
     const int tk = i / half_rot, pr = i - tk * half_rot;
     int64_t p;
     if (a.pos) {
@@ -156,95 +229,72 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
     } else {
       p = s_pos[tk];
     }
-    const int64_t f = (int64_t)((uint64_t)p * a.freq[pr]);  // in [-1/2, 1/2) turns
+    // turns in [-1/2, 1/2), to 2^-32 of one
+    const int32_t f = (int32_t)(((uint64_t)p * a.freq[pr]) >> 32);
     float s, c;
-    sincospif(__ll2float_rn(f) * 1.0842021724855044e-19f /* 2^-63 */, &s, &c);
-    cs_all[i] = make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
+    sincospif((float)f * 4.656612873077393e-10f /* 2^-31 */, &s, &c);
+    float* cs = cs_all + tk * a.rot + pr;
+    cs[0] = c * a.scale;
+    cs[half_rot] = (a.inverse ? -s : s) * a.scale;
   }
   __syncthreads();
+  if (!works) return;
 
-  const int u = threadIdx.x % a.units;  // this thread's place in a head
-  const int r0 = threadIdx.x / a.units;
-  if (r0 >= a.rows_at_once) return;
-  const bool rotates = u < a.turned_units;
-  // first channel of the place; the second of a half-layout pair lies half_rot on
-  int ch;
-  if (VEC)
-    ch = HALF ? (rotates ? u * V : a.rot + (u - a.turned_units) * V) : u * V;
-  else
-    ch = rotates ? (HALF ? u : 2 * u) : a.rot + (u - a.turned_units);
-  const bool two = rotates && (HALF || !VEC);
-  const int ch2 = HALF ? ch + half_rot : ch + 1;
-
-  const int rows = n * a.heads;
-  for (int base = r0; base < rows; base += a.rows_at_once * kBatch) {
-    const T* src[kBatch];
-    T* dst[kBatch];
-    int tok[kBatch];
-    bool turned[kBatch];
-    uint4 va[kBatch], vb[kBatch];
-    float fa[kBatch], fb[kBatch];
+  for (int w = first; w < work; w += a.lanes) {
+    if (w != first) place(w);
+    for (int tk = lane_token; tk < n; tk += a.side * kBatch) {
+      if (w != first || tk != lane_token) load(tk);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int r = base + i * a.rows_at_once;
-      dst[i] = nullptr;
-      if (r >= rows) continue;
-      const int tk = a.heads > 1 ? (int)__umulhi((uint32_t)r, a.heads_inv) : r;
-      int h = r - tk * a.heads;
-      tok[i] = tk;
-      if (!s_live[tk]) continue;
-      const Part* pt = &a.part[0];
-      if (h >= pt->heads) {
-        h -= pt->heads;
-        ++pt;
-        if (a.parts > 2 && h >= pt->heads) h -= pt->heads, ++pt;
-      }
-      const int64_t t = t0 + tk;
-      if (pt->paged) {
-        if (s_slot[tk] < 0) continue;
-        dst[i] = reinterpret_cast<T*>(pt->dst) + s_slot[tk] + h * pt->dst_head;
-      } else {
-        dst[i] = reinterpret_cast<T*>(pt->dst) + t * pt->dst_token + h * pt->dst_head;
-      }
-      src[i] = reinterpret_cast<const T*>(pt->src) + t * pt->src_token + h * pt->src_head;
-      turned[i] = pt->turned != 0;
-      if (VEC) {
-        va[i] = *reinterpret_cast<const uint4*>(src[i] + ch);
-        if (two) vb[i] = *reinterpret_cast<const uint4*>(src[i] + ch2);
-      } else {
-        fa[i] = Elem<T>::get(src[i][ch]);
-        if (two) fb[i] = Elem<T>::get(src[i][ch2]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (!dst[i]) continue;
-      const float2* cs = cs_all + tok[i] * half_rot;
-      const bool tr = rotates && turned[i];
-      if (VEC) {
-        if (tr) {
-          if (HALF) {
-            float x[V], y[V];
-            Elem<T>::unpack(va[i], x);
-            Elem<T>::unpack(vb[i], y);
-#pragma unroll
-            for (int j = 0; j < V; ++j) turn(x[j], y[j], cs[u * V + j]);
-            va[i] = Elem<T>::pack(x);
-            vb[i] = Elem<T>::pack(y);
-          } else {
+      for (int i = 0; i < kBatch; ++i) {
+        const int k = tk + i * a.side;
+        if (k >= n) break;
+        T* d = dst;
+        dst += dst_step;
+        if (a.cu) {
+          const int64_t slot = s_slot[k];
+          if (slot < (paged ? 0 : -1)) continue;
+          if (paged) d += slot;
+        }
+        if (VEC) {
+          if (tr) {
+            const float* cs = cs_all + k * a.rot;
             float x[V];
             Elem<T>::unpack(va[i], x);
+            if (HALF) {
+              float y[V];
+              Elem<T>::unpack(vb[i], y);
+              cs += u * V;
 #pragma unroll
-            for (int j = 0; j < V / 2; ++j) turn(x[2 * j], x[2 * j + 1], cs[u * (V / 2) + j]);
+              for (int j = 0; j < V; j += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(cs + j);
+                const float4 s = *reinterpret_cast<const float4*>(cs + half_rot + j);
+                turn2(x[j], x[j + 1], y[j], y[j + 1], c.x, c.y, s.x, s.y);
+                turn2(x[j + 2], x[j + 3], y[j + 2], y[j + 3], c.z, c.w, s.z, s.w);
+              }
+              vb[i] = Elem<T>::pack(y);
+            } else {
+              cs += u * (V / 2);
+#pragma unroll
+              for (int j = 0; j < V; j += 4) {
+                const float2 c = *reinterpret_cast<const float2*>(cs + j / 2);
+                const float2 s = *reinterpret_cast<const float2*>(cs + half_rot + j / 2);
+                turn2(x[j], x[j + 2], x[j + 1], x[j + 3], c.x, c.y, s.x, s.y);
+              }
+            }
             va[i] = Elem<T>::pack(x);
           }
+          *reinterpret_cast<uint4*>(d) = va[i];
+          if (two) *reinterpret_cast<uint4*>(d + ch2) = vb[i];
+        } else {
+          if (tr) {
+            const float c = cs_all[k * a.rot + u], s = cs_all[k * a.rot + half_rot + u];
+            const float x = fa[i], y = fb[i];
+            fa[i] = fmaf(x, c, -(y * s));
+            fb[i] = fmaf(y, c, x * s);
+          }
+          d[0] = Elem<T>::put(fa[i]);
+          if (two) d[ch2] = Elem<T>::put(fb[i]);
         }
-        *reinterpret_cast<uint4*>(dst[i] + ch) = va[i];
-        if (two) *reinterpret_cast<uint4*>(dst[i] + ch2) = vb[i];
-      } else {
-        if (tr) turn(fa[i], fb[i], cs[u]);
-        dst[i][ch] = Elem<T>::put(fa[i]);
-        if (two) dst[i][ch2] = Elem<T>::put(fb[i]);
       }
     }
   }
@@ -268,19 +318,25 @@ int launch(Args& a, bool half, cudaStream_t stream, const char* what) {
   // is not turned, a vector or a channel each
   a.turned_units = (half || !vec) ? a.rot / (2 * v) : a.rot / v;
   a.units = a.turned_units + (a.D - a.rot) / v;
-  a.rows_at_once = kThreads / a.units;
-  // row / heads as a multiplication: rows < 8 * 4096, so the reciprocal's excess (< heads) cannot
-  // carry (one head needs no division, and its reciprocal would not fit)
-  a.heads_inv = a.heads > 1 ? (uint32_t)(((1ull << 32) + a.heads - 1) / a.heads) : 0;
-  // one token a block until that fills the machine several times over, then as many as keep it full
+  // Threads: as many as a token has places, in equal rounds, or several tokens side by side.  Up to
+  // 512 of them where a block's latency is what counts (one token of 12 + 12 heads 2.7 us, with
+  // 256 3.3), 256 where the blocks of an SM cover each other's (4099 tokens of 24 + 4 heads
+  // of 80 in fp32 12.6 us, with 256 15).
+  const int most = a.T < 2 * (int64_t)sm_count() ? kThreads : kManyThreads;
+  const int work = a.heads * a.units;
+  const int rounds = (work + most - 1) / most;
+  a.lanes = (work + rounds - 1) / rounds;
+  a.side = most / a.lanes > 1 ? most / a.lanes : 1;
+  if (a.side > kMaxTokens / 4) a.side = kMaxTokens / 4;
+  const int threads = (a.lanes * a.side + 31) / 32 * 32;
+  // one token a block (a side) until that fills the machine several times over, then more
   const int64_t want = (int64_t)sm_count() * 8;
-  a.tokens = (int)(a.T / want);
-  if (a.tokens < 1) a.tokens = 1;
-  if (a.tokens > kMaxTokens) a.tokens = kMaxTokens;
+  int64_t tokens = (a.T + want - 1) / want;
+  tokens = (tokens + a.side - 1) / a.side * a.side;
+  a.tokens = (int)(tokens < kMaxTokens ? tokens : kMaxTokens / a.side * a.side);
   const int64_t grid = (a.T + a.tokens - 1) / a.tokens;
-  FVB_REQUIRE(grid < (1ll << 31), "%s: too many tokens", what);
-  const size_t smem = (size_t)a.tokens * (a.rot / 2) * sizeof(float2);
-  const dim3 g((unsigned)grid), b(kThreads);
+  const size_t smem = (size_t)a.tokens * a.rot * sizeof(float);
+  const dim3 g((unsigned)grid), b((unsigned)threads);
   if (half) {
     if (vec) rope_kernel<T, true, true><<<g, b, smem, stream>>>(a);
     else rope_kernel<T, true, false><<<g, b, smem, stream>>>(a);
