@@ -38,6 +38,7 @@ struct Args {
   const int32_t *table, *lens, *cu;  // cu NULL: one token a sequence
   int64_t T, width, pages;
   int B, Hk, g, page, causal, ctas;
+  int rows;  // packed rows of an item's tile
   float scale_log2;
   float* part;    // [2 ctas][rows][D]: O of an item begun before the CTA, of one begun in it
   float* part_ml; // [2 ctas][rows][2]
@@ -86,14 +87,14 @@ struct Segment {  // key tiles [t0, t1) of an item's [0, tiles)
 
 // Walks over a CTA's segments.  Items with no key count as one tile, so that their rows (zeros)
 // have an owner.
-template <int R, int KT>
+template <int KT>
 struct Walk {
   int64_t unit, end;
   int b, h, rt, t0;
   Seq s;
 
   __device__ int item_tiles(const Args& a) const {
-    const int t = tiles_of<KT>(a, s, rt * R, rt * R + R);
+    const int t = tiles_of<KT>(a, s, rt * a.rows, rt * a.rows + a.rows);
     return t > 0 ? t : 1;
   }
   __device__ bool next(const Args& a, Segment& g) {
@@ -104,7 +105,7 @@ struct Walk {
     unit += g.t1 - t0;
     t0 = 0;
     if (unit < end) {
-      if (++rt * R >= s.n * a.g) {
+      if (++rt * a.rows >= s.n * a.g) {
         rt = 0;
         if (++h == a.Hk) {
           h = 0;
@@ -117,9 +118,9 @@ struct Walk {
 };
 
 // units of one key head of a sequence
-template <int R, int KT>
+template <int KT>
 __device__ int64_t head_units(const Args& a, const Seq& s) {
-  const int rows = s.n * a.g;
+  const int rows = s.n * a.g, R = a.rows;
   if (!a.causal) {
     const int64_t t = ((int64_t)s.len + KT - 1) / KT;
     return (int64_t)((rows + R - 1) / R) * (t > 0 ? t : 1);
@@ -138,13 +139,13 @@ struct Found {
 };
 
 // Every thread of the block; finds the walk of this CTA.  Returns the tiles a CTA takes.
-template <int R, int KT, int kThreads, int kLeast>
-__device__ int64_t start_walk(const Args& a, Walk<R, KT>& w, Found* sh, int64_t* sums) {
+template <int KT, int kThreads, int kLeast>
+__device__ int64_t start_walk(const Args& a, Walk<KT>& w, Found* sh, int64_t* sums) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t first = 0, mine = 0;
   for (int64_t b = threadIdx.x; b < a.B; b += kThreads) {
-    const int64_t u = head_units<R, KT>(a, get_seq(a, (int)b)) * a.Hk;
+    const int64_t u = head_units<KT>(a, get_seq(a, (int)b)) * a.Hk;
     if (b < kThreads) first = u;
     mine += u;
   }
@@ -165,7 +166,7 @@ __device__ int64_t start_walk(const Args& a, Walk<R, KT>& w, Found* sh, int64_t*
   for (int64_t at = 0; at < a.B; at += kThreads) {
     const int64_t b = at + threadIdx.x;
     int64_t u = at == 0 ? first : 0;
-    if (at && b < a.B) u = head_units<R, KT>(a, get_seq(a, (int)b)) * a.Hk;
+    if (at && b < a.B) u = head_units<KT>(a, get_seq(a, (int)b)) * a.Hk;
     int64_t x = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -188,7 +189,7 @@ __device__ int64_t start_walk(const Args& a, Walk<R, KT>& w, Found* sh, int64_t*
   w.b = sh->b;
   int64_t rem = sh->rem;
   w.s = get_seq(a, w.b);
-  const int64_t hu = head_units<R, KT>(a, w.s);
+  const int64_t hu = head_units<KT>(a, w.s);
   w.h = (int)(rem / hu);
   rem -= w.h * hu;
   w.rt = 0;
@@ -204,8 +205,8 @@ __device__ int64_t start_walk(const Args& a, Walk<R, KT>& w, Found* sh, int64_t*
 }
 
 // One thread: the record of an item that begins in this CTA and ends in another.
-template <int R, int KT>
-__device__ void write_rec(const Args& a, Walk<R, KT> w, int64_t per) {
+template <int KT>
+__device__ void write_rec(const Args& a, Walk<KT> w, int64_t per) {
   int32_t* r = a.rec + (int64_t)blockIdx.x * 8;
   Segment g;
   int valid = 0;
@@ -219,6 +220,11 @@ __device__ void write_rec(const Args& a, Walk<R, KT> w, int64_t per) {
     at += g.t1 - g.t0;
   }
   r[0] = valid;
+}
+
+// Lets the merge kernel be set up while this one runs.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 template <typename T>
@@ -306,8 +312,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
   __shared__ float s_ml[4][kRows][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
-  Walk<kRows, kKeys> w;
-  const int64_t per = start_walk<kRows, kKeys, kThreads, kLeast>(a, w, &found, sums);
+  Walk<kKeys> w;
+  const int64_t per = start_walk<kKeys, kThreads, kLeast>(a, w, &found, sums);
+  let_next_start();
   if (threadIdx.x == 0) write_rec(a, w, per);
 
   uint8_t* ring = smem + warp * (S::kStages * S::kStage);
@@ -644,8 +651,8 @@ constexpr int kDescs = 4;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                 const int box, const Args a) {
+    chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const int box, const Args a) {
   using S = Shape<D>;
   constexpr int kSlots = S::kSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -655,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* const sK = base + 2 * S::kTile;
   uint8_t* const sV = sK + kSlots * S::kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kSlots * S::kTile);
-  enum { Q_FULL = 0, S_FULL, S_FREE, P_FULL, PV_DONE, DRAIN, kNB };
+  enum { Q_FULL = 0, Q_EMPTY, S_FULL, S_FREE, P_FULL, PV_DONE, DRAIN, kNB };
   auto BAR = [&](int x, int i) { return bars + x * kNB + i; };
   uint64_t* const k_full = bars + 2 * kNB;
   uint64_t* const k_empty = k_full + kSlots;
@@ -678,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     s_copied[0] = s_copied[1] = 0;
     for (int x = 0; x < 2; ++x)
       for (int b = 0; b < kNB; ++b)
-        mbar_init(BAR(x, b), (b == Q_FULL || b == S_FREE || b == P_FULL) ? 4u : 1u);
+        mbar_init(BAR(x, b), (b == S_FREE || b == P_FULL) ? 4u : 1u);
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(k_full + i, 1);
       mbar_init(v_full + i, 1);
@@ -695,8 +702,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  Walk<kRows, kKeys> w;
-  const int64_t per = start_walk<kRows, kKeys, kThreads, kLeast>(a, w, &found, sums);
+  Walk<kKeys> w;
+  const int64_t per = start_walk<kKeys, kThreads, kLeast>(a, w, &found, sums);
+  let_next_start();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -711,12 +719,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
+      prefetch_tmap(&tmQ);
       prefetch_tmap(&tmK);
       prefetch_tmap(&tmV);
     }
     const int boxes = kKeys / box;
+    const int half_rows = a.rows >> 1;
     bool ok = true;
-    int64_t nk = 0, nv = 0;  // tiles issued
+    int64_t nk = 0, nv = 0;       // tiles issued
+    uint32_t nq[2] = {0, 0};
     // a tile is `boxes` boxes of `box` rows, each inside one page; lane i loads box i
     auto tile = [&](uint8_t* ring, const CUtensorMap& tm, uint64_t* full, uint64_t* empty,
                     int64_t& count, int j) {
@@ -743,6 +754,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the MMA threads take K(0) K(1) V(0) K(2) V(1) ...
       for (int j = 0; j <= all && all > 0 && ok; ++j) {
         if (j < all) ok = tile(sK, tmK, k_full, k_empty, nk, j);
+        if (j == 0) {
+          // Q of both halves: boxes of a token's g heads for 128 / g tokens (rows past the
+          // sequence's end are other tokens', or zeros: nobody stores them)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || DESC().cnt[x] == 0) continue;
+            if (!__all_sync(0xffffffffu, mbar_wait(BAR(x, Q_EMPTY), (nq[x] & 1u) ^ 1u, 0x912u))) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) {
+              const Desc& g = DESC();
+              mbar_arrive_expect_tx(BAR(x, Q_FULL), (uint32_t)(half_rows * D * 2));
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c)
+                tma_load_4d(sQ + x * S::kTile + c * kAtom, &tmQ, BAR(x, Q_FULL), c * 64, g.h * a.g,
+                            (int)g.t0 + (g.row0 + x * half_rows) / a.g, 0);
+            }
+            __syncwarp();
+            ++nq[x];
+          }
+        }
         if (ok && j >= 1) ok = tile(sV, tmV, v_full, v_empty, nv, j - 1);
       }
       __syncwarp();
@@ -751,6 +784,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // no load may still be writing shared memory when the CTA exits
     if (lane == 0) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (nq[x]) mbar_wait(BAR(x, Q_FULL), (nq[x] - 1) & 1u, 0x902u);
       for (int64_t i = nk > kSlots ? nk - kSlots : 0; i < nk; ++i)
         mbar_wait(k_full + i % kSlots, (uint32_t)(i / kSlots) & 1u, 0x902u);
       for (int64_t i = nv > kSlots ? nv - kSlots : 0; i < nv; ++i)
@@ -759,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 9) {
     // ------------------------------------------------------------ segments
     if (lane == 0) {
-      const Walk<kRows, kKeys> start = w;
+      const Walk<kKeys> start = w;
       Segment g;
       for (bool more = true; more; ++seg) {
         more = w.next(a, g);
@@ -767,10 +803,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         Desc& d = descs[seg % kDescs];
         d.more = more;
         if (more) {
-          const int row0 = g.rt * kRows;
+          const int half_rows = a.rows >> 1, row0 = g.rt * a.rows;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int tl = tiles_of<kKeys>(a, g.s, row0 + x * 128, row0 + x * 128 + 128);
+            const int tl = tiles_of<kKeys>(a, g.s, row0 + x * half_rows, row0 + (x + 1) * half_rows);
             const int e = tl < g.t1 ? tl : g.t1;
             d.cnt[x] = e > g.t0 ? e - g.t0 : 0;
           }
@@ -844,6 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_commit(BAR(x, S_FULL));
           tc_commit(k_empty + ks);
+          if (j == cm - 1) tc_commit(BAR(x, Q_EMPTY));
         }
         __syncwarp();
         step(ks, kph);
@@ -900,6 +937,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tP = tmem + kColP + (uint32_t)(x * 64) + lane_addr;
     const uint32_t tO = tmem + kColO + (uint32_t)(x * 128) + lane_addr;
     const float c = a.scale_log2;
+    const int half_rows = a.rows >> 1;
     bool ok = true;
     uint32_t kv = 0, mine = 0;
     while (ok && __all_sync(0xffffffffu, next_segment())) {
@@ -907,27 +945,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       int lim = 0;  // keys that this row sees
       if (cnt > 0) {
         const Desc& g = DESC();
-        const int pr = g.row0 + x * 128 + row;
-        const bool row_ok = pr < g.n * a.g;
-        const int tok = row_ok ? pr / a.g : 0;
-        const int head = g.h * a.g + (row_ok ? pr - tok * a.g : 0);
-        if (row_ok) {
-          const int v = a.causal ? min(g.off + tok + 1, len) : len;
+        const int pr = g.row0 + x * half_rows + row;
+        if (row < half_rows && pr < g.n * a.g) {
+          const int v = a.causal ? min(g.off + pr / a.g + 1, len) : len;
           lim = v > 0 ? v : 0;
         }
-        // this row of Q, swizzled as TMA would (the MMAs of the last segment are done)
-        const uint4* src = reinterpret_cast<const uint4*>(
-            reinterpret_cast<const T*>(a.q) + (g.t0 + tok) * a.q_token + head * a.q_head);
-        uint8_t* dst = sQ + x * S::kTile + row * 128;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (row_ok) v = __ldg(src + i);
-          *reinterpret_cast<uint4*>(dst + (i >> 3) * kAtom + (((i & 7) ^ (row & 7)) << 4)) = v;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(x, Q_FULL));
       }
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < cnt; ++j) {
@@ -1026,11 +1048,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (have_o) tc_fence_after();
       else if (cnt > 0) ok = false;
       const Desc& g = DESC();
-      const int pr = g.row0 + x * 128 + row;
-      const bool row_ok = pr < g.n * a.g;
+      const int pr = g.row0 + x * half_rows + row;
+      const bool row_ok = row < half_rows && pr < g.n * a.g;
       const bool whole = g.whole;
       const float inv = (have_o && l > 0.f) ? 1.0f / l : 0.f;
-      const int64_t prow = ((int64_t)blockIdx.x * 2 + (key_t0 == 0)) * kRows + x * 128 + row;
+      const int64_t prow = ((int64_t)blockIdx.x * 2 + (key_t0 == 0)) * kRows + x * half_rows + row;
       const int tok = pr / a.g;
       uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (g.t0 + tok) * a.o_token +
                                             (int64_t)(g.h * a.g + pr - tok * a.g) * a.o_head);
@@ -1090,66 +1112,92 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace chunk
 
 // ===========================================================================
-// Joins the parts of an item that CTA boundaries cut, in their order.  WPR warps a row, each
-// taking every WPR-th part.
+// Joins the parts of an item that CTA boundaries cut, in their order.  D / 8 lanes take a row, or
+// with few rows a part of it (ROWS false: a block a row, its groups every G-th part).  Launched
+// while the kernel before it still runs, it waits for that one's end before it reads anything.
 // ===========================================================================
-template <typename T, int D, int R, int WPR>
+template <typename T, int D, int R, bool ROWS>
 __global__ void __launch_bounds__(128) merge_kernel(const Args a) {
-  constexpr int kE = D / 32;  // channels a lane
-  __shared__ float s_o[WPR > 1 ? WPR : 1][D];
-  __shared__ float s_l[WPR > 1 ? WPR : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kLanes = D / 8, G = 128 / kLanes;
+  __shared__ float s_o[ROWS ? 1 : G][D];
+  __shared__ float s_l[ROWS ? 1 : G];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int gl = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int c0 = blockIdx.x;
-  const int32_t* r = a.rec + (int64_t)c0 * 8;
-  if (!r[0]) return;
-  const int sub = WPR > 1 ? warp : 0;
-  const int row = WPR > 1 ? blockIdx.y : blockIdx.y * 4 + warp;
-  const Seq s = get_seq(a, r[1]);
-  const int64_t pr = (int64_t)r[3] * R + row;
-  if (pr >= (int64_t)s.n * a.g) return;  // with WPR > 1 the same for the whole block
-  const int parts = r[4] - c0 + 1;
+  const int4 rec = *reinterpret_cast<const int4*>(a.rec + (int64_t)c0 * 8);  // valid, b, h, rt
+  if (!rec.x) return;
+  const int parts = a.rec[(int64_t)c0 * 8 + 4] - c0 + 1;
+  const int row = ROWS ? blockIdx.y * G + group : blockIdx.y;
+  const Seq s = get_seq(a, rec.y);
+  const int64_t pr = (int64_t)rec.w * a.rows + row;
+  const bool live = row < a.rows && pr < (int64_t)s.n * a.g;
+  if (!ROWS && !live) return;  // the whole block
   auto slot = [&](int p) { return ((int64_t)(c0 + p) * 2 + (p == 0)) * R + row; };
   float mm = -INFINITY;
-  for (int p = lane; p < parts; p += 32) mm = fmaxf(mm, a.part_ml[slot(p) * 2]);
-  mm = warp_max(mm);
-  float acc[kE], l = 0.f;
+  if (live)
+    for (int p = ROWS ? gl : threadIdx.x & 31; p < parts; p += ROWS ? kLanes : 32)
+      mm = fmaxf(mm, a.part_ml[slot(p) * 2]);
 #pragma unroll
-  for (int i = 0; i < kE; ++i) acc[i] = 0.f;
-  for (int p = sub; p < parts; p += WPR) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(p) * 2);
-    if (ml.x == -INFINITY) continue;
-    const float f = ex2_approx(ml.x - mm);
-    const float* o = a.part + slot(p) * D + lane * kE;
+  for (int o = (ROWS ? kLanes : 32) / 2; o > 0; o >>= 1)
+    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  float acc[8], l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kE; ++i) acc[i] = fmaf(f, o[i], acc[i]);
-    l = fmaf(f, ml.y, l);
-  }
-  if (WPR > 1) {
-#pragma unroll
-    for (int i = 0; i < kE; ++i) s_o[sub][lane * kE + i] = acc[i];
-    if (lane == 0) s_l[sub] = l;
-    __syncthreads();
-    if (sub) return;
-#pragma unroll
-    for (int q = 1; q < WPR; ++q) {
-      l += s_l[q];
-#pragma unroll
-      for (int i = 0; i < kE; ++i) acc[i] += s_o[q][lane * kE + i];
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  if (live) {
+#pragma unroll 2
+    for (int p = ROWS ? 0 : group; p < parts; p += ROWS ? 1 : G) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(p) * 2);
+      if (ml.x == -INFINITY) continue;
+      const float f = ex2_approx(ml.x - mm);
+      const float4* o = reinterpret_cast<const float4*>(a.part + slot(p) * D + gl * 8);
+      const float4 x = o[0], y = o[1];
+      acc[0] = fmaf(f, x.x, acc[0]), acc[1] = fmaf(f, x.y, acc[1]);
+      acc[2] = fmaf(f, x.z, acc[2]), acc[3] = fmaf(f, x.w, acc[3]);
+      acc[4] = fmaf(f, y.x, acc[4]), acc[5] = fmaf(f, y.y, acc[5]);
+      acc[6] = fmaf(f, y.z, acc[6]), acc[7] = fmaf(f, y.w, acc[7]);
+      l = fmaf(f, ml.y, l);
     }
   }
+  if (!ROWS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_o[group][gl * 8 + i] = acc[i];
+    if (gl == 0) s_l[group] = l;
+    __syncthreads();
+    if (group) return;
+    for (int q = 1; q < G && q < parts; ++q) {
+      l += s_l[q];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += s_o[q][gl * 8 + i];
+    }
+  }
+  if (!live) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int64_t i = pr / a.g;
   T* dst = reinterpret_cast<T*>(a.out) + (s.t0 + i) * a.o_token +
-           ((int64_t)r[2] * a.g + pr - i * a.g) * a.o_head + lane * kE;
-#pragma unroll
-  for (int e = 0; e < kE; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + e) = Pair<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+           ((int64_t)rec.z * a.g + pr - i * a.g) * a.o_head + gl * 8;
+  *reinterpret_cast<uint4*>(dst) =
+      make_uint4(Pair<T>::pack(acc[0] * inv, acc[1] * inv), Pair<T>::pack(acc[2] * inv, acc[3] * inv),
+                 Pair<T>::pack(acc[4] * inv, acc[5] * inv), Pair<T>::pack(acc[6] * inv, acc[7] * inv));
 }
 
 // Whether the rows of the longest sequence fit the few-rows kernel.  Measured at 48 sequences of
 // about 9 k keys, 32 / 8 heads of 128: see the figures at the entry point.
 inline bool few_rows(int64_t max_new, int64_t g) { return max_new * g <= dec::kRows; }
 inline int ctas_of(bool few) { return sm_count() * (few ? 2 : 1); }
+
+int launch_merge(void (*kernel)(Args), dim3 grid, const Args& a, cudaStream_t stream) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(128);
+  c.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &early;
+  c.numAttrs = 1;
+  FVB_CUDA_TRY(cudaLaunchKernelEx(&c, kernel, a), "fvb_paged_attn merge launch");
+  return FVB_OK;
+}
 
 template <typename T, int D>
 int launch(Args& a, bool few, cudaStream_t stream) {
@@ -1170,13 +1218,12 @@ int launch(Args& a, bool few, cudaStream_t stream) {
     dec::decode_kernel<T, D><<<a.ctas, dec::kThreads, dec::kRing, stream>>>(a);
     int rc = check_launch("fvb_paged_attn");
     if (rc) return rc;
-    merge_kernel<T, D, dec::kRows, 4><<<dim3(a.ctas, dec::kRows), 128, 0, stream>>>(a);
-    return check_launch("fvb_paged_attn");
+    return launch_merge(merge_kernel<T, D, dec::kRows, false>, dim3(a.ctas, dec::kRows), a, stream);
   }
   // rows of a TMA box: a power of two that divides the page, at most a tile
   int box = 16;
   while (box < chunk::kKeys && a.page % (2 * box) == 0) box *= 2;
-  CUtensorMap tk, tv;
+  CUtensorMap tq, tk, tv;
   const CUtensorMapDataType dt = Pair<T>::kFmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t dims[4] = {(uint64_t)D, (uint64_t)a.Hk, (uint64_t)a.page, (uint64_t)a.pages};
@@ -1187,11 +1234,16 @@ int launch(Args& a, bool few, cudaStream_t stream) {
   if (rc) return rc;
   rc = make_tmap_4d(&tv, a.v, dt, dims, sv, bx);
   if (rc) return rc;
-  chunk::chunk_kernel<T, D><<<a.ctas, chunk::kThreads, chunk::Shape<D>::kSmem, stream>>>(tk, tv, box, a);
+  const uint64_t dq[4] = {(uint64_t)D, (uint64_t)a.Hk * a.g, (uint64_t)a.T, 1};
+  const uint64_t sq[3] = {(uint64_t)a.q_head * 2, (uint64_t)a.q_token * 2, (uint64_t)a.q_token * 2};
+  const uint32_t bq[4] = {64, (uint32_t)a.g, (uint32_t)(128 / a.g), 1};
+  rc = make_tmap_4d(&tq, a.q, dt, dq, sq, bq);
+  if (rc) return rc;
+  chunk::chunk_kernel<T, D><<<a.ctas, chunk::kThreads, chunk::Shape<D>::kSmem, stream>>>(tq, tk, tv, box, a);
   rc = check_launch("fvb_paged_attn");
   if (rc) return rc;
-  merge_kernel<T, D, chunk::kRows, 1><<<dim3(a.ctas, chunk::kRows / 4), 128, 0, stream>>>(a);
-  return check_launch("fvb_paged_attn");
+  return launch_merge(merge_kernel<T, D, chunk::kRows, true>, dim3(a.ctas, chunk::kRows * (D / 8) / 128), a,
+                      stream);
 }
 
 struct Workspace {
@@ -1243,6 +1295,8 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
                p->v_head | p->o_token | p->o_head) % 8 == 0,
               "fvb_paged_attn: strides must be multiples of 8 elements");
   const bool few = pattn::few_rows(p->max_new, p->Hq / p->Hk);
+  if (!few && p->Hq / p->Hk > 128)
+    return fail(FVB_ERR_UNSUPPORTED, "fvb_paged_attn: more than 128 query heads on a key head");
   const pattn::Workspace w = pattn::workspace(few, p->D);
   char* const ws = (char*)p->workspace;
   pattn::Args a = {};
@@ -1257,6 +1311,8 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
   a.B = (int)p->B, a.Hk = (int)p->Hk, a.g = (int)(p->Hq / p->Hk), a.page = (int)p->page;
   a.causal = p->causal != 0;
   a.ctas = pattn::ctas_of(few);
+  // many rows: halves of whole tokens
+  a.rows = few ? pattn::dec::kRows : 2 * (128 / a.g) * a.g;
   a.scale_log2 = (float)(p->scale * 1.4426950408889634);
   a.part = (float*)(ws + w.part);
   a.part_ml = (float*)(ws + w.ml);
