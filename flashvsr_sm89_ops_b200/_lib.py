@@ -103,7 +103,7 @@ _SIGS = {
     "fvb_pages_reserve": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "fvb_pages_fork": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64,
                               _i64, _i64, _i64, _vp, _vp]),
-    "fvb_pages_release": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "fvb_pages_release": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "fvb_pages_compact": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
                                  _i64, _vp, _vp]),
     "fvb_paged_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),

@@ -38,7 +38,7 @@ struct Args {
   const int32_t *table, *lens, *cu;  // cu NULL: one token a sequence
   int64_t T, width, pages;
   int B, Hk, g, page, causal, ctas;
-  int rows;  // packed rows of an item's tile
+  int rows, tokens;  // packed rows of an item's tile: whole tokens
   float scale_log2;
   float* part;    // [2 ctas][rows][D]: O of an item begun before the CTA, of one begun in it
   float* part_ml; // [2 ctas][rows][2]
@@ -64,20 +64,18 @@ __device__ __forceinline__ Seq get_seq(const Args& a, int b) {
   return s;
 }
 
-// keys that token i of the sequence sees
-__device__ __forceinline__ int sees(const Args& a, const Seq& s, int i) {
+// keys that the sequence's first `i` new tokens see
+__device__ __forceinline__ int seen_by(const Args& a, const Seq& s, int i) {
   if (!a.causal) return s.len;
-  const int v = s.off + i + 1;
+  const int v = s.off + i;
   return v < 0 ? 0 : (v < s.len ? v : s.len);
 }
 
-// key tiles of packed rows [r0, r1): 0 if there are no such rows
+// key tiles of tokens [i0, i1): 0 if there are no such tokens
 template <int KT>
-__device__ __forceinline__ int tiles_of(const Args& a, const Seq& s, int r0, int r1) {
-  const int rows = s.n * a.g;  // below 2^31: checked at the entry
-  if (r0 >= rows) return 0;
-  if (r1 > rows) r1 = rows;
-  return (int)(((uint32_t)sees(a, s, (r1 - 1) / a.g) + KT - 1) / KT);
+__device__ __forceinline__ int tiles_of(const Args& a, const Seq& s, int i0, int i1) {
+  if (i0 >= s.n) return 0;
+  return (int)(((uint32_t)seen_by(a, s, i1 < s.n ? i1 : s.n) + KT - 1) / KT);
 }
 
 struct Segment {  // key tiles [t0, t1) of an item's [0, tiles)
@@ -94,7 +92,7 @@ struct Walk {
   Seq s;
 
   __device__ int item_tiles(const Args& a) const {
-    const int t = tiles_of<KT>(a, s, rt * a.rows, rt * a.rows + a.rows);
+    const int t = tiles_of<KT>(a, s, rt * a.tokens, (rt + 1) * a.tokens);
     return t > 0 ? t : 1;
   }
   __device__ bool next(const Args& a, Segment& g) {
@@ -105,7 +103,7 @@ struct Walk {
     unit += g.t1 - t0;
     t0 = 0;
     if (unit < end) {
-      if (++rt * a.rows >= s.n * a.g) {
+      if (++rt * a.tokens >= s.n) {
         rt = 0;
         if (++h == a.Hk) {
           h = 0;
@@ -120,14 +118,14 @@ struct Walk {
 // units of one key head of a sequence
 template <int KT>
 __device__ int64_t head_units(const Args& a, const Seq& s) {
-  const int rows = s.n * a.g, R = a.rows;
+  const int tk = a.tokens;
   if (!a.causal) {
     const int64_t t = ((int64_t)s.len + KT - 1) / KT;
-    return (int64_t)((rows + R - 1) / R) * (t > 0 ? t : 1);
+    return (int64_t)((s.n + tk - 1) / tk) * (t > 0 ? t : 1);
   }
   int64_t u = 0;
-  for (int r = 0; r < rows; r += R) {
-    const int t = tiles_of<KT>(a, s, r, r + R);
+  for (int i = 0; i < s.n; i += tk) {
+    const int t = tiles_of<KT>(a, s, i, i + tk);
     u += t > 0 ? t : 1;
   }
   return u;
@@ -325,9 +323,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
 
   Segment g;
   while (w.next(a, g)) {
-    const int row0 = g.rt * kRows;
+    const int row0 = g.rt * a.rows;
     const int left = g.s.n * a.g - row0;
-    const int rows = left < kRows ? left : kRows;
+    const int rows = left < a.rows ? left : a.rows;
     // Q: fragments of the 16 x D tile
     uint32_t qf[D / 16][4];
     int lim[2];
@@ -339,14 +337,14 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
       const int i = pr / a.g;
       const T* qp = reinterpret_cast<const T*>(a.q) + (g.s.t0 + i) * a.q_token +
                     (int64_t)(g.h * a.g + pr - i * a.g) * a.q_head + qcol;
-      lim[hh] = ok ? sees(a, g.s, i) : 0;
+      lim[hh] = ok ? seen_by(a, g.s, i + 1) : 0;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         qf[kk][hh] = ok ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
         qf[kk][hh + 2] = ok ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
       }
     }
-    const int vis = sees(a, g.s, (row0 + rows - 1) / a.g);  // of the tile's last row
+    const int vis = seen_by(a, g.s, min(g.s.n, (g.rt + 1) * a.tokens));  // by the tile's last token
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -541,10 +539,10 @@ template <int D>
 struct Shape {
   static constexpr int kTile = D * 256;  // bytes of 128 rows
   static constexpr int kSlots = D == 128 ? 2 : 4;  // of K and of V
-  // Exponentials on the FMA pipe: a quarter of them takes the largest case (8448 over 33792 keys, D
-  // 128) from 2.12 to 1.95 million clocks and from 1390 to 1360 us (1620 to 1587 under a lasting
-  // load: the clock gives way); an eighth or three eighths gained less.
-  static constexpr uint32_t kFma = D == 128 ? 0x22u : 0u;
+  // Exponentials on the FMA pipe, pairs of each eight.  8448 over 33792 keys, D 128: a quarter takes
+  // 2.12 to 1.95 million clocks and 1390 to 1360 us (the clock gives way to the load); other shares
+  // gained less.  Ragged chunks of D 64: none 64.8 us, an eighth 62.1, a quarter 62.1.
+  static constexpr uint32_t kFma = D == 128 ? 0x22u : 0x10u;
   static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // align, barriers
 };
 
@@ -803,16 +801,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         Desc& d = descs[seg % kDescs];
         d.more = more;
         if (more) {
-          const int half_rows = a.rows >> 1, row0 = g.rt * a.rows;
+          const int half = a.tokens >> 1, i0 = g.rt * a.tokens;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int tl = tiles_of<kKeys>(a, g.s, row0 + x * half_rows, row0 + (x + 1) * half_rows);
+            const int tl = tiles_of<kKeys>(a, g.s, i0 + x * half, i0 + (x + 1) * half);
             const int e = tl < g.t1 ? tl : g.t1;
             d.cnt[x] = e > g.t0 ? e - g.t0 : 0;
           }
           d.all = d.cnt[0] > d.cnt[1] ? d.cnt[0] : d.cnt[1];
           d.key_t0 = g.t0, d.b = g.b, d.h = g.h, d.len = g.s.len, d.n = g.s.n, d.off = g.s.off;
-          d.row0 = row0, d.whole = g.t0 == 0 && g.t1 == g.tiles, d.t0 = g.s.t0;
+          d.row0 = g.rt * a.rows, d.whole = g.t0 == 0 && g.t1 == g.tiles, d.t0 = g.s.t0;
         }
         mbar_arrive(d_full + seg % kDescs);
       }
@@ -1311,8 +1309,9 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
   a.B = (int)p->B, a.Hk = (int)p->Hk, a.g = (int)(p->Hq / p->Hk), a.page = (int)p->page;
   a.causal = p->causal != 0;
   a.ctas = pattn::ctas_of(few);
-  // many rows: halves of whole tokens
-  a.rows = few ? pattn::dec::kRows : 2 * (128 / a.g) * a.g;
+  // whole tokens in a tile, and with many rows in each half of it
+  a.tokens = few ? pattn::dec::kRows / a.g : 2 * (128 / a.g);
+  a.rows = a.tokens * a.g;
   a.scale_log2 = (float)(p->scale * 1.4426950408889634);
   a.part = (float*)(ws + w.part);
   a.part_ml = (float*)(ws + w.ml);

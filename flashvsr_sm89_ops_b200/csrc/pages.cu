@@ -18,11 +18,24 @@ namespace fvb {
 namespace pages {
 
 constexpr int kThreads = 1024;
+constexpr int kSmall = 2048;  // lists up to this long are kept in shared memory
 constexpr int kNoPages = 1, kNoWidth = 2, kBadArgs = 4;
 
 struct Copy {
   int32_t from, to, rows, pad;
 };
+
+// Every kernel of this file is launched while its predecessor still runs, lets its own successor do
+// the same, and touches memory only after the predecessor's end: a chain of steps costs their
+// latencies, not their launches.
+__device__ __forceinline__ void chain() {
+  asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+}
+
+// one bit a sequence, in shared memory
+__device__ __forceinline__ bool test_and_set(uint32_t* bits, int64_t i) {
+  return atomicOr(bits + (i >> 5), 1u << (i & 31)) >> (i & 31) & 1;
+}
 
 // exclusive prefix sum over the block of one value a thread; total gets the sum
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
@@ -88,8 +101,9 @@ __device__ __forceinline__ int64_t held(const Cache& c, int64_t len) {  // pages
 __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const int32_t* more,
                                                            int32_t* ws) {
   __shared__ int sums[32];
-  int32_t* prefix = ws;
-  int32_t* list = ws + c.seqs + 1;
+  __shared__ int32_t s_prefix[kSmall], s_list[kSmall];
+  int32_t* const prefix = c.seqs <= kSmall ? s_prefix : ws;
+  chain();
   int64_t need = 0;
   int bad = 0;
   for (int64_t at = 0; at < c.seqs; at += kThreads) {
@@ -109,6 +123,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const 
   }
   bad = __syncthreads_or(bad & kBadArgs) ? kBadArgs : __syncthreads_or(bad & kNoWidth) ? kNoWidth : 0;
   if (!bad && need > c.pages) bad = kNoPages;
+  int32_t* const list = need <= kSmall ? s_list : ws + c.seqs + 1;
   if (!bad && free_pages(c.refs, c.pages, (int)need, list, sums) < need) bad = kNoPages;
   if (bad) {
     if (threadIdx.x == 0) atomicOr(c.status, bad);
@@ -127,45 +142,52 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const 
   for (int64_t b = threadIdx.x; b < c.seqs; b += kThreads) c.lens[b] += more[b];
 }
 
-// ws: count, copies [n], mark [seqs], list [n]
+// ws: count, copies [n], list [n]
 __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int32_t* src,
                                                         const int32_t* dst, int n, int32_t* ws) {
+  extern __shared__ uint32_t branch[];  // a bit a sequence: it is a branch
   __shared__ int sums[32];
+  __shared__ int32_t s_list[kSmall];
+  __shared__ int32_t s_rank[kSmall];
   Copy* copies = reinterpret_cast<Copy*>(ws + 4);
-  int32_t* mark = ws + 4 + 4 * (int64_t)n;
-  int32_t* list = mark + c.seqs;
-  for (int64_t b = threadIdx.x; b < c.seqs; b += kThreads) mark[b] = 0;
+  for (int i = threadIdx.x; i < (int)((c.seqs + 31) >> 5); i += kThreads) branch[i] = 0;
+  chain();
   __syncthreads();
   int bad = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int64_t a = src[i], d = dst[i];
     if (a < 0 || a >= c.seqs || d < 0 || d >= c.seqs) bad = kBadArgs;
-    else if (c.lens[d] != 0 || atomicExch(mark + d, 1) != 0) bad = kBadArgs;
+    else if (test_and_set(branch, d) || c.lens[d] != 0) bad = kBadArgs;
   }
-  bad = __syncthreads_or(bad) ? kBadArgs : 0;
-  if (!bad)
-    for (int i = threadIdx.x; i < n; i += kThreads)
-      if (mark[src[i]]) bad = kBadArgs;
   bad = __syncthreads_or(bad) ? kBadArgs : 0;
   int need = 0;
   if (!bad) {
     for (int at = 0; at < n; at += kThreads) {
       const int i = at + threadIdx.x;
       int part = 0;
-      if (i < n) part = (int)(c.lens[src[i]] % c.page);
+      int32_t len = 0;
+      int64_t a = 0;
+      if (i < n) {
+        a = src[i];
+        if (branch[a >> 5] >> (a & 31) & 1) bad = kBadArgs;
+        len = c.lens[a];
+        part = len % c.page;
+      }
       int total;
       const int r = need + block_scan(part > 0, sums, total);
       if (i < n) {
-        // rows 0: nothing to copy; `to` is the place in the list until the pages are known
-        const int64_t full = c.lens[src[i]] / c.page;
-        int32_t from = full < c.width ? c.table[src[i] * c.width + full] : -1;
+        if (n <= kSmall) s_rank[i] = r;
+        const int64_t full = len / c.page;
+        int32_t from = full < c.width ? c.table[a * c.width + full] : -1;
         if (from < 0 || from >= c.pages) part = 0, from = 0;
-        copies[i] = {from, r, part, 0};
+        copies[i] = {from, r, part, 0};  // rows 0: nothing to copy
       }
       need += total;
     }
-    if (need > c.pages || free_pages(c.refs, c.pages, need, list, sums) < need) bad = kNoPages;
+    bad = __syncthreads_or(bad) ? kBadArgs : 0;
   }
+  int32_t* const list = n <= kSmall ? s_list : ws + 4 + 4 * (int64_t)n;
+  if (!bad && (need > c.pages || free_pages(c.refs, c.pages, need, list, sums) < need)) bad = kNoPages;
   if (bad) {
     if (threadIdx.x == 0) {
       atomicOr(c.status, bad);
@@ -181,7 +203,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int
     const int32_t len = c.lens[a];
     int64_t full = len / c.page;
     if (full > c.width) full = c.width;
-    const int32_t fresh = len % c.page ? list[copies[i].to] : 0;
+    const int32_t fresh = len % c.page ? list[n <= kSmall ? s_rank[i] : copies[i].to] : 0;
     for (int64_t j = lane; j < c.width; j += 32) {
       int32_t p = -1;
       if (j < full) {
@@ -201,17 +223,17 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int
   }
 }
 
-// ws: mark [seqs].  drop NULL: everything; else leading pages, the others move to the front.
+// drop NULL: everything; else leading pages, the others move to the front.
 __global__ void __launch_bounds__(kThreads) release_kernel(const Cache c, const int32_t* seqs,
-                                                           const int32_t* drop, int n,
-                                                           int32_t* mark) {
-  for (int64_t b = threadIdx.x; b < c.seqs; b += kThreads) mark[b] = 0;
+                                                           const int32_t* drop, int n) {
+  extern __shared__ uint32_t named[];  // a bit a sequence
+  for (int i = threadIdx.x; i < (int)((c.seqs + 31) >> 5); i += kThreads) named[i] = 0;
+  chain();
   __syncthreads();
   int bad = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int64_t b = seqs[i];
-    if (b < 0 || b >= c.seqs || (drop && drop[i] < 0)) bad = 1;
-    else if (atomicExch(mark + b, 1) != 0) bad = 1;
+    if (b < 0 || b >= c.seqs || (drop && drop[i] < 0) || test_and_set(named, b)) bad = 1;
   }
   if (__syncthreads_or(bad)) {
     if (threadIdx.x == 0) atomicOr(c.status, kBadArgs);
@@ -223,19 +245,28 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Cache c, const 
     int32_t* row = c.table + b * c.width;
     const int64_t have = held(c, c.lens[b]);
     const int64_t gone = drop && drop[i] < have ? drop[i] : have;
-    for (int64_t j = lane; j < gone; j += 32) {
-      const int32_t p = row[j];
-      if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
+    if (gone == have) {
+      for (int64_t j = lane; j < have; j += 32) {
+        const int32_t p = row[j];
+        row[j] = -1;
+        if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
+      }
+    } else {
+      for (int64_t j = lane; j < gone; j += 32) {
+        const int32_t p = row[j];
+        if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
+      }
+      __syncwarp();
+      // 32 entries at a time: read, then written, so that a shift by less than 32 is safe
+      for (int64_t j0 = 0; j0 < have; j0 += 32) {
+        const int64_t j = j0 + lane;
+        const int32_t p = j + gone < have ? row[j + gone] : -1;
+        __syncwarp();
+        if (j < have) row[j] = p;
+        __syncwarp();
+      }
     }
     __syncwarp();
-    // 32 entries at a time: read, then written, so that a shift by less than 32 is safe
-    for (int64_t j0 = 0; j0 < have; j0 += 32) {
-      const int64_t j = j0 + lane;
-      const int32_t p = j + gone < have ? row[j + gone] : -1;
-      __syncwarp();
-      if (j < have) row[j] = p;
-      __syncwarp();
-    }
     if (lane == 0) {
       const int64_t left = (int64_t)c.lens[b] - gone * c.page;
       c.lens[b] = gone == have || left < 0 ? 0 : (int32_t)left;
@@ -249,6 +280,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const Cache c, int32_
   __shared__ int sums[32];
   Copy* copies = reinterpret_cast<Copy*>(ws + 4);
   int32_t* map = ws + 4 + 4 * (c.pages / 2 + 1);
+  chain();
   int64_t used = 0;
   for (int64_t p = threadIdx.x; p < c.pages; p += kThreads) used += c.refs[p] > 0;
   int total;
@@ -292,6 +324,7 @@ constexpr int kChunk = kCopyThreads * 4 * 16;  // bytes a block copies at a time
 __global__ void __launch_bounds__(kCopyThreads)
     copy_kernel(const Pools p, const int32_t* ws, const int32_t* map, int32_t* table,
                 int64_t entries, int64_t pages) {
+  chain();
   const int64_t count = ws[0];
   const Copy* copies = reinterpret_cast<const Copy*>(ws + 4);
   if (map) {
@@ -326,8 +359,25 @@ __global__ void __launch_bounds__(kCopyThreads)
   }
 }
 
+template <typename... P, typename... A>
+int launch(const char* what, cudaStream_t stream, void (*kernel)(P...), int64_t grid, int threads, size_t smem,
+           A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)grid);
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &early;
+  c.numAttrs = 1;
+  FVB_CUDA_TRY(cudaLaunchKernelEx(&c, kernel, args...), what);
+  return FVB_OK;
+}
+
 int check(const Cache& c, const char* what) {
-  FVB_REQUIRE(c.seqs >= 0 && c.width >= 0 && c.pages >= 0 && c.page > 0 && c.page < (1 << 24) &&
+  FVB_REQUIRE(c.seqs >= 0 && c.seqs <= (1 << 17) && c.width >= 0 && c.pages >= 0 && c.page > 0 && c.page < (1 << 24) &&
                   c.pages < (1ll << 31) && c.seqs * c.width < (1ll << 31),
               "%s: cache of %lld sequences x %lld pages of %d, pool of %lld", what, (long long)c.seqs,
               (long long)c.width, c.page, (long long)c.pages);
@@ -342,10 +392,12 @@ int launch_copy(const Pools& p, const int32_t* ws, const int32_t* map, const Cac
   const int64_t full = (int64_t)sm_count() * 8;
   if (grid > full) grid = full;
   if (grid < 1) grid = 1;
-  copy_kernel<<<(unsigned)grid, kCopyThreads, 0, stream>>>(p, ws, map, c.table, c.seqs * c.width,
-                                                           c.pages);
-  return check_launch(what);
+  return launch(what, stream, copy_kernel, grid, kCopyThreads, 0, p, ws, map, c.table, c.seqs * c.width,
+                c.pages);
 }
+
+// a bit a sequence, in whole words; sequences are limited so that these fit beside the lists
+inline size_t bits(int64_t seqs) { return (size_t)((seqs + 31) / 32 * 4); }
 
 int check_pools(const Pools& p, const char* what) {
   FVB_REQUIRE(p.layers >= 0 && p.row_bytes > 0 && p.row_bytes % 16 == 0 &&
@@ -364,7 +416,7 @@ extern "C" {
 size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages, int64_t n) {
   if (seqs < 0 || pages < 0 || n < 0) return 0;
   const int64_t reserve = seqs + 1 + pages;
-  const int64_t fork = 4 + 4 * n + seqs + n;
+  const int64_t fork = 4 + 4 * n + n;
   const int64_t compact = 4 + 4 * (pages / 2 + 1) + pages;
   int64_t m = reserve > fork ? reserve : fork;
   if (compact > m) m = compact;
@@ -381,9 +433,8 @@ int fvb_pages_reserve(const int32_t* more, int32_t* table, int32_t* lens, int32_
   if (rc) return rc;
   if (seqs == 0) return FVB_OK;
   FVB_REQUIRE(more && workspace, "fvb_pages_reserve: NULL pointer");
-  fvb::pages::reserve_kernel<<<1, fvb::pages::kThreads, 0, (cudaStream_t)stream>>>(
-      c, more, (int32_t*)workspace);
-  return check_launch("fvb_pages_reserve");
+  return fvb::pages::launch("fvb_pages_reserve", (cudaStream_t)stream, fvb::pages::reserve_kernel, 1,
+                            fvb::pages::kThreads, 0, c, more, (int32_t*)workspace);
 }
 
 int fvb_pages_fork(const int32_t* src, const int32_t* dst, int64_t n, int32_t* table, int32_t* lens,
@@ -404,15 +455,15 @@ int fvb_pages_fork(const int32_t* src, const int32_t* dst, int64_t n, int32_t* t
   FVB_REQUIRE(src && dst && workspace, "fvb_pages_fork: NULL pointer");
   FVB_REQUIRE(aligned16(workspace), "fvb_pages_fork: workspace must be 16-byte aligned");
   int32_t* ws = (int32_t*)workspace;
-  fvb::pages::fork_kernel<<<1, fvb::pages::kThreads, 0, (cudaStream_t)stream>>>(c, src, dst, (int)n, ws);
-  rc = check_launch("fvb_pages_fork");
+  rc = fvb::pages::launch("fvb_pages_fork", (cudaStream_t)stream, fvb::pages::fork_kernel, 1,
+                          fvb::pages::kThreads, fvb::pages::bits(seqs), c, src, dst, (int)n, ws);
   if (rc) return rc;
   return fvb::pages::launch_copy(p, ws, nullptr, c, n, (cudaStream_t)stream, "fvb_pages_fork");
 }
 
 int fvb_pages_release(const int32_t* rows, const int32_t* drop, int64_t n, int32_t* table,
                       int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs, int64_t width,
-                      int64_t pages, int64_t page, void* workspace, fvb_stream_t stream) {
+                      int64_t pages, int64_t page, fvb_stream_t stream) {
   using namespace fvb;
   FVB_REQUIRE(page > 0 && page < (1 << 24), "fvb_pages_release: page of %lld", (long long)page);
   const fvb::pages::Cache c = {table, lens, refs, status, seqs, width, pages, (int)page};
@@ -420,10 +471,9 @@ int fvb_pages_release(const int32_t* rows, const int32_t* drop, int64_t n, int32
   if (rc) return rc;
   FVB_REQUIRE(n >= 0 && n < (1 << 28), "fvb_pages_release: %lld sequences", (long long)n);
   if (n == 0) return FVB_OK;
-  FVB_REQUIRE(rows && workspace, "fvb_pages_release: NULL pointer");
-  fvb::pages::release_kernel<<<1, fvb::pages::kThreads, 0, (cudaStream_t)stream>>>(
-      c, rows, drop, (int)n, (int32_t*)workspace);
-  return check_launch("fvb_pages_release");
+  FVB_REQUIRE(rows, "fvb_pages_release: NULL pointer");
+  return fvb::pages::launch("fvb_pages_release", (cudaStream_t)stream, fvb::pages::release_kernel, 1,
+                            fvb::pages::kThreads, fvb::pages::bits(seqs), c, rows, drop, (int)n);
 }
 
 int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
@@ -442,8 +492,8 @@ int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* sta
   if (pages == 0) return FVB_OK;
   FVB_REQUIRE(workspace && aligned16(workspace), "fvb_pages_compact: workspace must be 16-byte aligned");
   int32_t* ws = (int32_t*)workspace;
-  fvb::pages::compact_kernel<<<1, fvb::pages::kThreads, 0, (cudaStream_t)stream>>>(c, ws);
-  rc = check_launch("fvb_pages_compact");
+  rc = fvb::pages::launch("fvb_pages_compact", (cudaStream_t)stream, fvb::pages::compact_kernel, 1,
+                          fvb::pages::kThreads, 0, c, ws);
   if (rc) return rc;
   return fvb::pages::launch_copy(p, ws, ws + 4 + 4 * (pages / 2 + 1), c, pages / 2 + 1,
                                  (cudaStream_t)stream, "fvb_pages_compact");

@@ -148,7 +148,8 @@ class PagedKV:
 
     The tensors are the state: read them, or hand in ones that hold one.  Free pages are given out
     lowest first in the order of sequences and of their pages.  A call on the device that cannot
-    be done (no pages, an index out of range) changes nothing and is recorded in `status`.
+    be done (no pages, an index out of range) changes nothing and is recorded in `status`.  At most
+    131072 sequences.
     """
 
     def __init__(self, k, v, table, lens, refs):
@@ -234,8 +235,8 @@ class PagedKV:
         seqs = _ints(seqs, None, "seqs", "PagedKV.release", self._index)
         if pages is not None:
             pages = _ints(pages, seqs.numel(), "pages", "PagedKV.release", self._index)
-        self._call("fvb_pages_release", seqs.data_ptr(), None if pages is None else pages.data_ptr(), seqs.numel(),
-                   *self._state)
+        _lib.call_on(self._index, "fvb_pages_release", seqs.data_ptr(), None if pages is None else pages.data_ptr(),
+                     seqs.numel(), *self._state, _lib.stream_of(self.table))
 
     def compact(self):
         """Moves the pages in use to the front of the pool, so that its end is free."""

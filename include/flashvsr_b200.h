@@ -444,6 +444,7 @@ FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
  * and sets a bit of *status: 1 no free pages, 2 a table row too short, 4 bad arguments (an index
  * out of range or twice, a negative count, a branch that is not empty).
  * workspace: fvb_pages_workspace_bytes(seqs, pages, n), 16-byte aligned; n branches of a fork.
+ * At most 131072 sequences.
  *   reserve  room for more[b] tokens in every sequence; lens grow
  *   fork     dst[i] becomes a branch of src[i]: full pages shared, the tokens of a partly filled
  *            last page copied to a page of its own in every layer's k and v
@@ -461,8 +462,7 @@ FVB_API int fvb_pages_fork(const int32_t* src, const int32_t* dst, int64_t n, in
                            int64_t row_bytes, void* workspace, fvb_stream_t stream);
 FVB_API int fvb_pages_release(const int32_t* rows, const int32_t* drop, int64_t n, int32_t* table,
                               int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
-                              int64_t width, int64_t pages, int64_t page, void* workspace,
-                              fvb_stream_t stream);
+                              int64_t width, int64_t pages, int64_t page, fvb_stream_t stream);
 FVB_API int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* status,
                               int64_t seqs, int64_t width, int64_t pages, int64_t page, void* k,
                               void* v, int64_t layers, int64_t layer_stride, int64_t page_stride,

@@ -106,6 +106,7 @@ def test_c_arguments():
     assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, 2, 2, 4, 0, 16, None) == bad
     assert lib.fvb_pages_reserve(16, None, 16, 16, 16, 2, 2, 4, 16, 16, None) == bad
     assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, 1 << 20, 1 << 20, 4, 16, 16, None) == bad
+    assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, (1 << 17) + 1, 2, 4, 16, 16, None) == bad
     assert lib.fvb_pages_reserve(None, 16, 16, 16, 16, 2, 2, 4, 16, 16, None) == bad
     assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, 0, 2, 4, 16, 16, None) == _lib.FVB_OK
     pools = (16, 16, 1, 1024, 256, 16)
@@ -114,8 +115,8 @@ def test_c_arguments():
     assert lib.fvb_pages_fork(16, 16, 1, 16, 16, 16, 16, 2, 2, 4, 16, 16, 24, 1, 1024, 256, 16, 16, None) == bad
     assert lib.fvb_pages_fork(16, None, 1, 16, 16, 16, 16, 2, 2, 4, 16, *pools, 16, None) == bad
     assert lib.fvb_pages_fork(16, 16, 0, 16, 16, 16, 16, 2, 2, 4, 16, *pools, 16, None) == _lib.FVB_OK
-    assert lib.fvb_pages_release(None, None, 1, 16, 16, 16, 16, 2, 2, 4, 16, 16, None) == bad
-    assert lib.fvb_pages_release(16, None, 0, 16, 16, 16, 16, 2, 2, 4, 16, 16, None) == _lib.FVB_OK
+    assert lib.fvb_pages_release(None, None, 1, 16, 16, 16, 16, 2, 2, 4, 16, None) == bad
+    assert lib.fvb_pages_release(16, None, 0, 16, 16, 16, 16, 2, 2, 4, 16, None) == _lib.FVB_OK
     assert lib.fvb_pages_compact(16, 16, 16, 16, 2, 2, 4, 16, *pools, None, None) == bad
     assert lib.fvb_pages_workspace_bytes(10, 100, 10) >= 4 * (11 + 100)
     assert lib.fvb_paged_attn_workspace_bytes(1, 8, 2, 128) < lib.fvb_paged_attn_workspace_bytes(64, 8, 2, 128)
