@@ -99,22 +99,21 @@ _SIGS = {
     # of them one by one costs 2.7 us a call, packing them 0.3
     "fvb_rope": (_int, [ctypes.c_char_p, _vp]),
     "fvb_kv_append": (_int, [ctypes.c_char_p, _vp]),
-    "fvb_pages_workspace_bytes": (_sz, [_i64, _i64, _i64]),
-    "fvb_pages_reserve": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
-    "fvb_pages_fork": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64,
-                              _i64, _i64, _i64, _vp, _vp]),
-    "fvb_pages_release": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
-    "fvb_pages_compact": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64,
-                                 _i64, _vp, _vp]),
+    "fvb_pages_workspace_bytes": (_sz, [_i64, _i64]),
+    "fvb_pages_reserve": (_int, [ctypes.c_char_p, _vp, _vp]),
+    "fvb_pages_fork": (_int, [ctypes.c_char_p, _vp, _vp, _i64, _vp]),
+    "fvb_pages_release": (_int, [ctypes.c_char_p, _vp, _vp, _i64, _vp]),
+    "fvb_pages_compact": (_int, [ctypes.c_char_p, _vp]),
     "fvb_paged_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "fvb_paged_attn": (_int, [ctypes.c_char_p, _vp]),
 }
 
 
-# fvb_rope_args, fvb_kv_append_args and fvb_paged_attn_args: every member is 8 bytes
+# fvb_rope_args, fvb_kv_append_args, fvb_paged_attn_args and fvb_pages: every member is 8 bytes
 ROPE_ARGS = struct.Struct("=24qdq").pack
 KV_APPEND_ARGS = struct.Struct("=24qd10q").pack
 PAGED_ATTN_ARGS = struct.Struct("=24qd5q").pack
+PAGES = struct.Struct("=15q").pack
 
 
 class FvbError(RuntimeError):

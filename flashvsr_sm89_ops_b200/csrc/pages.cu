@@ -197,29 +197,26 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int
   }
   __syncthreads();
   if (threadIdx.x == 0) ws[0] = n;
-  const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < n; i += kThreads / 32) {
-    const int64_t a = src[i], d = dst[i];
-    const int32_t len = c.lens[a];
-    int64_t full = len / c.page;
-    if (full > c.width) full = c.width;
-    const int32_t fresh = len % c.page ? list[n <= kSmall ? s_rank[i] : copies[i].to] : 0;
-    for (int64_t j = lane; j < c.width; j += 32) {
-      int32_t p = -1;
-      if (j < full) {
-        p = c.table[a * c.width + j];
-        if (p >= 0 && p < c.pages) atomicAdd(c.refs + p, 1);
-      } else if (j == full && len % c.page) {
-        p = fresh;
-        c.refs[p] = 1;
-      }
-      c.table[d * c.width + j] = p;
+  // a thread an entry of the branches' rows
+  for (int64_t e = threadIdx.x; e < n * c.width; e += kThreads) {
+    const int i = (int)(e / c.width);
+    const int64_t j = e - i * c.width, a = src[i], d = dst[i];
+    const int32_t len = c.lens[a], full = len / c.page;
+    int32_t p = -1;
+    if (j < full) {
+      p = c.table[a * c.width + j];
+      if (p >= 0 && p < c.pages) atomicAdd(c.refs + p, 1);
+    } else if (j == full && len % c.page) {
+      p = list[n <= kSmall ? s_rank[i] : copies[i].to];
+      c.refs[p] = 1;
     }
-    __syncwarp();
-    if (lane == 0) {
-      copies[i].to = fresh;
-      c.lens[d] = len;
-    }
+    c.table[d * c.width + j] = p;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int32_t len = c.lens[src[i]];
+    copies[i].to = len % c.page ? list[n <= kSmall ? s_rank[i] : copies[i].to] : 0;
+    c.lens[dst[i]] = len;
   }
 }
 
@@ -239,19 +236,21 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Cache c, const 
     if (threadIdx.x == 0) atomicOr(c.status, kBadArgs);
     return;
   }
+  // a thread an entry of the rows that go as a whole, a warp a row of the others
+  for (int64_t e = threadIdx.x; e < n * c.width; e += kThreads) {
+    const int i = (int)(e / c.width);
+    const int64_t j = e - i * c.width, b = seqs[i], have = held(c, c.lens[b]);
+    if (j >= have || (drop && drop[i] < have)) continue;
+    const int32_t p = c.table[b * c.width + j];
+    c.table[b * c.width + j] = -1;
+    if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
+  }
   const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < n; i += kThreads / 32) {
-    const int64_t b = seqs[i];
-    int32_t* row = c.table + b * c.width;
-    const int64_t have = held(c, c.lens[b]);
-    const int64_t gone = drop && drop[i] < have ? drop[i] : have;
-    if (gone == have) {
-      for (int64_t j = lane; j < have; j += 32) {
-        const int32_t p = row[j];
-        row[j] = -1;
-        if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
-      }
-    } else {
+  if (drop)
+    for (int i = threadIdx.x >> 5; i < n; i += kThreads / 32) {
+      const int64_t b = seqs[i], have = held(c, c.lens[b]), gone = drop[i];
+      int32_t* row = c.table + b * c.width;
+      if (gone >= have) continue;
       for (int64_t j = lane; j < gone; j += 32) {
         const int32_t p = row[j];
         if (p >= 0 && p < c.pages) atomicSub(c.refs + p, 1);
@@ -266,11 +265,11 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Cache c, const 
         __syncwarp();
       }
     }
-    __syncwarp();
-    if (lane == 0) {
-      const int64_t left = (int64_t)c.lens[b] - gone * c.page;
-      c.lens[b] = gone == have || left < 0 ? 0 : (int32_t)left;
-    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int64_t b = seqs[i], have = held(c, c.lens[b]);
+    const int64_t left = (int64_t)c.lens[b] - (int64_t)(drop ? drop[i] : 0) * c.page;
+    c.lens[b] = !drop || drop[i] >= have ? 0 : (int32_t)(left > 0 ? left : 0);
   }
 }
 
@@ -376,14 +375,32 @@ int launch(const char* what, cudaStream_t stream, void (*kernel)(P...), int64_t 
   return FVB_OK;
 }
 
-int check(const Cache& c, const char* what) {
-  FVB_REQUIRE(c.seqs >= 0 && c.seqs <= (1 << 17) && c.width >= 0 && c.pages >= 0 && c.page > 0 && c.page < (1 << 24) &&
-                  c.pages < (1ll << 31) && c.seqs * c.width < (1ll << 31),
-              "%s: cache of %lld sequences x %lld pages of %d, pool of %lld", what, (long long)c.seqs,
-              (long long)c.width, c.page, (long long)c.pages);
-  FVB_REQUIRE(c.table && c.lens && c.refs && c.status, "%s: NULL pointer", what);
+int cache_of(const fvb_pages* p, Cache& c, const char* what) {
+  FVB_REQUIRE(p, "%s: NULL pointer", what);
+  // a bit a sequence has to fit in shared memory beside the lists
+  FVB_REQUIRE(p->seqs >= 0 && p->seqs <= (1 << 17) && p->width >= 0 && p->width < (1ll << 31) &&
+                  p->pages >= 0 && p->pages < (1ll << 31) && p->page > 0 && p->page < (1 << 24) &&
+                  p->seqs * p->width < (1ll << 31),
+              "%s: cache of %lld sequences x %lld pages of %lld, pool of %lld", what, (long long)p->seqs,
+              (long long)p->width, (long long)p->page, (long long)p->pages);
+  FVB_REQUIRE(p->table && p->lens && p->refs && p->status && p->workspace, "%s: NULL pointer", what);
+  FVB_REQUIRE(aligned16(p->workspace), "%s: workspace must be 16-byte aligned", what);
+  c = {p->table, p->lens, p->refs, p->status, p->seqs, p->width, p->pages, (int)p->page};
   return FVB_OK;
 }
+
+int pools_of(const fvb_pages* p, Pools& q, const char* what) {
+  FVB_REQUIRE(p->layers >= 0 && p->row_bytes > 0 && p->row_bytes % 16 == 0 &&
+                  p->layer_stride % 16 == 0 && p->page_stride % 16 == 0,
+              "%s: rows and strides must be multiples of 16 bytes", what);
+  FVB_REQUIRE(p->layers == 0 || (p->k && p->v && aligned16(p->k) && aligned16(p->v)),
+              "%s: pools must be 16-byte aligned", what);
+  q = {(uint8_t*)p->k, (uint8_t*)p->v, p->layers, p->layer_stride, p->page_stride, p->row_bytes,
+       p->row_bytes * p->page};
+  return FVB_OK;
+}
+
+inline size_t bits(int64_t seqs) { return (size_t)((seqs + 31) / 32 * 4); }  // a bit a sequence
 
 int launch_copy(const Pools& p, const int32_t* ws, const int32_t* map, const Cache& c, int64_t most,
                 cudaStream_t stream, const char* what) {
@@ -396,107 +413,76 @@ int launch_copy(const Pools& p, const int32_t* ws, const int32_t* map, const Cac
                 c.pages);
 }
 
-// a bit a sequence, in whole words; sequences are limited so that these fit beside the lists
-inline size_t bits(int64_t seqs) { return (size_t)((seqs + 31) / 32 * 4); }
-
-int check_pools(const Pools& p, const char* what) {
-  FVB_REQUIRE(p.layers >= 0 && p.row_bytes > 0 && p.row_bytes % 16 == 0 &&
-                  p.layer_stride % 16 == 0 && p.page_stride % 16 == 0,
-              "%s: rows and strides must be multiples of 16 bytes", what);
-  FVB_REQUIRE(p.layers == 0 || (p.k && p.v && aligned16(p.k) && aligned16(p.v)),
-              "%s: pools must be 16-byte aligned", what);
-  return FVB_OK;
-}
-
 }  // namespace pages
 }  // namespace fvb
 
 extern "C" {
 
-size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages, int64_t n) {
-  if (seqs < 0 || pages < 0 || n < 0) return 0;
+size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages) {
+  if (seqs < 0 || pages < 0) return 0;
   const int64_t reserve = seqs + 1 + pages;
-  const int64_t fork = 4 + 4 * n + n;
+  const int64_t fork = 4 + 4 * seqs + seqs;
   const int64_t compact = 4 + 4 * (pages / 2 + 1) + pages;
   int64_t m = reserve > fork ? reserve : fork;
   if (compact > m) m = compact;
   return (size_t)(4 * m + 16);
 }
 
-int fvb_pages_reserve(const int32_t* more, int32_t* table, int32_t* lens, int32_t* refs,
-                      int32_t* status, int64_t seqs, int64_t width, int64_t pages, int64_t page,
-                      void* workspace, fvb_stream_t stream) {
+int fvb_pages_reserve(const fvb_pages* p, const int32_t* more, fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(page > 0 && page < (1 << 24), "fvb_pages_reserve: page of %lld", (long long)page);
-  const fvb::pages::Cache c = {table, lens, refs, status, seqs, width, pages, (int)page};
-  int rc = fvb::pages::check(c, "fvb_pages_reserve");
-  if (rc) return rc;
-  if (seqs == 0) return FVB_OK;
-  FVB_REQUIRE(more && workspace, "fvb_pages_reserve: NULL pointer");
-  return fvb::pages::launch("fvb_pages_reserve", (cudaStream_t)stream, fvb::pages::reserve_kernel, 1,
-                            fvb::pages::kThreads, 0, c, more, (int32_t*)workspace);
+  pages::Cache c;
+  int rc = pages::cache_of(p, c, "fvb_pages_reserve");
+  if (rc || p->seqs == 0) return rc;
+  FVB_REQUIRE(more, "fvb_pages_reserve: NULL pointer");
+  return pages::launch("fvb_pages_reserve", (cudaStream_t)stream, pages::reserve_kernel, 1, pages::kThreads, 0,
+                       c, more, (int32_t*)p->workspace);
 }
 
-int fvb_pages_fork(const int32_t* src, const int32_t* dst, int64_t n, int32_t* table, int32_t* lens,
-                   int32_t* refs, int32_t* status, int64_t seqs, int64_t width, int64_t pages,
-                   int64_t page, void* k, void* v, int64_t layers, int64_t layer_stride,
-                   int64_t page_stride, int64_t row_bytes, void* workspace, fvb_stream_t stream) {
+int fvb_pages_fork(const fvb_pages* p, const int32_t* src, const int32_t* dst, int64_t n,
+                   fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(page > 0 && page < (1 << 24), "fvb_pages_fork: page of %lld", (long long)page);
-  const fvb::pages::Cache c = {table, lens, refs, status, seqs, width, pages, (int)page};
-  int rc = fvb::pages::check(c, "fvb_pages_fork");
+  pages::Cache c;
+  pages::Pools pools;
+  int rc = pages::cache_of(p, c, "fvb_pages_fork");
+  if (!rc) rc = pages::pools_of(p, pools, "fvb_pages_fork");
   if (rc) return rc;
-  const fvb::pages::Pools p = {(uint8_t*)k, (uint8_t*)v, layers, layer_stride, page_stride, row_bytes,
-                               row_bytes * page};
-  rc = fvb::pages::check_pools(p, "fvb_pages_fork");
-  if (rc) return rc;
-  FVB_REQUIRE(n >= 0 && n < (1 << 28), "fvb_pages_fork: %lld branches", (long long)n);
+  FVB_REQUIRE(n >= 0 && n <= p->seqs, "fvb_pages_fork: %lld branches of %lld sequences", (long long)n,
+              (long long)p->seqs);
   if (n == 0) return FVB_OK;
-  FVB_REQUIRE(src && dst && workspace, "fvb_pages_fork: NULL pointer");
-  FVB_REQUIRE(aligned16(workspace), "fvb_pages_fork: workspace must be 16-byte aligned");
-  int32_t* ws = (int32_t*)workspace;
-  rc = fvb::pages::launch("fvb_pages_fork", (cudaStream_t)stream, fvb::pages::fork_kernel, 1,
-                          fvb::pages::kThreads, fvb::pages::bits(seqs), c, src, dst, (int)n, ws);
+  FVB_REQUIRE(src && dst, "fvb_pages_fork: NULL pointer");
+  int32_t* ws = (int32_t*)p->workspace;
+  rc = pages::launch("fvb_pages_fork", (cudaStream_t)stream, pages::fork_kernel, 1, pages::kThreads,
+                     pages::bits(p->seqs), c, src, dst, (int)n, ws);
   if (rc) return rc;
-  return fvb::pages::launch_copy(p, ws, nullptr, c, n, (cudaStream_t)stream, "fvb_pages_fork");
+  return pages::launch_copy(pools, ws, nullptr, c, n, (cudaStream_t)stream, "fvb_pages_fork");
 }
 
-int fvb_pages_release(const int32_t* rows, const int32_t* drop, int64_t n, int32_t* table,
-                      int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs, int64_t width,
-                      int64_t pages, int64_t page, fvb_stream_t stream) {
+int fvb_pages_release(const fvb_pages* p, const int32_t* rows, const int32_t* drop, int64_t n,
+                      fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(page > 0 && page < (1 << 24), "fvb_pages_release: page of %lld", (long long)page);
-  const fvb::pages::Cache c = {table, lens, refs, status, seqs, width, pages, (int)page};
-  int rc = fvb::pages::check(c, "fvb_pages_release");
+  pages::Cache c;
+  int rc = pages::cache_of(p, c, "fvb_pages_release");
   if (rc) return rc;
   FVB_REQUIRE(n >= 0 && n < (1 << 28), "fvb_pages_release: %lld sequences", (long long)n);
   if (n == 0) return FVB_OK;
   FVB_REQUIRE(rows, "fvb_pages_release: NULL pointer");
-  return fvb::pages::launch("fvb_pages_release", (cudaStream_t)stream, fvb::pages::release_kernel, 1,
-                            fvb::pages::kThreads, fvb::pages::bits(seqs), c, rows, drop, (int)n);
+  return pages::launch("fvb_pages_release", (cudaStream_t)stream, pages::release_kernel, 1, pages::kThreads,
+                       pages::bits(p->seqs), c, rows, drop, (int)n);
 }
 
-int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
-                      int64_t width, int64_t pages, int64_t page, void* k, void* v, int64_t layers,
-                      int64_t layer_stride, int64_t page_stride, int64_t row_bytes, void* workspace,
-                      fvb_stream_t stream) {
+int fvb_pages_compact(const fvb_pages* p, fvb_stream_t stream) {
   using namespace fvb;
-  FVB_REQUIRE(page > 0 && page < (1 << 24), "fvb_pages_compact: page of %lld", (long long)page);
-  const fvb::pages::Cache c = {table, lens, refs, status, seqs, width, pages, (int)page};
-  int rc = fvb::pages::check(c, "fvb_pages_compact");
+  pages::Cache c;
+  pages::Pools pools;
+  int rc = pages::cache_of(p, c, "fvb_pages_compact");
+  if (!rc) rc = pages::pools_of(p, pools, "fvb_pages_compact");
+  if (rc || p->pages == 0) return rc;
+  int32_t* ws = (int32_t*)p->workspace;
+  rc = pages::launch("fvb_pages_compact", (cudaStream_t)stream, pages::compact_kernel, 1, pages::kThreads, 0, c,
+                     ws);
   if (rc) return rc;
-  const fvb::pages::Pools p = {(uint8_t*)k, (uint8_t*)v, layers, layer_stride, page_stride, row_bytes,
-                               row_bytes * page};
-  rc = fvb::pages::check_pools(p, "fvb_pages_compact");
-  if (rc) return rc;
-  if (pages == 0) return FVB_OK;
-  FVB_REQUIRE(workspace && aligned16(workspace), "fvb_pages_compact: workspace must be 16-byte aligned");
-  int32_t* ws = (int32_t*)workspace;
-  rc = fvb::pages::launch("fvb_pages_compact", (cudaStream_t)stream, fvb::pages::compact_kernel, 1,
-                          fvb::pages::kThreads, 0, c, ws);
-  if (rc) return rc;
-  return fvb::pages::launch_copy(p, ws, ws + 4 + 4 * (pages / 2 + 1), c, pages / 2 + 1,
-                                 (cudaStream_t)stream, "fvb_pages_compact");
+  return pages::launch_copy(pools, ws, ws + 4 + 4 * (p->pages / 2 + 1), c, p->pages / 2 + 1,
+                            (cudaStream_t)stream, "fvb_pages_compact");
 }
 
 }  // extern "C"

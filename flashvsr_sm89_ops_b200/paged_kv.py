@@ -180,18 +180,17 @@ class PagedKV:
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.device = dev
         seqs, width = table.shape
-        n = _lib.load().fvb_pages_workspace_bytes(seqs, P, seqs)
+        n = _lib.load().fvb_pages_workspace_bytes(seqs, P)
         self._ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        self._ws_ptr = self._ws.data_ptr()
-        # what every step of the pages takes: the state, then its sizes
-        self._state = (table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.status.data_ptr(), seqs, width, P,
-                       page)
         self._pools = (k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0) * 2, k.stride(1) * 2, H * D * 2)
-        # what every append and attention takes
+        # what every step of the pages takes
+        self._pages = _lib.PAGES(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.status.data_ptr(), seqs, width,
+                                 P, page, *self._pools, self._ws.data_ptr())
+        # and every append and attention
         self._index, self._dt, self._dtype = k.get_device(), _DTYPES[k.dtype], k.dtype
         self._shape = (H, D, P, page)
         self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
-        self._tail = (table.data_ptr(), seqs, width, P, page)
+        self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads: int, head_dim: int, seqs: int,
@@ -210,37 +209,35 @@ class PagedKV:
             self.status.zero_()
             raise RuntimeError("PagedKV: " + "; ".join(m for bit, m in _STATUS.items() if s & bit))
 
-    def _call(self, name, *args):
-        _lib.call_on(self._index, name, *args, self._ws_ptr, _lib.stream_of(self.table))
-
     def reserve(self, more: torch.Tensor):
         """Room for more[b] tokens (int32 [seqs]) behind every sequence; lens grow by them."""
-        more = _ints(more, self.lens.numel(), "more", "PagedKV.reserve", self._index)
-        self._call("fvb_pages_reserve", more.data_ptr(), *self._state)
+        more = _ints(more, self._tail[2], "more", "PagedKV.reserve", self._index)
+        _lib.call_on(self._index, "fvb_pages_reserve", self._pages, more.data_ptr(), _lib.stream_of(more))
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor):
         """Sequence dst[i] becomes a branch of src[i] (int32 [n]; a parent may come several times,
         the branches are empty, distinct and no parents).  Full pages are shared; the tokens in a
         partly filled last page are copied, in every layer."""
         src = _ints(src, None, "src", "PagedKV.fork", self._index)
-        dst = _ints(dst, src.numel(), "dst", "PagedKV.fork", self._index)
-        if src.numel() > self.lens.numel():
-            raise ValueError(f"PagedKV.fork: {src.numel()} branches of {self.lens.numel()} sequences")
-        self._call("fvb_pages_fork", src.data_ptr(), dst.data_ptr(), src.numel(), *self._state, *self._pools)
+        n = src.shape[0]
+        dst = _ints(dst, n, "dst", "PagedKV.fork", self._index)
+        _lib.call_on(self._index, "fvb_pages_fork", self._pages, src.data_ptr(), dst.data_ptr(), n,
+                     _lib.stream_of(src))
 
     def release(self, seqs: torch.Tensor, pages: torch.Tensor | None = None):
         """Sequences (int32 [n], distinct) give back all their pages and become empty, or with
         `pages` (int32 [n]) that many of their first ones: a stream's oldest tokens.  Pages that
         other sequences hold stay."""
         seqs = _ints(seqs, None, "seqs", "PagedKV.release", self._index)
+        n = seqs.shape[0]
         if pages is not None:
-            pages = _ints(pages, seqs.numel(), "pages", "PagedKV.release", self._index)
-        _lib.call_on(self._index, "fvb_pages_release", seqs.data_ptr(), None if pages is None else pages.data_ptr(),
-                     seqs.numel(), *self._state, _lib.stream_of(self.table))
+            pages = _ints(pages, n, "pages", "PagedKV.release", self._index)
+        _lib.call_on(self._index, "fvb_pages_release", self._pages, seqs.data_ptr(),
+                     None if pages is None else pages.data_ptr(), n, _lib.stream_of(seqs))
 
     def compact(self):
         """Moves the pages in use to the front of the pool, so that its end is free."""
-        self._call("fvb_pages_compact", *self._state, *self._pools)
+        _lib.call_on(self._index, "fvb_pages_compact", self._pages, _lib.stream_of(self.table))
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
                q: torch.Tensor | None = None, rope: Rope | None = None, positions: torch.Tensor | None = None,
@@ -263,7 +260,7 @@ class PagedKV:
             raise ValueError(f"{name}: k and v must be {dt} on {self.device}")
         if not 0 <= layer < self._pools[2]:
             raise ValueError(f"{name}: layer {layer} of {self._pools[2]}")
-        table, seqs, width, P, page = self._tail
+        lens, table, seqs, width, P, page = self._tail
         cu = _ints(cu_seqlens, seqs + 1, "cu_seqlens", name, index)
         if q is None:
             if out_q is not None:
@@ -302,7 +299,7 @@ class PagedKV:
         at = layer * layer_bytes
         _lib.call_on(index, "fvb_kv_append",
                      _lib.KV_APPEND_ARGS(*qargs, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, H, T, D, *rargs,
-                                         cu.data_ptr(), self._state[1], table, seqs, width, P, page, kp + at, vp + at,
+                                         cu.data_ptr(), lens, table, seqs, width, P, page, kp + at, vp + at,
                                          self._strides[0]), _lib.stream_of(k))
         return oq
 
@@ -320,6 +317,6 @@ class PagedKV:
                              f"{tuple(q.shape)} on {q.device}")
         kp, vp, _, layer_bytes, _, _ = self._pools
         at, s = layer * layer_bytes, self._strides
-        table, seqs, width, _, _ = self._tail
-        return _attend(name, q, self._dt, (kp + at, *s, vp + at, *s), self._shape, table, width, self._state[1], seqs,
+        lens, table, seqs, width, _, _ = self._tail
+        return _attend(name, q, self._dt, (kp + at, *s, vp + at, *s), self._shape, table, width, lens, seqs,
                        cu_seqlens, causal, sm_scale, max_new, out)

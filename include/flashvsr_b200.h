@@ -443,30 +443,27 @@ FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
  * first, in the order of sequences and of their pages.  A step that cannot be done changes nothing
  * and sets a bit of *status: 1 no free pages, 2 a table row too short, 4 bad arguments (an index
  * out of range or twice, a negative count, a branch that is not empty).
- * workspace: fvb_pages_workspace_bytes(seqs, pages, n), 16-byte aligned; n branches of a fork.
- * At most 131072 sequences.
+ * workspace: fvb_pages_workspace_bytes(seqs, pages), 16-byte aligned.  At most 131072 sequences.
  *   reserve  room for more[b] tokens in every sequence; lens grow
  *   fork     dst[i] becomes a branch of src[i]: full pages shared, the tokens of a partly filled
  *            last page copied to a page of its own in every layer's k and v
  *   release  all of rows[i]'s pages (drop NULL) or its drop[i] first ones; the rest moves forward
  *   compact  pages in use move to the front of the pool, both in ascending order
  * Pools: layer_stride, page_stride, row_bytes (a token in one layer) in bytes, multiples of 16. */
-FVB_API size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages, int64_t n);
-FVB_API int fvb_pages_reserve(const int32_t* more, int32_t* table, int32_t* lens, int32_t* refs,
-                              int32_t* status, int64_t seqs, int64_t width, int64_t pages,
-                              int64_t page, void* workspace, fvb_stream_t stream);
-FVB_API int fvb_pages_fork(const int32_t* src, const int32_t* dst, int64_t n, int32_t* table,
-                           int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
-                           int64_t width, int64_t pages, int64_t page, void* k, void* v,
-                           int64_t layers, int64_t layer_stride, int64_t page_stride,
-                           int64_t row_bytes, void* workspace, fvb_stream_t stream);
-FVB_API int fvb_pages_release(const int32_t* rows, const int32_t* drop, int64_t n, int32_t* table,
-                              int32_t* lens, int32_t* refs, int32_t* status, int64_t seqs,
-                              int64_t width, int64_t pages, int64_t page, fvb_stream_t stream);
-FVB_API int fvb_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* status,
-                              int64_t seqs, int64_t width, int64_t pages, int64_t page, void* k,
-                              void* v, int64_t layers, int64_t layer_stride, int64_t page_stride,
-                              int64_t row_bytes, void* workspace, fvb_stream_t stream);
+typedef struct {
+  int32_t *table, *lens, *refs, *status;
+  int64_t seqs, width, pages, page;
+  void *k, *v; /* reserve and release do without the pools */
+  int64_t layers, layer_stride, page_stride, row_bytes;
+  void* workspace;
+} fvb_pages;
+FVB_API size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages);
+FVB_API int fvb_pages_reserve(const fvb_pages* cache, const int32_t* more, fvb_stream_t stream);
+FVB_API int fvb_pages_fork(const fvb_pages* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                           fvb_stream_t stream);
+FVB_API int fvb_pages_release(const fvb_pages* cache, const int32_t* rows, const int32_t* drop, int64_t n,
+                              fvb_stream_t stream);
+FVB_API int fvb_pages_compact(const fvb_pages* cache, fvb_stream_t stream);
 
 /* Attention of new tokens over a paged cache.  q, out [T][Hq][D], k and v [pages][page][Hk][D], all
  * with strides in elements (multiples of 8, 16-byte aligned pointers); query head h reads key head

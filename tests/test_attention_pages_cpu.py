@@ -103,20 +103,27 @@ def test_c_arguments():
     assert attn(D=96) == unsupported and attn(D=256) == unsupported
     assert attn(T=0) == _lib.FVB_OK and attn(B=0) == _lib.FVB_OK
 
-    assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, 2, 2, 4, 0, 16, None) == bad
-    assert lib.fvb_pages_reserve(16, None, 16, 16, 16, 2, 2, 4, 16, 16, None) == bad
-    assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, 1 << 20, 1 << 20, 4, 16, 16, None) == bad
-    assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, (1 << 17) + 1, 2, 4, 16, 16, None) == bad
-    assert lib.fvb_pages_reserve(None, 16, 16, 16, 16, 2, 2, 4, 16, 16, None) == bad
-    assert lib.fvb_pages_reserve(16, 16, 16, 16, 16, 0, 2, 4, 16, 16, None) == _lib.FVB_OK
-    pools = (16, 16, 1, 1024, 256, 16)
-    assert lib.fvb_pages_fork(16, 16, -1, 16, 16, 16, 16, 2, 2, 4, 16, *pools, 16, None) == bad
-    assert lib.fvb_pages_fork(16, 16, 1, 16, 16, 16, 16, 2, 2, 4, 16, 16, 16, 1, 1024, 250, 16, 16, None) == bad
-    assert lib.fvb_pages_fork(16, 16, 1, 16, 16, 16, 16, 2, 2, 4, 16, 16, 24, 1, 1024, 256, 16, 16, None) == bad
-    assert lib.fvb_pages_fork(16, None, 1, 16, 16, 16, 16, 2, 2, 4, 16, *pools, 16, None) == bad
-    assert lib.fvb_pages_fork(16, 16, 0, 16, 16, 16, 16, 2, 2, 4, 16, *pools, 16, None) == _lib.FVB_OK
-    assert lib.fvb_pages_release(None, None, 1, 16, 16, 16, 16, 2, 2, 4, 16, None) == bad
-    assert lib.fvb_pages_release(16, None, 0, 16, 16, 16, 16, 2, 2, 4, 16, None) == _lib.FVB_OK
-    assert lib.fvb_pages_compact(16, 16, 16, 16, 2, 2, 4, 16, *pools, None, None) == bad
-    assert lib.fvb_pages_workspace_bytes(10, 100, 10) >= 4 * (11 + 100)
+    def pages(table=16, seqs=2, width=2, pages=4, page=16, k=16, layers=1, layer=1024, stride=256, row=16, ws=16):
+        return _lib.PAGES(table, 16, 16, 16, seqs, width, pages, page, k, 16, layers, layer, stride, row, ws)
+
+    fns = [lambda c: lib.fvb_pages_reserve(c, 16, None), lambda c: lib.fvb_pages_fork(c, 16, 16, 1, None),
+           lambda c: lib.fvb_pages_release(c, 16, None, 1, None), lambda c: lib.fvb_pages_compact(c, None)]
+    for fn in fns:
+        assert fn(None) == bad
+        for kw in ({"page": 0}, {"page": 1 << 24}, {"table": 0}, {"seqs": -1}, {"seqs": (1 << 17) + 1}, {"width": -1},
+                   {"seqs": 1 << 17, "width": 1 << 14}, {"pages": -1}, {"ws": 0}, {"ws": 24}):
+            assert fn(pages(**kw)) == bad, kw
+    for fn in fns[1::2]:
+        for kw in ({"k": 24}, {"k": 0}, {"layer": 8}, {"stride": 250}, {"row": 8}, {"row": 0}, {"layers": -1}):
+            assert fn(pages(**kw)) == bad, kw
+    assert lib.fvb_pages_reserve(pages(), None, None) == bad
+    assert lib.fvb_pages_reserve(pages(seqs=0), 16, None) == _lib.FVB_OK
+    assert lib.fvb_pages_fork(pages(), 16, 16, -1, None) == bad
+    assert lib.fvb_pages_fork(pages(), 16, 16, 3, None) == bad  # more branches than sequences
+    assert lib.fvb_pages_fork(pages(), 16, None, 1, None) == bad
+    assert lib.fvb_pages_fork(pages(), 16, 16, 0, None) == _lib.FVB_OK
+    assert lib.fvb_pages_release(pages(), None, None, 1, None) == bad
+    assert lib.fvb_pages_release(pages(), 16, None, 0, None) == _lib.FVB_OK
+    assert lib.fvb_pages_compact(pages(pages=0), None) == _lib.FVB_OK
+    assert lib.fvb_pages_workspace_bytes(10, 100) >= 4 * (11 + 100)
     assert lib.fvb_paged_attn_workspace_bytes(1, 8, 2, 128) < lib.fvb_paged_attn_workspace_bytes(64, 8, 2, 128)
