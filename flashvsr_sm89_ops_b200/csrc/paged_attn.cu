@@ -39,6 +39,7 @@ struct Args {
   int64_t T, width, pages;
   int B, Hk, g, page, causal, ctas;
   int rows, tokens;  // packed rows of an item's tile: whole tokens
+  int few_rows;      // rows that the caller's bound on new tokens announces
   float scale_log2;
   float* part;    // [2 ctas][rows][D]: O of an item begun before the CTA, of one begun in it
   float* part_ml; // [2 ctas][rows][2]
@@ -115,91 +116,239 @@ struct Walk {
   }
 };
 
-// units of one key head of a sequence
-template <int KT>
-__device__ int64_t head_units(const Args& a, const Seq& s) {
-  const int tk = a.tokens;
-  if (!a.causal) {
-    const int64_t t = ((int64_t)s.len + KT - 1) / KT;
-    return (int64_t)((s.n + tk - 1) / tk) * (t > 0 ? t : 1);
-  }
-  int64_t u = 0;
-  for (int i = 0; i < s.n; i += tk) {
-    const int t = tiles_of<KT>(a, s, i, i + tk);
-    u += t > 0 ? t : 1;
-  }
-  return u;
-}
-
 struct Found {
-  int64_t total, rem;
+  int64_t rem, head;  // the walk's place in its sequence, tiles of a key head there
   int b;
 };
 
-// Every thread of the block; finds the walk of this CTA.  Returns the tiles a CTA takes.
-template <int KT, int kThreads, int kLeast>
-__device__ int64_t start_walk(const Args& a, Walk<KT>& w, Found* sh, int64_t* sums) {
+// What all items together are.
+struct Total {
+  int64_t units, items;
+  int most;  // the longest item
+};
+
+template <int KT>
+__device__ __forceinline__ int item_units(const Args& a, const Seq& s, int rt) {
+  const int t = tiles_of<KT>(a, s, rt * a.tokens, (rt + 1) * a.tokens);
+  return t > 0 ? t : 1;
+}
+
+// Work on all sequences, `lanes` threads a sequence (a power of two, a warp at most).
+template <int KT, int kThreads>
+struct Crew {
+  int lanes, seqs, me, at;  // sequences side by side; this thread's among them, and its place there
+
+  __device__ explicit Crew(int B) {
+    lanes = 32;
+    while (lanes > 1 && B * lanes > kThreads) lanes >>= 1;
+    seqs = kThreads / lanes;
+    me = threadIdx.x / lanes;
+    at = threadIdx.x & (lanes - 1);
+  }
+  // units of one key head of sequence b, on all of its threads; 0 past the last
+  __device__ int64_t head_units(const Args& a, int64_t b, int& tiles) const {
+    tiles = 0;
+    int64_t u = 0;
+    if (b < a.B) {
+      const Seq s = get_seq(a, (int)b);
+      tiles = (s.n + a.tokens - 1) / a.tokens;
+      if (a.causal) {
+        for (int r = at; r < tiles; r += lanes) u += item_units<KT>(a, s, r);
+      } else if (at == 0 && tiles) {
+        u = (int64_t)tiles * item_units<KT>(a, s, 0);
+      }
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    return u;
+  }
+};
+
+// Inclusive prefix sum over the warp.
+template <typename I>
+__device__ __forceinline__ I warp_scan(I x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const I y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// What a thread knows of its sequence of the first round: tiles of a key head, of all, and of the
+// sequences before it.
+struct First {
+  int64_t head, units, before;
+};
+
+// Every thread of the block.  kItems: also their number and the longest one.
+template <int KT, int kThreads, bool kItems>
+__device__ Total count_all(const Args& a, const Crew<KT, kThreads>& crew, First& first, int64_t* sums) {
+  constexpr int kWarps = kThreads / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t units = 0, items = 0;
+  int most = 0;
+  for (int64_t b0 = 0; b0 < a.B; b0 += crew.seqs) {
+    int tiles;
+    const int64_t hu = crew.head_units(a, b0 + crew.me, tiles);
+    const int64_t u = crew.at == 0 ? hu * a.Hk : 0;
+    if (b0 == 0) first.head = hu, first.units = u;
+    units += u;
+    if (kItems && crew.at == 0 && tiles) {
+      items += (int64_t)tiles * a.Hk;
+      most = max(most, item_units<KT>(a, get_seq(a, (int)(b0 + crew.me)), tiles - 1));
+    }
+  }
+  // with one round the sum's own prefix is the place of each sequence
+  const int64_t x = warp_scan(units);
+  if (lane == 31) sums[warp] = x;
+  if (kItems) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      items += __shfl_xor_sync(0xffffffffu, items, o);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    if (lane == 0) sums[kWarps + warp] = items, sums[2 * kWarps + warp] = most;
+  }
+  __syncthreads();
+  Total t = {0, 0, 0};
+  first.before = x - units;
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) first.before += sums[i];
+    t.units += sums[i];
+    if (kItems) t.items += sums[kWarps + i], t.most = max(t.most, (int)sums[2 * kWarps + i]);
+  }
+  return t;
+}
+
+// Every thread of the block; finds the walk of this CTA, `per` tiles a CTA.
+template <int KT, int kThreads>
+__device__ void start_walk(const Args& a, const Crew<KT, kThreads>& crew, const Total& total,
+                           const First& first, int64_t per, Walk<KT>& w, Found* sh, int64_t* sums) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t first = 0, mine = 0;
-  for (int64_t b = threadIdx.x; b < a.B; b += kThreads) {
-    const int64_t u = head_units<KT>(a, get_seq(a, (int)b)) * a.Hk;
-    if (b < kThreads) first = u;
-    mine += u;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
-  if (threadIdx.x == 0) sh->b = -1;
-  __syncthreads();
-  int64_t total = 0;
-  for (int i = 0; i < kWarps; ++i) total += sums[i];
-  int64_t per = (total + a.ctas - 1) / a.ctas;
-  if (per < kLeast) per = kLeast;
   const int64_t unit = (int64_t)blockIdx.x * per;
   w.unit = unit;
-  w.end = unit + per < total ? unit + per : total;
-  if (unit >= total) return per;  // nothing here (the same for every thread)
-  int64_t base = 0;
-  for (int64_t at = 0; at < a.B; at += kThreads) {
-    const int64_t b = at + threadIdx.x;
-    int64_t u = at == 0 ? first : 0;
-    if (at && b < a.B) u = head_units<KT>(a, get_seq(a, (int)b)) * a.Hk;
-    int64_t x = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+  w.end = unit + per < total.units ? unit + per : total.units;
+  if (unit >= total.units) return;  // nothing here (the same for every thread)
+  if (a.B <= crew.seqs) {
+    if (first.units > 0 && first.before <= unit && unit < first.before + first.units)
+      sh->b = crew.me, sh->rem = unit - first.before, sh->head = first.head;
+    __syncthreads();
+  } else {
+    int64_t base = 0;
+    for (int64_t b0 = 0; b0 < a.B; b0 += crew.seqs) {
+      int tiles;
+      const int64_t hu = crew.head_units(a, b0 + crew.me, tiles);
+      const int64_t u = crew.at == 0 ? hu * a.Hk : 0;
+      const int64_t x = warp_scan(u);
+      __syncthreads();
+      if (lane == 31) sums[warp] = x;
+      __syncthreads();
+      int64_t before = base + x - u, all = 0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) before += sums[i];
+        all += sums[i];
+      }
+      if (u > 0 && before <= unit && unit < before + u)
+        sh->b = (int)(b0 + crew.me), sh->rem = unit - before, sh->head = hu;
+      base += all;
+      __syncthreads();
+      if (base > unit) break;
     }
-    __syncthreads();
-    if (lane == 31) sums[warp] = x;
-    __syncthreads();
-    int64_t before = base + x - u, all = 0;
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) before += sums[i];
-      all += sums[i];
-    }
-    if (u > 0 && before <= unit && unit < before + u) sh->b = (int)b, sh->rem = unit - before;
-    base += all;
-    __syncthreads();
-    if (base > unit) break;
   }
   w.b = sh->b;
   int64_t rem = sh->rem;
   w.s = get_seq(a, w.b);
-  const int64_t hu = head_units<KT>(a, w.s);
-  w.h = (int)(rem / hu);
-  rem -= w.h * hu;
+  w.h = (int)(rem / sh->head);
+  rem -= w.h * sh->head;
   w.rt = 0;
   if (!a.causal) {
     const int t = w.item_tiles(a);
     w.rt = (int)(rem / t);
     rem -= (int64_t)w.rt * t;
   } else {
-    for (int t = w.item_tiles(a); rem >= t; t = w.item_tiles(a)) rem -= t, ++w.rt;
+    // a warp at a time: 32 items
+    for (;; w.rt += 32) {
+      const int x = warp_scan(item_units<KT>(a, w.s, w.rt + lane));
+      const uint32_t past = __ballot_sync(0xffffffffu, x > rem);
+      const int to = past ? __ffs(past) - 1 : 32;
+      rem -= to ? __shfl_sync(0xffffffffu, x, to - 1) : 0;
+      if (past) {
+        w.rt += to;
+        break;
+      }
+    }
   }
   w.t0 = (int)rem;
-  return per;
+}
+
+// One warp: item number `place` of all items in the order of their length, longest first.  Items
+// of a sequence grow along it, so how many have at least t tiles follows from one division; a
+// binary search over t, a sum over the sequences a step, finds the length at that place.  `mine`:
+// sequence number `lane`, read once.
+template <int KT>
+__device__ Segment item_at(const Args& a, uint32_t place, int most, const Seq& mine) {
+  const int lane = threadIdx.x & 31;
+  auto seq = [&](int b) { return b < 32 ? mine : get_seq(a, b); };  // b % 32 == lane
+  // items of a key head of sequence b with at least t tiles (every item counts as one)
+  auto at_least = [&](const Seq& s, int t) -> int {
+    const int tiles = (int)((uint32_t)(s.n + a.tokens - 1) / (uint32_t)a.tokens);
+    if (t <= 1 || tiles == 0) return tiles;
+    const int64_t x = (int64_t)(t - 1) * KT;  // seen keys > x
+    if (s.len <= x) return 0;
+    if (!a.causal) return tiles;
+    const int64_t i = x - s.off;  // tokens of the chunk that do not reach
+    if (i >= s.n) return 0;
+    const int first = i < 0 ? 0 : (int)((uint32_t)i / (uint32_t)a.tokens);
+    return tiles - min(first, tiles - 1);
+  };
+  auto all_at_least = [&](int t) {  // there are fewer than 2^30 items
+    uint32_t n = 0;
+    for (int b = lane; b < a.B; b += 32) n += at_least(seq(b), t);
+    return __reduce_add_sync(0xffffffffu, n) * (uint32_t)a.Hk;
+  };
+  int lo = 1, hi = most;  // the largest t with more than `place` items of at least t
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (all_at_least(mid) > place) lo = mid; else hi = mid - 1;
+  }
+  uint32_t k = place - all_at_least(lo + 1);  // among those of lo tiles
+  Segment g;
+  for (int b0 = 0;; b0 += 32) {
+    const int b = b0 + lane;
+    Seq s = {};
+    int n = 0, above = 0;
+    if (b < a.B) {
+      s = seq(b);
+      above = at_least(s, lo + 1);
+      n = at_least(s, lo) - above;
+    }
+    const uint32_t x = warp_scan((uint32_t)n * (uint32_t)a.Hk);
+    const uint32_t past = __ballot_sync(0xffffffffu, x > k);
+    if (!past) {
+      if (b0 + 32 >= a.B) {  // not reached: every place has an item
+        g.b = -1;
+        return g;
+      }
+      k -= __shfl_sync(0xffffffffu, x, 31);
+      continue;
+    }
+    const int to = __ffs(past) - 1;
+    k -= __shfl_sync(0xffffffffu, x - (uint32_t)n * (uint32_t)a.Hk, to);
+    n = __shfl_sync(0xffffffffu, n, to);
+    above = __shfl_sync(0xffffffffu, above, to);
+    g.b = b0 + to;
+    g.s.n = __shfl_sync(0xffffffffu, s.n, to);
+    g.s.len = __shfl_sync(0xffffffffu, s.len, to);
+    g.s.off = __shfl_sync(0xffffffffu, s.off, to);
+    g.s.t0 = __shfl_sync(0xffffffffu, s.t0, to);
+    g.h = (int)(k / (uint32_t)n);
+    g.rt = (int)((uint32_t)(g.s.n + a.tokens - 1) / (uint32_t)a.tokens) - above - 1 - ((int)k - g.h * n);
+    g.t0 = 0;
+    g.t1 = g.tiles = item_units<KT>(a, g.s, g.rt);
+    return g;
+  }
 }
 
 // One thread: the record of an item that begins in this CTA and ends in another.
@@ -276,7 +425,7 @@ struct Shape {
   static constexpr int kRowBytes = D * 2, kChunks = D / 8;
   static constexpr int kStage = 2 * 16 * kRowBytes;           // K and V strip of a warp
   static constexpr int kStages = kRing / (4 * kStage);
-  static constexpr int kPad = D + 4;                           // floats a row of the join
+  static_assert(kStage == 16 * D * 4, "a stage holds 16 rows of floats");
 };
 
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
@@ -306,13 +455,18 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
   using S = Shape<D>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Found found;
-  __shared__ int64_t sums[4];
+  __shared__ int64_t sums[3 * kThreads / 32];
   __shared__ float s_ml[4][kRows][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
-  Walk<kKeys> w;
-  const int64_t per = start_walk<kKeys, kThreads, kLeast>(a, w, &found, sums);
   let_next_start();
+  Walk<kKeys> w;
+  const Crew<kKeys, kThreads> crew(a.B);
+  First first;
+  const Total total = count_all<kKeys, kThreads, false>(a, crew, first, sums);
+  int64_t per = (total.units + a.ctas - 1) / a.ctas;
+  if (per < kLeast) per = kLeast;
+  start_walk<kKeys>(a, crew, total, first, per, w, &found, sums);
   if (threadIdx.x == 0) write_rec(a, w, per);
 
   uint8_t* ring = smem + warp * (S::kStages * S::kStage);
@@ -321,8 +475,54 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
   const T* const vp = reinterpret_cast<const T*>(a.v);
   const int qrow = lane >> 2, qcol = (lane & 3) * 2;
 
+  int base = 0;  // ring stage of a segment's first strip
+  int pid = -1;  // page of the strip that is loaded next
+  auto strip = [&](const Segment& g, int j) { return (g.t0 + j) * kKeys + warp * 16; };
+  // keys that the tile's last token sees: those past them are not loaded
+  auto last_seen = [&](const Segment& g) { return seen_by(a, g.s, min(g.s.n, (g.rt + 1) * a.tokens)); };
+  auto page_of = [&](const Segment& g, int vis, int j) {  // (pages are multiples of 16 rows)
+    const int key = strip(g, j);
+    return j < g.t1 - g.t0 && key < vis ? __ldg(a.table + (int64_t)g.b * a.width + key / a.page) : -1;
+  };
+  auto load = [&](const Segment& g, int vis, int j, int stage) {
+    const int key = strip(g, j);
+    if (j < g.t1 - g.t0 && key < vis) {
+      const bool in = pid >= 0 && pid < a.pages;
+      const int slot = key % a.page;
+      const int64_t p = in ? pid : 0;
+      const T* ks = kp + p * a.k_page + (int64_t)slot * a.k_slot + g.h * a.k_head;
+      const T* vs = vp + p * a.v_page + (int64_t)slot * a.v_slot + g.h * a.v_head;
+      const uint32_t st = ring_u + (uint32_t)(stage * S::kStage);
+      const int c = lane % S::kChunks;
+#pragma unroll
+      for (int i = 0; i < S::kChunks / 2; ++i) {
+        const int r = i * (32 / S::kChunks) + lane / S::kChunks;
+        const uint32_t dst = st + (uint32_t)(r * S::kRowBytes + ((c ^ (r & 7)) << 4));
+        const bool take = in && key + r < g.s.len;
+        const int rr = take ? r : 0;
+        cp_async16_or_zero(dst, ks + rr * a.k_slot + c * 8, take);
+        cp_async16_or_zero(dst + S::kStage / 2, vs + rr * a.v_slot + c * 8, take);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // a segment's first strips, but for one stage of the ring; page numbers are fetched one strip
+  // ahead of the strip that needs them
+  auto begin = [&](const Segment& g, int vis) {
+    pid = page_of(g, vis, 0);
+#pragma unroll 1
+    for (int j = 0; j < S::kStages - 1; ++j) {
+      const int nx = page_of(g, vis, j + 1);
+      load(g, vis, j, (base + j) % S::kStages);
+      pid = nx;
+    }
+  };
+
   Segment g;
-  while (w.next(a, g)) {
+  bool more = w.next(a, g);
+  int vis = more ? last_seen(g) : 0;
+  if (more) begin(g, vis);
+  while (more) {
     const int row0 = g.rt * a.rows;
     const int left = g.s.n * a.g - row0;
     const int rows = left < a.rows ? left : a.rows;
@@ -344,60 +544,25 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         qf[kk][hh + 2] = ok ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
       }
     }
-    const int vis = seen_by(a, g.s, min(g.s.n, (g.rt + 1) * a.tokens));  // by the tile's last token
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     const int steps = g.t1 - g.t0;
-    const int32_t* row = a.table + (int64_t)g.b * a.width;
-    auto strip = [&](int j) { return (g.t0 + j) * kKeys + warp * 16; };
-    auto page_of = [&](int j) {  // page of a strip (pages are multiples of 16 rows)
-      const int key = strip(j);
-      return j < steps && key < vis ? __ldg(row + key / a.page) : -1;
-    };
-    auto load = [&](int j, int pid) {
-      const int key = strip(j);
-      if (j < steps && key < vis) {
-        const bool in = pid >= 0 && pid < a.pages;
-        const int slot = key % a.page;
-        const int64_t p = in ? pid : 0;
-        const T* ks = kp + p * a.k_page + (int64_t)slot * a.k_slot + g.h * a.k_head;
-        const T* vs = vp + p * a.v_page + (int64_t)slot * a.v_slot + g.h * a.v_head;
-        const uint32_t st = ring_u + (uint32_t)((j % S::kStages) * S::kStage);
-        const int c = lane % S::kChunks;
-#pragma unroll
-        for (int i = 0; i < S::kChunks / 2; ++i) {
-          const int r = i * (32 / S::kChunks) + lane / S::kChunks;
-          const uint32_t dst = st + (uint32_t)(r * S::kRowBytes + ((c ^ (r & 7)) << 4));
-          const bool take = in && key + r < g.s.len;
-          const int rr = take ? r : 0;
-          cp_async16_or_zero(dst, ks + rr * a.k_slot + c * 8, take);
-          cp_async16_or_zero(dst + S::kStage / 2, vs + rr * a.v_slot + c * 8, take);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    // page numbers are fetched one strip ahead of the strip that needs them
-    int pid = page_of(0);
-#pragma unroll 1
-    for (int j = 0; j < S::kStages - 1; ++j) {
-      const int nx = page_of(j + 1);
-      load(j, pid);
-      pid = nx;
-    }
+    int stage = base;  // of strip j; the one before it is loaded next
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
-      const int nx = page_of(j + S::kStages);
+      const int nx = page_of(g, vis, j + S::kStages);
       cp_async_wait<S::kStages - 2>();
       __syncwarp();  // strip j is there for every lane, strip j - 1 has been read by every lane
-      load(j + S::kStages - 1, pid);
+      load(g, vis, j + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
       pid = nx;
-      const int key0 = strip(j);
-      if (key0 >= vis) continue;
-      const uint32_t ks = ring_u + (uint32_t)((j % S::kStages) * S::kStage);
+      const int key0 = strip(g, j);
+      const uint32_t ks = ring_u + (uint32_t)(stage * S::kStage);
       const uint32_t vs = ks + S::kStage / 2;
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+      if (key0 >= vis) continue;
       float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       {
         const int r = ((lane >> 4) << 3) + (lane & 7);
@@ -459,28 +624,41 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         Pair<T>::mma(o[2 * i + 1], p, b[2], b[3]);
       }
     }
-    cp_async_wait<0>();
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
       l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
     }
-    __syncthreads();  // every warp is done with its ring: the join takes its place
-    float* const so = reinterpret_cast<float*>(smem);
+    __syncwarp();  // every lane has read the last strip
+    // The next segment's first strips are loaded while this one is joined; the join takes the
+    // stage that they leave out, the last strip's: 16 rows of D floats fill it, its 16-byte chunks
+    // in an order of their row's against bank conflicts.
+    base = stage;
+    const int free_stage = (stage == 0 ? S::kStages : stage) - 1;
+    const Segment was = g;
+    more = w.next(a, g);
+    if (more) {
+      vis = last_seen(g);
+      begin(g, vis);
+    }
+    auto joint = [&](int wp, int r, int chunk) {
+      return reinterpret_cast<float*>(smem + (wp * S::kStages + free_stage) * S::kStage) + r * D +
+             ((chunk ^ (r & 7)) << 2);
+    };
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int r = qrow + 8 * hh;
       if (r < rows) {
-        float* dst = so + (warp * kRows + r) * S::kPad + qcol;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hh], o[i][2 * hh + 1]);
+          *reinterpret_cast<float2*>(joint(warp, r, i * 2 + (qcol >> 2)) + (qcol & 3)) =
+              make_float2(o[i][2 * hh], o[i][2 * hh + 1]);
         if ((lane & 3) == 0) s_ml[warp][r][0] = m[hh], s_ml[warp][r][1] = l[hh];
       }
     }
     __syncthreads();
-    const bool whole = g.t0 == 0 && g.t1 == g.tiles;
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (g.t0 == 0);
+    const bool whole = was.t0 == 0 && was.t1 == was.tiles;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (was.t0 == 0);
     for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
       const int r = idx / (D / 4), c = (idx % (D / 4)) * 4;
       float mm = s_ml[0][r][0];
@@ -492,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float f = ex2_approx(s_ml[i][r][0] - sub);
-        const float4 v = *reinterpret_cast<const float4*>(so + (i * kRows + r) * S::kPad + c);
+        const float4 v = *reinterpret_cast<const float4*>(joint(i, r, c >> 2));
         acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y);
         acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
         ll = fmaf(f, s_ml[i][r][1], ll);
@@ -502,8 +680,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         // a row that sees no key is 0, whatever the values that other rows of its tile see
         if (mm == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const int pr = row0 + r, i = pr / a.g;
-        T* dst = reinterpret_cast<T*>(a.out) + (g.s.t0 + i) * a.o_token +
-                 (int64_t)(g.h * a.g + pr - i * a.g) * a.o_head + c;
+        T* dst = reinterpret_cast<T*>(a.out) + (was.s.t0 + i) * a.o_token +
+                 (int64_t)(was.h * a.g + pr - i * a.g) * a.o_head + c;
         *reinterpret_cast<uint2*>(dst) =
             make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
       } else {
@@ -512,8 +690,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
           *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(mm, ll);
       }
     }
-    __syncthreads();  // the ring is loaded again
+    __syncthreads();  // the joint's stage is loaded again
   }
+  cp_async_wait<0>();
 }
 
 }  // namespace dec
@@ -531,6 +710,10 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
 namespace chunk {
 
 constexpr int kThreads = 384, kRows = 256, kKeys = 128, kLeast = 2;
+#ifndef KCUT
+#define KCUT 12
+#endif
+constexpr int kCut = KCUT;  // key tiles, see where items are dealt out
 constexpr int kAtom = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzle
 constexpr float kLazy = 8.0f;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
@@ -543,7 +726,9 @@ struct Shape {
   // 2.12 to 1.95 million clocks and 1390 to 1360 us (the clock gives way to the load); other shares
   // gained less.  Ragged chunks of D 64: none 64.8 us, an eighth 62.1, a quarter 62.1.
   static constexpr uint32_t kFma = D == 128 ? 0x22u : 0x10u;
-  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // align, barriers
+  // alignment, barriers, and each softmax warp's 32 rows of 64 bytes (pitch 80) on their way out
+  static constexpr int kStage = 32 * 80;
+  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024 + 8 * kStage;
 };
 
 // 2^x of two numbers without the special-function unit, which at 16 a clock and SM would need as
@@ -675,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // that sits out keys which the other one sees falls further behind than that.
   __shared__ uint32_t s_copied[2];
   __shared__ Found found;
-  __shared__ int64_t sums[kThreads / 32];
+  __shared__ int64_t sums[3 * kThreads / 32];
 
   const int warp = warp_id_uniform();
   const int lane = threadIdx.x & 31;
@@ -700,9 +885,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  Walk<kKeys> w;
-  const int64_t per = start_walk<kKeys, kThreads, kLeast>(a, w, &found, sums);
   let_next_start();
+  // Cut items at CTA boundaries, or whole ones to each CTA, longest first and there and back (so the
+  // longest is paired with the shortest of the next round)?  A cut costs both CTAs a write of 256 rows
+  // of floats and the join their reads: 18 us for all, about kCut tiles' time.  Whole items cost
+  // what the last, incomplete round leaves idle, or an item longer than a CTA's share.
+  Walk<kKeys> w = {};
+  const Crew<kKeys, kThreads> crew(a.B);
+  First first;
+  const Total total = count_all<kKeys, kThreads, true>(a, crew, first, sums);
+  int64_t per = (total.units + a.ctas - 1) / a.ctas;
+  if (per < kLeast) per = kLeast;
+  const int64_t rounds = (total.items + a.ctas - 1) / a.ctas;
+  const bool cut = total.items < a.ctas || total.most > per + kCut ||
+                   (rounds * a.ctas - total.items) * total.units > kCut * a.ctas * total.items;
+  if (cut) start_walk<kKeys>(a, crew, total, first, per, w, &found, sums);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -726,55 +923,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int64_t nk = 0, nv = 0;       // tiles issued
     uint32_t nq[2] = {0, 0};
-    // a tile is `boxes` boxes of `box` rows, each inside one page; lane i loads box i
-    auto tile = [&](uint8_t* ring, const CUtensorMap& tm, uint64_t* full, uint64_t* empty,
-                    int64_t& count, int j) {
-      const int s = (int)(count % kSlots);
-      const uint32_t ph = (uint32_t)(count / kSlots) & 1u;
+    // a tile is `boxes` boxes of `box` rows, each inside one page; lane i loads box i.  Page
+    // numbers are fetched a tile ahead, and V takes K's.
+    struct Place {
+      int row, page;  // in the page; past the sequence's end, and numbers outside the pool: zeros
+    };
+    auto look = [&](int j) {
       const Desc& g = DESC();
       const int key = (g.key_t0 + j) * kKeys + lane * box;
-      int pid = -1;  // past the end, and numbers outside the pool: zeros
-      if (lane < boxes && key < g.len) pid = __ldg(a.table + g.b * a.width + key / a.page);
+      const int at = (int)((uint32_t)key / (uint32_t)a.page);
+      Place p = {key - at * a.page, -1};
+      if (lane < boxes && key < g.len) p.page = __ldg(a.table + g.b * a.width + at);
+      return p;
+    };
+    auto tile = [&](uint8_t* ring, const CUtensorMap& tm, uint64_t* full, uint64_t* empty,
+                    int64_t& count, const Place& p) {
+      const int s = (int)(count % kSlots);
+      const uint32_t ph = (uint32_t)(count / kSlots) & 1u;
       if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ph ^ 1u, 0x901u))) return false;
       if (lane == 0) mbar_arrive_expect_tx(full + s, S::kTile);
       __syncwarp();
       if (lane < boxes) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(ring + s * S::kTile + c * kAtom + lane * box * 128, &tm, full + s, c * 64, g.h,
-                      key % a.page, pid);
+          tma_load_4d(ring + s * S::kTile + c * kAtom + lane * box * 128, &tm, full + s, c * 64, DESC().h,
+                      p.row, p.page);
       }
       ++count;
       return true;
     };
     while (ok && __all_sync(0xffffffffu, next_segment())) {
       const int all = DESC().all;
+      Place now = look(0), before = now;
+      // Q of both halves: boxes of a token's g heads for 128 / g tokens (rows past the
+      // sequence's end are other tokens', or zeros: nobody stores them)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (!ok || DESC().cnt[x] == 0) continue;
+        if (!__all_sync(0xffffffffu, mbar_wait(BAR(x, Q_EMPTY), (nq[x] & 1u) ^ 1u, 0x912u))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const Desc& g = DESC();
+          mbar_arrive_expect_tx(BAR(x, Q_FULL), (uint32_t)(half_rows * D * 2));
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(sQ + x * S::kTile + c * kAtom, &tmQ, BAR(x, Q_FULL), c * 64, g.h * a.g,
+                        (int)g.t0 + (g.row0 + x * half_rows) / a.g, 0);
+        }
+        __syncwarp();
+        ++nq[x];
+      }
       // the MMA threads take K(0) K(1) V(0) K(2) V(1) ...
       for (int j = 0; j <= all && all > 0 && ok; ++j) {
-        if (j < all) ok = tile(sK, tmK, k_full, k_empty, nk, j);
-        if (j == 0) {
-          // Q of both halves: boxes of a token's g heads for 128 / g tokens (rows past the
-          // sequence's end are other tokens', or zeros: nobody stores them)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!ok || DESC().cnt[x] == 0) continue;
-            if (!__all_sync(0xffffffffu, mbar_wait(BAR(x, Q_EMPTY), (nq[x] & 1u) ^ 1u, 0x912u))) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) {
-              const Desc& g = DESC();
-              mbar_arrive_expect_tx(BAR(x, Q_FULL), (uint32_t)(half_rows * D * 2));
-#pragma unroll
-              for (int c = 0; c < D / 64; ++c)
-                tma_load_4d(sQ + x * S::kTile + c * kAtom, &tmQ, BAR(x, Q_FULL), c * 64, g.h * a.g,
-                            (int)g.t0 + (g.row0 + x * half_rows) / a.g, 0);
-            }
-            __syncwarp();
-            ++nq[x];
-          }
-        }
-        if (ok && j >= 1) ok = tile(sV, tmV, v_full, v_empty, nv, j - 1);
+        const Place next = j + 1 < all ? look(j + 1) : now;
+        if (j < all) ok = tile(sK, tmK, k_full, k_empty, nk, now);
+        if (ok && j >= 1) ok = tile(sV, tmV, v_full, v_empty, nv, before);
+        before = now;
+        now = next;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(d_empty + seg % kDescs);
@@ -792,12 +999,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ segments
-    if (lane == 0) {
-      const Walk<kKeys> start = w;
-      Segment g;
-      for (bool more = true; more; ++seg) {
+    const Walk<kKeys> start = w;
+    Seq mine = {};
+    if (lane < a.B) mine = get_seq(a, lane);
+    Segment g;
+    int64_t round = 0;
+    for (bool more = true; more; ++seg) {
+      if (cut) {
         more = w.next(a, g);
-        if (!mbar_wait(d_empty + seg % kDescs, ((seg / kDescs) & 1u) ^ 1u, 0x90fu)) break;
+      } else {
+        const int64_t place = round * a.ctas + (round & 1 ? a.ctas - 1 - blockIdx.x : blockIdx.x);
+        more = place < total.items;
+        if (more) g = item_at<kKeys>(a, (uint32_t)place, total.most, mine);
+        more = more && g.b >= 0;
+        ++round;
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(d_empty + seg % kDescs, ((seg / kDescs) & 1u) ^ 1u, 0x90fu)))
+        break;
+      if (lane == 0) {
         Desc& d = descs[seg % kDescs];
         d.more = more;
         if (more) {
@@ -814,7 +1033,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_arrive(d_full + seg % kDescs);
       }
-      write_rec(a, start, per);
+      __syncwarp();
+    }
+    if (lane == 0) {
+      if (cut) write_rec(a, start, per);
+      else a.rec[(int64_t)blockIdx.x * 8] = 0;
     }
   } else if (warp >= 10) {
     // ------------------------------------------------------------ MMA issuer of tile x
@@ -936,6 +1159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tO = tmem + kColO + (uint32_t)(x * 128) + lane_addr;
     const float c = a.scale_log2;
     const int half_rows = a.rows >> 1;
+    uint8_t* const stage = reinterpret_cast<uint8_t*>(bars) + 1024 + warp * S::kStage;
     bool ok = true;
     uint32_t kv = 0, mine = 0;
     while (ok && __all_sync(0xffffffffu, next_segment())) {
@@ -1110,13 +1334,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace chunk
 
 // ===========================================================================
-// Joins the parts of an item that CTA boundaries cut, in their order.  D / 8 lanes take a row, or
-// with few rows a part of it (ROWS false: a block a row, its groups every G-th part).  Launched
-// while the kernel before it still runs, it waits for that one's end before it reads anything.
+// Joins the parts of an item that CTA boundaries cut, in their order.  D / 8 lanes take a row
+// (ROWS), or with few rows and hundreds of parts a block takes a row and its groups every G-th part,
+// four of them in flight.  Launched while the kernel before it still runs, it waits for that one's
+// end before it reads anything.
 // ===========================================================================
 template <typename T, int D, int R, bool ROWS>
-__global__ void __launch_bounds__(128) merge_kernel(const Args a) {
-  constexpr int kLanes = D / 8, G = 128 / kLanes;
+__global__ void __launch_bounds__(256) merge_kernel(const Args a) {
+  constexpr int kLanes = D / 8, G = 256 / kLanes;
+  constexpr int kFlight = ROWS ? 2 : 4;
   __shared__ float s_o[ROWS ? 1 : G][D];
   __shared__ float s_l[ROWS ? 1 : G];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1125,57 +1351,73 @@ __global__ void __launch_bounds__(128) merge_kernel(const Args a) {
   const int4 rec = *reinterpret_cast<const int4*>(a.rec + (int64_t)c0 * 8);  // valid, b, h, rt
   if (!rec.x) return;
   const int parts = a.rec[(int64_t)c0 * 8 + 4] - c0 + 1;
-  const int row = ROWS ? blockIdx.y * G + group : blockIdx.y;
   const Seq s = get_seq(a, rec.y);
-  const int64_t pr = (int64_t)rec.w * a.rows + row;
-  const bool live = row < a.rows && pr < (int64_t)s.n * a.g;
-  if (!ROWS && !live) return;  // the whole block
-  auto slot = [&](int p) { return ((int64_t)(c0 + p) * 2 + (p == 0)) * R + row; };
-  float mm = -INFINITY;
-  if (live)
-    for (int p = ROWS ? gl : threadIdx.x & 31; p < parts; p += ROWS ? kLanes : 32)
-      mm = fmaxf(mm, a.part_ml[slot(p) * 2]);
+  // ROWS: one pass, a row a group; else a row a block
+  for (int row = ROWS ? blockIdx.y * G + group : blockIdx.y; ROWS || row < a.rows; row += gridDim.y) {
+    const int64_t pr = (int64_t)rec.w * a.rows + row;
+    const bool live = row < a.rows && pr < (int64_t)s.n * a.g;
+    if (!ROWS && !live) return;  // the whole block: later rows are not there either
+    auto slot = [&](int p) { return ((int64_t)(c0 + p) * 2 + (p == 0)) * R + row; };
+    float mm = -INFINITY;
+    if (live)
+      for (int p = ROWS ? gl : threadIdx.x & 31; p < parts; p += ROWS ? kLanes : 32)
+        mm = fmaxf(mm, a.part_ml[slot(p) * 2]);
 #pragma unroll
-  for (int o = (ROWS ? kLanes : 32) / 2; o > 0; o >>= 1)
-    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  float acc[8], l = 0.f;
+    for (int o = (ROWS ? kLanes : 32) / 2; o > 0; o >>= 1)
+      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    float acc[8], l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-  if (live) {
-#pragma unroll 2
-    for (int p = ROWS ? 0 : group; p < parts; p += ROWS ? 1 : G) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(p) * 2);
-      if (ml.x == -INFINITY) continue;
-      const float f = ex2_approx(ml.x - mm);
-      const float4* o = reinterpret_cast<const float4*>(a.part + slot(p) * D + gl * 8);
-      const float4 x = o[0], y = o[1];
-      acc[0] = fmaf(f, x.x, acc[0]), acc[1] = fmaf(f, x.y, acc[1]);
-      acc[2] = fmaf(f, x.z, acc[2]), acc[3] = fmaf(f, x.w, acc[3]);
-      acc[4] = fmaf(f, y.x, acc[4]), acc[5] = fmaf(f, y.y, acc[5]);
-      acc[6] = fmaf(f, y.z, acc[6]), acc[7] = fmaf(f, y.w, acc[7]);
-      l = fmaf(f, ml.y, l);
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    if (live) {
+      constexpr int kStep = ROWS ? 1 : G;
+      for (int p0 = ROWS ? 0 : group; p0 < parts; p0 += kStep * kFlight) {
+        float2 ml[kFlight];
+        float4 x[kFlight], y[kFlight];
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+          const int p = p0 + i * kStep;
+          ml[i] = make_float2(-INFINITY, 0.f);
+          if (p >= parts) continue;
+          ml[i] = *reinterpret_cast<const float2*>(a.part_ml + slot(p) * 2);
+          const float4* o = reinterpret_cast<const float4*>(a.part + slot(p) * D + gl * 8);
+          x[i] = o[0], y[i] = o[1];  // whatever it is where the part saw no key: not used then
+        }
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+          if (ml[i].x == -INFINITY) continue;
+          const float f = ex2_approx(ml[i].x - mm);
+          acc[0] = fmaf(f, x[i].x, acc[0]), acc[1] = fmaf(f, x[i].y, acc[1]);
+          acc[2] = fmaf(f, x[i].z, acc[2]), acc[3] = fmaf(f, x[i].w, acc[3]);
+          acc[4] = fmaf(f, y[i].x, acc[4]), acc[5] = fmaf(f, y[i].y, acc[5]);
+          acc[6] = fmaf(f, y[i].z, acc[6]), acc[7] = fmaf(f, y[i].w, acc[7]);
+          l = fmaf(f, ml[i].y, l);
+        }
+      }
     }
-  }
-  if (!ROWS) {
+    if (!ROWS) {
+      __syncthreads();  // the last row's sums have been read
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s_o[group][gl * 8 + i] = acc[i];
-    if (gl == 0) s_l[group] = l;
-    __syncthreads();
-    if (group) return;
-    for (int q = 1; q < G && q < parts; ++q) {
-      l += s_l[q];
+      for (int i = 0; i < 8; ++i) s_o[group][gl * 8 + i] = acc[i];
+      if (gl == 0) s_l[group] = l;
+      __syncthreads();
+      if (group) continue;
+      for (int q = 1; q < G && q < parts; ++q) {
+        l += s_l[q];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += s_o[q][gl * 8 + i];
+        for (int i = 0; i < 8; ++i) acc[i] += s_o[q][gl * 8 + i];
+      }
     }
+    if (live) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const int64_t i = pr / a.g;
+      T* dst = reinterpret_cast<T*>(a.out) + (s.t0 + i) * a.o_token +
+               ((int64_t)rec.z * a.g + pr - i * a.g) * a.o_head + gl * 8;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(
+          Pair<T>::pack(acc[0] * inv, acc[1] * inv), Pair<T>::pack(acc[2] * inv, acc[3] * inv),
+          Pair<T>::pack(acc[4] * inv, acc[5] * inv), Pair<T>::pack(acc[6] * inv, acc[7] * inv));
+    }
+    if (ROWS) return;
   }
-  if (!live) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const int64_t i = pr / a.g;
-  T* dst = reinterpret_cast<T*>(a.out) + (s.t0 + i) * a.o_token +
-           ((int64_t)rec.z * a.g + pr - i * a.g) * a.o_head + gl * 8;
-  *reinterpret_cast<uint4*>(dst) =
-      make_uint4(Pair<T>::pack(acc[0] * inv, acc[1] * inv), Pair<T>::pack(acc[2] * inv, acc[3] * inv),
-                 Pair<T>::pack(acc[4] * inv, acc[5] * inv), Pair<T>::pack(acc[6] * inv, acc[7] * inv));
 }
 
 // Whether the rows of the longest sequence fit the few-rows kernel.  Measured at 48 sequences of
@@ -1186,7 +1428,7 @@ inline int ctas_of(bool few) { return sm_count() * (few ? 2 : 1); }
 int launch_merge(void (*kernel)(Args), dim3 grid, const Args& a, cudaStream_t stream) {
   cudaLaunchConfig_t c = {};
   c.gridDim = grid;
-  c.blockDim = dim3(128);
+  c.blockDim = dim3(256);
   c.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1216,7 +1458,8 @@ int launch(Args& a, bool few, cudaStream_t stream) {
     dec::decode_kernel<T, D><<<a.ctas, dec::kThreads, dec::kRing, stream>>>(a);
     int rc = check_launch("fvb_paged_attn");
     if (rc) return rc;
-    return launch_merge(merge_kernel<T, D, dec::kRows, false>, dim3(a.ctas, dec::kRows), a, stream);
+    // a block a row; a few of them look after the rows that a false max_new did not announce
+    return launch_merge(merge_kernel<T, D, dec::kRows, false>, dim3(a.ctas, a.few_rows), a, stream);
   }
   // rows of a TMA box: a power of two that divides the page, at most a tile
   int box = 16;
@@ -1240,7 +1483,7 @@ int launch(Args& a, bool few, cudaStream_t stream) {
   chunk::chunk_kernel<T, D><<<a.ctas, chunk::kThreads, chunk::Shape<D>::kSmem, stream>>>(tq, tk, tv, box, a);
   rc = check_launch("fvb_paged_attn");
   if (rc) return rc;
-  return launch_merge(merge_kernel<T, D, chunk::kRows, true>, dim3(a.ctas, chunk::kRows * (D / 8) / 128), a,
+  return launch_merge(merge_kernel<T, D, chunk::kRows, true>, dim3(a.ctas, chunk::kRows * (D / 8) / 256), a,
                       stream);
 }
 
@@ -1312,6 +1555,7 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
   // whole tokens in a tile, and with many rows in each half of it
   a.tokens = few ? pattn::dec::kRows / a.g : 2 * (128 / a.g);
   a.rows = a.tokens * a.g;
+  a.few_rows = (int)(few ? p->max_new * a.g : a.rows);
   a.scale_log2 = (float)(p->scale * 1.4426950408889634);
   a.part = (float*)(ws + w.part);
   a.part_ml = (float*)(ws + w.ml);

@@ -23,7 +23,8 @@ _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
 
 
 def _ints(t, n, what, name, index):
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
+    s = t.shape
+    if t.dtype != torch.int32 or len(s) != 1 or (n is not None and s[0] != n):
         raise ValueError(f"{name}: {what} must be int32 [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
     if t.get_device() != index:
         raise ValueError(f"{name}: {what} is on {t.device}, the cache on cuda:{index}")
@@ -252,9 +253,9 @@ class PagedKV:
         H, D, P, page = self._shape
         if not (k.is_cuda and v.is_cuda and cu_seqlens.is_cuda):
             _lib.require_cuda(k, v, cu_seqlens)
-        k, v = _rows(k, "k", name), _rows(v, "v", name)
-        T, Hk, Dk = k.shape
-        if Hk != H or Dk != D or v.shape != k.shape:
+        k, T, Hk, Dk, kt, kh = _rows(k, "k", name)
+        v, Tv, Hv, Dv, vt, vh = _rows(v, "v", name)
+        if Hk != H or Dk != D or Tv != T or Hv != H or Dv != D:
             raise ValueError(f"{name}: k and v must be [T, {H}, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
         if k.dtype != dt or v.dtype != dt or k.get_device() != index or v.get_device() != index:
             raise ValueError(f"{name}: k and v must be {dt} on {self.device}")
@@ -271,12 +272,10 @@ class PagedKV:
                 raise ValueError(f"{name}: q without a Rope has nothing to be done to it")
             if q.dtype != dt or q.get_device() != index:
                 raise ValueError(f"{name}: q must be {dt} on {self.device}")
-            q3 = _rows(q, "q", name)
-            Tq, Hq, Dq = q3.shape
+            q3, Tq, Hq, Dq, st, sh = _rows(q, "q", name)
             if Tq != T or Dq != D:
                 raise ValueError(f"{name}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
             oq, ot, oh = _out(out_q, q, "out_q", name)
-            st, sh, _ = q3.stride()
             qargs = (q3.data_ptr(), st, sh, Hq, oq.data_ptr(), ot, oh)
         if rope is None:
             if positions is not None:
@@ -293,8 +292,6 @@ class PagedKV:
                 positions = _positions(positions, rope, T, index, name)
                 pos, pos64 = positions.data_ptr(), _POS64[positions.dtype]
             rargs = (rope.rotary_dim, rope.half, self._dt, pos, pos64, rope.axes, rope._freq, rope._axis, rope.scale)
-        kt, kh, _ = k.stride()
-        vt, vh, _ = v.stride()
         kp, vp, _, layer_bytes, _, _ = self._pools
         at = layer * layer_bytes
         _lib.call_on(index, "fvb_kv_append",

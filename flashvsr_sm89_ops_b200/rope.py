@@ -89,12 +89,18 @@ class Rope:
 
 
 def _rows(x, what, name):
-    """x as [T, H, D] with unit stride inside a head."""
-    if x.dim() == 4:
-        x = x.flatten(0, 1) if x.stride(0) == x.shape[1] * x.stride(1) else x.contiguous().flatten(0, 1)
+    """x [T, H, D] or [B, L, H, D] as rows with unit stride inside a head: (x, T, H, D, its strides of
+    tokens and heads)."""
+    s, n = x.stride(), x.shape
+    if len(n) == 3 and (s[2] == 1 or n[2] < 2):
+        return x, n[0], n[1], n[2], s[0], s[1]
+    if len(n) == 4:
+        x = x.flatten(0, 1) if s[0] == n[1] * s[1] else x.contiguous().flatten(0, 1)
     if x.dim() != 3:
         raise ValueError(f"{name}: {what} must be [T, H, D] or [B, L, H, D], got {tuple(x.shape)}")
-    return x if x.shape[2] < 2 or x.stride(2) == 1 else x.contiguous()
+    if x.shape[2] > 1 and x.stride(2) != 1:
+        x = x.contiguous()
+    return x, *x.shape, x.stride(0), x.stride(1)
 
 
 def _positions(positions, rope, T, index, name):
@@ -111,8 +117,9 @@ def _positions(positions, rope, T, index, name):
 def _out(out, x, what, name):
     """The tensor that x's rotation goes to, and its rows' strides of tokens and heads."""
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        n = x.shape
+        return torch.empty_like(x, memory_format=torch.contiguous_format), n[-2] * n[-1], n[-1]
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{name}: {what} must be {x.dtype} {tuple(x.shape)} on {x.device}")
     s = out.stride()
     if len(s) == 4 and s[0] != out.shape[1] * s[1] and out.shape[0] > 1:
@@ -126,15 +133,13 @@ def _run(q, k, positions, rope, inverse, out_q, out_k):
     name = "fused_rope"
     dt = _dtype_code(q.dtype, name)
     index = q.get_device()
-    q3 = _rows(q, "q", name)
-    T, Hq, D = q3.shape
+    q3, T, Hq, D, st, sh = _rows(q, "q", name)
     if rope.rotary_dim > D:
         raise ValueError(f"{name}: rotary_dim {rope.rotary_dim} of a head of {D}")
     if rope.index != index:
         raise ValueError(f"{name}: the Rope is on {rope.device}, q on {q.device}")
     positions = _positions(positions, rope, T, index, name)
     oq, ot, oh = _out(out_q, q, "out_q", name)
-    st, sh, _ = q3.stride()
     if k is None:
         if out_k is not None:
             raise ValueError(f"{name}: out_k without k")
@@ -142,12 +147,10 @@ def _run(q, k, positions, rope, inverse, out_q, out_k):
     else:
         if k.dtype != q.dtype or k.get_device() != index:
             raise ValueError(f"{name}: k is {k.dtype} on {k.device}, q {q.dtype} on {q.device}")
-        k3 = _rows(k, "k", name)
-        Tk, Hk, Dk = k3.shape
+        k3, Tk, Hk, Dk, kt, kh = _rows(k, "k", name)
         if Tk != T or Dk != D:
             raise ValueError(f"{name}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         ok, kot, koh = _out(out_k, k, "out_k", name)
-        kt, kh, _ = k3.stride()
         kargs = (k3.data_ptr(), kt, kh, Hk, ok.data_ptr(), kot, koh)
     _lib.call_on(index, "fvb_rope",
                  _lib.ROPE_ARGS(q3.data_ptr(), st, sh, Hq, oq.data_ptr(), ot, oh, *kargs, T, D, rope.rotary_dim,

@@ -545,6 +545,10 @@ SHAPES = [
     ([1537, 600, 900], [100, 300, 7], 16, 4, 64, 16),
     ([1100, 700], [3, 0], 12, 12, 128, 64),
     ([1500, 2000, 900, 700], [0, 0, 0, 0], 8, 1, 64, 32),
+    # more items than the machine has SMs, of many lengths: whole ones dealt out by length
+    ([0 if i % 7 == 0 else 1 + 41 * i % 131 for i in range(90)], [97 * i % 1300 for i in range(90)], 8, 4, 128, 16),
+    ([300] * 40, [0] * 40, 4, 4, 64, 64),
+    ([130, 1, 1, 2, 64] * 12, [0, 700, 3000, 128, 5] * 12, 12, 4, 128, 32),
 ]
 
 
