@@ -518,17 +518,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
     }
   };
 
-  Segment g;
-  bool more = w.next(a, g);
-  int vis = more ? last_seen(g) : 0;
-  if (more) begin(g, vis);
-  while (more) {
-    const int row0 = g.rt * a.rows;
-    const int left = g.s.n * a.g - row0;
-    const int rows = left < a.rows ? left : a.rows;
-    // Q: fragments of the 16 x D tile
-    uint32_t qf[D / 16][4];
-    int lim[2];
+  // Q of a segment: fragments of its tile, and the keys that this thread's two rows see
+  uint32_t qf[D / 16][4];
+  int lim[2], row0, rows;
+  auto load_q = [&](const Segment& g) {
+    row0 = g.rt * a.rows;
+    rows = min(g.s.n * a.g - row0, a.rows);
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int r = qrow + 8 * hh;
@@ -544,6 +539,16 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         qf[kk][hh + 2] = ok ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
       }
     }
+  };
+
+  Segment g;
+  bool more = w.next(a, g);
+  int vis = more ? last_seen(g) : 0;
+  if (more) {
+    begin(g, vis);
+    load_q(g);
+  }
+  while (more) {
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -636,10 +641,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
     base = stage;
     const int free_stage = (stage == 0 ? S::kStages : stage) - 1;
     const Segment was = g;
+    const int was_row0 = row0, was_rows = rows;
     more = w.next(a, g);
     if (more) {
       vis = last_seen(g);
       begin(g, vis);
+      load_q(g);
     }
     auto joint = [&](int wp, int r, int chunk) {
       return reinterpret_cast<float*>(smem + (wp * S::kStages + free_stage) * S::kStage) + r * D +
@@ -648,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int r = qrow + 8 * hh;
-      if (r < rows) {
+      if (r < was_rows) {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
           *reinterpret_cast<float2*>(joint(warp, r, i * 2 + (qcol >> 2)) + (qcol & 3)) =
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
     __syncthreads();
     const bool whole = was.t0 == 0 && was.t1 == was.tiles;
     const int64_t slot = (int64_t)blockIdx.x * 2 + (was.t0 == 0);
-    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
+    for (int idx = threadIdx.x; idx < was_rows * (D / 4); idx += kThreads) {
       const int r = idx / (D / 4), c = (idx % (D / 4)) * 4;
       float mm = s_ml[0][r][0];
 #pragma unroll
@@ -679,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         const float inv = ll > 0.f ? 1.f / ll : 0.f;
         // a row that sees no key is 0, whatever the values that other rows of its tile see
         if (mm == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int pr = row0 + r, i = pr / a.g;
+        const int pr = was_row0 + r, i = pr / a.g;
         T* dst = reinterpret_cast<T*>(a.out) + (was.s.t0 + i) * a.o_token +
                  (int64_t)(was.h * a.g + pr - i * a.g) * a.o_head + c;
         *reinterpret_cast<uint2*>(dst) =
@@ -710,10 +717,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
 namespace chunk {
 
 constexpr int kThreads = 384, kRows = 256, kKeys = 128, kLeast = 2;
-#ifndef KCUT
-#define KCUT 12
-#endif
-constexpr int kCut = KCUT;  // key tiles, see where items are dealt out
+constexpr int kCut = 12;  // key tiles, see where items are dealt out
 constexpr int kAtom = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzle
 constexpr float kLazy = 8.0f;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
@@ -1334,48 +1338,52 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace chunk
 
 // ===========================================================================
-// Joins the parts of an item that CTA boundaries cut, in their order.  D / 8 lanes take a row
-// (ROWS), or with few rows and hundreds of parts a block takes a row and its groups every G-th part,
-// four of them in flight.  Launched while the kernel before it still runs, it waits for that one's
-// end before it reads anything.
+// Joins the parts of an item that CTA boundaries cut, in their order.  D / 8 lanes (a group) take a
+// row.  With few rows an item can have hundreds of parts: beyond kWide a block takes a row, its groups
+// every G-th part, four in flight, and the groups are joined through shared memory.  Launched while
+// the kernel before it still runs, it waits for that one's end before it reads anything.
 // ===========================================================================
-template <typename T, int D, int R, bool ROWS>
+template <typename T, int D, int R, bool FEW>
 __global__ void __launch_bounds__(256) merge_kernel(const Args a) {
-  constexpr int kLanes = D / 8, G = 256 / kLanes;
-  constexpr int kFlight = ROWS ? 2 : 4;
-  __shared__ float s_o[ROWS ? 1 : G][D];
-  __shared__ float s_l[ROWS ? 1 : G];
+  constexpr int kLanes = D / 8, G = 256 / kLanes, kFlight = 4, kWide = 8;
+  __shared__ float s_o[FEW ? G : 1][D];
+  __shared__ float s_l[FEW ? G : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int gl = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int c0 = blockIdx.x;
   const int4 rec = *reinterpret_cast<const int4*>(a.rec + (int64_t)c0 * 8);  // valid, b, h, rt
   if (!rec.x) return;
   const int parts = a.rec[(int64_t)c0 * 8 + 4] - c0 + 1;
+  const bool wide = FEW && parts > kWide;
   const Seq s = get_seq(a, rec.y);
-  // ROWS: one pass, a row a group; else a row a block
-  for (int row = ROWS ? blockIdx.y * G + group : blockIdx.y; ROWS || row < a.rows; row += gridDim.y) {
-    const int64_t pr = (int64_t)rec.w * a.rows + row;
-    const bool live = row < a.rows && pr < (int64_t)s.n * a.g;
-    if (!ROWS && !live) return;  // the whole block: later rows are not there either
+  const int rows = min(a.rows, s.n * a.g - rec.w * a.rows);
+  // wide: a row a block; else a row a group (a few rows are one block's)
+  if (FEW && !wide && blockIdx.y) return;
+  for (int row0 = wide ? blockIdx.y : blockIdx.y * G; row0 < rows; row0 += wide ? gridDim.y : gridDim.y * G) {
+    const int row = wide ? row0 : row0 + group;
+    const bool live = row < rows;
     auto slot = [&](int p) { return ((int64_t)(c0 + p) * 2 + (p == 0)) * R + row; };
     float mm = -INFINITY;
     if (live)
-      for (int p = ROWS ? gl : threadIdx.x & 31; p < parts; p += ROWS ? kLanes : 32)
+      for (int p = wide ? threadIdx.x & 31 : gl; p < parts; p += wide ? 32 : kLanes)
         mm = fmaxf(mm, a.part_ml[slot(p) * 2]);
 #pragma unroll
-    for (int o = (ROWS ? kLanes : 32) / 2; o > 0; o >>= 1)
-      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    for (int o = kLanes / 2; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    if (wide) {
+#pragma unroll
+      for (int o = kLanes; o < 32; o <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    }
     float acc[8], l = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     if (live) {
-      constexpr int kStep = ROWS ? 1 : G;
-      for (int p0 = ROWS ? 0 : group; p0 < parts; p0 += kStep * kFlight) {
+      const int step = wide ? G : 1;
+      for (int p0 = wide ? group : 0; p0 < parts; p0 += step * kFlight) {
         float2 ml[kFlight];
         float4 x[kFlight], y[kFlight];
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) {
-          const int p = p0 + i * kStep;
+          const int p = p0 + i * step;
           ml[i] = make_float2(-INFINITY, 0.f);
           if (p >= parts) continue;
           ml[i] = *reinterpret_cast<const float2*>(a.part_ml + slot(p) * 2);
@@ -1394,29 +1402,28 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a) {
         }
       }
     }
-    if (!ROWS) {
+    if (wide) {
       __syncthreads();  // the last row's sums have been read
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s_o[group][gl * 8 + i] = acc[i];
-      if (gl == 0) s_l[group] = l;
+      for (int i = 0; i < 8; ++i) s_o[FEW ? group : 0][gl * 8 + i] = acc[i];
+      if (gl == 0) s_l[FEW ? group : 0] = l;
       __syncthreads();
       if (group) continue;
       for (int q = 1; q < G && q < parts; ++q) {
-        l += s_l[q];
+        l += s_l[FEW ? q : 0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += s_o[q][gl * 8 + i];
+        for (int i = 0; i < 8; ++i) acc[i] += s_o[FEW ? q : 0][gl * 8 + i];
       }
     }
     if (live) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int64_t i = pr / a.g;
+      const int64_t pr = (int64_t)rec.w * a.rows + row, i = pr / a.g;
       T* dst = reinterpret_cast<T*>(a.out) + (s.t0 + i) * a.o_token +
                ((int64_t)rec.z * a.g + pr - i * a.g) * a.o_head + gl * 8;
       *reinterpret_cast<uint4*>(dst) = make_uint4(
           Pair<T>::pack(acc[0] * inv, acc[1] * inv), Pair<T>::pack(acc[2] * inv, acc[3] * inv),
           Pair<T>::pack(acc[4] * inv, acc[5] * inv), Pair<T>::pack(acc[6] * inv, acc[7] * inv));
     }
-    if (ROWS) return;
   }
 }
 
@@ -1458,8 +1465,8 @@ int launch(Args& a, bool few, cudaStream_t stream) {
     dec::decode_kernel<T, D><<<a.ctas, dec::kThreads, dec::kRing, stream>>>(a);
     int rc = check_launch("fvb_paged_attn");
     if (rc) return rc;
-    // a block a row; a few of them look after the rows that a false max_new did not announce
-    return launch_merge(merge_kernel<T, D, dec::kRows, false>, dim3(a.ctas, a.few_rows), a, stream);
+    return launch_merge(merge_kernel<T, D, dec::kRows, true>, dim3(a.ctas, a.few_rows < 4 ? a.few_rows : 4), a,
+                        stream);
   }
   // rows of a TMA box: a power of two that divides the page, at most a tile
   int box = 16;
@@ -1483,7 +1490,7 @@ int launch(Args& a, bool few, cudaStream_t stream) {
   chunk::chunk_kernel<T, D><<<a.ctas, chunk::kThreads, chunk::Shape<D>::kSmem, stream>>>(tq, tk, tv, box, a);
   rc = check_launch("fvb_paged_attn");
   if (rc) return rc;
-  return launch_merge(merge_kernel<T, D, chunk::kRows, true>, dim3(a.ctas, chunk::kRows * (D / 8) / 256), a,
+  return launch_merge(merge_kernel<T, D, chunk::kRows, false>, dim3(a.ctas, chunk::kRows * (D / 8) / 256), a,
                       stream);
 }
 
