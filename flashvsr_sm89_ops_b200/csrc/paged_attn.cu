@@ -7,12 +7,13 @@
 //
 // Work is cut the same way in both kernels.  An item is (sequence, key head, tile of packed
 // rows); its length is the number of key tiles that its last row sees.  The items of all
-// sequences lie end to end on one line of `total` key tiles, and CTA c takes tiles [c per,
-// (c+1) per): uneven sequences and causal triangles balance by themselves, few rows over a long
-// cache spread over the machine, and a last partial wave does not exist.  An item cut by a
-// boundary leaves unnormalised partial sums (fp32 O, row maximum and sum) that merge_kernel
-// joins in the order of the cut, so results do not depend on timing.  Lengths are read on the
-// device only: a captured graph follows them.
+// sequences lie end to end on one line of key tiles, and each CTA takes an equal stretch of it:
+// uneven sequences and causal triangles balance by themselves, few rows over a long cache spread
+// over the machine, and a last partial wave does not exist.  An item cut by a boundary leaves
+// unnormalised partial sums (fp32 O, row maximum and sum) that merge_kernel joins in the order of
+// the cut, so results do not depend on timing.  Where there are many rows and items enough, whole
+// items are dealt out by length instead (see chunk_kernel).  Lengths are read on the device only:
+// every CTA counts the work itself, and a captured graph follows them.
 //
 //   decode_kernel  up to 16 packed rows a tile: single tokens, a few drafted ones.  Bound by the
 //                  bytes of the cache.
@@ -708,8 +709,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
 // Many rows: 256 packed rows (two tiles of 128, "A" and "B") against 128 keys a step.
 //
 // Both tiles read the same key and value tiles from one ring, so a key crosses L2 once for 256
-// rows.  Per tile a warpgroup of softmax threads (a thread owns a row) and one MMA-issuing
-// thread; one warp loads.  Tensor memory: one score buffer that the tiles take in turn (a tile's
+// rows.  Per tile a warpgroup of softmax threads (a thread owns a row) and one warp that issues
+// its MMAs; one warp loads, one works the segments out.  Tensor memory: one score buffer that the tiles take in turn (a tile's
 // softmax copies its scores to registers, and the buffer is the other's), P_A, P_B as packed
 // 16-bit pairs, O_A, O_B.  O stays there for a whole segment; the running maximum is raised only
 // when a tile's exceeds it by more than 2^8, and O is rescaled in place then.
@@ -730,9 +731,7 @@ struct Shape {
   // 2.12 to 1.95 million clocks and 1390 to 1360 us (the clock gives way to the load); other shares
   // gained less.  Ragged chunks of D 64: none 64.8 us, an eighth 62.1, a quarter 62.1.
   static constexpr uint32_t kFma = D == 128 ? 0x22u : 0x10u;
-  // alignment, barriers, and each softmax warp's 32 rows of 64 bytes (pitch 80) on their way out
-  static constexpr int kStage = 32 * 80;
-  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024 + 8 * kStage;
+  static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // alignment, barriers
 };
 
 // 2^x of two numbers without the special-function unit, which at 16 a clock and SM would need as
@@ -1163,7 +1162,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tO = tmem + kColO + (uint32_t)(x * 128) + lane_addr;
     const float c = a.scale_log2;
     const int half_rows = a.rows >> 1;
-    uint8_t* const stage = reinterpret_cast<uint8_t*>(bars) + 1024 + warp * S::kStage;
     bool ok = true;
     uint32_t kv = 0, mine = 0;
     while (ok && __all_sync(0xffffffffu, next_segment())) {
@@ -1194,7 +1192,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR(x, S_FREE));
         const int key0 = (key_t0 + j) * kKeys;
-        if (key0 + kKeys > lim) {
+        const bool masked = __any_sync(0xffffffffu, key0 + kKeys > lim);
+        if (masked) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (key0 + i >= lim) s[i] = __float_as_uint(-INFINITY);
@@ -1213,7 +1212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t nm = f2_pack(-msub, -msub);
         uint64_t acc2 = f2_pack(0.f, 0.f);
         uint32_t pk[32];
-        exp_pack64<T, S::kFma>(s, cc, nm, acc2, pk);
+        if (masked) exp_pack64<T, 0>(s, cc, nm, acc2, pk);
+        else exp_pack64<T, S::kFma>(s, cc, nm, acc2, pk);
         if (j > 0) {
           // P_x and O_x are free once the product of tile j - 1 is done
           if (!__all_sync(0xffffffffu,
@@ -1235,7 +1235,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tmem_st_32x32b_x32(tP, pk);
-        exp_pack64<T, S::kFma>(s + 64, cc, nm, acc2, pk);
+        if (masked) exp_pack64<T, 0>(s + 64, cc, nm, acc2, pk);
+        else exp_pack64<T, S::kFma>(s + 64, cc, nm, acc2, pk);
         tmem_st_32x32b_x32(tP + 32, pk);
         float la, lb;
         f2_unpack(acc2, la, lb);
@@ -1427,8 +1428,9 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a) {
   }
 }
 
-// Whether the rows of the longest sequence fit the few-rows kernel.  Measured at 48 sequences of
-// about 9 k keys, 32 / 8 heads of 128: see the figures at the entry point.
+// Whether the rows of the longest sequence fit a tile of the few-rows kernel.  16 streams of up to 4000
+// keys, D 128, few rows against many: 1 row a key head 29.5 and 46.2 us, 4 rows 35.1 and 48.9, 16 rows
+// 34.0 and 44.6; 32 rows, two tiles of it that read the cache twice, 50.2 and 49.9.
 inline bool few_rows(int64_t max_new, int64_t g) { return max_new * g <= dec::kRows; }
 inline int ctas_of(bool few) { return sm_count() * (few ? 2 : 1); }
 

@@ -49,7 +49,7 @@ def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal
     if Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError(f"{name}: {Hq} query heads on {Hk} key heads")
     st, sh, sd = q.stride()
-    if sd != 1 or (st | sh) & 7 or q.data_ptr() & 15:
+    if sd != 1 or (st | sh) & 7 or st <= 0 or sh <= 0 or q.data_ptr() & 15:
         q = q.clone(memory_format=torch.contiguous_format)
         st, sh, _ = q.stride()
     if out is None:
@@ -176,9 +176,8 @@ class PagedKV:
                 raise ValueError(f"PagedKV: {what} must be contiguous int32 [{n}] on {dev}")
         if v.device != dev:
             raise ValueError(f"PagedKV: k is on {dev}, v on {v.device}")
-        self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
+        self._tensors = (k, v, table, lens, refs, torch.zeros(1, dtype=torch.int32, device=dev))
         self.page = page
-        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.device = dev
         seqs, width = table.shape
         n = _lib.load().fvb_pages_workspace_bytes(seqs, P)
@@ -202,6 +201,14 @@ class PagedKV:
                    torch.full((seqs, pages if width is None else width), -1, dtype=torch.int32, device=device),
                    torch.zeros(seqs, dtype=torch.int32, device=device),
                    torch.zeros(pages, dtype=torch.int32, device=device))
+
+    # the calls hold the addresses of these, so they can be written to but not replaced
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    table = property(lambda self: self._tensors[2])
+    lens = property(lambda self: self._tensors[3])
+    refs = property(lambda self: self._tensors[4])
+    status = property(lambda self: self._tensors[5])
 
     def check(self):
         """Waits for the device and raises what a step since the last check could not do."""

@@ -77,12 +77,16 @@ class Rope:
         self.scale = 1.0
         if scaling == "yarn":
             self.scale = 0.1 * math.log(factor) + 1 if attention_factor is None else float(attention_factor)
-        self.freq = torch.tensor(turns, dtype=torch.int64, device=device)
-        self.axis = torch.tensor([a for a, d in enumerate(dims) for _ in range(d // 2)], dtype=torch.int32,
-                                 device=device)
+        self._tensors = (torch.tensor(turns, dtype=torch.int64, device=device),
+                         torch.tensor([a for a, d in enumerate(dims) for _ in range(d // 2)], dtype=torch.int32,
+                                      device=device))
         self.device = self.freq.device
         self.index = self.freq.get_device()  # -1 on the host
         self._freq, self._axis = self.freq.data_ptr(), self.axis.data_ptr()
+
+    # the calls hold the addresses of these
+    freq = property(lambda self: self._tensors[0])
+    axis = property(lambda self: self._tensors[1])
 
     def __repr__(self):
         return f"Rope({self.rotary_dim}, layout={self.layout!r}, axes={self.axes}, scale={self.scale})"

@@ -592,6 +592,23 @@ def test_attend_rows_that_see_nothing(max_new):
     assert (out[:250] == 0).all() and not out[250:400].isfinite().any()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attend_masked_values_weigh_nothing(dtype, D):
+    """The largest values of the type behind the mask: the rows before them are the same to the bit."""
+    new, had = [200, 70], [300, 0]
+    q, k, v, table, lens, ks, vs = _case(new, had, 4, 2, D, 32, dtype, 27)
+    for max_new in (1, 200):
+        want = ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=max_new)
+        loud = v.clone()
+        for b, (n, h) in enumerate(zip(new, had)):
+            i = torch.arange(h + n // 2, h + n, device=DEV)
+            loud[table[b].long()[i // 32], i % 32] = torch.finfo(dtype).max
+        got = ops.paged_attention(q, k, loud, table, lens, _cu(new), max_new=max_new)
+        for at, n in ((0, 200), (200, 70)):
+            assert torch.equal(got[at:at + n // 2], want[at:at + n // 2])
+
+
 @pytest.mark.parametrize("max_new", [1, 64])
 def test_attend_sharp_scores(max_new):
     """Scores of hundreds, maxima that rise along the keys: the running maximum is moved many times."""
@@ -625,6 +642,10 @@ def test_attend_layouts(max_new):
     wide.fill_(5.0)
     ops.paged_attention(qpad, k, v, table, lens, _cu(new), max_new=max_new, out=wide[..., :D])
     assert torch.equal(wide[:93, :, :D], want) and (wide[93:] == 5).all() and (wide[..., D:] == 5).all()
+    # one query for all heads and tokens, without a copy of its own
+    flat = q[:1, :1].expand(93, 6, D)
+    assert torch.equal(ops.paged_attention(flat, k, v, table, lens, _cu(new), max_new=max_new),
+                       ops.paged_attention(flat.contiguous(), k, v, table, lens, _cu(new), max_new=max_new))
     # an unaligned q is copied
     odd = torch.randn(93 * 6 * D + 1, device=DEV).half()
     odd[1:] = q.reshape(-1)
@@ -850,6 +871,9 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+    for obj, name in ((kv, "table"), (kv, "k"), (kv, "status"), (rope, "freq")):
+        with pytest.raises(AttributeError):
+            setattr(obj, name, None)
     wide = ops.PagedKV.empty(1, 4, 16, 2, 72, 2, 3)
     with pytest.raises(NotImplementedError):
         wide.attend(0, torch.zeros(4, 2, 72, device=DEV, dtype=bf), cu)
