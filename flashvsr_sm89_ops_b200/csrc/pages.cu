@@ -10,7 +10,9 @@
 //
 // The bookkeeping is one block: it scans refs (4 bytes a page) and touches one table row a
 // sequence, microseconds against the copies.  Copies are bound by memory: read and written once,
-// 64 bytes in flight a thread over all layers' k and v in one launch.  A step whose arguments or
+// 64 bytes in flight a thread over all layers' k and v in one launch (100 pages of 128 x 12 x 128 in 4
+// layers: 629 MB in 101 us, 6.2 TB/s).  The bookkeeping of a step takes 3.5-6 us, a chain of dependent
+// accesses.  A step whose arguments or
 // whose room do not suffice changes nothing and records a code in `status`.
 #include "common.cuh"
 

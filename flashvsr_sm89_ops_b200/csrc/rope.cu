@@ -12,9 +12,9 @@
 // memory, serves every head of q and k.
 //
 // Bound by memory: q and k are read and written once (append: q, k and v, with k and v written
-// to their pages).  Measured (B200, cold inputs): 8448 tokens of 12 + 12 heads of 128 in bf16 20.5 us
-// (104 MB at 5.1 TB/s), 16896 tokens appended 51 us (261 MB at 5.1 TB/s), 4099 tokens of 24 + 4 heads
-// of 80 in fp32 12.6 us (73 MB at 5.8 TB/s).  An earlier form that dealt rows of heads to threads
+// to their pages).  Measured (B200, cold inputs): 8448 tokens of 12 + 12 heads of 128 in bf16 19.7 us
+// (104 MB at 5.3 TB/s), 16896 tokens appended 50 us (261 MB at 5.2 TB/s), 4099 tokens of 24 + 4 heads
+// of 80 in fp32 11.6 us (73 MB at 6.3 TB/s).  An earlier form that dealt rows of heads to threads
 // spent 63% of its issue slots on indexes (27, 54 and 21 us); one that kept blocks resident and
 // prefetched the next tokens' angles held too many registers to cover latency (34, 74 and 20 us).
 #include "common.cuh"
