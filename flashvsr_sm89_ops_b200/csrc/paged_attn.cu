@@ -727,62 +727,22 @@ template <int D>
 struct Shape {
   static constexpr int kTile = D * 256;  // bytes of 128 rows
   static constexpr int kSlots = D == 128 ? 2 : 4;  // of K and of V
-  // Exponentials on the FMA pipe, pairs of each eight.  8448 over 33792 keys, D 128: a quarter takes
-  // 2.12 to 1.95 million clocks and 1390 to 1360 us (the clock gives way to the load); other shares
-  // gained less.  Ragged chunks of D 64: none 64.8 us, an eighth 62.1, a quarter 62.1.
-  static constexpr uint32_t kFma = D == 128 ? 0x22u : 0x10u;
   static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // alignment, barriers
 };
 
-// 2^x of two numbers without the special-function unit, which at 16 a clock and SM would need as
-// long for a tile's exponentials as the tensor cores for its products: x = n + f with f in
-// [-1/2, 1/2] (n by adding and subtracting 1.5 2^23), a polynomial in f, and n added to the
-// exponent.  The polynomials minimise the largest relative error (fitted by reweighted least
-// squares): 2^-13.7 with degree 3, for probabilities that are rounded to bf16 (2^-9), 2^-18.5
-// with degree 4 for fp16 (2^-12).  Below -126 the result is 2^-126, which counts as nothing.
+// p = 2^(s c - m) of 64 scores, packed; fp32 row sum into acc2.  All on the special-function unit: an
+// eighth or a quarter of them as polynomials on the FMA pipe took 8448 over 33792 keys from 1424 to
+// 1412 us, and ragged chunks from 169 to 186-189 us (65 to 66-67 at D 64).
 template <typename T>
-__device__ __forceinline__ void exp2_fma(uint64_t x, float& p0, float& p1) {
-  float x0, x1;
-  f2_unpack(x, x0, x1);
-  x = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t t = f2_add(x, f2_pack(12582912.f, 12582912.f));
-  const uint64_t n = f2_add(t, f2_pack(-12582912.f, -12582912.f));
-  const uint64_t f = f2_fma(n, f2_pack(-1.f, -1.f), x);
-  uint64_t p;
-  if (Pair<T>::kFmt) {
-    p = f2_fma(f, f2_pack(0.0551716685f, 0.0551716685f), f2_pack(0.242611125f, 0.242611125f));
-    p = f2_fma(f, p, f2_pack(0.693260968f, 0.693260968f));
-    p = f2_fma(f, p, f2_pack(0.999928057f, 0.999928057f));
-  } else {
-    p = f2_fma(f, f2_pack(0.0095701022f, 0.0095701022f), f2_pack(0.0559178591f, 0.0559178591f));
-    p = f2_fma(f, p, f2_pack(0.240247443f, 0.240247443f));
-    p = f2_fma(f, p, f2_pack(0.693121791f, 0.693121791f));
-    p = f2_fma(f, p, f2_pack(0.999999285f, 0.999999285f));
-  }
-  float t0, t1;
-  f2_unpack(t, t0, t1);
-  f2_unpack(p, p0, p1);
-  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
-}
-
-// p = 2^(s c - m) of 64 scores, packed; fp32 row sum into acc2.  kFma: which pairs of each eight
-// take exp2_fma.
-template <typename T, uint32_t kFma>
 __device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint64_t nm,
                                            uint64_t& acc2, uint32_t* pk) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const uint64_t xv =
         f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, nm);
-    float p0, p1;
-    if (kFma >> (i & 7) & 1) {
-      exp2_fma<T>(xv, p0, p1);
-    } else {
-      float x0, x1;
-      f2_unpack(xv, x0, x1);
-      p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-    }
+    float x0, x1;
+    f2_unpack(xv, x0, x1);
+    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
     acc2 = f2_add(acc2, f2_pack(p0, p1));
     pk[i] = Pair<T>::pack(p0, p1);
   }
@@ -1212,8 +1172,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t nm = f2_pack(-msub, -msub);
         uint64_t acc2 = f2_pack(0.f, 0.f);
         uint32_t pk[32];
-        if (masked) exp_pack64<T, 0>(s, cc, nm, acc2, pk);
-        else exp_pack64<T, S::kFma>(s, cc, nm, acc2, pk);
+        // twice the same: with the two kinds of tiles apart the compiler keeps all scores in registers
+        // (ragged chunks of D 64 65.3 us; in one path it spills ten of them, 67.1)
+        if (masked) exp_pack64<T>(s, cc, nm, acc2, pk);
+        else exp_pack64<T>(s, cc, nm, acc2, pk);
         if (j > 0) {
           // P_x and O_x are free once the product of tile j - 1 is done
           if (!__all_sync(0xffffffffu,
@@ -1235,8 +1197,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tmem_st_32x32b_x32(tP, pk);
-        if (masked) exp_pack64<T, 0>(s + 64, cc, nm, acc2, pk);
-        else exp_pack64<T, S::kFma>(s + 64, cc, nm, acc2, pk);
+        if (masked) exp_pack64<T>(s + 64, cc, nm, acc2, pk);
+        else exp_pack64<T>(s + 64, cc, nm, acc2, pk);
         tmem_st_32x32b_x32(tP + 32, pk);
         float la, lb;
         f2_unpack(acc2, la, lb);

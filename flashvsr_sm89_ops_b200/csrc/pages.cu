@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const 
     if (b < c.seqs) {
       const int64_t len = c.lens[b], add = more[b];
       const int64_t want = (len + add + c.page - 1) / c.page;
-      if (add < 0 || len + add > INT32_MAX) bad |= kBadArgs;
+      if (len < 0 || add < 0 || len + add > INT32_MAX) bad |= kBadArgs;
       else if (want > c.width) bad |= kNoWidth;
       else n = (int)(want - held(c, len));
     }
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int64_t a = src[i], d = dst[i];
     if (a < 0 || a >= c.seqs || d < 0 || d >= c.seqs) bad = kBadArgs;
-    else if (test_and_set(branch, d) || c.lens[d] != 0) bad = kBadArgs;
+    else if (test_and_set(branch, d) || c.lens[d] != 0 || c.lens[a] < 0) bad = kBadArgs;
   }
   bad = __syncthreads_or(bad) ? kBadArgs : 0;
   int need = 0;

@@ -19,7 +19,8 @@ from .rope import _POS64, Rope, _out, _positions, _rows
 
 _DTYPES = {torch.bfloat16: _lib.FVB_BF16, torch.float16: _lib.FVB_F16}
 _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
-           4: "bad arguments (an index out of range or twice, a negative count, a branch that was not empty)"}
+           4: "bad arguments (an index out of range or twice, a negative count or length, a branch that was not "
+              "empty)"}
 
 
 def _ints(t, n, what, name, index):

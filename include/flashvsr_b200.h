@@ -442,7 +442,7 @@ FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
 /* Pages.  refs [pages]: how many sequences hold a page (0: free).  Free pages are given out lowest
  * first, in the order of sequences and of their pages.  A step that cannot be done changes nothing
  * and sets a bit of *status: 1 no free pages, 2 a table row too short, 4 bad arguments (an index
- * out of range or twice, a negative count, a branch that is not empty).
+ * out of range or twice, a negative count or length, a branch that is not empty).
  * workspace: fvb_pages_workspace_bytes(seqs, pages), 16-byte aligned.  At most 131072 sequences.
  *   reserve  room for more[b] tokens in every sequence; lens grow
  *   fork     dst[i] becomes a branch of src[i]: full pages shared, the tokens of a partly filled

@@ -383,6 +383,13 @@ def test_pages_refuse_what_cannot_be_done():
             kv.check()
         book.check(kv)
         kv.check()
+    kv.lens[2] = -5  # a state that was handed in broken
+    for call in (lambda: kv.reserve(_i32([0] * 4)), lambda: kv.fork(_i32([2]), _i32([3]))):
+        call()
+        with pytest.raises(RuntimeError, match="bad arguments"):
+            kv.check()
+    kv.release(_i32([2]))
+    book.check(kv)
     kv.reserve(_i32([0, 0, 80, 0]))
     book.reserve([0, 0, 80, 0])
     kv.fork(_i32([0]), _i32([3]))  # its last page is partly filled, and none is free
@@ -474,12 +481,10 @@ def _attend_64(q, k, v, n, causal, scale):
 def _attend_bound(o, a, size, L, D, dtype):
     """Half a step of the result.  Each probability is rounded to the type (u, relative) and off by
     what its exponent is off: D products summed in fp32 (D 2^-23 of sum |q||k| scale), its scaling and
-    subtraction (2^-22 of the same), and the exponential's own error: ex2's 2^-22, or that of a
-    polynomial of degree 3 (bf16, 7.5e-5) or 4 (fp16, 2.6e-6) fitted on [-1/2, 1/2], each
-    evaluated with roundings of 2^-23 in all; numerator and sum alike (twice).  Sums of L terms
-    in fp32 are off by L 2^-23."""
+    subtraction (2^-22 of the same), and ex2's own 2^-22; numerator and sum alike (twice).  Sums of L
+    terms in fp32 are off by L 2^-23."""
     u = U[dtype]
-    d = size * (D * 2.0 ** -23 + 2.0 ** -22) + 2.0 ** -22 + (7.5e-5 if dtype == torch.bfloat16 else 2.6e-6)
+    d = size * (D * 2.0 ** -23 + 2.0 ** -22) + 2.0 ** -22
     return u * o.abs() + a * (u + 2 * d + L * 2.0 ** -23) * (1 + 2 * u) + TINY[dtype]
 
 
