@@ -13,7 +13,8 @@
 // 64 bytes in flight a thread over all layers' k and v in one launch (100 pages of 128 x 12 x 128 in 4
 // layers: 629 MB in 101 us, 6.2 TB/s).  The bookkeeping of a step takes 3.5-6 us, a chain of dependent
 // accesses.  A step whose arguments or
-// whose room do not suffice changes nothing and records a code in `status`.
+// whose room do not suffice changes nothing and records a code in `status`; a reserve also records in
+// `refused` whether it was done, for the appends behind it (the host does not know).
 #include "common.cuh"
 
 namespace fvb {
@@ -89,7 +90,7 @@ __device__ int free_pages(const int32_t* refs, int64_t pages, int need, int32_t*
 }
 
 struct Cache {
-  int32_t *table, *lens, *refs, *status;
+  int32_t *table, *lens, *refs, *status, *refused;
   int64_t seqs, width, pages;
   int page;
 };
@@ -127,10 +128,11 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const 
   if (!bad && need > c.pages) bad = kNoPages;
   int32_t* const list = need <= kSmall ? s_list : ws + c.seqs + 1;
   if (!bad && free_pages(c.refs, c.pages, (int)need, list, sums) < need) bad = kNoPages;
-  if (bad) {
-    if (threadIdx.x == 0) atomicOr(c.status, bad);
-    return;
+  if (threadIdx.x == 0) {
+    if (bad) atomicOr(c.status, bad);
+    if (c.refused) *c.refused = bad != 0;
   }
+  if (bad) return;
   for (int i = threadIdx.x; i < need; i += kThreads) {
     int64_t lo = 0, hi = c.seqs;  // the last sequence whose pages start at or before i
     while (lo + 1 < hi) {
@@ -387,7 +389,7 @@ int cache_of(const fvb_pages* p, Cache& c, const char* what) {
               (long long)p->width, (long long)p->page, (long long)p->pages);
   FVB_REQUIRE(p->table && p->lens && p->refs && p->status && p->workspace, "%s: NULL pointer", what);
   FVB_REQUIRE(aligned16(p->workspace), "%s: workspace must be 16-byte aligned", what);
-  c = {p->table, p->lens, p->refs, p->status, p->seqs, p->width, p->pages, (int)p->page};
+  c = {p->table, p->lens, p->refs, p->status, p->refused, p->seqs, p->width, p->pages, (int)p->page};
   return FVB_OK;
 }
 

@@ -57,7 +57,11 @@ struct Args {
   int64_t B, width, pages;
   int page;
   int64_t page_stride, slot_stride;  // of the pools
+  const int32_t* refused;  // not 0: the chunk has no room (NULL: it has)
+  int32_t* status;
 };
+
+constexpr int kNotAppended = 8;  // in status
 
 template <typename T>
 struct Elem;
@@ -206,7 +210,12 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
         if (a.cu[mid] <= t) lo = mid; else hi = mid;
       }
       const int64_t c0 = a.cu[lo], c1 = a.cu[lo + 1];
-      const bool live = c0 <= t && t < c1;
+      bool live = c0 <= t && t < c1;
+      // without the room that a reserve makes, the places counted back from lens are cached tokens'
+      if (live && a.refused && *a.refused) {
+        live = false;
+        atomicOr(a.status, kNotAppended);
+      }
       const int64_t at = (int64_t)a.lens[lo] - (c1 - c0) + (t - c0);
       int64_t slot = -1;
       if (live && at >= 0) {
@@ -409,6 +418,7 @@ extern "C" int fvb_kv_append(const fvb_kv_append_args* p, fvb_stream_t stream) {
                   p->k_pool && p->v_pool,
               "fvb_kv_append: NULL pointer");
   FVB_REQUIRE(p->rot == 0 || (p->freq && (p->axes == 1 || p->axis)), "fvb_kv_append: NULL pointer");
+  FVB_REQUIRE(!p->refused || p->status, "fvb_kv_append: refused without status");
   const int turned = p->rot > 0;
   rope::Args a = {};
   if (p->Hq)
@@ -434,5 +444,7 @@ extern "C" int fvb_kv_append(const fvb_kv_append_args* p, fvb_stream_t stream) {
   a.page = (int)p->page;
   a.page_stride = p->page_stride;
   a.slot_stride = p->Hk * p->D;
+  a.refused = p->refused;
+  a.status = p->status;
   return rope::launch_dtype(a, (int)p->dtype, p->half != 0, (cudaStream_t)stream, "fvb_kv_append");
 }

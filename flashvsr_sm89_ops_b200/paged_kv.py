@@ -20,7 +20,8 @@ from .rope import _POS64, Rope, _out, _positions, _rows
 _DTYPES = {torch.bfloat16: _lib.FVB_BF16, torch.float16: _lib.FVB_F16}
 _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
            4: "bad arguments (an index out of range or twice, a negative count or length, a branch that was not "
-              "empty)"}
+              "empty)",
+           8: "tokens were not appended, as the reserve() before them could not be done"}
 
 
 def _ints(t, n, what, name, index):
@@ -150,8 +151,10 @@ class PagedKV:
 
     The tensors are the state: read them, or hand in ones that hold one.  Free pages are given out
     lowest first in the order of sequences and of their pages.  A call on the device that cannot
-    be done (no pages, an index out of range) changes nothing and is recorded in `status`.  At most
-    131072 sequences.
+    be done (no pages, an index out of range) changes nothing and is recorded in `status`.  Behind a
+    reserve() that could not be done, no append() writes anything until one is (`refused` int32 [1] is
+    not 0): a step that found no room can be done again, and its results so far mean nothing.  At
+    most 131072 sequences.
     """
 
     def __init__(self, k, v, table, lens, refs):
@@ -177,7 +180,7 @@ class PagedKV:
                 raise ValueError(f"PagedKV: {what} must be contiguous int32 [{n}] on {dev}")
         if v.device != dev:
             raise ValueError(f"PagedKV: k is on {dev}, v on {v.device}")
-        self._tensors = (k, v, table, lens, refs, torch.zeros(1, dtype=torch.int32, device=dev))
+        self._tensors = (k, v, table, lens, refs, *torch.zeros(2, dtype=torch.int32, device=dev).split(1))
         self.page = page
         self.device = dev
         seqs, width = table.shape
@@ -186,12 +189,13 @@ class PagedKV:
         self._pools = (k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0) * 2, k.stride(1) * 2, H * D * 2)
         # what every step of the pages takes
         self._pages = _lib.PAGES(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.status.data_ptr(), seqs, width,
-                                 P, page, *self._pools, self._ws.data_ptr())
+                                 P, page, *self._pools, self._ws.data_ptr(), refused=self.refused.data_ptr())
         # and every append and attention
         self._index, self._dt, self._dtype = k.get_device(), _DTYPES[k.dtype], k.dtype
         self._shape = (H, D, P, page)
         self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
         self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
+        self._room = {"refused": self.refused.data_ptr(), "status": self.status.data_ptr()}
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads: int, head_dim: int, seqs: int,
@@ -210,6 +214,7 @@ class PagedKV:
     lens = property(lambda self: self._tensors[3])
     refs = property(lambda self: self._tensors[4])
     status = property(lambda self: self._tensors[5])
+    refused = property(lambda self: self._tensors[6])
 
     def check(self):
         """Waits for the device and raises what a step since the last check could not do."""
@@ -255,7 +260,8 @@ class PagedKV:
         [T, heads, D] of all sequences, sequence b's at cu_seqlens[b] .. cu_seqlens[b + 1] (int32
         [seqs + 1]).  With a Rope, k is rotated on the way and so is q [T, Hq, D], which is
         returned; positions (as in fused_rope) default to the tokens' places in their sequences.
-        Tokens past cu_seqlens[seqs] are ignored, and rows of out_q for them stay as they are."""
+        Tokens past cu_seqlens[seqs] are ignored, and rows of out_q for them stay as they are.  If
+        the last reserve() could not be done, nothing is written, out_q neither, and check() raises."""
         name = "PagedKV.append"
         index, dt = self._index, self._dtype
         H, D, P, page = self._shape
@@ -305,7 +311,7 @@ class PagedKV:
         _lib.call_on(index, "fvb_kv_append",
                      _lib.KV_APPEND_ARGS(*qargs, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, H, T, D, *rargs,
                                          cu.data_ptr(), lens, table, seqs, width, P, page, kp + at, vp + at,
-                                         self._strides[0]), _lib.stream_of(k))
+                                         self._strides[0], **self._room), _lib.stream_of(k))
         return oq
 
     def attend(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, causal: bool = True,

@@ -416,7 +416,9 @@ FVB_API int fvb_rope(const fvb_rope_args* args, fvb_stream_t stream);
  * cu[b] .. cu[b + 1] are the last ones of sequence b's lens[b].
  * Writes k (rotated, rot = 0: as it is) and v of T new tokens to their places, and q rotated to
  * q_out (Hq = 0: no q).  pos NULL: a token's position is its place in the sequence.  Tokens
- * outside cu, and places without a page, are left alone.  bf16 / fp16. */
+ * outside cu, and places without a page, are left alone.  bf16 / fp16.
+ * refused, status: those of the cache's fvb_pages (NULL: not looked at).  Where the last reserve was
+ * refused nothing is written, q_out neither, and bit 8 of *status is set. */
 typedef struct {
   const void* q;
   int64_t q_token, q_head, Hq;
@@ -436,13 +438,16 @@ typedef struct {
   int64_t B, width, pages, page;
   void *k_pool, *v_pool;
   int64_t page_stride;
+  const int32_t* refused;
+  int32_t* status;
 } fvb_kv_append_args;
 FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
 
 /* Pages.  refs [pages]: how many sequences hold a page (0: free).  Free pages are given out lowest
  * first, in the order of sequences and of their pages.  A step that cannot be done changes nothing
  * and sets a bit of *status: 1 no free pages, 2 a table row too short, 4 bad arguments (an index
- * out of range or twice, a negative count or length, a branch that is not empty).
+ * out of range or twice, a negative count or length, a branch that is not empty), 8 see fvb_kv_append.
+ * refused (NULL: not kept): 1 when the last reserve could not be done, else 0.
  * workspace: fvb_pages_workspace_bytes(seqs, pages), 16-byte aligned.  At most 131072 sequences.
  *   reserve  room for more[b] tokens in every sequence; lens grow
  *   fork     dst[i] becomes a branch of src[i]: full pages shared, the tokens of a partly filled
@@ -456,6 +461,7 @@ typedef struct {
   void *k, *v; /* reserve and release do without the pools */
   int64_t layers, layer_stride, page_stride, row_bytes;
   void* workspace;
+  int32_t* refused;
 } fvb_pages;
 FVB_API size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages);
 FVB_API int fvb_pages_reserve(const fvb_pages* cache, const int32_t* more, fvb_stream_t stream);
