@@ -58,6 +58,7 @@ struct Args {
   int page;
   int64_t page_stride, slot_stride;  // of the pools
   const int32_t* refused;  // not 0: the chunk has no room (NULL: it has)
+  const int32_t* refs;     // sequences that hold a page (NULL: one)
   int32_t* status;
 };
 
@@ -221,7 +222,10 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
       if (live && at >= 0) {
         const int64_t j = at / a.page;
         const int32_t p = j < a.width ? a.table[lo * a.width + j] : -1;
-        if (p >= 0 && p < a.pages) slot = p * a.page_stride + (at - j * a.page) * a.slot_stride;
+        if (p >= 0 && p < a.pages) {
+          if (a.refs && a.refs[p] > 1) atomicOr(a.status, kNotAppended);  // other sequences' tokens too
+          else slot = p * a.page_stride + (at - j * a.page) * a.slot_stride;
+        }
       }
       s_pos[threadIdx.x] = at;
       s_slot[threadIdx.x] = live ? slot : -2;  // -1: no place in the pool, -2: no token at all
@@ -418,7 +422,7 @@ extern "C" int fvb_kv_append(const fvb_kv_append_args* p, fvb_stream_t stream) {
                   p->k_pool && p->v_pool,
               "fvb_kv_append: NULL pointer");
   FVB_REQUIRE(p->rot == 0 || (p->freq && (p->axes == 1 || p->axis)), "fvb_kv_append: NULL pointer");
-  FVB_REQUIRE(!p->refused || p->status, "fvb_kv_append: refused without status");
+  FVB_REQUIRE((!p->refused && !p->refs) || p->status, "fvb_kv_append: refused and refs need status");
   const int turned = p->rot > 0;
   rope::Args a = {};
   if (p->Hq)
@@ -445,6 +449,7 @@ extern "C" int fvb_kv_append(const fvb_kv_append_args* p, fvb_stream_t stream) {
   a.page_stride = p->page_stride;
   a.slot_stride = p->Hk * p->D;
   a.refused = p->refused;
+  a.refs = p->refs;
   a.status = p->status;
   return rope::launch_dtype(a, (int)p->dtype, p->half != 0, (cudaStream_t)stream, "fvb_kv_append");
 }

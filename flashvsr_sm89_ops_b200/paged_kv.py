@@ -21,7 +21,8 @@ _DTYPES = {torch.bfloat16: _lib.FVB_BF16, torch.float16: _lib.FVB_F16}
 _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
            4: "bad arguments (an index out of range or twice, a negative count or length, a branch that was not "
               "empty)",
-           8: "tokens were not appended, as the reserve() before them could not be done"}
+           8: "tokens were not appended: the reserve() before them could not be done, or other sequences hold their "
+              "page too"}
 
 
 def _ints(t, n, what, name, index):
@@ -195,7 +196,7 @@ class PagedKV:
         self._shape = (H, D, P, page)
         self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
         self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
-        self._room = {"refused": self.refused.data_ptr(), "status": self.status.data_ptr()}
+        self._room = {"refused": self.refused.data_ptr(), "refs": refs.data_ptr(), "status": self.status.data_ptr()}
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads: int, head_dim: int, seqs: int,
@@ -231,7 +232,8 @@ class PagedKV:
     def fork(self, src: torch.Tensor, dst: torch.Tensor):
         """Sequence dst[i] becomes a branch of src[i] (int32 [n]; a parent may come several times,
         the branches are empty, distinct and no parents).  Full pages are shared; the tokens in a
-        partly filled last page are copied, in every layer."""
+        partly filled last page are copied, in every layer: what reserve() made room for is appended
+        first."""
         src = _ints(src, None, "src", "PagedKV.fork", self._index)
         n = src.shape[0]
         dst = _ints(dst, n, "dst", "PagedKV.fork", self._index)
@@ -261,7 +263,8 @@ class PagedKV:
         [seqs + 1]).  With a Rope, k is rotated on the way and so is q [T, Hq, D], which is
         returned; positions (as in fused_rope) default to the tokens' places in their sequences.
         Tokens past cu_seqlens[seqs] are ignored, and rows of out_q for them stay as they are.  If
-        the last reserve() could not be done, nothing is written, out_q neither, and check() raises."""
+        the last reserve() could not be done, nothing is written, out_q neither, and check() raises; so
+        it does where a token's page belongs to other sequences too, which is left as it is."""
         name = "PagedKV.append"
         index, dt = self._index, self._dtype
         H, D, P, page = self._shape

@@ -417,8 +417,9 @@ FVB_API int fvb_rope(const fvb_rope_args* args, fvb_stream_t stream);
  * Writes k (rotated, rot = 0: as it is) and v of T new tokens to their places, and q rotated to
  * q_out (Hq = 0: no q).  pos NULL: a token's position is its place in the sequence.  Tokens
  * outside cu, and places without a page, are left alone.  bf16 / fp16.
- * refused, status: those of the cache's fvb_pages (NULL: not looked at).  Where the last reserve was
- * refused nothing is written, q_out neither, and bit 8 of *status is set. */
+ * refused, refs, status: those of the cache's fvb_pages (NULL: not looked at).  Where the last reserve
+ * was refused nothing is written, q_out neither; places in a page that several sequences hold are left
+ * alone.  Either sets bit 8 of *status. */
 typedef struct {
   const void* q;
   int64_t q_token, q_head, Hq;
@@ -438,7 +439,7 @@ typedef struct {
   int64_t B, width, pages, page;
   void *k_pool, *v_pool;
   int64_t page_stride;
-  const int32_t* refused;
+  const int32_t *refused, *refs;
   int32_t* status;
 } fvb_kv_append_args;
 FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);

@@ -5,7 +5,7 @@ import torch
 
 import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
-from test_attention_pages_gpu import _fill, _gen, _i32, _tokens
+from test_attention_pages_gpu import _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -99,3 +99,26 @@ def test_captured_step_runs_into_a_full_pool():
     graph.replay()
     kv.check()
     assert kv.lens.tolist() == [17, 1] and (_tokens(kv, 0)[0][0, 16:] == 9).all() and (_tokens(kv, 1)[0] == 9).all()
+
+
+def test_append_leaves_shared_pages_alone():
+    """A page of several sequences is not written to, whatever lens say: each keeps what it has."""
+    H, D, page = 1, 64, 16
+    kv = ops.PagedKV.empty(1, 8, page, H, D, 3, 4)
+    _fill(kv, 3)
+    kv.reserve(_i32([32, 16, 0]))
+    kv.append(0, *_chunk(48, H, D, 4)[:2], _i32([0, 32, 48, 48]))
+    kv.fork(_i32([0]), _i32([2]))
+    kv.check()
+    want_k, want_v = kv.k.clone(), kv.v.clone()
+    q, k, v = _chunk(24, H, D, 5)
+    oq = kv.append(0, k, v, _i32([0, 8, 16, 24]), q=q, rope=ops.Rope(D))  # nobody reserved anything
+    with pytest.raises(RuntimeError, match="not appended"):
+        kv.check()
+    p = kv.table[1, 0].long()  # the middle stream's page is its own
+    want_k[0, p, 8:], want_v[0, p, 8:] = kv.k[0, p, 8:], v[8:16]
+    assert torch.equal(kv.k, want_k) and torch.equal(kv.v, want_v)
+    f, axis = _freqs((D,))
+    pos = torch.cat([torch.arange(24, 32), torch.arange(8, 16), torch.arange(24, 32)]).to(DEV)
+    y, both = _rope_64(q, pos[:, None], D, False, f, axis, 1.0, False)
+    assert ((oq.double() - y).abs() <= _rope_bound(y, both, q.dtype)).all()
