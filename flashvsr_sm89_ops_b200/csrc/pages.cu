@@ -15,6 +15,10 @@
 // accesses.  A step whose arguments or
 // whose room do not suffice changes nothing and records a code in `status`; a reserve also records in
 // `refused` whether it was done, for the appends behind it (the host does not know).
+//
+// Keys stay as they were rotated when a sequence's first pages are given back, so its next tokens'
+// positions go on from all that it ever held: `dropped` counts what it held before lens.  A sequence
+// without tokens begins at 0 again (there is no key that a distance could be wrong to).
 #include "common.cuh"
 
 namespace fvb {
@@ -91,6 +95,7 @@ __device__ int free_pages(const int32_t* refs, int64_t pages, int need, int32_t*
 
 struct Cache {
   int32_t *table, *lens, *refs, *status, *refused;
+  int64_t* dropped;
   int64_t seqs, width, pages;
   int page;
 };
@@ -143,7 +148,10 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const 
     c.refs[list[i]] = 1;
   }
   __syncthreads();
-  for (int64_t b = threadIdx.x; b < c.seqs; b += kThreads) c.lens[b] += more[b];
+  for (int64_t b = threadIdx.x; b < c.seqs; b += kThreads) {
+    if (c.dropped && c.lens[b] == 0) c.dropped[b] = 0;  // begins anew
+    c.lens[b] += more[b];
+  }
 }
 
 // ws: count, copies [n], list [n]
@@ -221,6 +229,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int
     const int32_t len = c.lens[src[i]];
     copies[i].to = len % c.page ? list[n <= kSmall ? s_rank[i] : copies[i].to] : 0;
     c.lens[dst[i]] = len;
+    if (c.dropped) c.dropped[dst[i]] = c.dropped[src[i]];
   }
 }
 
@@ -272,8 +281,10 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Cache c, const 
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const int64_t b = seqs[i], have = held(c, c.lens[b]);
-    const int64_t left = (int64_t)c.lens[b] - (int64_t)(drop ? drop[i] : 0) * c.page;
-    c.lens[b] = !drop || drop[i] >= have ? 0 : (int32_t)(left > 0 ? left : 0);
+    const int64_t len = c.lens[b], left = len - (int64_t)(drop ? drop[i] : 0) * c.page;
+    const int32_t now = !drop || drop[i] >= have ? 0 : (int32_t)(left > 0 ? left : 0);
+    c.lens[b] = now;
+    if (c.dropped) c.dropped[b] = now ? c.dropped[b] + (len - now) : 0;
   }
 }
 
@@ -389,7 +400,7 @@ int cache_of(const fvb_pages* p, Cache& c, const char* what) {
               (long long)p->width, (long long)p->page, (long long)p->pages);
   FVB_REQUIRE(p->table && p->lens && p->refs && p->status && p->workspace, "%s: NULL pointer", what);
   FVB_REQUIRE(aligned16(p->workspace), "%s: workspace must be 16-byte aligned", what);
-  c = {p->table, p->lens, p->refs, p->status, p->refused, p->seqs, p->width, p->pages, (int)p->page};
+  c = {p->table, p->lens, p->refs, p->status, p->refused, p->dropped, p->seqs, p->width, p->pages, (int)p->page};
   return FVB_OK;
 }
 

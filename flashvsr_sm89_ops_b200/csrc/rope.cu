@@ -46,7 +46,7 @@ struct Args {
   int D, rot, tokens;  // tokens: a block's share
   int units, turned_units;  // places of a head, those that are turned
   int lanes, side;          // threads of a token, tokens side by side
-  const void* pos;  // NULL: the token's place in its sequence
+  const void* pos;  // NULL: the token's place in its sequence, dropped tokens counted
   int pos64, axes;
   const uint64_t* freq;  // [rot / 2] turns a position, 2^64 to a turn
   const int32_t* axis;   // [rot / 2]
@@ -59,6 +59,7 @@ struct Args {
   int64_t page_stride, slot_stride;  // of the pools
   const int32_t* refused;  // not 0: the chunk has no room (NULL: it has)
   const int32_t* refs;     // sequences that hold a page (NULL: one)
+  const int64_t* dropped;  // tokens that a sequence had before those of lens (NULL: none)
   int32_t* status;
 };
 
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
           else slot = p * a.page_stride + (at - j * a.page) * a.slot_stride;
         }
       }
-      s_pos[threadIdx.x] = at;
+      s_pos[threadIdx.x] = at + (a.dropped ? a.dropped[lo] : 0);
       s_slot[threadIdx.x] = live ? slot : -2;  // -1: no place in the pool, -2: no token at all
     }
     __syncthreads();
@@ -450,6 +451,7 @@ extern "C" int fvb_kv_append(const fvb_kv_append_args* p, fvb_stream_t stream) {
   a.slot_stride = p->Hk * p->D;
   a.refused = p->refused;
   a.refs = p->refs;
+  a.dropped = p->dropped;
   a.status = p->status;
   return rope::launch_dtype(a, (int)p->dtype, p->half != 0, (cudaStream_t)stream, "fvb_kv_append");
 }

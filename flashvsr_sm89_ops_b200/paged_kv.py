@@ -148,6 +148,8 @@ class PagedKV:
     table   int32 [seqs, width]: page numbers of each sequence, -1 for none
     lens    int32 [seqs]: tokens of each sequence
     refs    int32 [P]: how many sequences hold a page, 0 for free
+    dropped int64 [seqs]: tokens that a sequence gave back at its start (all 0 if not handed in); its
+            next token's position is dropped + its place.  0 again once it has no tokens
     status  int32 [1]: what went wrong, see :meth:`check`
 
     The tensors are the state: read them, or hand in ones that hold one.  Free pages are given out
@@ -158,8 +160,8 @@ class PagedKV:
     most 131072 sequences.
     """
 
-    def __init__(self, k, v, table, lens, refs):
-        _lib.require_cuda(k, v, table, lens, refs)
+    def __init__(self, k, v, table, lens, refs, dropped=None):
+        _lib.require_cuda(k, v, table, lens, refs, dropped)
         if k.dim() != 5 or v.shape != k.shape or k.dtype not in _DTYPES or v.dtype != k.dtype:
             raise ValueError(f"PagedKV: k and v must be bf16 or fp16 [layers, P, page, heads, D], got "
                              f"{k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
@@ -181,7 +183,12 @@ class PagedKV:
                 raise ValueError(f"PagedKV: {what} must be contiguous int32 [{n}] on {dev}")
         if v.device != dev:
             raise ValueError(f"PagedKV: k is on {dev}, v on {v.device}")
-        self._tensors = (k, v, table, lens, refs, *torch.zeros(2, dtype=torch.int32, device=dev).split(1))
+        if dropped is None:
+            dropped = torch.zeros(table.shape[0], dtype=torch.int64, device=dev)
+        elif dropped.dtype != torch.int64 or dropped.shape != lens.shape or not dropped.is_contiguous() \
+                or dropped.device != dev:
+            raise ValueError(f"PagedKV: dropped must be contiguous int64 [{table.shape[0]}] on {dev}")
+        self._tensors = (k, v, table, lens, refs, *torch.zeros(2, dtype=torch.int32, device=dev).split(1), dropped)
         self.page = page
         self.device = dev
         seqs, width = table.shape
@@ -190,13 +197,15 @@ class PagedKV:
         self._pools = (k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0) * 2, k.stride(1) * 2, H * D * 2)
         # what every step of the pages takes
         self._pages = _lib.PAGES(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.status.data_ptr(), seqs, width,
-                                 P, page, *self._pools, self._ws.data_ptr(), refused=self.refused.data_ptr())
+                                 P, page, *self._pools, self._ws.data_ptr(), refused=self.refused.data_ptr(),
+                                 dropped=dropped.data_ptr())
         # and every append and attention
         self._index, self._dt, self._dtype = k.get_device(), _DTYPES[k.dtype], k.dtype
         self._shape = (H, D, P, page)
         self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
         self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
-        self._room = {"refused": self.refused.data_ptr(), "refs": refs.data_ptr(), "status": self.status.data_ptr()}
+        self._room = {"refused": self.refused.data_ptr(), "refs": refs.data_ptr(), "status": self.status.data_ptr(),
+                      "dropped": dropped.data_ptr()}
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads: int, head_dim: int, seqs: int,
@@ -216,6 +225,7 @@ class PagedKV:
     refs = property(lambda self: self._tensors[4])
     status = property(lambda self: self._tensors[5])
     refused = property(lambda self: self._tensors[6])
+    dropped = property(lambda self: self._tensors[7])
 
     def check(self):
         """Waits for the device and raises what a step since the last check could not do."""
@@ -243,7 +253,8 @@ class PagedKV:
     def release(self, seqs: torch.Tensor, pages: torch.Tensor | None = None):
         """Sequences (int32 [n], distinct) give back all their pages and become empty, or with
         `pages` (int32 [n]) that many of their first ones: a stream's oldest tokens.  Pages that
-        other sequences hold stay."""
+        other sequences hold stay.  What a sequence keeps is as it was rotated, and its next tokens'
+        positions go on from there (`dropped`)."""
         seqs = _ints(seqs, None, "seqs", "PagedKV.release", self._index)
         n = seqs.shape[0]
         if pages is not None:
@@ -261,7 +272,8 @@ class PagedKV:
         """Writes the last tokens of each sequence, those that reserve() made room for: k, v
         [T, heads, D] of all sequences, sequence b's at cu_seqlens[b] .. cu_seqlens[b + 1] (int32
         [seqs + 1]).  With a Rope, k is rotated on the way and so is q [T, Hq, D], which is
-        returned; positions (as in fused_rope) default to the tokens' places in their sequences.
+        returned; positions (as in fused_rope) default to the tokens' places in their sequences, tokens
+        that release() dropped at their start counted.
         Tokens past cu_seqlens[seqs] are ignored, and rows of out_q for them stay as they are.  If
         the last reserve() could not be done, nothing is written, out_q neither, and check() raises; so
         it does where a token's page belongs to other sequences too, which is left as it is."""

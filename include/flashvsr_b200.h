@@ -415,7 +415,8 @@ FVB_API int fvb_rope(const fvb_rope_args* args, fvb_stream_t stream);
  * table [B][width] of page numbers (-1: none), lens [B] tokens a sequence.  cu [B + 1]: new tokens
  * cu[b] .. cu[b + 1] are the last ones of sequence b's lens[b].
  * Writes k (rotated, rot = 0: as it is) and v of T new tokens to their places, and q rotated to
- * q_out (Hq = 0: no q).  pos NULL: a token's position is its place in the sequence.  Tokens
+ * q_out (Hq = 0: no q).  pos NULL: a token's position is its place in the sequence plus dropped[b]
+ * (NULL: 0), the tokens that the sequence gave back at its start.  Tokens
  * outside cu, and places without a page, are left alone.  bf16 / fp16.
  * refused, refs, status: those of the cache's fvb_pages (NULL: not looked at).  Where the last reserve
  * was refused nothing is written, q_out neither; places in a page that several sequences hold are left
@@ -441,6 +442,7 @@ typedef struct {
   int64_t page_stride;
   const int32_t *refused, *refs;
   int32_t* status;
+  const int64_t* dropped;
 } fvb_kv_append_args;
 FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
 
@@ -449,6 +451,8 @@ FVB_API int fvb_kv_append(const fvb_kv_append_args* args, fvb_stream_t stream);
  * and sets a bit of *status: 1 no free pages, 2 a table row too short, 4 bad arguments (an index
  * out of range or twice, a negative count or length, a branch that is not empty), 8 see fvb_kv_append.
  * refused (NULL: not kept): 1 when the last reserve could not be done, else 0.
+ * dropped [seqs] (NULL: not kept): the tokens that a sequence gave back at its start; 0 again once it
+ * has none left; a branch's is its parent's.
  * workspace: fvb_pages_workspace_bytes(seqs, pages), 16-byte aligned.  At most 131072 sequences.
  *   reserve  room for more[b] tokens in every sequence; lens grow
  *   fork     dst[i] becomes a branch of src[i]: full pages shared, the tokens of a partly filled
@@ -463,6 +467,7 @@ typedef struct {
   int64_t layers, layer_stride, page_stride, row_bytes;
   void* workspace;
   int32_t* refused;
+  int64_t* dropped;
 } fvb_pages;
 FVB_API size_t fvb_pages_workspace_bytes(int64_t seqs, int64_t pages);
 FVB_API int fvb_pages_reserve(const fvb_pages* cache, const int32_t* more, fvb_stream_t stream);

@@ -1,11 +1,14 @@
 """The paged cache, attention over it and rotary positions where a call could go wrong without an error:
 refused room, streams that slide, values that are not finite, outputs that overlap, gradients."""
+import math
+import random
+
 import pytest
 import torch
 
 import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
-from test_attention_pages_gpu import _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
+from test_attention_pages_gpu import _check, _cu, _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -122,3 +125,156 @@ def test_append_leaves_shared_pages_alone():
     pos = torch.cat([torch.arange(24, 32), torch.arange(8, 16), torch.arange(24, 32)]).to(DEV)
     y, both = _rope_64(q, pos[:, None], D, False, f, axis, 1.0, False)
     assert ((oq.double() - y).abs() <= _rope_bound(y, both, q.dtype)).all()
+
+
+# ------------------------------------------------------------------------------- streams that slide
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_positions_of_a_stream_that_slides(layout):
+    """Default positions count every token that a stream ever had; branches go on where their parent is;
+    a stream without tokens begins anew."""
+    H, D, page, seqs = 2, 64, 16, 4
+    dt = torch.float16
+    kv = ops.PagedKV.empty(1, 60, page, H, D, seqs, 12, dtype=dt)
+    rope = ops.Rope(D, layout=layout)
+    f, axis = _freqs((D,))
+    ever = [0] * seqs
+    seed = 60
+
+    def chunk(new):
+        nonlocal seed
+        seed += 1
+        q, k, v = _chunk(sum(new), H, D, seed, dt)
+        kv.reserve(_i32(new))
+        oq = kv.append(0, k, v, _cu(new), q=q, rope=rope)
+        pos = torch.cat([torch.arange(a, a + n) for a, n in zip(ever, new)]).to(DEV)
+        y, both = _rope_64(q, pos[:, None], D, layout == "half", f, axis, 1.0, False)
+        assert ((oq.double() - y).abs() <= _rope_bound(y, both, dt)).all()
+        y, both = _rope_64(k, pos[:, None], D, layout == "half", f, axis, 1.0, False)
+        t = 0
+        for b, n in enumerate(new):
+            if n:
+                here = _tokens(kv, b)[0][0, -n:]
+                assert ((here.double() - y[t:t + n]).abs() <= _rope_bound(y, both, dt)[t:t + n]).all()
+            t += n
+            ever[b] += n
+
+    chunk([70, 40, 0, 5])
+    kv.release(_i32([0, 1]), _i32([2, 1]))
+    chunk([1, 1, 0, 1])
+    chunk([20, 3, 0, 40])
+    kv.release(_i32([3, 0]), _i32([0, 3]))
+    kv.fork(_i32([0]), _i32([2]))
+    ever[2] = ever[0]
+    chunk([2, 2, 9, 1])
+    assert kv.dropped.tolist() == [80, 16, 80, 0]
+    kv.release(_i32([2]))             # all of it
+    kv.release(_i32([1]), _i32([9]))  # more pages than it has
+    ever[1] = ever[2] = 0
+    assert kv.dropped.tolist() == [80, 0, 0, 0]
+    chunk([1, 4, 3, 17])
+    kv.compact()
+    chunk([1, 1, 1, 1])
+    kv.check()
+
+
+def test_a_stream_that_slides_attends_as_one_that_does_not():
+    """The same tokens with and without their oldest pages given back: attention of the next ones over what is
+    kept is the same, as rotation goes by distance."""
+    H, D, page = 2, 64, 16
+    rope = ops.Rope(D)
+    q, k, v = _chunk(100, H, D, 70, torch.float16)
+    outs = []
+    for slide in (False, True):
+        kv = ops.PagedKV.empty(1, 10, page, H, D, 1, 10, dtype=torch.float16)
+        kv.reserve(_i32([96])), kv.append(0, k[:96], v[:96], _i32([0, 96]), rope=rope)
+        if slide:
+            kv.release(_i32([0]), _i32([3]))
+        kv.reserve(_i32([4]))
+        q2 = kv.append(0, k[96:], v[96:], _i32([0, 4]), q=q[96:], rope=rope)
+        if not slide:  # hide the first 48 keys by hand
+            kv.table[0, :7] = kv.table[0, 3:].clone()
+            kv.lens.sub_(48)
+        outs.append(kv.attend(0, q2, _i32([0, 4])))
+    assert torch.equal(*outs)
+
+
+def test_streams_slide_branch_and_go_on():
+    """Two layers: prompts, single tokens, branches, dropped windows, a compaction; every chunk's attention
+    against the tokens that each stream has, rotated by their place among all that it ever had."""
+    layers, Hq, Hk, D, page, seqs = 2, 6, 2, 64, 16, 6
+    dt = torch.float16
+    r = random.Random(5)
+    kv = ops.PagedKV.empty(layers, 160, page, Hk, D, seqs, 40, dtype=dt)
+    kv.k.fill_(math.nan), kv.v.fill_(math.nan)
+    rope = ops.Rope(D, scaling="linear", factor=2.0)
+    f, axis = _freqs((D,))
+    f = f / 2
+    held = [[torch.empty(layers, 0, Hk, D, device=DEV, dtype=dt)] * 2 for _ in range(seqs)]  # of each stream: k and v
+    ever = [0] * seqs
+    g = _gen(6)
+
+    def chunk(new):
+        kv.reserve(_i32(new))
+        pos = torch.cat([torch.arange(a, a + n) for a, n in zip(ever, new)]).to(DEV)
+        for b, n in enumerate(new):
+            ever[b] += n
+            held[b] = [torch.cat([t, t.new_zeros(layers, n, Hk, D)], 1) for t in held[b]]
+        for layer in range(layers):
+            x = torch.randn(sum(new), Hq + 2 * Hk, D, device=DEV, generator=g).to(dt)
+            q, k, v = x.split((Hq, Hk, Hk), 1)
+            q2 = kv.append(layer, k, v, _cu(new), q=q, rope=rope)
+            for t, y in ((q, q2), (k, torch.cat([_tokens(kv, b)[0][layer, -n:] for b, n in enumerate(new) if n]))):
+                want, both = _rope_64(t, pos[:, None], D, False, f, axis, 1.0, False)
+                assert ((y.double() - want).abs() <= _rope_bound(want, both, dt)).all()
+            t0 = 0
+            for b, n in enumerate(new):
+                if n:  # what the cache holds is what attention is judged by
+                    held[b][0][layer, -n:] = _tokens(kv, b)[0][layer, -n:]
+                    held[b][1][layer, -n:] = v[t0:t0 + n]
+                t0 += n
+            out = kv.attend(layer, q2, _cu(new), max_new=max(new))
+            _check(out, q2, [h[0][layer] for h in held], [h[1][layer] for h in held], new, True, D ** -0.5, dt)
+
+    def branch(src, dst):
+        kv.fork(_i32(src), _i32(dst))
+        for a, d in zip(src, dst):
+            held[d], ever[d] = [t.clone() for t in held[a]], ever[a]
+
+    def drop(b, n):
+        kv.release(_i32([b]), None if n is None else _i32([n]))
+        held[b] = [t[:, t.shape[1] if n is None else n * page:] for t in held[b]]
+        if n is None:
+            ever[b] = 0
+
+    chunk([100, 33, 0, 0, 0, 0])
+    chunk([1, 1, 0, 0, 0, 0])
+    branch([0, 1, 0], [2, 3, 5])
+    for _ in range(3):
+        chunk([1, 1, 1, 1, 0, 1])
+    chunk([40, 0, 17, 3, 50, 1])
+    drop(0, 2), drop(3, 1)
+    drop(5, None)
+    kv.compact()
+    used = int((kv.refs > 0).sum())
+    assert (kv.refs[:used] > 0).all() and (kv.refs[used:] == 0).all()
+    branch([0], [5])
+    for _ in range(2):
+        chunk([r.randint(0, 5) for _ in range(seqs - 1)] + [1])
+    drop(5, 3)
+    chunk([64, 20, 1, 130, 2, 16])
+    kv.check()
+
+
+def test_dropped_can_be_handed_in():
+    D = 64
+    rope = ops.Rope(D)
+    kv = ops.PagedKV.empty(1, 4, 16, 1, D, 2, 2)
+    far = torch.tensor([2 ** 33, 5], dtype=torch.int64, device=DEV)
+    kv = ops.PagedKV(kv.k, kv.v, _i32([[0, 1], [2, 3]]), _i32([20, 3]), _i32([1] * 4), far)
+    q, k, v = _chunk(5, 1, D, 80)
+    got = kv.append(0, k, v, _i32([0, 2, 5]), q=q, rope=rope)
+    pos = torch.tensor([2 ** 33 + 18, 2 ** 33 + 19, 5, 6, 7], device=DEV)
+    assert torch.equal(got, ops.fused_rope(q, None, pos, rope)[0])
+    for bad in (far.int(), far[:1], far.cpu(), far.view(2, 1)):
+        with pytest.raises(ValueError):
+            ops.PagedKV(kv.k, kv.v, kv.table, kv.lens, kv.refs, bad)
