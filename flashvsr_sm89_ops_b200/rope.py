@@ -31,7 +31,8 @@ def _frequencies(d: int, theta: float, scaling, factor: float, original_len, bet
         def pair(turns):
             return d * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), d // 2 - 1)
+        # (published as clipped to the channels, not to the pairs: the ramp may end behind the last pair)
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), d - 1)
         ramp = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(d // 2)]
         w = [x * (1 - r) + x / factor * r for x, r in zip(w, ramp)]
     return w

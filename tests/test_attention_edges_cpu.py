@@ -1,5 +1,30 @@
-"""Host side of the paged cache and of rotary positions: what the C entry points and the handles refuse."""
+"""Host side of the paged cache and of rotary positions: frequencies, what the C entry points and the handles refuse."""
+import math
+
+import pytest
+
+import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
+
+
+@pytest.mark.parametrize("d,original,theta", [(128, 131072, 10000.0), (128, 4096, 10000.0), (64, 32768, 500.0),
+                                              (4, 4096, 10000.0), (6, 4096, 10000.0), (2, 4096, 10000.0),
+                                              (96, 8, 10000.0), (80, 1 << 40, 10000.0)])
+def test_yarn_by_its_definition(d, original, theta):
+    """Pair i turns n = original theta^(-2i/d) / 2 pi times.  The pair (a real number) of n = 32 rounded down and
+    that of n = 1 rounded up, both kept within the d channels, are the ends of the ramp."""
+    s = 8.0
+    rope = ops.Rope(d, theta=theta, scaling="yarn", factor=s, original_len=original, device="cpu")
+    got = [(t % 2 ** 64) / 2 ** 64 * 2 * math.pi for t in rope.freq.tolist()]
+    at = [d / 2 * math.log(original / (2 * math.pi * n)) / math.log(theta) for n in (32, 1)]
+    low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), d - 1)
+    for i, w in enumerate(got):
+        plain = theta ** (-2 * i / d)
+        turns = original * plain / (2 * math.pi)
+        r = 0.0 if i <= low else 1.0 if i >= high else (i - low) / (high - low)
+        assert w == pytest.approx(plain * (1 - r) + plain / s * r, rel=1e-12)
+        if turns > 1 and at[1] <= d - 1:
+            assert w > plain / s  # it turns in the original length: not stretched in full
 
 
 def test_append_needs_a_place_for_its_refusal():
