@@ -684,10 +684,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         ll = fmaf(f, s_ml[i][r][1], ll);
       }
       if (whole) {
-        const float inv = ll > 0.f ? 1.f / ll : 0.f;
-        // a row that sees no key is 0, whatever the values that other rows of its tile see
-        if (mm == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const int pr = was_row0 + r, i = pr / a.g;
+        // A row that sees no key is 0, whatever the values that other rows of its tile see.  One that
+        // sees some is not: without a finite score its maximum is -inf too, and the result NaN.
+        const bool sees = seen_by(a, was.s, i + 1) > 0;
+        const float inv = sees ? 1.f / ll : 0.f;
+        if (!sees) acc = make_float4(0.f, 0.f, 0.f, 0.f);
         T* dst = reinterpret_cast<T*>(a.out) + (was.s.t0 + i) * a.o_token +
                  (int64_t)(was.h * a.g + pr - i * a.g) * a.o_head + c;
         *reinterpret_cast<uint2*>(dst) =
@@ -1240,7 +1242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int pr = g.row0 + x * half_rows + row;
       const bool row_ok = row < half_rows && pr < g.n * a.g;
       const bool whole = g.whole;
-      const float inv = (have_o && l > 0.f) ? 1.0f / l : 0.f;
+      const float inv = (have_o && lim > 0) ? 1.0f / l : 0.f;
       const int64_t prow = ((int64_t)blockIdx.x * 2 + (key_t0 == 0)) * kRows + x * half_rows + row;
       const int tok = pr / a.g;
       uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (g.t0 + tok) * a.o_token +
@@ -1257,8 +1259,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
         if (row_ok && whole) {
-          // a row that sees no key is 0, whatever the values that other rows of its tile see
-          if (m_used == -INFINITY) {
+          // a row that sees no key is 0, whatever the values that other rows of its tile see; one that
+          // has no finite score (its maximum is -inf too) is NaN by its sum, 0 or NaN
+          if (lim == 0) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
@@ -1301,7 +1304,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace chunk
 
 // ===========================================================================
-// Joins the parts of an item that CTA boundaries cut, in their order.  D / 8 lanes (a group) take a
+// Joins the parts of an item that CTA boundaries cut, in their order.  A part whose maximum is -inf and
+// whose sum is 0 has no weight (its O may not have been written); with a sum of NaN it has NaN scores,
+// which the result shows.  D / 8 lanes (a group) take a
 // row.  With few rows an item can have hundreds of parts: beyond kWide a block takes a row, its groups
 // every G-th part, four in flight, and the groups are joined through shared memory.  Launched while
 // the kernel before it still runs, it waits for that one's end before it reads anything.
@@ -1355,7 +1360,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a) {
         }
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) {
-          if (ml[i].x == -INFINITY) continue;
+          if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;
           const float f = ex2_approx(ml[i].x - mm);
           acc[0] = fmaf(f, x[i].x, acc[0]), acc[1] = fmaf(f, x[i].y, acc[1]);
           acc[2] = fmaf(f, x[i].z, acc[2]), acc[3] = fmaf(f, x[i].w, acc[3]);
@@ -1379,8 +1384,8 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a) {
       }
     }
     if (live) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
       const int64_t pr = (int64_t)rec.w * a.rows + row, i = pr / a.g;
+      const float inv = seen_by(a, s, (int)i + 1) > 0 ? 1.f / l : 0.f;
       T* dst = reinterpret_cast<T*>(a.out) + (s.t0 + i) * a.o_token +
                ((int64_t)rec.z * a.g + pr - i * a.g) * a.o_head + gl * 8;
       *reinterpret_cast<uint4*>(dst) = make_uint4(

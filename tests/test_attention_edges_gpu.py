@@ -8,7 +8,7 @@ import torch
 
 import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
-from test_attention_pages_gpu import _check, _cu, _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
+from test_attention_pages_gpu import _attend_64, _case, _check, _cu, _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -278,3 +278,47 @@ def test_dropped_can_be_handed_in():
     for bad in (far.int(), far[:1], far.cpu(), far.view(2, 1)):
         with pytest.raises(ValueError):
             ops.PagedKV(kv.k, kv.v, kv.table, kv.lens, kv.refs, bad)
+
+
+# ------------------------------------------------------------------------------- not finite
+@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("D", [64, 128])
+def test_nan_queries_reach_their_rows(D, max_new):
+    """A head of a token that is NaN is NaN in the result, and the others are what they were."""
+    new, had = [300, 1, 40], [700, 9000, 0]  # cut items and whole ones
+    for dtype in (torch.bfloat16, torch.float16):
+        q, k, v, table, lens, ks, vs = _case(new, had, 4, 2, D, 32, dtype, 90)
+        want = ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=max_new)
+        rows = [(0, 1), (17, 0), (299, 3), (300, 2), (301, 0), (340, 1)]
+        for t, h in rows:
+            q[t, h, 5] = math.nan
+        got = ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=max_new)
+        for t, h in rows:
+            assert got[t, h].isnan().all(), (t, h)
+            got[t, h] = want[t, h]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("max_new", [1, 200])
+@pytest.mark.parametrize("bad", [math.nan, -math.inf])
+def test_rows_whose_scores_are_not_finite(bad, max_new):
+    """A row that sees keys, but has only NaN or -inf for scores, is NaN as its softmax is; 0 is for rows that see
+    none.  And a stretch of NaN keys in a long cache is not lost between two parts of an item."""
+    new, had = [200, 3], [0, 0]
+    q, k, v, table, lens, ks, vs = _case(new, had, 2, 1, 64, 16, torch.bfloat16, 91)
+    q = q.abs() + 0.5
+    broken = k.clone()
+    broken[table[1, 0].long(), :3] = bad  # all keys of the second sequence
+    broken[table[0, 0].long(), 0] = bad   # and the only one of the first row
+    out = ops.paged_attention(q, broken, v, table, lens, _cu(new), max_new=max_new)
+    assert out[200:].isnan().all() and out[0].isnan().all()
+    if bad == -math.inf:  # a weight of exactly nothing in the others
+        x = ks[0].clone()
+        x[0] = bad
+        o, a, size = _attend_64(q[1:200], x, vs[0], 199, True, 0.125)
+        assert out[1:200].isfinite().all() and (out[1:200].double() - o).abs().max() <= 2 * 2.0 ** -8 * 2 * a.max()
+    none = ops.paged_attention(q, broken, v, table, _i32([0, 2]), _cu(new), max_new=max_new)
+    assert (none[:200] == 0).all() and (none[200] == 0).all() and none[201:].isnan().all()
+    q, k, v, table, lens, ks, vs = _case([1], [40000], 2, 1, 64, 16, torch.bfloat16, 92)
+    k[table[0, 500:900].long()] = math.nan
+    assert ops.paged_attention(q, k, v, table, lens, _cu([1]), max_new=max_new).isnan().all()
