@@ -375,11 +375,17 @@ __device__ __forceinline__ void let_next_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// kRange: the largest power of two that weights have room for.  A weight is rounded to the type for
+// its product with v, and below the type's normal numbers that is no longer relative to it: in fp16 the
+// many small weights of a long cache would be lost beside one that is 2^25 times each of them.  So all
+// weights carry a factor 2^shift, sum and O alike, that takes the largest near the top of the range;
+// it drops out in the division.
 template <typename T>
 struct Pair;
 template <>
 struct Pair<__nv_bfloat16> {
   static constexpr uint32_t kFmt = 1;  // tcgen05 operand format
+  static constexpr float kRange = 0.f;  // normal numbers go down to 2^-126: no need
   __device__ static uint32_t pack(float lo, float hi) {
     __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&b);
@@ -395,6 +401,7 @@ struct Pair<__nv_bfloat16> {
 template <>
 struct Pair<__half> {
   static constexpr uint32_t kFmt = 0;
+  static constexpr float kRange = 15.f;
   __device__ static uint32_t pack(float lo, float hi) {
     __half2 b = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&b);
@@ -599,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         alpha[hh] = mn == -INFINITY ? 1.f : ex2_approx(m[hh] - mn);
         grew |= mn > m[hh];
         m[hh] = mn;
-        const float sub = mn == -INFINITY ? 0.f : mn;
+        const float sub = mn == -INFINITY ? 0.f : mn - Pair<T>::kRange;  // weights up to 2^kRange
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -618,7 +625,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
           o[i][2] *= alpha[1], o[i][3] *= alpha[1];
         }
       }
-      // P rounded to 16 bits, as the tensor cores take it: 2^-9 (bf16) or 2^-12 (fp16) a term
+      // P rounded to 16 bits, as the tensor cores take it: off by up to 2^-8 (bf16) or 2^-11 (fp16) of a
+      // weight (fp16: or 2^-40 of the largest, if that is more); the sum takes it unrounded
       const uint32_t p[4] = {Pair<T>::pack(sc[0][0], sc[0][1]), Pair<T>::pack(sc[0][2], sc[0][3]),
                              Pair<T>::pack(sc[1][0], sc[1][1]), Pair<T>::pack(sc[1][2], sc[1][3])};
       const int r = (((lane >> 3) & 1) << 3) + (lane & 7);
@@ -724,6 +732,9 @@ constexpr int kCut = 12;  // key tiles, see where items are dealt out
 constexpr int kAtom = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzle
 constexpr float kLazy = 8.0f;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
+// the factor of all weights: with kLazy above it they fill the range
+template <typename T>
+constexpr float kShift = Pair<T>::kRange > kLazy ? Pair<T>::kRange - kLazy : 0.f;
 
 template <int D>
 struct Shape {
@@ -732,7 +743,8 @@ struct Shape {
   static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // alignment, barriers
 };
 
-// p = 2^(s c - m) of 64 scores, packed; fp32 row sum into acc2.  All on the special-function unit: an
+// p = 2^(s c - m) of 64 scores, packed (rounded to 16 bits: off by up to 2^-8 of itself in bf16, 2^-11 or
+// 2^-32 of the largest in fp16); fp32 row sum of the unrounded ones into acc2.  All on the special-function unit: an
 // eighth or a quarter of them as polynomials on the FMA pipe took 8448 over 33792 keys from 1424 to
 // 1412 us, and ragged chunks from 169 to 186-189 us (65 to 66-67 at D 64).
 template <typename T>
@@ -1169,7 +1181,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // tcgen05.ld / st are warp-wide: the warp rescales when any of its rows does
         const bool rescale = __any_sync(0xffffffffu, raise);
-        const float msub = (m_used == -INFINITY) ? 0.f : m_used;
+        const float msub = (m_used == -INFINITY) ? 0.f : m_used - kShift<T>;
         const uint64_t cc = f2_pack(c, c);
         const uint64_t nm = f2_pack(-msub, -msub);
         uint64_t acc2 = f2_pack(0.f, 0.f);

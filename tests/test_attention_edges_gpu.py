@@ -8,7 +8,7 @@ import torch
 
 import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
-from test_attention_pages_gpu import _attend_64, _case, _check, _cu, _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
+from test_attention_pages_gpu import U, _attend_64, _case, _check, _cu, _fill, _freqs, _gen, _i32, _rope_64, _rope_bound, _tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -322,3 +322,27 @@ def test_rows_whose_scores_are_not_finite(bad, max_new):
     q, k, v, table, lens, ks, vs = _case([1], [40000], 2, 1, 64, 16, torch.bfloat16, 92)
     k[table[0, 500:900].long()] = math.nan
     assert ops.paged_attention(q, k, v, table, lens, _cu([1]), max_new=max_new).isnan().all()
+
+
+@pytest.mark.parametrize("max_new,shift", [(1, 15), (130, 7)])
+@pytest.mark.parametrize("L", [40, 3000, 60000])
+def test_many_small_weights_in_fp16(L, max_new, shift):
+    """One key outweighs each of the others by 2^25: together they count all the same.  Weights are held as
+    fp16 times 2^shift, so one is off by 2^-11 of itself or 2^-25-shift, whichever is more."""
+    n, D = 2, 64
+    kv = ops.PagedKV.empty(1, -(-L // 16) + 1, 16, 1, D, 1, dtype=torch.float16)
+    kv.reserve(_i32([L]))
+    k = torch.zeros(L, 1, D, device=DEV, dtype=torch.float16)
+    g = _gen(93)
+    k[:, 0, 0] = -17.5 + torch.rand(L, device=DEV, generator=g) * 0.1
+    k[L // 3, 0, 0] = 0
+    v = torch.rand(L, 1, D, device=DEV, generator=g).half() + 0.5
+    v[L // 3] = 0
+    kv.append(0, k, v, _i32([0, L]))
+    q = torch.zeros(n, 1, D, device=DEV, dtype=torch.float16)
+    q[:, :, 0] = 1
+    out = kv.attend(0, q, _i32([0, n]), sm_scale=1.0, max_new=max_new, causal=False).double()
+    want, a, _ = _attend_64(q, k, v, n, False, 1.0)
+    # the exponent of each weight: 17.5 log2 e in fp32 and its subtraction, 2^-18; then as in _attend_bound
+    tol = want * (2 * U[torch.float16] + 2.0 ** -18 + L * 2.0 ** -23) + L * 1.5 * 2.0 ** (-25 - shift) + 2.0 ** -25
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() / tol).max()
