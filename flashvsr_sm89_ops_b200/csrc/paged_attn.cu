@@ -1410,7 +1410,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Args a) {
 // Whether the rows of the longest sequence fit a tile of the few-rows kernel.  16 streams of up to 4000
 // keys, D 128, few rows against many: 1 row a key head 29.5 and 46.2 us, 4 rows 35.1 and 48.9, 16 rows
 // 34.0 and 44.6; 32 rows, two tiles of it that read the cache twice, 50.2 and 49.9.
-inline bool few_rows(int64_t max_new, int64_t g) { return max_new * g <= dec::kRows; }
+inline bool few_rows(int64_t max_new, int64_t g) { return max_new <= dec::kRows / g; }  // (max_new may be huge)
 inline int ctas_of(bool few) { return sm_count() * (few ? 2 : 1); }
 
 int launch_merge(void (*kernel)(Args), dim3 grid, const Args& a, cudaStream_t stream) {

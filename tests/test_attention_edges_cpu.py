@@ -32,3 +32,12 @@ def test_append_needs_a_place_for_its_refusal():
             16, 16, 2048)
     for kw in ({"refused": 16}, {"refs": 16}):
         assert _lib.load().fvb_kv_append(_lib.KV_APPEND_ARGS(*args, **kw), None) == _lib.FVB_ERR_INVALID
+
+
+@pytest.mark.parametrize("max_new,Hq,Hk", [(1 << 59, 64, 2), (1 << 62, 16, 4), ((1 << 63) - 1, 8, 4), (17, 4, 4),
+                                           (1, 17, 1), (9, 2, 1)])
+def test_many_rows_however_large_their_bound(max_new, Hq, Hk):
+    """The kernel for few rows takes tiles of 16 / (Hq / Hk) whole tokens: none at all for larger groups."""
+    ws = _lib.load().fvb_paged_attn_workspace_bytes
+    assert ws(max_new, Hq, Hk, 128) == ws(17, 1, 1, 128) > ws(16, 1, 1, 128)
+    assert ws(16, 4, 4, 128) == ws(1, 16, 1, 128) == ws(8, 2, 1, 128) == ws(5, 3, 1, 128) == ws(16, 1, 1, 128)

@@ -346,3 +346,13 @@ def test_many_small_weights_in_fp16(L, max_new, shift):
     # the exponent of each weight: 17.5 log2 e in fp32 and its subtraction, 2^-18; then as in _attend_bound
     tol = want * (2 * U[torch.float16] + 2.0 ** -18 + L * 2.0 ** -23) + L * 1.5 * 2.0 ** (-25 - shift) + 2.0 ** -25
     assert ((out - want).abs() <= tol).all(), ((out - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("max_new", [1 << 58, 1 << 59, (1 << 63) - 1])
+def test_huge_bounds_on_the_new_tokens(max_new):
+    """max_new only picks the kernel: one that no product of it fits is that of many rows."""
+    new, had = [3, 1], [50, 200]
+    q, k, v, table, lens, ks, vs = _case(new, had, 64, 2, 64, 16, torch.bfloat16, 102)
+    want = ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=4)
+    assert torch.equal(ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=max_new), want)
+    _check(want, q, ks, vs, new, True, 0.125, torch.bfloat16)
