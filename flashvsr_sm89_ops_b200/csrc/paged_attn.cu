@@ -1510,7 +1510,9 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
                   p->pages > 0 && p->pages < (1ll << 31) && p->width * p->page < (1ll << 31) &&
                   p->T < (1ll << 30) && p->T * p->Hq < (1ll << 30),
               "fvb_paged_attn: shape");
-  FVB_REQUIRE(p->scale > 0 && p->scale < 1e30, "fvb_paged_attn: scale %g", p->scale);
+  // (one that is 0 in fp32 would make -inf * 0 of masked scores)
+  const float scale_log2 = (float)(p->scale * 1.4426950408889634);
+  FVB_REQUIRE(p->scale > 0 && p->scale < 1e30 && scale_log2 > 0.f, "fvb_paged_attn: scale %g", p->scale);
   FVB_REQUIRE(p->max_new >= 1, "fvb_paged_attn: max_new %lld", (long long)p->max_new);
   if (p->T == 0 || p->B == 0) return FVB_OK;
   FVB_REQUIRE(p->cu || p->T == p->B, "fvb_paged_attn: %lld tokens of %lld sequences need cu_seqlens",
@@ -1544,7 +1546,7 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
   a.tokens = few ? pattn::dec::kRows / a.g : 2 * (128 / a.g);
   a.rows = a.tokens * a.g;
   a.few_rows = (int)(few ? p->max_new * a.g : a.rows);
-  a.scale_log2 = (float)(p->scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   a.part = (float*)(ws + w.part);
   a.part_ml = (float*)(ws + w.ml);
   a.rec = (int32_t*)(ws + w.rec);

@@ -41,3 +41,14 @@ def test_many_rows_however_large_their_bound(max_new, Hq, Hk):
     ws = _lib.load().fvb_paged_attn_workspace_bytes
     assert ws(max_new, Hq, Hk, 128) == ws(17, 1, 1, 128) > ws(16, 1, 1, 128)
     assert ws(16, 4, 4, 128) == ws(1, 16, 1, 128) == ws(8, 2, 1, 128) == ws(5, 3, 1, 128) == ws(16, 1, 1, 128)
+
+
+def _attend(T=4, B=4, Hq=2, D=64, page=16, width=2, scale=0.1, q=16):
+    return _lib.load().fvb_paged_attn(_lib.PAGED_ATTN_ARGS(q, Hq * D, D, 16, 8, 8, 8, 16, 8, 8, 8, 16, width, 16, 0, T, B,
+                                                           Hq, Hq, D, 4, page, 1, 1, scale, 0, 32, Hq * D, D, 16), None)
+
+
+@pytest.mark.parametrize("scale", [1e-60, 2.0 ** -151, 5e-324])
+def test_scales_that_are_nothing_in_fp32(scale):
+    assert _attend(scale=scale, T=0, B=0) == _lib.FVB_ERR_INVALID
+    assert _attend(scale=2.0 ** -149, T=0, B=0) == _lib.FVB_OK

@@ -356,3 +356,15 @@ def test_huge_bounds_on_the_new_tokens(max_new):
     want = ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=4)
     assert torch.equal(ops.paged_attention(q, k, v, table, lens, _cu(new), max_new=max_new), want)
     _check(want, q, ks, vs, new, True, 0.125, torch.bfloat16)
+
+
+# ------------------------------------------------------------------------------- refusals
+@pytest.mark.parametrize("scale", [1e-60, 2.0 ** -151])
+def test_scales_that_fp32_does_not_hold(scale):
+    q, k, v, table, lens, ks, vs = _case([130], [3], 2, 2, 64, 16, torch.bfloat16, 95)
+    for m in (1, 130):
+        with pytest.raises(ValueError):
+            ops.paged_attention(q, k, v, table, lens, _cu([130]), sm_scale=scale, max_new=m)
+        for small in (2.0 ** -120, 2.0 ** -140):
+            out = ops.paged_attention(q, k, v, table, lens, _cu([130]), sm_scale=small, max_new=m)
+            _check(out, q, ks, vs, [130], True, small, torch.bfloat16)
