@@ -30,6 +30,9 @@
 namespace fvb {
 namespace pattn {
 
+// Keys of a sequence: the end of their last tile, and of tiles loaded ahead of it, is an int.
+constexpr int64_t kMostKeys = (1ll << 31) - 1024;
+
 struct Args {
   const void* q;
   void* out;
@@ -1507,7 +1510,7 @@ extern "C" int fvb_paged_attn(const fvb_paged_attn_args* p, fvb_stream_t stream)
   FVB_REQUIRE(p->page > 0 && p->page % 16 == 0 && p->page < (1 << 24),
               "fvb_paged_attn: pages must hold a multiple of 16 tokens (got %lld)", (long long)p->page);
   FVB_REQUIRE(p->T >= 0 && p->B >= 0 && p->B < (1 << 30) && p->width >= 0 && p->width < (1ll << 31) &&
-                  p->pages > 0 && p->pages < (1ll << 31) && p->width * p->page < (1ll << 31) &&
+                  p->pages > 0 && p->pages < (1ll << 31) && p->width * p->page <= pattn::kMostKeys &&
                   p->T < (1ll << 30) && p->T * p->Hq < (1ll << 30),
               "fvb_paged_attn: shape");
   // (one that is 0 in fp32 would make -inf * 0 of masked scores)

@@ -483,9 +483,9 @@ FVB_API int fvb_pages_compact(const fvb_pages* cache, fvb_stream_t stream);
  * lens.  A row that sees no key is 0; rows outside cu are left as they were; what lies past lens in
  * a page is not seen.  A page number outside the pool reads as zeros.  cu NULL: one token a sequence
  * (T = B).  max_new: new tokens of the longest sequence; it picks the kernel and need not be exact
- * for the result to be right.  bf16 / fp16, D 64 or 128, pages of a multiple of 16 tokens, scale
- * positive (in fp32 too: above 2^-150).  fp32 scores, statistics and sums; the probabilities are rounded to the input's type
- * for their product with v. */
+ * for the result to be right.  bf16 / fp16, D 64 or 128, pages of a multiple of 16 tokens, tables of at
+ * most 2^31 - 1024 tokens a sequence, scale positive (in fp32 too: above 2^-150).  fp32 scores,
+ * statistics and sums; the probabilities are rounded to the input's type for their product with v. */
 FVB_API size_t fvb_paged_attn_workspace_bytes(int64_t max_new, int64_t Hq, int64_t Hk, int64_t D);
 typedef struct {
   const void* q;

@@ -52,3 +52,9 @@ def _attend(T=4, B=4, Hq=2, D=64, page=16, width=2, scale=0.1, q=16):
 def test_scales_that_are_nothing_in_fp32(scale):
     assert _attend(scale=scale, T=0, B=0) == _lib.FVB_ERR_INVALID
     assert _attend(scale=2.0 ** -149, T=0, B=0) == _lib.FVB_OK
+
+
+def test_tables_up_to_the_last_key():
+    for page, width, rc in ((16, (1 << 27) - 1, _lib.FVB_ERR_INVALID), (1024, (1 << 21) - 1, _lib.FVB_OK),
+                            (16, (1 << 27) - 63, _lib.FVB_ERR_INVALID), (16, (1 << 27) - 64, _lib.FVB_OK)):
+        assert _attend(page=page, width=width, T=0, B=0) == rc, (page, width)
