@@ -64,7 +64,7 @@ def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal
         ot, oh, od = out.stride()
         if od != 1 or (ot | oh) & 7 or out.data_ptr() & 15:
             raise ValueError(f"{name}: out must be 16-byte aligned, with strides that are multiples of 8")
-        if out.data_ptr() == q.data_ptr():
+        if T and out.data_ptr() == q.data_ptr():
             raise ValueError(f"{name}: out cannot be q")
     few = max_new * (Hq // Hk) <= 16
     ws = torch.empty(_WS.get((few, D, index)) or _workspace_bytes(few, D, index), dtype=torch.uint8, device=q.device)

@@ -359,6 +359,16 @@ def test_huge_bounds_on_the_new_tokens(max_new):
 
 
 # ------------------------------------------------------------------------------- refusals
+def test_nothing_to_write():
+    kv = ops.PagedKV.empty(1, 4, 16, 2, 64, 2, 2)
+    z = torch.empty(0, 2, 64, device=DEV, dtype=torch.bfloat16)
+    out = torch.empty_like(z)
+    assert kv.attend(0, z, _i32([0, 0, 0]), out=out) is out
+    assert ops.paged_attention(z, kv.k[0], kv.v[0], kv.table, kv.lens, _i32([0, 0, 0]), out=out) is out
+    rope = ops.Rope(64)
+    assert ops.fused_rope(z, z, _i32([]), rope, out_q=out, out_k=out)[0] is out
+
+
 @pytest.mark.parametrize("scale", [1e-60, 2.0 ** -151])
 def test_scales_that_fp32_does_not_hold(scale):
     q, k, v, table, lens, ks, vs = _case([130], [3], 2, 2, 64, 16, torch.bfloat16, 95)
