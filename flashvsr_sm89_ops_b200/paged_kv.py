@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .rope import _POS64, Rope, _out, _positions, _rows
+from .rope import _POS64, Rope, _apart, _out, _positions, _rows
 
 _DTYPES = {torch.bfloat16: _lib.FVB_BF16, torch.float16: _lib.FVB_F16}
 _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
@@ -32,6 +32,15 @@ def _ints(t, n, what, name, index):
     if t.get_device() != index:
         raise ValueError(f"{name}: {what} is on {t.device}, the cache on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _beside(out, pools, shape, name):
+    """Refuses an output that reaches into the pages of a layer."""
+    Hk, D, P, page = shape
+    at, end = out.data_ptr(), out.data_ptr() + 2 * (1 + sum((n - 1) * s for n, s in zip(out.shape, out.stride())))
+    for p, sp, ss, sh in (pools[:4], pools[4:]):
+        if out.numel() and P and at < p + 2 * ((P - 1) * sp + (page - 1) * ss + (Hk - 1) * sh + D) and p < end:
+            raise ValueError(f"{name}: the output lies over the pages")
 
 
 def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal, sm_scale, max_new, out):
@@ -64,8 +73,8 @@ def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal
         ot, oh, od = out.stride()
         if od != 1 or (ot | oh) & 7 or out.data_ptr() & 15:
             raise ValueError(f"{name}: out must be 16-byte aligned, with strides that are multiples of 8")
-        if T and out.data_ptr() == q.data_ptr():
-            raise ValueError(f"{name}: out cannot be q")
+        _apart((out.data_ptr(), T, Hq, ot, oh, 2), [((q.data_ptr(), T, Hq, st, sh, 2), "q", False)], D, "out", name)
+        _beside(out, pools, shape, name)
     few = max_new * (Hq // Hk) <= 16
     ws = torch.empty(_WS.get((few, D, index)) or _workspace_bytes(few, D, index), dtype=torch.uint8, device=q.device)
     _lib.call_on(index, "fvb_paged_attn",
@@ -97,7 +106,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     head h reads key head h // (Hq / Hk).  table int32 [B, width]; lens int32 [B] with the new
     tokens counted in.  Token i of n sees the first lens - n + i + 1 keys (causal) or all lens.
     D 64 or 128.  Returns [T, Hq, D]; a row that sees no key is 0, and rows past cu_seqlens[B]
-    are left as `out` had them (undefined in a new tensor).
+    are left as `out` had them (undefined in a new tensor).  `out` shares no element with q or the
+    pages.
 
     max_new, the most new tokens a sequence has, picks the kernel: with max_new * Hq / Hk <= 16
     the one for few rows.  It defaults to T (1 without cu_seqlens); any value gives the same
@@ -306,6 +316,13 @@ class PagedKV:
                 raise ValueError(f"{name}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
             oq, ot, oh = _out(out_q, q, "out_q", name)
             qargs = (q3.data_ptr(), st, sh, Hq, oq.data_ptr(), ot, oh)
+            if out_q is not None:
+                _apart((oq.data_ptr(), T, Hq, ot, oh, 2), [((q3.data_ptr(), T, Hq, st, sh, 2), "q", True),
+                                                           ((k.data_ptr(), T, H, kt, kh, 2), "k", False),
+                                                           ((v.data_ptr(), T, H, vt, vh, 2), "v", False)], D, "out_q", name)
+                kp, vp, _, layer_bytes, _, _ = self._pools
+                at = layer * layer_bytes
+                _beside(oq, (kp + at, *self._strides, vp + at, *self._strides), self._shape, name)
         if rope is None:
             if positions is not None:
                 raise ValueError(f"{name}: positions without a Rope")

@@ -134,6 +134,52 @@ def _out(out, x, what, name):
     return out, s[-3], s[-2]
 
 
+def _clash(a, b, D):
+    """Whether two sets of rows share an element.  Each: address, T, H, strides of tokens and heads, bytes an
+    element; rows of D elements.  Sets of different strides that reach into each other count as such."""
+    pa, Ta, Ha, ta, ha, e = a
+    pb, Tb, Hb, tb, hb, _ = b
+    if not Ta or not Tb or not Ha or not Hb:
+        return False
+    if pa + ((Ta - 1) * ta + (Ha - 1) * ha + D) * e <= pb or pb + ((Tb - 1) * tb + (Hb - 1) * hb + D) * e <= pa:
+        return False
+    t, h = (ta if Ta > 1 else tb), (ha if Ha > 1 else hb)  # the stride of an axis of one is any number
+    if (Tb > 1 and t != tb) or (Hb > 1 and h != hb) or (pb - pa) % e:
+        return True
+    d = (pb - pa) // e
+    if Ta == 1 and Tb == 1:
+        t = 0
+    elif t and (Ha - 1) * h + D <= d % t <= t - (Hb - 1) * h - D:
+        return False  # beside each other in every token
+    for i in range(1 - Ha, Hb):
+        c = d + i * h
+        at = (-c // t, -(c // t)) if t else (0,)
+        if any(abs(c + min(max(n, 1 - Ta), Tb - 1) * t) < D for n in at):
+            return True
+    return False
+
+
+def _own(rows, D, what, name):
+    """Refuses an output whose rows lie over each other."""
+    _, T, H, t, h, _ = rows
+    (s0, n0), (s1, n1) = sorted(((t, T), (h, H))) if T > 1 and H > 1 else ((h, H), (t, T))
+    inner = (n0 - 1) * s0 + D if n0 > 1 else D
+    if T and H and ((n0 > 1 and s0 < D) or (n1 > 1 and s1 < inner)):
+        raise ValueError(f"{name}: rows of {what} lie over each other")
+
+
+def _apart(rows, others, D, what, name):
+    """Refuses an output that shares elements with another tensor of the call: others are (rows, its
+    name, whether being that very tensor is fine)."""
+    _own(rows, D, what, name)
+    for other, named, same in others:
+        if same and rows[0] == other[0] and rows[1:3] == other[1:3] and \
+                (rows[1] < 2 or rows[3] == other[3]) and (rows[2] < 2 or rows[4] == other[4]):
+            continue
+        if _clash(rows, other, D):
+            raise ValueError(f"{name}: {what} lies over {named}")
+
+
 def _run(q, k, positions, rope, inverse, out_q, out_k):
     name = "fused_rope"
     dt = _dtype_code(q.dtype, name)
@@ -157,6 +203,17 @@ def _run(q, k, positions, rope, inverse, out_q, out_k):
             raise ValueError(f"{name}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         ok, kot, koh = _out(out_k, k, "out_k", name)
         kargs = (k3.data_ptr(), kt, kh, Hk, ok.data_ptr(), kot, koh)
+    if out_q is not None or out_k is not None:
+        e = q.element_size()
+        ins = [((q3.data_ptr(), T, Hq, st, sh, e), "q")]
+        if k is not None:
+            ins.append(((k3.data_ptr(), T, Hk, kt, kh, e), "k"))
+        rows = (oq.data_ptr(), T, Hq, ot, oh, e)
+        if out_q is not None:
+            _apart(rows, [(r, n, n == "q") for r, n in ins], D, "out_q", name)
+        if out_k is not None:
+            _apart((ok.data_ptr(), T, Hk, kot, koh, e), [(r, n, n == "k") for r, n in ins] + [(rows, "out_q", False)], D,
+                   "out_k", name)
     _lib.call_on(index, "fvb_rope",
                  _lib.ROPE_ARGS(q3.data_ptr(), st, sh, Hq, oq.data_ptr(), ot, oh, *kargs, T, D, rope.rotary_dim,
                                 rope.half, dt, positions.data_ptr(), _POS64[positions.dtype], rope.axes, rope._freq,
@@ -189,7 +246,8 @@ def fused_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     q [T, Hq, D] or [B, L, Hq, D], k the same with its own heads; bf16, fp16 or fp32; any strides
     of tokens and heads (slices of a fused projection are read as they lie).  positions int32 or
     int64, one a token ([T] or [B, L]), or [.., axes] with a Rope of several axes; negative ones
-    turn backwards.  fp32 between loads and stores, one rounding.  out_q / out_k may be q / k.
+    turn backwards.  fp32 between loads and stores, one rounding.  out_q / out_k may be q / k, and
+    otherwise share no element with them or each other.
     inverse turns back, which is the gradient; autograd (once) goes through the call unless
     outputs are given.  D at most 256.
     """

@@ -1,10 +1,12 @@
 """Host side of the paged cache and of rotary positions: frequencies, what the C entry points and the handles refuse."""
 import math
+import random
 
 import pytest
 
 import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
+from flashvsr_sm89_ops_b200.rope import _clash, _own
 
 
 @pytest.mark.parametrize("d,original,theta", [(128, 131072, 10000.0), (128, 4096, 10000.0), (64, 32768, 500.0),
@@ -58,3 +60,40 @@ def test_tables_up_to_the_last_key():
     for page, width, rc in ((16, (1 << 27) - 1, _lib.FVB_ERR_INVALID), (1024, (1 << 21) - 1, _lib.FVB_OK),
                             (16, (1 << 27) - 63, _lib.FVB_ERR_INVALID), (16, (1 << 27) - 64, _lib.FVB_OK)):
         assert _attend(page=page, width=width, T=0, B=0) == rc, (page, width)
+
+
+def _elements(rows, D):
+    p, T, H, t, h, e = rows
+    return {p // e + i * t + j * h + c for i in range(T) for j in range(H) for c in range(D)}
+
+
+def test_rows_that_share_elements():
+    """Against the sets themselves: nothing shared is missed, and of rows of equal strides nothing else refused."""
+    r = random.Random(1)
+    shared = apart = 0
+    for _ in range(20000):
+        D = r.choice((1, 2, 4))
+        h = r.choice((D, D + 1, 2 * D, 3 * D, 40))
+        t = r.choice((h, 3 * h, 4 * h + 1, 7 * D, 2))
+        sets = []
+        for _ in range(2):
+            same = r.random() < 0.8
+            sets.append((2 * r.randint(0, 60), r.randint(0, 4), r.randint(0, 3), t if same else r.choice((h, 5 * h, D)),
+                         h if same else r.choice((D, t)), 2))
+        a, b = sets
+        want = bool(_elements(a, D) & _elements(b, D))
+        got = _clash(a, b, D)
+        assert got or not want, (a, b, D)
+        if (a[3:5] == b[3:5]) and a[1] and b[1]:
+            assert got == want, (a, b, D)
+            shared += want
+            apart += not want
+        rows = _elements(a, D)
+        if len(rows) < a[1] * a[2] * D:
+            with pytest.raises(ValueError):
+                _own(a, D, "out", "test")
+    assert shared > 1000 and apart > 1000
+    _own((0, 8, 4, 640, 64, 2), 64, "out", "test")
+    _own((0, 8, 4, 64, 512, 2), 64, "out", "test")  # heads outside tokens
+    _own((0, 8, 1, 64, 1, 2), 64, "out", "test")
+    _own((0, 1, 4, 0, 64, 2), 64, "out", "test")

@@ -359,6 +359,53 @@ def test_huge_bounds_on_the_new_tokens(max_new):
 
 
 # ------------------------------------------------------------------------------- refusals
+def test_outputs_that_overlap_are_refused():
+    bf = torch.bfloat16
+    x = torch.randn(8, 10, 64, device=DEV, generator=_gen(94)).to(bf)
+    q, k, free = x[:, :4], x[:, 4:6], x[:, 6:]
+    pos = torch.arange(8, device=DEV)
+    rope = ops.Rope(64)
+    one = torch.empty(1, 4, 64, device=DEV, dtype=bf)
+    flat = x.view(-1)
+    shifted = flat.as_strided((8, 4, 64), (640, 64, 1), 64)
+    other = flat.as_strided((8, 4, 64), (256, 64, 1), 0)
+    twice = torch.empty(8, 4, 64, device=DEV, dtype=bf)
+    was = x.clone()
+    for kw in ({"out_q": one.expand(8, 4, 64)}, {"out_q": twice[:, :1].expand(8, 4, 64)}, {"out_q": shifted},
+               {"out_q": other}, {"out_q": k.repeat_interleave(2, 1), "out_k": k[:, :1].expand(8, 2, 64)},
+               {"out_q": free, "out_k": free[:, 1:3]}, {"out_k": q[:, :2]}, {"out_q": x[:, 2:6]},
+               {"out_q": twice.as_strided((8, 4, 64), (64, 64, 1))}):
+        with pytest.raises(ValueError):
+            ops.fused_rope(q, k, pos, rope, **kw)
+            pytest.fail(str(kw.keys()))
+    assert torch.equal(x, was)
+    # what does not overlap is taken, in the same storage too
+    want_q, want_k = ops.fused_rope(q, k, pos, rope)
+    oq, ok = ops.fused_rope(q, k, pos, rope, out_q=free, out_k=k)
+    assert torch.equal(oq, want_q) and torch.equal(ok, want_k) and torch.equal(x[:, :4], was[:, :4])
+    halves = torch.zeros(8, 4, 128, device=DEV, dtype=bf)
+    halves[..., :64] = q
+    oq, _ = ops.fused_rope(halves[..., :64], None, pos, rope, out_q=halves[..., 64:])
+    assert torch.equal(oq, want_q) and torch.equal(halves[..., :64], q)
+
+    new = [5, 3]
+    kv = ops.PagedKV.empty(1, 4, 16, 2, 64, 2, 2)
+    kv.reserve(_i32(new)), kv.append(0, k, k, _cu(new))
+    q = was[:, :4]
+    for out in (one.expand(8, 4, 64), twice[:, :1].expand(8, 4, 64), was.view(-1).as_strided((8, 4, 64), (640, 64, 1), 64),
+                was[:, 2:6], kv.k.view(-1)[:2048].view(8, 4, 64), kv.v.view(-1)[2048:4096].view(8, 4, 64),
+                twice.as_strided((8, 4, 64), (64, 64, 1))):
+        with pytest.raises(ValueError):
+            kv.attend(0, q, _cu(new), out=out)
+        with pytest.raises(ValueError):
+            ops.paged_attention(q, kv.k[0], kv.v[0], kv.table, kv.lens, _cu(new), out=out)
+    want = kv.attend(0, q, _cu(new))
+    assert torch.equal(kv.attend(0, q, _cu(new), out=was[:, 6:]), want)
+    for out in (one.expand(8, 4, 64), was[:, 1:5], kv.k.view(-1)[:2048].view(8, 4, 64)):
+        with pytest.raises(ValueError):
+            kv.append(0, was[:, 4:6], was[:, 4:6], _cu(new), q=q, rope=rope, out_q=out)
+
+
 def test_nothing_to_write():
     kv = ops.PagedKV.empty(1, 4, 16, 2, 64, 2, 2)
     z = torch.empty(0, 2, 64, device=DEV, dtype=torch.bfloat16)
