@@ -10,6 +10,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 from .fp4_quant import _dtype_code
@@ -225,7 +226,8 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, rope, inverse):
         ctx.save_for_backward(positions)
-        ctx.rope, ctx.inverse = rope, inverse
+        ctx.save_for_forward(positions)
+        ctx.rope, ctx.inverse, ctx.two = rope, inverse, k is not None
         oq, ok = _run(q, k, positions, rope, inverse, None, None)
         return (oq, ok) if k is not None else oq
 
@@ -238,6 +240,24 @@ class _Rotate(torch.autograd.Function):
         gq, gk = _run(gq, gk, positions, ctx.rope, not ctx.inverse, None, None)
         return gq, gk, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # linear: tangents are rotated as their tensors are (one that is absent stays so)
+        positions, = ctx.saved_tensors
+        tq, tk = (None if t is None else _run(t, None, positions, ctx.rope, ctx.inverse, None, None)[0] for t in (tq, tk))
+        return (tq, tk) if ctx.two else tq
+
+
+def _tracked(*ts):
+    """Whether autograd has an interest in a call with these tensors, backward or forward."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    # (there are no tangents outside of a dual level, where this costs a comparison)
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in ts)
+
 
 def fused_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rope: Rope, *,
                inverse: bool = False, out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None):
@@ -248,14 +268,14 @@ def fused_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     int64, one a token ([T] or [B, L]), or [.., axes] with a Rope of several axes; negative ones
     turn backwards.  fp32 between loads and stores, one rounding.  out_q / out_k may be q / k, and
     otherwise share no element with them or each other.
-    inverse turns back, which is the gradient; autograd (once) goes through the call unless
-    outputs are given.  D at most 256.
+    inverse turns back, which is the gradient; autograd (once, backward or forward) goes through the
+    call unless outputs are given.  D at most 256.
     """
     if not (q.is_cuda and positions.is_cuda and (k is None or k.is_cuda)):
         _lib.require_cuda(q, k, positions)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _tracked(q, k):
         if out_q is not None or out_k is not None:
-            raise ValueError("fused_rope: out_q / out_k with inputs that require a gradient")
+            raise ValueError("fused_rope: out_q / out_k with inputs that require a gradient or carry a tangent")
         r = _Rotate.apply(q, k, positions, rope, bool(inverse))
         return r if k is not None else (r, None)
     return _run(q, k, positions, rope, bool(inverse), out_q, out_k)

@@ -425,3 +425,27 @@ def test_scales_that_fp32_does_not_hold(scale):
         for small in (2.0 ** -120, 2.0 ** -140):
             out = ops.paged_attention(q, k, v, table, lens, _cu([130]), sm_scale=small, max_new=m)
             _check(out, q, ks, vs, [130], True, small, torch.bfloat16)
+
+
+# ------------------------------------------------------------------------------- gradients
+def test_rope_tangents():
+    import torch.autograd.forward_ad as fwd
+    g = _gen(96)
+    q, k, tq, tk = (torch.randn(9, h, 32, device=DEV, generator=g) for h in (4, 2, 4, 2))
+    pos = torch.arange(9, device=DEV)
+    rope = ops.Rope(24, scaling="yarn", factor=2.0, original_len=512)
+    for inverse in (False, True):
+        wq, wk = ops.fused_rope(tq, tk, pos, rope, inverse=inverse)
+        pq, pk = ops.fused_rope(q, k, pos, rope, inverse=inverse)
+        with fwd.dual_level():
+            oq, ok = (fwd.unpack_dual(x) for x in ops.fused_rope(fwd.make_dual(q, tq), fwd.make_dual(k, tk), pos, rope,
+                                                                 inverse=inverse))
+            assert torch.equal(oq.primal, pq) and torch.equal(ok.primal, pk)
+            assert torch.equal(oq.tangent, wq) and torch.equal(ok.tangent, wk)
+            oq, ok = (fwd.unpack_dual(x) for x in ops.fused_rope(q, fwd.make_dual(k, tk), pos, rope, inverse=inverse))
+            assert oq.tangent is None or (oq.tangent == 0).all()
+            assert torch.equal(ok.tangent, wk)
+            y, none = ops.fused_rope(fwd.make_dual(q, tq), None, pos, rope, inverse=inverse)
+            assert none is None and torch.equal(fwd.unpack_dual(y).tangent, wq)
+            with pytest.raises(ValueError):
+                ops.fused_rope(fwd.make_dual(q, tq), None, pos, rope, out_q=torch.empty_like(q))
