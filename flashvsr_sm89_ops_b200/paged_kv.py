@@ -8,14 +8,15 @@ heads; this is the form for many streams of uneven length, shared key heads and 
 
 All state is device memory and every call is launches on the current stream, so a step over the
 cache can be captured in a graph and replayed while the lengths grow.  Calls that change a cache
-belong on one stream, or must be ordered by the caller.  Inference only.
+belong on one stream, or must be ordered by the caller.  Inference only: inputs may require gradients,
+but a backward pass through a result raises.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
-from .rope import _POS64, Rope, _apart, _out, _positions, _rows
+from .rope import _POS64, Rope, _apart, _out, _positions, _rows, _tracked
 
 _DTYPES = {torch.bfloat16: _lib.FVB_BF16, torch.float16: _lib.FVB_F16}
 _STATUS = {1: "no free pages left", 2: "a sequence outgrew its table row",
@@ -34,6 +35,32 @@ def _ints(t, n, what, name, index):
     return t if t.is_contiguous() else t.contiguous()
 
 
+class _NoGradient(torch.autograd.Function):
+    """A result of inputs that autograd follows.  It is what it is without them, but a backward pass through it
+    raises where it would otherwise go by without these inputs' share."""
+
+    @staticmethod
+    def forward(ctx, name, y, *inputs):
+        ctx.name = name
+        ctx.mark_dirty(y)
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError(f"{ctx.name} has no gradient (inference only)")
+
+
+def _followed(name, y, *inputs):
+    """y, the result of these inputs, for autograd: itself where that can be, else another name of it (a
+    leaf, one of several views of a tensor)."""
+    if not _tracked(*inputs):
+        return y
+    try:
+        return _NoGradient.apply(name, y, *inputs)
+    except RuntimeError:
+        return _NoGradient.apply(name, y.detach(), *inputs)
+
+
 def _beside(out, pools, shape, name):
     """Refuses an output that reaches into the pages of a layer."""
     Hk, D, P, page = shape
@@ -43,8 +70,9 @@ def _beside(out, pools, shape, name):
             raise ValueError(f"{name}: the output lies over the pages")
 
 
-def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal, sm_scale, max_new, out):
-    """The call itself.  pools: k, its three strides, v, its three strides; shape: Hk, D, P, page."""
+def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal, sm_scale, max_new, out, inputs):
+    """The call itself.  pools: k, its three strides, v, its three strides; shape: Hk, D, P, page; inputs: what
+    autograd could follow."""
     index = q.get_device()
     T, Hq, D = q.shape
     Hk, _, P, page = shape
@@ -81,7 +109,7 @@ def _attend(name, q, dt, pools, shape, table, width, lens, B, cu_seqlens, causal
                  _lib.PAGED_ATTN_ARGS(q.data_ptr(), st, sh, *pools, table, width, lens, cu, T, B, Hq, Hk, D, P, page,
                                       max_new, causal, D ** -0.5 if sm_scale is None else sm_scale, dt,
                                       out.data_ptr(), ot, oh, ws.data_ptr()), _lib.stream_of(q))
-    return out
+    return _followed(name, out, *inputs)
 
 
 _WS: dict = {}
@@ -147,7 +175,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             elif s[i] & 7 or s[i] <= 0:
                 raise ValueError(f"{name}: strides of the pages must be positive multiples of 8, got {tuple(t.stride())}")
     return _attend(name, q, dt, (k_pages.data_ptr(), *ks[:3], v_pages.data_ptr(), *vs[:3]), (Hk, D, P, page),
-                   table.data_ptr(), table.shape[1], lens.data_ptr(), B, cu_seqlens, causal, sm_scale, max_new, out)
+                   table.data_ptr(), table.shape[1], lens.data_ptr(), B, cu_seqlens, causal, sm_scale, max_new, out,
+                   (q, k_pages, v_pages))
 
 
 class PagedKV:
@@ -344,7 +373,7 @@ class PagedKV:
                      _lib.KV_APPEND_ARGS(*qargs, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, H, T, D, *rargs,
                                          cu.data_ptr(), lens, table, seqs, width, P, page, kp + at, vp + at,
                                          self._strides[0], **self._room), _lib.stream_of(k))
-        return oq
+        return None if oq is None else _followed(name, oq, q, k, v)
 
     def attend(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, causal: bool = True,
                sm_scale: float | None = None, max_new: int | None = None,
@@ -362,4 +391,4 @@ class PagedKV:
         at, s = layer * layer_bytes, self._strides
         lens, table, seqs, width, _, _ = self._tail
         return _attend(name, q, self._dt, (kp + at, *s, vp + at, *s), self._shape, table, width, lens, seqs,
-                       cu_seqlens, causal, sm_scale, max_new, out)
+                       cu_seqlens, causal, sm_scale, max_new, out, (q,))

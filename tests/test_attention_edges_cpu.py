@@ -3,9 +3,11 @@ import math
 import random
 
 import pytest
+import torch
 
 import flashvsr_sm89_ops_b200 as ops
 from flashvsr_sm89_ops_b200 import _lib
+from flashvsr_sm89_ops_b200.paged_kv import _followed
 from flashvsr_sm89_ops_b200.rope import _clash, _own
 
 
@@ -97,3 +99,22 @@ def test_rows_that_share_elements():
     _own((0, 8, 4, 64, 512, 2), 64, "out", "test")  # heads outside tokens
     _own((0, 8, 1, 64, 1, 2), 64, "out", "test")
     _own((0, 1, 4, 0, 64, 2), 64, "out", "test")
+
+
+def test_results_that_autograd_follows():
+    w = torch.randn(3, 4, requires_grad=True)
+    x = w * 1
+    for y in (torch.zeros(3, 4), torch.zeros(3, 8)[:, 4:], torch.zeros(4, 3, 4).unbind(0)[1], torch.zeros(3, 8).chunk(2, 1)[0]):
+        z = _followed("this", y, None, x)
+        assert z.data_ptr() == y.data_ptr() and z.stride() == y.stride()
+        with pytest.raises(RuntimeError, match="this has no gradient"):
+            z.sum().backward()
+    for y in (x, w):  # an input as the result, a leaf too
+        z = _followed("this", y, y)
+        assert z.data_ptr() == y.data_ptr()
+        with pytest.raises(RuntimeError, match="this has no gradient"):
+            z.sum().backward()
+    y = torch.zeros(3, 4)
+    assert _followed("this", y, w.detach(), None) is y and not y.requires_grad
+    with torch.no_grad():
+        assert _followed("this", y, w) is y and not y.requires_grad

@@ -449,3 +449,35 @@ def test_rope_tangents():
             assert none is None and torch.equal(fwd.unpack_dual(y).tangent, wq)
             with pytest.raises(ValueError):
                 ops.fused_rope(fwd.make_dual(q, tq), None, pos, rope, out_q=torch.empty_like(q))
+
+
+def test_what_has_no_gradient_says_so():
+    """Results are what they are without gradients; a backward pass through them raises."""
+    import torch.autograd.forward_ad as fwd
+    bf = torch.bfloat16
+    new = [5, 3]
+    kv = ops.PagedKV.empty(1, 4, 16, 2, 64, 2, 2)
+    kv.reserve(_i32(new))
+    x = torch.randn(8, 8, 64, device=DEV, generator=_gen(97)).to(bf)
+    rope = ops.Rope(64)
+    want_q = kv.append(0, x[:, 4:6], x[:, 6:], _cu(new), q=x[:, :4], rope=rope)
+    want = kv.attend(0, want_q, _cu(new))
+    w = x.clone().requires_grad_()
+    y = w * 1
+    q2 = kv.append(0, y[:, 4:6], y[:, 6:], _cu(new), q=y[:, :4], rope=rope)
+    assert torch.equal(q2.detach(), want_q)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        q2.sum().backward(retain_graph=True)
+    wide = torch.zeros(8, 4, 128, device=DEV, dtype=bf)
+    for out in (kv.attend(0, q2, _cu(new)), kv.attend(0, y[:, :4], _cu(new)), kv.attend(0, q2, _cu(new), out=wide[..., 64:]),
+                ops.paged_attention(x[:, :4], (kv.k[0].clone().requires_grad_() * 1), kv.v[0], kv.table, kv.lens, _cu(new))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.float().sum().backward(retain_graph=True)
+    assert torch.equal(wide[..., 64:].detach(), want) and w.grad is None
+    with torch.no_grad():
+        assert not kv.attend(0, q2, _cu(new)).requires_grad
+    assert not kv.attend(0, x[:, :4], _cu(new)).requires_grad
+    with fwd.dual_level():
+        assert torch.equal(kv.attend(0, want_q, _cu(new)), want)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            kv.attend(0, fwd.make_dual(want_q, want_q.clone()), _cu(new))
