@@ -228,23 +228,36 @@ class PagedKV:
                 or dropped.device != dev:
             raise ValueError(f"PagedKV: dropped must be contiguous int64 [{table.shape[0]}] on {dev}")
         self._tensors = (k, v, table, lens, refs, *torch.zeros(2, dtype=torch.int32, device=dev).split(1), dropped)
+        self._bind()
+
+    def _bind(self):
+        k, v, table, lens, refs, status, refused, dropped = self._tensors
+        _, P, page, H, D = k.shape
         self.page = page
-        self.device = dev
+        self.device = dev = k.device
         seqs, width = table.shape
         n = _lib.load().fvb_pages_workspace_bytes(seqs, P)
         self._ws = torch.empty(n, dtype=torch.uint8, device=dev)
         self._pools = (k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0) * 2, k.stride(1) * 2, H * D * 2)
         # what every step of the pages takes
-        self._pages = _lib.PAGES(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.status.data_ptr(), seqs, width,
-                                 P, page, *self._pools, self._ws.data_ptr(), refused=self.refused.data_ptr(),
+        self._pages = _lib.PAGES(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), status.data_ptr(), seqs, width, P,
+                                 page, *self._pools, self._ws.data_ptr(), refused=refused.data_ptr(),
                                  dropped=dropped.data_ptr())
         # and every append and attention
         self._index, self._dt, self._dtype = k.get_device(), _DTYPES[k.dtype], k.dtype
         self._shape = (H, D, P, page)
         self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
         self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
-        self._room = {"refused": self.refused.data_ptr(), "refs": refs.data_ptr(), "status": self.status.data_ptr(),
+        self._room = {"refused": refused.data_ptr(), "refs": refs.data_ptr(), "status": status.data_ptr(),
                       "dropped": dropped.data_ptr()}
+
+    # a copy has tensors, and so addresses, of its own
+    def __getstate__(self):
+        return {"_tensors": self._tensors}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     @classmethod
     def empty(cls, layers: int, pages: int, page: int, heads: int, head_dim: int, seqs: int,

@@ -82,9 +82,17 @@ class Rope:
         self._tensors = (torch.tensor(turns, dtype=torch.int64, device=device),
                          torch.tensor([a for a, d in enumerate(dims) for _ in range(d // 2)], dtype=torch.int32,
                                       device=device))
+        self._bind()
+
+    def _bind(self):
         self.device = self.freq.device
         self.index = self.freq.get_device()  # -1 on the host
         self._freq, self._axis = self.freq.data_ptr(), self.axis.data_ptr()
+
+    # a copy (of a model that holds one, say) has tensors, and so addresses, of its own
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     # the calls hold the addresses of these
     freq = property(lambda self: self._tensors[0])

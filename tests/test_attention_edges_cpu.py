@@ -1,5 +1,7 @@
 """Host side of the paged cache and of rotary positions: frequencies, what the C entry points and the handles refuse."""
+import copy
 import math
+import pickle
 import random
 
 import pytest
@@ -118,3 +120,13 @@ def test_results_that_autograd_follows():
     assert _followed("this", y, w.detach(), None) is y and not y.requires_grad
     with torch.no_grad():
         assert _followed("this", y, w) is y and not y.requires_grad
+
+
+def test_copies_of_a_rope_have_their_own_tensors():
+    rope = ops.Rope(64, axes=(32, 32), scaling="yarn", factor=2.0, original_len=512, device="cpu")
+    for twin in (copy.deepcopy(rope), pickle.loads(pickle.dumps(rope)), copy.deepcopy({"a": [rope]})["a"][0]):
+        assert twin._freq == twin.freq.data_ptr() != rope.freq.data_ptr()
+        assert twin._axis == twin.axis.data_ptr() != rope.axis.data_ptr()
+        assert torch.equal(twin.freq, rope.freq) and torch.equal(twin.axis, rope.axis) and repr(twin) == repr(rope)
+    same = copy.copy(rope)
+    assert same._freq == rope._freq == rope.freq.data_ptr()

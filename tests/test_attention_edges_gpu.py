@@ -1,5 +1,6 @@
 """The paged cache, attention over it and rotary positions where a call could go wrong without an error:
 refused room, streams that slide, values that are not finite, outputs that overlap, gradients."""
+import copy
 import math
 import random
 
@@ -481,3 +482,27 @@ def test_what_has_no_gradient_says_so():
         assert torch.equal(kv.attend(0, want_q, _cu(new)), want)
         with pytest.raises((RuntimeError, NotImplementedError)):
             kv.attend(0, fwd.make_dual(want_q, want_q.clone()), _cu(new))
+
+
+# ------------------------------------------------------------------------------- copies of a handle
+def test_copies_have_their_own_tensors():
+    rope = ops.Rope(64, axes=(32, 32))
+    x = torch.randn(4, 2, 64, device=DEV, generator=_gen(98)).bfloat16()
+    pos = torch.arange(8, device=DEV).view(4, 2)
+    want = ops.fused_rope(x, None, pos, rope)[0]
+    twin = copy.deepcopy(rope)
+    rope.freq.zero_()
+    assert torch.equal(ops.fused_rope(x, None, pos, twin)[0], want)
+    kv = ops.PagedKV.empty(2, 8, 16, 2, 64, 3, 4)
+    kv.reserve(_i32([20, 3, 0]))
+    kv.append(1, *_chunk(23, 2, 64, 99)[:2], _i32([0, 20, 23, 23]))
+    q = _chunk(23, 4, 64, 100)[0]
+    want = kv.attend(1, q, _i32([0, 20, 23, 23]))
+    twin = copy.deepcopy(kv)
+    twin.release(_i32([0]))
+    twin.reserve(_i32([0, 17, 4]))
+    twin.append(1, *_chunk(21, 2, 64, 101)[:2], _i32([0, 0, 17, 21]))
+    assert kv.lens.tolist() == [20, 3, 0] and kv.refs.tolist() == [1, 1, 1, 0, 0, 0, 0, 0]
+    assert torch.equal(kv.attend(1, q, _i32([0, 20, 23, 23])), want)
+    assert twin.lens.tolist() == [0, 20, 4]
+    kv.check(), twin.check()
