@@ -506,3 +506,44 @@ def test_copies_have_their_own_tensors():
     assert torch.equal(kv.attend(1, q, _i32([0, 20, 23, 23])), want)
     assert twin.lens.tolist() == [0, 20, 4]
     kv.check(), twin.check()
+
+
+# ------------------------------------------------------------------------------- long lists
+def test_lists_too_long_for_shared_memory():
+    """More sequences, pages of one call and branches than the kernels keep in shared memory."""
+    from test_attention_pages_gpu import Book
+    seqs, page = 6000, 16
+    r = random.Random(8)
+    kv = ops.PagedKV.empty(1, 30000, page, 1, 8, seqs, 6, dtype=torch.float16)
+    _fill(kv, 9)
+    book = Book.of(kv)
+    more = [r.choice((0, 5, 16, 40, 48)) if b % 2 else 0 for b in range(seqs)]
+    assert sum(book.pages(n) for n in more) > 2048
+    kv.reserve(_i32(more))
+    book.reserve(more)
+    book.check(kv)
+    dst = [b for b in range(0, seqs, 2)]
+    r.shuffle(dst)
+    dst = dst[:2500]
+    src = [r.randrange(1, seqs, 2) for _ in dst]
+    some = r.sample(range(len(dst)), 40)
+    before = [_tokens(kv, src[i]) for i in some]
+    kv.fork(_i32(src), _i32(dst))
+    book.fork(src, dst)
+    book.check(kv)
+    for i, (k, v) in zip(some, before):
+        k2, v2 = _tokens(kv, dst[i])
+        assert torch.equal(k, k2) and torch.equal(v, v2)
+    drop = r.sample(range(seqs), 3000)
+    count = [r.choice((0, 1, 2, 100)) for _ in drop]
+    kv.release(_i32(drop), _i32(count))
+    book.release(drop, count)
+    book.check(kv)
+    kv.compact()
+    book.compact()
+    book.check(kv)
+    more = [r.choice((0, 1, 20)) if n <= 40 else 0 for n in book.lens]
+    kv.reserve(_i32(more))
+    book.reserve(more)
+    book.check(kv)
+    kv.check()
