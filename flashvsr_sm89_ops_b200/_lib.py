@@ -112,12 +112,12 @@ _SIGS = {
 # fvb_rope_args, fvb_kv_append_args, fvb_paged_attn_args and fvb_pages: every member is 8 bytes
 ROPE_ARGS = struct.Struct("=24qdq").pack
 PAGED_ATTN_ARGS = struct.Struct("=24qd5q").pack
-_KV_APPEND = struct.Struct("=24qd14q").pack
+KV_APPEND_ALL = struct.Struct("=24qd14q").pack
 _PAGES = struct.Struct("=17q").pack
 
 
 def KV_APPEND_ARGS(*members, refused=0, refs=0, status=0, dropped=0):
-    return _KV_APPEND(*members, refused, refs, status, dropped)
+    return KV_APPEND_ALL(*members, refused, refs, status, dropped)
 
 
 def PAGES(*members, refused=0, dropped=0):

@@ -149,8 +149,9 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const Cache c, const 
   }
   __syncthreads();
   for (int64_t b = threadIdx.x; b < c.seqs; b += kThreads) {
-    if (c.dropped && c.lens[b] == 0) c.dropped[b] = 0;  // begins anew
-    c.lens[b] += more[b];
+    const int32_t len = c.lens[b];
+    c.lens[b] = len + more[b];
+    if (c.dropped && len == 0) c.dropped[b] = 0;  // begins anew
   }
 }
 
@@ -226,10 +227,11 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const Cache c, const int
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int32_t len = c.lens[src[i]];
+    const int32_t a = src[i], d = dst[i], len = c.lens[a];
+    const int64_t before = c.dropped ? c.dropped[a] : 0;
     copies[i].to = len % c.page ? list[n <= kSmall ? s_rank[i] : copies[i].to] : 0;
-    c.lens[dst[i]] = len;
-    if (c.dropped) c.dropped[dst[i]] = c.dropped[src[i]];
+    c.lens[d] = len;
+    if (c.dropped) c.dropped[d] = before;
   }
 }
 
@@ -280,11 +282,12 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const Cache c, const 
     }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int64_t b = seqs[i], have = held(c, c.lens[b]);
-    const int64_t len = c.lens[b], left = len - (int64_t)(drop ? drop[i] : 0) * c.page;
+    const int64_t b = seqs[i], len = c.lens[b], have = held(c, len);
+    const int64_t before = drop && c.dropped ? c.dropped[b] : 0;
+    const int64_t left = len - (int64_t)(drop ? drop[i] : 0) * c.page;
     const int32_t now = !drop || drop[i] >= have ? 0 : (int32_t)(left > 0 ? left : 0);
     c.lens[b] = now;
-    if (c.dropped) c.dropped[b] = now ? c.dropped[b] + (len - now) : 0;
+    if (c.dropped) c.dropped[b] = now ? before + (len - now) : 0;
   }
 }
 

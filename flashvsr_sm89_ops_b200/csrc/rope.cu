@@ -202,8 +202,10 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
     load(lane_token);
   }
 
+  int32_t refs = 0;  // sequences that hold this thread's token's page: they arrive while the angles are formed
   if (a.cu) {
     if (threadIdx.x < n) {
+      const int32_t refused = a.refused ? *a.refused : 0;
       const int64_t t = t0 + threadIdx.x;
       // last sequence that starts at or before t; tokens behind the last sequence are left alone
       int64_t lo = 0, hi = a.B;
@@ -214,21 +216,22 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
       const int64_t c0 = a.cu[lo], c1 = a.cu[lo + 1];
       bool live = c0 <= t && t < c1;
       // without the room that a reserve makes, the places counted back from lens are cached tokens'
-      if (live && a.refused && *a.refused) {
+      if (live && refused) {
         live = false;
         atomicOr(a.status, kNotAppended);
       }
+      const int64_t before = a.dropped ? a.dropped[lo] : 0;
       const int64_t at = (int64_t)a.lens[lo] - (c1 - c0) + (t - c0);
       int64_t slot = -1;
       if (live && at >= 0) {
         const int64_t j = at / a.page;
         const int32_t p = j < a.width ? a.table[lo * a.width + j] : -1;
         if (p >= 0 && p < a.pages) {
-          if (a.refs && a.refs[p] > 1) atomicOr(a.status, kNotAppended);  // other sequences' tokens too
-          else slot = p * a.page_stride + (at - j * a.page) * a.slot_stride;
+          if (a.refs) refs = a.refs[p];
+          slot = p * a.page_stride + (at - j * a.page) * a.slot_stride;
         }
       }
-      s_pos[threadIdx.x] = at + (a.dropped ? a.dropped[lo] : 0);
+      s_pos[threadIdx.x] = at + before;
       s_slot[threadIdx.x] = live ? slot : -2;  // -1: no place in the pool, -2: no token at all
     }
     __syncthreads();
@@ -250,6 +253,10 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const Args a) {
     float* cs = cs_all + tk * a.rot + pr;
     cs[0] = c * a.scale;
     cs[half_rot] = (a.inverse ? -s : s) * a.scale;
+  }
+  if (refs > 1) {  // other sequences' tokens too
+    s_slot[threadIdx.x] = -1;
+    atomicOr(a.status, kNotAppended);
   }
   __syncthreads();
   if (!works) return;

@@ -121,7 +121,7 @@ int make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
 
 extern "C" {
 
-int fvb_abi_version(void) { return 1; }
+int fvb_abi_version(void) { return 2; }
 
 const char* fvb_last_error(void) { return fvb::t_err; }
 

@@ -248,8 +248,7 @@ class PagedKV:
         self._shape = (H, D, P, page)
         self._strides = (k.stride(1) if P > 1 else page * H * D, H * D, D)
         self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
-        self._room = {"refused": refused.data_ptr(), "refs": refs.data_ptr(), "status": status.data_ptr(),
-                      "dropped": dropped.data_ptr()}
+        self._room = (refused.data_ptr(), refs.data_ptr(), status.data_ptr(), dropped.data_ptr())
 
     # a copy has tensors, and so addresses, of its own
     def __getstate__(self):
@@ -383,9 +382,9 @@ class PagedKV:
         kp, vp, _, layer_bytes, _, _ = self._pools
         at = layer * layer_bytes
         _lib.call_on(index, "fvb_kv_append",
-                     _lib.KV_APPEND_ARGS(*qargs, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, H, T, D, *rargs,
-                                         cu.data_ptr(), lens, table, seqs, width, P, page, kp + at, vp + at,
-                                         self._strides[0], **self._room), _lib.stream_of(k))
+                     _lib.KV_APPEND_ALL(*qargs, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, H, T, D, *rargs,
+                                        cu.data_ptr(), lens, table, seqs, width, P, page, kp + at, vp + at,
+                                        self._strides[0], *self._room), _lib.stream_of(k))
         return None if oq is None else _followed(name, oq, q, k, v)
 
     def attend(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, causal: bool = True,

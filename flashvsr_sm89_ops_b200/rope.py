@@ -258,10 +258,9 @@ class _Rotate(torch.autograd.Function):
 
 def _tracked(*ts):
     """Whether autograd has an interest in a call with these tensors, backward or forward."""
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return True
+    for t in ts:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            return True
     # (there are no tangents outside of a dual level, where this costs a comparison)
     return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
                                                   for t in ts)
