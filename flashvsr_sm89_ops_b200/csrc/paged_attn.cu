@@ -749,7 +749,8 @@ struct Shape {
 // p = 2^(s c - m) of 64 scores, packed (rounded to 16 bits: off by up to 2^-8 of itself in bf16, 2^-11 or
 // 2^-32 of the largest in fp16); fp32 row sum of the unrounded ones into acc2.  All on the special-function unit: an
 // eighth or a quarter of them as polynomials on the FMA pipe took 8448 over 33792 keys from 1424 to
-// 1412 us, and ragged chunks from 169 to 186-189 us (65 to 66-67 at D 64).
+// 1412 us, and ragged chunks (32 of up to 600 tokens over up to 600, 32 / 8 heads of 128, pages of 16)
+// from 169 to 186-189 us; 7 of up to 1537 over up to 1001, 16 / 4 x 64, from 65 to 66-67.
 template <typename T>
 __device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint64_t nm,
                                            uint64_t& acc2, uint32_t* pk) {

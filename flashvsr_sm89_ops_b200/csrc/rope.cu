@@ -7,14 +7,17 @@
 // scaling for long contexts.
 //
 // Angles: w_i / 2 pi is held as a 64-bit fraction of a turn, so p * w_i modulo one turn is an
-// integer product that drops whole turns exactly: the angle of a position of any size is good to
-// fp32, where p * w in fp32 has lost it by p = 2^16.  One angle a token and pair, in shared
-// memory, serves every head of q and k.
+// integer product that drops whole turns exactly: the angle is good to fp32 up to positions of about
+// 2^30, where p * w in fp32 has lost it by p = 2^16.  (w itself comes from a 64-bit float: beyond, the
+// angle is off by up to p w 2^-52.)  One angle a token and pair, in shared memory, serves every head
+// of q and k.
 //
 // Bound by memory: q and k are read and written once (append: q, k and v, with k and v written
-// to their pages).  Measured (B200, cold inputs): 8448 tokens of 12 + 12 heads of 128 in bf16 19.7 us
-// (104 MB at 5.3 TB/s), 16896 tokens appended 50 us (261 MB at 5.2 TB/s), 4099 tokens of 24 + 4 heads
-// of 80 in fp32 11.6 us (73 MB at 6.3 TB/s).  An earlier form that dealt rows of heads to threads
+// to their pages).  Measured (B200, cold inputs): 8448 tokens of 12 + 12 heads of 128 in bf16 19.5 us
+// (104 MB at 5.3 TB/s), 16896 tokens appended 51.6 us (261 MB at 5.1 TB/s), 4099 tokens of 24 + 4 heads
+// of 80 in fp32 11.4 us (73 MB at 6.4 TB/s).  Where vectors do not fit, an element at a time: 8448
+// tokens of 12 + 12 heads of 96 in bf16, 24 of them turned in halves, 57 us (1.4 TB/s; 32 of them,
+// with vectors, 14.4).  An earlier form that dealt rows of heads to threads
 // spent 63% of its issue slots on indexes (27, 54 and 21 us); one that kept blocks resident and
 // prefetched the next tokens' angles held too many registers to cover latency (34, 74 and 20 us).
 #include "common.cuh"
@@ -340,9 +343,10 @@ int launch(Args& a, bool half, cudaStream_t stream, const char* what) {
   a.turned_units = (half || !vec) ? a.rot / (2 * v) : a.rot / v;
   a.units = a.turned_units + (a.D - a.rot) / v;
   // Threads: as many as a token has places, in equal rounds, or several tokens side by side.  Up to
-  // 512 of them where a block's latency is what counts (one token of 12 + 12 heads 2.7 us, with
-  // 256 3.3), 256 where the blocks of an SM cover each other's (4099 tokens of 24 + 4 heads
-  // of 80 in fp32 12.6 us, with 256 15).
+  // 512 of them where a block's latency is what counts (one token of 12 + 12 heads 2.4 us, with
+  // 256 3.1; 64 tokens appended 4.45, with 256 5.1), 192 where the blocks of an SM cover each other's
+  // (4099 tokens of 24 + 4 heads of 80 in fp32 11.6 us, with 128 12.5, with 256 13.3; 16896 tokens
+  // appended 51.5, 52.9 and 51.5; 8448 tokens of 12 + 12 heads in bf16 19.2, 17.3 and 19.2).
   const int most = a.T < 2 * (int64_t)sm_count() ? kThreads : kManyThreads;
   const int work = a.heads * a.units;
   const int rounds = (work + most - 1) / most;

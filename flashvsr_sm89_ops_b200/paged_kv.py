@@ -141,7 +141,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     the one for few rows.  It defaults to T (1 without cu_seqlens); any value gives the same
     results up to rounding.  What a page holds past a sequence's end is never seen, NaN or not.
     A NaN or an infinity among a sequence's own values can reach every row of the chunk that
-    shares a tile with it, rows before it included.
+    shares a tile with it, rows before it included.  A row that sees keys, but has only NaN or
+    -inf for scores, is NaN.  Inference only: a backward pass through the result raises.
     """
     name = "paged_attention"
     _lib.require_cuda(q, k_pages, v_pages, table, lens, cu_seqlens)
@@ -390,7 +391,8 @@ class PagedKV:
     def attend(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, causal: bool = True,
                sm_scale: float | None = None, max_new: int | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
-        """paged_attention of q over one layer of this cache."""
+        """paged_attention of q over one layer of this cache.  With cu_seqlens, max_new says where there are few
+        new tokens a sequence (1: single ones): without it the kernel for many rows is taken."""
         name = "PagedKV.attend"
         if not 0 <= layer < self._pools[2]:
             raise ValueError(f"{name}: layer {layer} of {self._pools[2]}")
