@@ -609,14 +609,16 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const Args a) {
         alpha[hh] = mn == -INFINITY ? 1.f : ex2_approx(m[hh] - mn);
         grew |= mn > m[hh];
         m[hh] = mn;
-        const float sub = mn == -INFINITY ? 0.f : mn - Pair<T>::kRange;  // weights up to 2^kRange
+        const float sub = mn == -INFINITY ? 0.f : mn;
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float& x = sc[t][hh * 2 + e];
-            x = ex2_approx(x - sub);
+            x -= sub;
+            if (Pair<T>::kRange > 0.f) x += Pair<T>::kRange;  // (of the difference: exact however large x is)
+            x = ex2_approx(x);
             sum += x;
           }
         l[hh] = l[hh] * alpha[hh] + sum;  // this lane's four keys; the quad joins at the end
@@ -735,9 +737,11 @@ constexpr int kCut = 12;  // key tiles, see where items are dealt out
 constexpr int kAtom = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzle
 constexpr float kLazy = 8.0f;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
-// the factor of all weights: with kLazy above it they fill the range
+// the factor of all weights: with kLazy above it they fill the range.  Maxima from kShifted on do
+// without it: their difference from it would be rounded, by whole powers of two in the end.
 template <typename T>
 constexpr float kShift = Pair<T>::kRange > kLazy ? Pair<T>::kRange - kLazy : 0.f;
+constexpr float kShifted = 1048576.f;
 
 template <int D>
 struct Shape {
@@ -746,18 +750,25 @@ struct Shape {
   static constexpr size_t kSmem = (size_t)kTile * (2 + 2 * kSlots) + 1024 + 1024;  // alignment, barriers
 };
 
-// p = 2^(s c - m) of 64 scores, packed (rounded to 16 bits: off by up to 2^-8 of itself in bf16, 2^-11 or
-// 2^-32 of the largest in fp16); fp32 row sum of the unrounded ones into acc2.  All on the special-function unit: an
-// eighth or a quarter of them as polynomials on the FMA pipe took 8448 over 33792 keys from 1424 to
-// 1412 us, and ragged chunks (32 of up to 600 tokens over up to 600, 32 / 8 heads of 128, pages of 16)
-// from 169 to 186-189 us; 7 of up to 1537 over up to 1001, 16 / 4 x 64, from 65 to 66-67.
+// p = 2^(round(s c) - m) of 64 scores, m one of those products: near it the difference is exact.  In one
+// rounding, 2^(s c - m), every weight would carry what the maximum's own product was rounded by, up to
+// half a step of m: by it fp16 overflows from scores of 2^27 on, bf16 from 2^31 (finite scores, NaN
+// results).  `zero` keeps the compiler from joining the two.  That costs 1-6%: 7 of up to 1537 tokens over
+// up to 1001, 16 / 4 x 64, 64.7 -> 66.5 us; 8448 over 33792 keys 1675 -> 1697 under lasting load; 32 of
+// up to 600 over up to 600, 32 / 8 x 128, pages of 16, 160 -> 170.  Branches to a rare exact path cost
+// 10-15%, predicated differences 20-30%.
+//
+// Packed as 16 bits (a weight is off by up to 2^-8 of itself in bf16, by 2^-11 or 2^-32 of the largest in
+// fp16); fp32 row sum of the unrounded ones into acc2.  All on the special-function unit: an eighth or a
+// quarter of them as polynomials on the FMA pipe took 8448 over 33792 keys from 1424 to 1412 us, the
+// ragged chunks above from 169 to 186-189 us, those of D 64 from 65 to 66-67 (before `zero`).
 template <typename T>
-__device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint64_t nm,
+__device__ __forceinline__ void exp_pack64(const uint32_t* s, uint64_t cc, uint64_t zero, uint64_t nm,
                                            uint64_t& acc2, uint32_t* pk) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const uint64_t xv =
-        f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, nm);
+        f2_add(f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, zero), nm);
     float x0, x1;
     f2_unpack(xv, x0, x1);
     const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
@@ -1139,6 +1150,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tP = tmem + kColP + (uint32_t)(x * 64) + lane_addr;
     const uint32_t tO = tmem + kColO + (uint32_t)(x * 128) + lane_addr;
     const float c = a.scale_log2;
+    const float zero = fminf(c, 0.f);  // c is positive, which the compiler does not know
+    // what a maximum's weights are taken relative to
+    auto ref = [](float m) { return kShift<T> > 0.f && fabsf(m) < kShifted ? m - kShift<T> : m; };
     const int half_rows = a.rows >> 1;
     bool ok = true;
     uint32_t kv = 0, mine = 0;
@@ -1180,20 +1194,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         float alpha = 1.f;
         const bool raise = mb > m_used + kLazy;
         if (raise) {
-          alpha = (m_used == -INFINITY) ? 0.f : ex2_approx(m_used - mb);
+          alpha = (m_used == -INFINITY) ? 0.f : ex2_approx(ref(m_used) - ref(mb));
           m_used = mb;
         }
         // tcgen05.ld / st are warp-wide: the warp rescales when any of its rows does
         const bool rescale = __any_sync(0xffffffffu, raise);
-        const float msub = (m_used == -INFINITY) ? 0.f : m_used - kShift<T>;
-        const uint64_t cc = f2_pack(c, c);
+        const float msub = (m_used == -INFINITY) ? 0.f : ref(m_used);
+        const uint64_t cc = f2_pack(c, c), zz = f2_pack(zero, zero);
         const uint64_t nm = f2_pack(-msub, -msub);
         uint64_t acc2 = f2_pack(0.f, 0.f);
         uint32_t pk[32];
         // twice the same: with the two kinds of tiles apart the compiler keeps all scores in registers
         // (ragged chunks of D 64 65.3 us; in one path it spills ten of them, 67.1)
-        if (masked) exp_pack64<T>(s, cc, nm, acc2, pk);
-        else exp_pack64<T>(s, cc, nm, acc2, pk);
+        if (masked) exp_pack64<T>(s, cc, zz, nm, acc2, pk);
+        else exp_pack64<T>(s, cc, zz, nm, acc2, pk);
         if (j > 0) {
           // P_x and O_x are free once the product of tile j - 1 is done
           if (!__all_sync(0xffffffffu,
@@ -1215,8 +1229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tmem_st_32x32b_x32(tP, pk);
-        if (masked) exp_pack64<T>(s + 64, cc, nm, acc2, pk);
-        else exp_pack64<T>(s + 64, cc, nm, acc2, pk);
+        if (masked) exp_pack64<T>(s + 64, cc, zz, nm, acc2, pk);
+        else exp_pack64<T>(s + 64, cc, zz, nm, acc2, pk);
         tmem_st_32x32b_x32(tP + 32, pk);
         float la, lb;
         f2_unpack(acc2, la, lb);
@@ -1300,7 +1314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (row_ok && !whole)
         *reinterpret_cast<float2*>(a.part_ml + prow * 2) =
-            make_float2(have_o ? m_used : -INFINITY, have_o ? l : 0.f);
+            make_float2(have_o ? ref(m_used) : -INFINITY, have_o ? l : 0.f);
       tc_fence_before();
       kv += g.all;
       mine += cnt;

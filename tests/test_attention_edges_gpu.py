@@ -349,6 +349,31 @@ def test_many_small_weights_in_fp16(L, max_new, shift):
     assert ((out - want).abs() <= tol).all(), ((out - want).abs() / tol).max()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("max_new", [1, 200])
+def test_scores_of_any_size(max_new, dtype):
+    """Two kinds of keys, one score S for the one and -S for the other: the result is the mean of the first
+    kind's values, whatever S is, though fp32 holds log2 e S to no better than 1 from 2^24 on."""
+    n, L, D = 3, 900, 64
+    g = _gen(103)
+    kv = ops.PagedKV.empty(1, 60, 16, 1, D, 1, dtype=dtype)
+    kv.reserve(_i32([L]))
+    v = torch.randn(L, 1, D, device=DEV, generator=g).to(dtype)
+    up = torch.rand(L, device=DEV, generator=g) < 0.3
+    want = v[up].double().mean(0)
+    # P in 16 bits (all of one value, so that is in the numerator alone), the sums, the output
+    tol = v[up].double().abs().mean(0) * (U[dtype] + 2 * L * 2.0 ** -23) + U[dtype] * want.abs() + 2.0 ** -25
+    for e in (*range(8, 15), *((20, 30, 50) if dtype == torch.bfloat16 else ())):
+        for m in (1.0, 1.1, 1.3, 1.7, 1.9):
+            k = torch.zeros(L, 1, D, device=DEV, dtype=dtype)
+            k[:, 0, 0] = torch.where(up, m * 2.0 ** e, -m * 2.0 ** e)
+            kv.append(0, k, v, _i32([0, L]))
+            q = torch.zeros(n, 1, D, device=DEV, dtype=dtype)
+            q[:, :, 0] = 2.0 ** e
+            out = kv.attend(0, q, _i32([0, n]), sm_scale=1.0, max_new=max_new, causal=False).double()
+            assert ((out - want).abs() <= tol).all(), (e, m, out[0, 0, :4])
+
+
 @pytest.mark.parametrize("max_new", [1 << 58, 1 << 59, (1 << 63) - 1])
 def test_huge_bounds_on_the_new_tokens(max_new):
     """max_new only picks the kernel: one that no product of it fits is that of many rows."""
