@@ -251,9 +251,9 @@ class PagedKV:
         self._tail = (lens.data_ptr(), table.data_ptr(), seqs, width, P, page)
         self._room = (refused.data_ptr(), refs.data_ptr(), status.data_ptr(), dropped.data_ptr())
 
-    # a copy has tensors, and so addresses, of its own
+    # a copy has tensors, and so addresses and a workspace, of its own
     def __getstate__(self):
-        return {"_tensors": self._tensors}
+        return {k: v for k, v in self.__dict__.items() if k != "_ws"}
 
     def __setstate__(self, state):
         self.__dict__.update(state)

@@ -523,7 +523,11 @@ def test_copies_have_their_own_tensors():
     kv.append(1, *_chunk(23, 2, 64, 99)[:2], _i32([0, 20, 23, 23]))
     q = _chunk(23, 4, 64, 100)[0]
     want = kv.attend(1, q, _i32([0, 20, 23, 23]))
+    kv.name = "mine"
     twin = copy.deepcopy(kv)
+    assert twin.name == "mine" and twin.status.data_ptr() + 4 == twin.refused.data_ptr()
+    assert not {t.data_ptr() for t in (twin.k, twin.v, twin.table, twin.lens, twin.refs, twin.dropped, twin.status, twin._ws)} \
+        & {t.data_ptr() for t in (kv.k, kv.v, kv.table, kv.lens, kv.refs, kv.dropped, kv.status, kv._ws)}
     twin.release(_i32([0]))
     twin.reserve(_i32([0, 17, 4]))
     twin.append(1, *_chunk(21, 2, 64, 101)[:2], _i32([0, 0, 17, 21]))
